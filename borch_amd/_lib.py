@@ -33,6 +33,7 @@ _c_i64 = ctypes.c_int64
 _c_p = ctypes.c_void_p
 _c_int = ctypes.c_int
 _c_size = ctypes.c_size_t
+_c_f = ctypes.c_float
 
 
 
@@ -41,6 +42,12 @@ class ConvDesc(ctypes.Structure):
     _fields_ = [("w", _c_p), ("O", _c_i64), ("KH", _c_i64), ("KW", _c_i64), ("stride", _c_i64), ("pad", _c_i64),
                 ("sW", _c_p), ("bias", _c_p), ("residual", _c_p), ("act", _c_int), ("out", _c_p),
                 ("s_out", _c_p), ("q_out", _c_p), ("amax", _c_p)]
+
+
+class Kv4Desc(ctypes.Structure):
+    """``bq_kv4_cache`` (include/bq.h): a key-value cache held in 4 bits."""
+    _fields_ = [("k", _c_p), ("k_scales", _c_p), ("v", _c_p), ("v_scales", _c_p), ("pages", _c_i64),
+                ("heads", _c_i64), ("page", _c_i64), ("dim", _c_i64)]
 
 
 # name -> (restype, argtypes); mirrors include/bq.h one for one.
@@ -105,6 +112,14 @@ SIGNATURES = {
     "bq_se_gate_absmax_parts": (_c_i64, [_c_i64, _c_i64]),
     "bq_se_gate_nhwc": (_c_int, [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p,
                                  _c_size, _c_p]),
+    "bq_prompt_attention": (_c_int, [_c_p, _c_p, _c_p, _c_int, *[_c_i64] * 10, _c_p, _c_i64, _c_int, _c_f, _c_p, _c_p]),
+    "bq_kv4_append": (_c_int, [_c_p, _c_p, _c_p, _c_int, *[_c_i64] * 5, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p]),
+    "bq_kv4_read": (_c_int, [_c_p, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_p]),
+    "bq_kv4_attend_ws_bytes": (_c_size, [_c_i64] * 5),
+    "bq_kv4_attend": (_c_int, [_c_p, _c_p, _c_int, *[_c_i64] * 5, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_f, _c_p,
+                               _c_p, _c_i64, _c_i64, _c_p, _c_size, _c_p]),
+    "bq_kv4_evict": (_c_int, [_c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64,
+                              _c_i64, _c_p, _c_p, _c_p, _c_p]),
 }
 
 _lock = threading.Lock()

@@ -1,0 +1,605 @@
+// Attention of the newest tokens over a cache held in 4 bits (its form: bq_kv4.h).
+//
+// For sequence b with n = lens[b] cached tokens, the newest T of them the queries', query token t
+// of query head h sees the first n - T + 1 + t: out = sum_i p_i v_i with p = softmax(scale q . k_i),
+// zeros where it sees nothing. The G = q_heads / heads query heads of a key-value head and the T
+// tokens are the rows of one product, R = T G.
+//
+// A wave takes 32 cached tokens at a time, straight from memory into MFMA operands (no LDS): the
+// scores transposed, S^T = k q^T, 16 x 16 x 32, so that lane (n, g) of column n = lane % 16 and
+// g = lane / 16 holds row n's scores for tokens 8 g .. 8 g + 7, which is the second product's
+// operand as it stands: O^T = v^T p^T. The codes become bf16 exactly (a code has 2 significant
+// bits, bf16 the exponents of f32). q enters as the exact sum of bf16 pieces (f32: 3, f16: 2,
+// bf16: 1) and p, in [0, 1], as pieces too (f32: 3, the 16-bit types: 2, so that p's error is
+// 2^-17 where the output's rounding is 2^-9 or 2^-12), with f32 accumulation.
+// The contracted index of the scores is permuted (lane group g takes a quarter of the channels) and
+// so are the rows of v^T (row m of product j is channel DIM / 16 m + j), both to load whole pieces.
+//
+// Each row keeps its running maximum, sum and output (one pass over the cache). A workgroup of four
+// waves takes a chunk of a sequence for one key-value head and 16 RT rows, and joins its waves in
+// LDS; where a sequence is cut into several chunks, they leave (maximum, sum, output) in the
+// workspace and a second kernel joins them. What the cached tokens received (the softmax weights
+// summed over the rows) needs the final maximum and sum of each row: a last kernel takes the scores
+// again, each token by one wave, so that sums are added without atomics, in one order.
+#include <math.h>
+
+#include "bq_bf16x3.h"
+#include "bq_kv4.h"
+
+namespace bq {
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+template <typename T>
+constexpr int Q_PIECES = __is_same(T, float) ? 3 : __is_same(T, _Float16) ? 2 : 1;
+template <typename T>
+constexpr int P_PIECES = __is_same(T, float) ? 3 : 2;
+
+struct Attend {
+  Kv4 c;
+  const int* lens;
+  const void* q;
+  int64_t qb, qt, qh;  // strides in elements: sequence, token, head
+  int tokens, group, rows, row_groups, max_len, chunk, splits;
+  FastDiv by_group;
+  float scale2;  // scale * log2(e)
+  void* out;     // [B][tokens][heads * group][DIM]
+  float *part, *stats;  // partial outputs [B heads][splits][rows][DIM + 2]; [B heads][rows][2]
+  float* weights;
+  int64_t wb, wh;
+};
+
+template <int P>
+struct Pieces {
+  v8bf p[P];
+};
+
+template <int P>
+__device__ __forceinline__ Pieces<P> pieces_of(const float x[8]) {
+  Pieces<P> r;
+  uint32_t w[P][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      w[k][i] = bf2(a, b);
+      if (k + 1 < P) {
+        a = __fsub_rn(a, __uint_as_float(w[k][i] << 16));
+        b = __fsub_rn(b, __uint_as_float(w[k][i] & 0xffff0000u));
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < P; ++k) r.p[k] = __builtin_bit_cast(v8bf, make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]));
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void load8f(const T* p, float x[8]) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  } else if constexpr (__is_same(T, __bf16)) {
+    const v8bf a = *reinterpret_cast<const v8bf*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
+  } else {
+    const v8h a = *reinterpret_cast<const v8h*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
+  }
+}
+
+// q's pieces as the score product's second operand: row 16 tile + n, step s, channels
+// DIM / 4 g + 8 s ..; rows past the last as zeros.
+template <typename T, int DIM>
+struct QFrag {
+  Pieces<Q_PIECES<T>> s[DIM / 32];
+  __device__ __forceinline__ void load(const Attend& a, int b, int h, int row0) {
+    const int lane = threadIdx.x & 63, row = row0 + (lane & 15), g = lane >> 4;
+    const int t = fdiv(row, a.by_group.mul, a.by_group.shift), j = row - t * a.group;
+    const T* p = (const T*)a.q + b * a.qb + t * a.qt + (int64_t)(h * a.group + j) * a.qh + DIM / 4 * g;
+#pragma unroll
+    for (int i = 0; i < DIM / 32; ++i) {
+      float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (row < a.rows) load8f(p + 8 * i, x);
+      s[i] = pieces_of<Q_PIECES<T>>(x);
+    }
+  }
+};
+
+__device__ __forceinline__ float scale_bits(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// Eight codes (one dword, low half byte first) times a scale, in bf16, exactly.
+__device__ __forceinline__ v8bf codes8(uint32_t w, float scale) {
+  const v2bf a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1),
+             c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3);
+  return v8bf{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// What a lane loads of 32 tokens' keys: of token 8 (n / 4) + 4 t + n % 4, its quarter g of the
+// channels (row n of score tile t), and the scale bytes of both tiles' tokens.
+template <int DIM>
+struct KBlock {
+  uint32_t w[2][DIM / 32];
+  uint32_t scales;
+  __device__ __forceinline__ void load(const Kv4& c, int at, int h, int off0) {
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const size_t row = Kv4At<DIM>::row(c, at, h, off0);
+    const uint8_t* p = c.k + Kv4At<DIM>::k(row) + (8 * (n >> 2) + (n & 3)) * (DIM / 2) + g * (DIM / 8);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if constexpr (DIM == 128) {
+        const uint4 x = *reinterpret_cast<const uint4*>(p + t * 4 * (DIM / 2));
+        w[t][0] = x.x, w[t][1] = x.y, w[t][2] = x.z, w[t][3] = x.w;
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(p + t * 4 * (DIM / 2));
+        w[t][0] = x.x, w[t][1] = x.y;
+      }
+    }
+    scales = *reinterpret_cast<const uint16_t*>(c.ks + row * (DIM / 32) + ((n & 3) * (DIM / 32) + g * (DIM / 32) / 4) * 8 +
+                                                2 * (n >> 2));
+  }
+  // The scores of 16 rows, before the scale: [4 t + i] is token 8 g + 4 t + i
+  template <typename T>
+  __device__ __forceinline__ void scores(const QFrag<T, DIM>& q, float s[8]) const {
+    constexpr int P = Q_PIECES<T>;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const float f = scale_bits((scales >> (8 * t)) & 255);
+      v4f acc = {0.f, 0.f, 0.f, 0.f};
+      v8bf kf[DIM / 32];
+#pragma unroll
+      for (int i = 0; i < DIM / 32; ++i) kf[i] = codes8(w[t][i], f);
+#pragma unroll
+      for (int k = P - 1; k >= 0; --k)  // the smallest pieces first
+#pragma unroll
+        for (int i = 0; i < DIM / 32; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i], q.s[i].p[k], acc, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[4 * t + i] = acc[i];
+    }
+  }
+};
+
+// Of 32 tokens' values: of tokens 8 g .. 8 g + 7, channel slice n (DIM / 16 channels).
+template <int DIM>
+struct VBlock {
+  uint32_t w[8];  // token i's slice: 8 codes (DIM 128), or two tokens' 4 codes each
+  uint32_t s[2];  // scale bytes, four tokens a dword
+  __device__ __forceinline__ void load(const Kv4& c, int at, int h, int off0) {
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const size_t row = Kv4At<DIM>::row(c, at, h, off0);
+    const uint8_t* p = c.v + row * (DIM / 2);
+    if constexpr (DIM == 128) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint4 x = *reinterpret_cast<const uint4*>(p + (2 * g + e) * 256 + n * 16);
+        w[4 * e] = x.x, w[4 * e + 1] = x.y, w[4 * e + 2] = x.z, w[4 * e + 3] = x.w;
+      }
+    } else {
+      const uint4 x = *reinterpret_cast<const uint4*>(p + g * 256 + n * 16);
+      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    }
+    const uint2 y = *reinterpret_cast<const uint2*>(c.vs + row * (DIM / 32) + n * (DIM / 32) / 16 * 32 + 8 * g);
+    s[0] = y.x, s[1] = y.y;
+  }
+  __device__ __forceinline__ uint32_t byte(int i) const { return (s[i >> 2] >> (8 * (i & 3))) & 255; }
+  __device__ __forceinline__ void clear(int i) {  // token i reads as zeros
+    s[i >> 2] = (s[i >> 2] & ~(255u << (8 * (i & 3)))) | (127u << (8 * (i & 3)));
+    if constexpr (DIM == 128) w[i] = 0;
+    else w[i >> 1] &= i & 1 ? 0xffffu : 0xffff0000u;
+  }
+  // The first operand of products 2 k and 2 k + 1 (channels DIM / 16 n + 2 k and + 1), 8 tokens each.
+  template <int K>
+  __device__ __forceinline__ void frags(v8bf& even, v8bf& odd) const {
+    uint32_t e[4], o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t a, b;
+      if constexpr (DIM == 128) {
+        a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[2 * i], scale_bits(byte(2 * i)), K));
+        b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[2 * i + 1], scale_bits(byte(2 * i + 1)), K));
+      } else {
+        a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[i], scale_bits(byte(2 * i)), K));
+        b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[i], scale_bits(byte(2 * i + 1)), K + 2));
+      }
+      e[i] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+      o[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    }
+    even = __builtin_bit_cast(v8bf, make_uint4(e[0], e[1], e[2], e[3]));
+    odd = __builtin_bit_cast(v8bf, make_uint4(o[0], o[1], o[2], o[3]));
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+  } else if constexpr (__is_same(T, __bf16)) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(bf2(a, b), bf2(c, d));
+  } else {
+    typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<v4h*>(p) = v4h{(_Float16)a, (_Float16)b, (_Float16)c, (_Float16)d};
+  }
+}
+
+// exp2(c (s - m)) with an empty row's maximum, -infinity, taken as 0
+__device__ __forceinline__ float weight_of(float s, float base, float c) {
+  return __builtin_amdgcn_exp2f(__fmul_rn(__fsub_rn(s, base), c));
+}
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+
+template <typename T, int DIM, int RT>
+__global__ __launch_bounds__(256) void kv4_attend_kernel(Attend a) {
+  constexpr int PP = P_PIECES<T>, NJ = DIM / 16, PITCH = DIM + 4;
+  __shared__ __attribute__((aligned(16))) float so[4][16][PITCH];
+  __shared__ float sm[4][16], sl[4][16];
+  const int split = blockIdx.x, h = blockIdx.y % a.c.heads, rg = blockIdx.y / a.c.heads, b = blockIdx.z;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+  const int len = max(0, min(a.lens[b], a.max_len));
+  const int t0 = split * a.chunk;
+  if (t0 >= len && split > 0) return;  // the first chunk of an empty sequence writes its zeros
+  const int t1 = min(len, t0 + a.chunk);
+  const int row0 = rg * 16 * RT;
+  const int sure = len - a.tokens + 1;  // tokens that every row sees
+
+  // this wave's blocks of 32 tokens: wave, wave + 4, ...; their pages, one a lane
+  const int blocks = (t1 - t0 + 31) >> 5;
+  const int first = (t0 >> 5) + wave;
+  const int bpp = a.c.page >> 5;
+  const int mine = blocks > wave ? (blocks - wave + 3) >> 2 : 0;
+  int pages = -1;
+  if (lane < mine) {
+    const int pi = fdiv(first + 4 * lane, a.c.by_blocks.mul, a.c.by_blocks.shift);
+    pages = kv4_page(a.c, b, pi);
+  }
+
+  QFrag<T, DIM> q[RT];
+  int end[RT];  // what this lane's row sees
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    q[r].load(a, b, h, row0 + 16 * r);
+    const int t = fdiv(row0 + 16 * r + n, a.by_group.mul, a.by_group.shift);
+    end[r] = min(len, sure + t);
+  }
+  float m[RT], l[RT];
+  v4f o[RT][NJ];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) o[r][j] = v4f{0.f, 0.f, 0.f, 0.f};
+  }
+
+  KBlock<DIM> kb, kn;
+  VBlock<DIM> vb, vn;
+  auto fetch = [&](int i, KBlock<DIM>& k, VBlock<DIM>& v) {
+    const int blk = first + 4 * i;
+    const int at = max(0, __builtin_amdgcn_readlane(pages, i));
+    const int off0 = (blk - fdiv(blk, a.c.by_blocks.mul, a.c.by_blocks.shift) * bpp) << 5;
+    k.load(a.c, at, h, off0);
+    v.load(a.c, at, h, off0);
+  };
+  if (mine > 0) fetch(0, kn, vn);
+  for (int i = 0; i < mine; ++i) {
+    kb = kn;
+    vb = vn;
+    if (i + 1 < mine) fetch(i + 1, kn, vn);
+    const int tok = (first + 4 * i) << 5;
+    if (__builtin_amdgcn_readlane(pages, i) < 0) continue;  // no page: nothing to see
+    float s[RT][8];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) kb.template scores<T>(q[r], s[r]);
+    uint32_t lost = 0;  // bit e: token 8 g + e of this lane's slice is NaN and not seen by every row
+    const bool edge = tok + 32 > sure;
+    if (edge) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int t = tok + 8 * g + e;
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+          if (t >= end[r]) s[r][e] = -INFINITY;
+        if (t >= sure && (t >= len || vb.byte(e) == 255)) {
+          if (t < len) lost |= 1u << e;
+          vb.clear(e);
+        }
+      }
+    }
+    Pieces<PP> p[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      float top = m[r];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, s[r][e]);
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float base = base_of(top);
+      if (__any(top > m[r])) {
+        const float f = weight_of(m[r], base, a.scale2);
+        l[r] = __fmul_rn(l[r], f);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[r][j] *= f;
+        m[r] = top;
+      }
+      float w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        w[e] = weight_of(s[r][e], base, a.scale2);
+        l[r] = __fadd_rn(l[r], w[e]);
+      }
+      p[r] = pieces_of<PP>(w);
+    }
+    auto product = [&]<int K>() {
+      v8bf f[2];
+      vb.template frags<K>(f[0], f[1]);
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int z = 0; z < 2; ++z)
+#pragma unroll
+          for (int k = PP - 1; k >= 0; --k)
+            o[r][2 * K + z] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[z], p[r].p[k], o[r][2 * K + z], 0, 0, 0);
+    };
+    product.template operator()<0>();
+    product.template operator()<1>();
+    if constexpr (DIM == 128) {
+      product.template operator()<2>();
+      product.template operator()<3>();
+    }
+    if (edge && __any(lost != 0)) {
+      // NaN values that some rows see and others do not: they left the products; the rows that see
+      // them get NaN in the 32 channels that share the scale. Lane (n, g) of O holds channels
+      // DIM / 4 g .., of v's lanes those of slice 4 g (a token group u): its block's scale.
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint64_t who = __ballot((lost >> e) & 1);
+        for (int u = 0; u < 4; ++u)
+          if ((who >> (16 * u + 4 * g)) & 1)
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+              if (tok + 8 * u + e < end[r])
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) o[r][j] = v4f{NAN, NAN, NAN, NAN};
+      }
+    }
+  }
+
+  // the four waves' rows together: lane (n, g) holds channels DIM / 4 g + DIM / 16 i + j of row n
+  const size_t bh = (size_t)b * a.c.heads + h;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    l[r] = __fadd_rn(l[r], __shfl_xor(l[r], 16));
+    l[r] = __fadd_rn(l[r], __shfl_xor(l[r], 32));
+    if (r) __syncthreads();
+    if (g == 0) {
+      sm[wave][n] = m[r];
+      sl[wave][n] = l[r];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; j += 4)
+        *reinterpret_cast<float4*>(&so[wave][n][DIM / 4 * g + NJ * i + j]) =
+            make_float4(o[r][j][i], o[r][j + 1][i], o[r][j + 2][i], o[r][j + 3][i]);
+    __syncthreads();
+    constexpr int LANES = DIM / 4;  // threads a row, four channels each
+    for (int x = threadIdx.x; x < 16 * LANES; x += 256) {
+      const int rr = x / LANES, c4 = x % LANES * 4, row = row0 + 16 * r + rr;
+      if (row >= a.rows) continue;
+      const float top = fmaxf(fmaxf(sm[0][rr], sm[1][rr]), fmaxf(sm[2][rr], sm[3][rr])), base = base_of(top);
+      float sum = 0.f;
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = weight_of(sm[w][rr], base, a.scale2);
+        const float4 z = *reinterpret_cast<const float4*>(&so[w][rr][c4]);
+        sum = __fmaf_rn(f, sl[w][rr], sum);
+        y.x = __fmaf_rn(f, z.x, y.x);
+        y.y = __fmaf_rn(f, z.y, y.y);
+        y.z = __fmaf_rn(f, z.z, y.z);
+        y.w = __fmaf_rn(f, z.w, y.w);
+      }
+      if (a.splits > 1) {
+        float* to = a.part + ((bh * a.splits + split) * a.rows + row) * (DIM + 2);
+        *reinterpret_cast<float2*>(to + c4) = make_float2(y.x, y.y);
+        *reinterpret_cast<float2*>(to + c4 + 2) = make_float2(y.z, y.w);
+        if (c4 == 0) *reinterpret_cast<float2*>(to + DIM) = make_float2(top, sum);
+      } else {
+        const float d = sum == 0.f ? 1.f : sum;
+        const int t = fdiv(row, a.by_group.mul, a.by_group.shift), j = row - t * a.group;
+        T* to = (T*)a.out + (((size_t)b * a.tokens + t) * a.c.heads * a.group + h * a.group + j) * DIM + c4;
+        store4(to, __fdiv_rn(y.x, d), __fdiv_rn(y.y, d), __fdiv_rn(y.z, d), __fdiv_rn(y.w, d));
+        if (a.weights && c4 == 0) *reinterpret_cast<float2*>(a.stats + (bh * a.rows + row) * 2) = make_float2(top, d);
+      }
+    }
+  }
+}
+
+// The chunks of one row joined, a workgroup a row: four waves a quarter of the chunks each.
+template <typename T, int DIM>
+__global__ __launch_bounds__(256) void kv4_join_kernel(Attend a) {
+  __shared__ float sm[4], sl[4], so[4][DIM];
+  const int row = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const size_t bh = (size_t)b * a.c.heads + h;
+  const int len = max(0, min(a.lens[b], a.max_len));
+  const int splits = max(1, (len + a.chunk - 1) / a.chunk);
+  const float* part = a.part + (bh * a.splits * a.rows + row) * (DIM + 2);
+  const size_t step = (size_t)a.rows * (DIM + 2);
+  constexpr int C = DIM / 64;
+  float top = -INFINITY, sum = 0.f, y[C] = {};
+  for (int s = wave; s < splits; s += 4) {
+    const float* p = part + s * step;
+    const float2 ms = *reinterpret_cast<const float2*>(p + DIM);
+    float x[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) x[c] = p[C * lane + c];
+    const float now = fmaxf(top, ms.x), base = base_of(now);
+    const float f = weight_of(top, base, a.scale2), e = weight_of(ms.x, base, a.scale2);
+    sum = __fmaf_rn(sum, f, __fmul_rn(ms.y, e));
+#pragma unroll
+    for (int c = 0; c < C; ++c) y[c] = __fmaf_rn(y[c], f, __fmul_rn(x[c], e));
+    top = now;
+  }
+  if (lane == 0) sm[wave] = top, sl[wave] = sum;
+#pragma unroll
+  for (int c = 0; c < C; ++c) so[wave][C * lane + c] = y[c];
+  __syncthreads();
+  if (wave) return;
+  const float now = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), base = base_of(now);
+  sum = 0.f;
+#pragma unroll
+  for (int c = 0; c < C; ++c) y[c] = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float f = weight_of(sm[w], base, a.scale2);
+    sum = __fmaf_rn(f, sl[w], sum);
+#pragma unroll
+    for (int c = 0; c < C; ++c) y[c] = __fmaf_rn(f, so[w][C * lane + c], y[c]);
+  }
+  const float d = sum == 0.f ? 1.f : sum;
+  const int t = fdiv(row, a.by_group.mul, a.by_group.shift), j = row - t * a.group;
+  T* to = (T*)a.out + (((size_t)b * a.tokens + t) * a.c.heads * a.group + h * a.group + j) * DIM + C * lane;
+#pragma unroll
+  for (int c = 0; c < C; ++c) to[c] = (T)__fdiv_rn(y[c], d);
+  if (a.weights && lane == 0) *reinterpret_cast<float2*>(a.stats + (bh * a.rows + row) * 2) = make_float2(now, d);
+}
+
+// What each cached token received, added to its sum: the scores of 32 tokens a wave once more, each
+// row's weight from its final maximum and sum, rows in order.
+template <typename T, int DIM>
+__global__ __launch_bounds__(256) void kv4_weights_kernel(Attend a, int blocks) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int blk = blockIdx.x * 4 + wave, h = blockIdx.y, b = blockIdx.z;
+  const int len = max(0, min(a.lens[b], a.max_len)), tok = blk << 5;
+  if (tok >= len) return;
+  const int pi = fdiv(blk, a.c.by_blocks.mul, a.c.by_blocks.shift);
+  const int at = kv4_page(a.c, b, pi);
+  if (at < 0) return;
+  const size_t bh = (size_t)b * a.c.heads + h;
+  KBlock<DIM> kb;
+  kb.load(a.c, at, h, (blk - pi * (a.c.page >> 5)) << 5);
+  float total[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int row0 = 0; row0 < a.rows; row0 += 16) {
+    QFrag<T, DIM> q;
+    q.load(a, b, h, row0);
+    const int row = row0 + n, t = fdiv(row, a.by_group.mul, a.by_group.shift);
+    const int end = row < a.rows ? min(len, len - a.tokens + 1 + t) : 0;
+    float2 st = make_float2(0.f, 1.f);
+    if (row < a.rows) st = *reinterpret_cast<const float2*>(a.stats + (bh * a.rows + row) * 2);
+    float s[8];
+    kb.template scores<T>(q, s);
+    const float base = base_of(st.x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (tok + 8 * g + e < end)
+        total[e] = __fadd_rn(total[e], __fdiv_rn(weight_of(s[e], base, a.scale2), st.y));
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) total[e] = __fadd_rn(total[e], __shfl_xor(total[e], d));
+  }
+  float mine = total[0];  // lane n < 8 writes token 8 g + n
+#pragma unroll
+  for (int e = 1; e < 8; ++e) mine = n == e ? total[e] : mine;
+  const int t = tok + 8 * g + n;
+  if (n < 8 && t < len) {
+    float* to = a.weights + b * a.wb + h * a.wh + t;
+    *to = __fadd_rn(*to, mine);
+  }
+}
+
+// The tokens a chunk takes and how many chunks that makes of the longest sequence.
+static int chunk_of(int64_t B, int64_t heads, int64_t rows, int64_t max_len, int64_t* splits) {
+  const int64_t groups = B * heads * ((rows + 31) / 32);
+  int64_t chunk = 512;
+  while (chunk < 4096 && groups * ((max_len + 2 * chunk - 1) / (2 * chunk)) >= 4096) chunk *= 2;
+  while (chunk > 128 && groups * ((max_len + chunk - 1) / chunk) < 512) chunk /= 2;
+  *splits = (max_len + chunk - 1) / chunk;
+  if (*splits < 1) *splits = 1;
+  return (int)chunk;
+}
+
+template <typename T, int DIM>
+static int launch(const char* what, const Attend& a, int B, hipStream_t st) {
+  if (a.rows <= 16)
+    kv4_attend_kernel<T, DIM, 1><<<dim3(a.splits, a.c.heads, B), 256, 0, st>>>(a);
+  else
+    kv4_attend_kernel<T, DIM, 2><<<dim3(a.splits, a.c.heads * a.row_groups, B), 256, 0, st>>>(a);
+  if (a.splits > 1) kv4_join_kernel<T, DIM><<<dim3(a.rows, a.c.heads, B), 256, 0, st>>>(a);
+  if (a.weights && a.max_len > 0) {
+    const int blocks = (a.max_len + 31) / 32;
+    kv4_weights_kernel<T, DIM><<<dim3((blocks + 3) / 4, a.c.heads, B), 256, 0, st>>>(a, blocks);
+  }
+  return check_launch(what);
+}
+
+}  // namespace bq
+
+using namespace bq;
+
+size_t bq_kv4_attend_ws_bytes(int64_t B, int64_t heads, int64_t rows, int64_t dim, int64_t max_len) {
+  if (B < 1 || heads < 1 || rows < 1 || dim < 1 || max_len < 0) return 0;
+  int64_t splits;
+  chunk_of(B, heads, rows, max_len, &splits);
+  const size_t r = (size_t)B * heads * rows;
+  return r * 8 + (splits > 1 ? r * splits * (dim + 2) * 4 : 0);
+}
+
+int bq_kv4_attend(const bq_kv4_cache* cache, const void* q, int type, int64_t tokens, int64_t q_heads, int64_t q_seq,
+                  int64_t q_token, int64_t q_head, const int32_t* table, int64_t B, int64_t width, const int32_t* lens,
+                  int64_t max_len, float scale, void* out, float* weights, int64_t w_seq, int64_t w_head, void* ws,
+                  size_t ws_bytes, bq_stream_t stream) {
+  const char* what = "bq_kv4_attend";
+  Attend a;
+  if (const int rc = kv4_of(what, cache, table, B, width, &a.c)) return rc;
+  if (type < 0 || type > 2) return set_error(BQ_ERR_ARG, "%s: type %d", what, type);
+  if (tokens < 0 || q_heads < 1 || max_len < 0 || max_len > 0x7fffffff - 8192)
+    return set_error(BQ_ERR_ARG, "%s: bad sizes", what);
+  if (q_heads % cache->heads)
+    return set_error(BQ_ERR_ARG, "%s: %lld query heads over %lld key-value heads", what, (long long)q_heads,
+                     (long long)cache->heads);
+  if (!(scale > 0.f) || !(scale < 1e30f)) return set_error(BQ_ERR_ARG, "%s: scale %g", what, (double)scale);
+  if (B == 0 || tokens == 0) return BQ_OK;
+  const int64_t group = q_heads / cache->heads;
+  if (tokens > 1 << 20 || group > 1 << 10 || B > 65535) return set_error(BQ_ERR_ARG, "%s: size too large", what);
+  const int64_t rows = tokens * group, row_groups = (rows + 31) / 32;
+  if (cache->heads * row_groups > 65535 || rows > 1 << 20) return set_error(BQ_ERR_ARG, "%s: size too large", what);
+  if (!q || !lens || !out) return set_error(BQ_ERR_ARG, "%s: null pointer", what);
+  const int64_t size = type == KV4_F32 ? 4 : 2;
+  if ((((uintptr_t)q | (uintptr_t)out) & 15) || (q_seq | q_token | q_head) * size % 16)
+    return set_error(BQ_ERR_ARG, "%s: rows that are not 16-byte aligned", what);
+  int64_t splits;
+  a.chunk = chunk_of(B, cache->heads, rows, max_len, &splits);
+  const size_t need = bq_kv4_attend_ws_bytes(B, cache->heads, rows, cache->dim, max_len);
+  if ((weights || splits > 1) && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
+    return set_error(BQ_ERR_ARG, "%s: a workspace of %zu bytes, given %zu", what, need, ws ? ws_bytes : 0);
+  const int64_t held = cache->pages ? width * cache->page : 0;  // tokens that a sequence's pages have room for
+  a.splits = (int)splits;
+  a.lens = lens;
+  a.q = q;
+  a.qb = q_seq;
+  a.qt = q_token;
+  a.qh = q_head;
+  a.tokens = (int)tokens;
+  a.group = (int)group;
+  a.rows = (int)rows;
+  a.row_groups = (int)row_groups;
+  a.max_len = (int)(max_len < held ? max_len : held);
+  a.by_group = fast_div((uint32_t)group);
+  a.scale2 = scale * 1.4426950408889634f;
+  a.out = out;
+  a.stats = (float*)ws;
+  a.part = a.stats + (size_t)B * cache->heads * rows * 2;
+  a.weights = weights;
+  a.wb = w_seq;
+  a.wh = w_head;
+  hipStream_t st = (hipStream_t)stream;
+  const bool wide = cache->dim == 128;
+  if (type == KV4_F32) return wide ? launch<float, 128>(what, a, (int)B, st) : launch<float, 64>(what, a, (int)B, st);
+  if (type == KV4_BF16) return wide ? launch<__bf16, 128>(what, a, (int)B, st) : launch<__bf16, 64>(what, a, (int)B, st);
+  return wide ? launch<_Float16, 128>(what, a, (int)B, st) : launch<_Float16, 64>(what, a, (int)B, st);
+}

@@ -470,6 +470,83 @@ int bq_gemv_w8a32(const float* x, const int8_t* W, int64_t M, int64_t N, int64_t
  * (borch-ts/src/kernels.ts:1264-1274). */
 int bq_dequant_i8(const int8_t* q, int64_t N, int64_t K, const float* s, float* w, bq_stream_t stream);
 
+/* ---- a decoder's attention: whole prompts, and a key-value cache held in 4 bits ----
+ *
+ * Element types of `type`: 0 f32, 1 bf16, 2 f16. Strides are in elements; channels are contiguous
+ * and every row starts 16-byte aligned. scale > 0 multiplies the scores (0 < scale < 1e30). */
+#define BQ_TYPE_F32 0
+#define BQ_TYPE_BF16 1
+#define BQ_TYPE_F16 2
+
+/* Softmax attention over whole prompts: B sequences packed one after another, sequence b the rows
+ * cu[b] .. cu[b + 1] - 1 (cu i32 [B + 1], ascending) of q [n, q_heads, dim] and of k, v [n, heads,
+ * dim]; query head j attends with key-value head j / (q_heads / heads).
+ *   out [n, q_heads, dim] (contiguous, of q's type) = softmax(scale q k^T) v
+ * over the sequence's rows, causal: up to the query's own. Rows of no sequence get zeros. f32
+ * accumulation; f32 products as exact sums of bf16 pieces, to f32's accuracy (values below 2^-109
+ * lose up to 2^-134); p rounded to the 16-bit types. What a query does not see never reaches its
+ * output, infinities and NaN included. dim 64 or 128. Beside the path, as bq_attention_f32
+ * (scaled_dot_product_attention, borch/_nn.py:2143-2170, with is_causal and enable_gqa). */
+int bq_prompt_attention(const void* q, const void* k, const void* v, int type, int64_t n, int64_t q_heads,
+                        int64_t heads, int64_t dim, int64_t q_token, int64_t q_head, int64_t k_token, int64_t k_head,
+                        int64_t v_token, int64_t v_head, const int32_t* cu, int64_t B, int causal, float scale,
+                        void* out, bq_stream_t stream);
+
+/* A key-value cache in pages of `page` tokens (a multiple of 32), for heads of dim 64 or 128. A
+ * value is +-{0, 1/2, 1, 3/2, 2, 3, 4, 6} (4 bits: sign, two of exponent, one of mantissa) times the
+ * power of two 2^(byte - 127) of its 32 channels; byte 255 stands for NaN. Arrays (contiguous,
+ * 16-byte aligned), first [pages][heads], then of each page and head, with tb = 512 / dim:
+ *   k         [page][dim / 2]               channels 2 i, 2 i + 1 in byte i's low and high half
+ *   k_scales  [page / 32][4][dim / 32][8]   token 32 a + 4 c + b at [a][b][:][c]
+ *   v         [page / tb][16][tb][dim / 32] token tb a + b, channels dim / 16 n .. at [a][n][b]
+ *   v_scales  [page / 32][dim / 32][32]     token 32 a + b at [a][:][b]
+ * Callers keep table i32 [B, width], each sequence's pages in order, and lens i32 [B], its cached
+ * tokens. An entry that is no page (outside 0 .. pages - 1) holds nothing: tokens there are not
+ * written, read as zeros, are not attended to and not moved. */
+typedef struct bq_kv4_cache {
+  uint8_t *k, *k_scales, *v, *v_scales;
+  int64_t pages, heads, page, dim;
+} bq_kv4_cache;
+
+/* New tokens into the cache: new_k, new_v [n, heads, dim], sequence b's the rows cu[b] .. cu[b + 1]
+ * - 1, the last ones of its lens[b] tokens (lens counts them). Each 32 channels take the least
+ * exponent (byte >= 1) that brings the largest magnitude to 6 or below, the codes round to nearest,
+ * ties to even; a block with a value that is not finite gets byte 255. */
+int bq_kv4_append(const bq_kv4_cache* cache, const void* new_k, const void* new_v, int type, int64_t n,
+                  int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, const int32_t* table, int64_t B,
+                  int64_t width, const int32_t* lens, const int32_t* cu, bq_stream_t stream);
+
+/* The values held: k, v f32 [B, heads, most, dim], zeros from lens[b] on. */
+int bq_kv4_read(const bq_kv4_cache* cache, const int32_t* table, int64_t B, int64_t width, const int32_t* lens,
+                int64_t most, float* k, float* v, bq_stream_t stream);
+
+/* Workspace bytes of bq_kv4_attend (rows = tokens * q_heads / heads). */
+size_t bq_kv4_attend_ws_bytes(int64_t B, int64_t heads, int64_t rows, int64_t dim, int64_t max_len);
+
+/* Attention of each sequence's newest `tokens` tokens over the cache: q [B, tokens, q_heads, dim];
+ * token t sees the first min(lens[b], max_len) - tokens + 1 + t cached tokens:
+ *   out [B, tokens, q_heads, dim] (contiguous, of q's type) = softmax(scale q k^T) v
+ * over the values that the cache stands for, zeros where nothing is seen; what a token does not see
+ * never reaches its output. f32 accumulation, f32 products to f32's accuracy. weights (nullable) f32,
+ * at w_seq and w_head elements from sequence to sequence and head to head, has each cached token's
+ * softmax weights added, summed over the queries of its key-value head (no atomics: the same bits in
+ * every run). ws: bq_kv4_attend_ws_bytes bytes, 16-byte aligned, need not be cleared. */
+int bq_kv4_attend(const bq_kv4_cache* cache, const void* q, int type, int64_t tokens, int64_t q_heads, int64_t q_seq,
+                  int64_t q_token, int64_t q_head, const int32_t* table, int64_t B, int64_t width, const int32_t* lens,
+                  int64_t max_len, float scale, void* out, float* weights, int64_t w_seq, int64_t w_head, void* ws,
+                  size_t ws_bytes, bq_stream_t stream);
+
+/* Eviction: of each (sequence, head) with more than `keep` cached tokens the `recent` last ones stay
+ * and, of the others, the keep - recent of largest weight in sums f32 (`most` a row, rows at sums_b
+ * and sums_h elements; ties to the earlier token, NaN above all); the tokens that stay move in
+ * order to the pages of new_table i32 [B, new_width], which are none of those in use.
+ *   kept i32 [B, heads, keep]: their former places (-1 past the last); weights f32 [B, heads, keep]:
+ *   their sums (0 past the last); left i32 [B]: min(lens[b], keep). lens beyond `most` are cut. */
+int bq_kv4_evict(const bq_kv4_cache* cache, const float* sums, int64_t sums_b, int64_t sums_h, int64_t most,
+                 const int32_t* table, int64_t B, int64_t width, const int32_t* lens, const int32_t* new_table,
+                 int64_t new_width, int64_t keep, int64_t recent, int32_t* kept, float* weights, int32_t* left,
+                 bq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
