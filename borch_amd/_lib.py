@@ -112,7 +112,9 @@ SIGNATURES = {
     "bq_se_gate_absmax_parts": (_c_i64, [_c_i64, _c_i64]),
     "bq_se_gate_nhwc": (_c_int, [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p,
                                  _c_size, _c_p]),
-    "bq_prompt_attention": (_c_int, [_c_p, _c_p, _c_p, _c_int, *[_c_i64] * 10, _c_p, _c_i64, _c_int, _c_f, _c_p, _c_p]),
+    "bq_prompt_attention": (_c_int, [_c_p, _c_p, _c_p, _c_int, *[_c_i64] * 10, _c_p, _c_i64, _c_int, _c_f, _c_p, _c_p,
+                                   _c_size, _c_p]),
+    "bq_prompt_attention_ws_bytes": (_c_size, [_c_int, _c_i64, _c_i64, _c_i64]),
     "bq_kv4_append": (_c_int, [_c_p, _c_p, _c_p, _c_int, *[_c_i64] * 5, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p]),
     "bq_kv4_read": (_c_int, [_c_p, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_p]),
     "bq_kv4_attend_ws_bytes": (_c_size, [_c_i64] * 5),

@@ -77,9 +77,12 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
     out = torch.empty((n, hq, dim), dtype=q.dtype, device=q.device)
     if n == 0 or hq == 0:
         return out
-    q, k, v = rows(q), rows(k), rows(v)
+    q, k, v = (x if max(strides(x)) <= 1 << 23 else x.contiguous() for x in (rows(q), rows(k), rows(v)))
+    need = lib().bq_prompt_attention_ws_bytes(code, n, h, dim)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     with torch.cuda.device(q.device):
         check(lib().bq_prompt_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), code, n, hq, h, dim, *strides(q),
                                         *strides(k), *strides(v), cu.data_ptr(), cu.shape[0] - 1, int(causal),
-                                        1.0 / math.sqrt(dim) if scale is None else scale, out.data_ptr(), _stream(q)))
+                                        1.0 / math.sqrt(dim) if scale is None else scale, out.data_ptr(),
+                                        None if ws is None else ws.data_ptr(), need, _stream(q)))
     return out

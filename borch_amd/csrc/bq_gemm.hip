@@ -27,6 +27,7 @@
 #include <utility>
 
 #include "bq_common.h"
+#include "bq_dma.h"
 
 namespace bq {
 
@@ -144,29 +145,6 @@ template <int MASK, int COUNT, int NMMA, int SPREAD>
 __device__ __forceinline__ void interleave_front() {
   interleave_impl<MASK, COUNT, SPREAD>(std::make_integer_sequence<int, SPREAD>{});
   sched_group<0x008, NMMA - SPREAD>();
-}
-
-// One 16-byte-per-lane load straight into LDS (no VGPR staging): lane l's 16 bytes land at
-// LDS byte address m0v + 16 * l. Issued from inline assembly so that the compiler, which
-// cannot tell these writes from the fragment reads of the other buffer, does not add a
-// full vmcnt wait before every LDS read; the caller waits (vmcnt) before the barrier that
-// publishes a stage. M0 is written here and used by nothing else in these kernels; the
-// s_nop covers the M0-write -> LDS-DMA hazard.
-__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t m0v) {
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(r), "s"(m0v)
-               : "m0");
-#pragma clang diagnostic pop
-}
-__device__ __forceinline__ void wait_dma_all() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-// A barrier orders LDS stores, not loads still in flight: before a barrier after which a
-// buffer this wave read is refilled, its reads must have returned.
-__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void wait_dma() {
-  static_assert(N >= 0 && N <= 63, "vmcnt range");
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
 // Main loop with direct-to-LDS loads into a ring of NBUF stage buffers. A stage's LDS image

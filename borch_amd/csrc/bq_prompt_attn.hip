@@ -14,12 +14,13 @@
 // The 16-bit types multiply as they are and p is rounded to their type (half a step of 2^-8 or
 // 2^-11 on each term, where the output takes one as large). f32 operands are the exact sums of
 // three bf16 pieces (bq_bf16x3.h), of whose nine products the six of weight 2^-18 and above are
-// added. What the pieces cannot hold is taken apart: a score that is not finite is computed again
-// in plain f32, a value that is not finite leaves the products (nonfinite_values).
+// added. Outputs that do not come out finite are taken again in plain f32 (plain_row), so that
+// infinities and NaN act as f32 has them, and only on the queries that see them.
 #include <math.h>
 
 #include "bq_bf16x3.h"
 #include "bq_common.h"
+#include "bq_dma.h"
 
 namespace bq {
 
@@ -37,21 +38,55 @@ struct Prompt {
   const int* cu;
   int n, B, heads, group, tiles, causal;
   float scale2;  // scale * log2(e)
+  void* ws;      // f32: the planes of k, then of v
 };
 
+// A workgroup's head and queries.
+struct Place {
+  int head, start, len, q0;  // the sequence's first row and length, the first query in it
+  bool keys;                 // whether it is a sequence (else rows of none, which see nothing)
+};
+
+// Places from the last down (the causal ones with most keys first), the heads of one place side by
+// side; with a multiple of 8 heads each XCD (ids modulo 8) keeps to its own. A place is a tile of
+// what lies before cu[0], of each sequence in turn, or of what lies past the last. False: the grid
+// has more workgroups than there are tiles.
+__device__ __forceinline__ bool place_of(const Prompt& a, Place* out) {
+  const int heads = a.heads * a.group, lane = threadIdx.x & 63;
+  int head = blockIdx.x % heads;
+  if (heads % 8 == 0) head = (head % 8) * (heads / 8) + head / 8;
+  int place = a.tiles - 1 - blockIdx.x / heads;
+  for (int base = 0; base < a.B + 2; base += 64) {
+    const int i = base + lane;
+    int s = 0, e = 0;
+    if (i <= a.B + 1) {
+      s = i == 0 ? 0 : min(max(a.cu[i - 1], 0), a.n);
+      e = i == a.B + 1 ? a.n : min(max(a.cu[i], 0), a.n);
+    }
+    const int mine = max(0, e - s + PROMPT_ROWS - 1) / PROMPT_ROWS;
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int y = __shfl_up(upto, d);
+      if (lane >= d) upto += y;
+    }
+    const uint64_t hit = __ballot(upto > place);
+    if (hit) {
+      const int at = __builtin_ctzll(hit);
+      // one value for the wave, in scalar registers
+      const int start = __builtin_amdgcn_readlane(s, at), end = __builtin_amdgcn_readlane(e, at);
+      place -= __builtin_amdgcn_readlane(upto - mine, at);
+      *out = Place{head, start, end - start, place * PROMPT_ROWS, base + at > 0 && base + at <= a.B};
+      return true;
+    }
+    place -= __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
 template <typename T>
-struct Kind;
-template <>
-struct Kind<float> {
-  static constexpr int P = 3, KT = 32;  // pieces, keys a tile
-};
-template <>
-struct Kind<__bf16> {
-  static constexpr int P = 1, KT = 64;
-};
-template <>
-struct Kind<_Float16> {
-  static constexpr int P = 1, KT = 64;
+struct Kind {
+  static constexpr int P = sizeof(T) == 4 ? 3 : 1;  // pieces
 };
 
 template <int P>
@@ -119,24 +154,6 @@ struct Piece {
       return Frag<1>{{__builtin_bit_cast(v8s, x[0])}};
     }
   }
-  // Whether an element's exponent is all ones.
-  __device__ __forceinline__ bool odd() const {
-    bool bad = false;
-#pragma unroll
-    for (const uint4& v : x) {
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 4) {
-          bad |= (w[i] & 0x7f800000u) == 0x7f800000u;
-        } else {
-          constexpr uint32_t E = __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
-          bad |= (w[i] & E) == E || (w[i] & (E << 16)) == (E << 16);
-        }
-      }
-    }
-    return bad;
-  }
 };
 
 // Where a 16-byte piece of a row lies in a staged tile. k's rows are read 16 at a time at one
@@ -155,92 +172,200 @@ __device__ __forceinline__ v4s read_tr(const unsigned char* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(const __attribute__((address_space(3))) unsigned char*)p);
 }
 
-template <typename T, int DIM>
-struct PromptTile {
-  static constexpr int P = Kind<T>::P, KT = Kind<T>::KT, PLANE = KT * DIM * 2, STEPS = DIM / 16, VT = DIM / 32;
-  static constexpr int PER = KT * DIM / 8 / (PROMPT_WAVES * 64);  // pieces a thread
-  unsigned char k[P * PLANE], v[P * PLANE];
-  int odd[2];  // whether v's tile holds a value that is not finite, tiles in turn
-
-  // v's operand of 32 channels from 32 d, tokens of step s: lane l is channel 32 d + l % 32
-  __device__ __forceinline__ Frag<P> v_frag(int d, int s) const {
-    const int lane = threadIdx.x & 63;
-    const int row = 16 * s + 4 * (lane >> 5) + ((lane & 15) >> 2);
-    const int piece = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), half = (lane & 1) * 8;
-    Frag<P> f;
+__device__ __forceinline__ v16f zeros16() {
+  v16f z;
 #pragma unroll
-    for (int e = 0; e < P; ++e) {
-      const v4s a = read_tr(v + e * PLANE + v_at<DIM>(row, piece) + half);
-      const v4s b = read_tr(v + e * PLANE + v_at<DIM>(row + 8, piece) + half);
-      f.p[e] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
-    return f;
-  }
-};
-
-// The scores of a lane that did not come out finite, in plain f32: infinities and NaN among q and k
-// as f32 gives them.
-__device__ __attribute__((noinline)) void plain_scores(const float* q, const float* k, int64_t kt, int dim, int tokens,
-                                                       int half, float* s) {
-  for (int i = 0; i < 16; ++i) {
-    const int t = 8 * (i / 4) + 4 * half + i % 4;
-    if (t >= tokens || __builtin_isfinite(s[i])) continue;
-    float x = 0.f;
-    for (int d = 0; d < dim; ++d) x = __fmaf_rn(q[d], k[t * kt + d], x);
-    s[i] = x;
-  }
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
 }
 
+// v's operand of 32 channels from 32 d, tokens of step s: lane l is channel 32 d + l % 32
+template <int DIM, int P>
+__device__ __forceinline__ Frag<P> v_frag(const unsigned char* v, int plane, int d, int s) {
+  const int lane = threadIdx.x & 63;
+  const int row = 16 * s + 4 * (lane >> 5) + ((lane & 15) >> 2);
+  const int piece = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), half = (lane & 1) * 8;
+  Frag<P> f;
+#pragma unroll
+  for (int e = 0; e < P; ++e) {
+    const v4s a = read_tr(v + e * plane + v_at<DIM>(row, piece) + half);
+    const v4s b = read_tr(v + e * plane + v_at<DIM>(row + 8, piece) + half);
+    f.p[e] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  return f;
+}
+
+// One query's attention by one wave in plain f32, for outputs that are not finite: what infinities
+// among q, k and v come to is f32's matter, not that of pieces of either sign or of weights rounded
+// to 0. Lane l scores keys l, l + 64, ..., and sums channels l (and l + 64).
+template <typename T, int DIM>
+__device__ __attribute__((noinline)) void plain_row(const T* q, const T* k, int64_t kt, const T* v, int64_t vt, T* to,
+                                                    int sees, float scale2) {
+  constexpr int C = DIM / 64;
+  const int lane = threadIdx.x & 63;
+  float m = -INFINITY, l = 0.f, o[C] = {};
+  for (int t0 = 0; t0 < sees; t0 += 64) {
+    const int t = t0 + lane;
+    float s = -INFINITY;
+    if (t < sees) {
+      s = 0.f;
+      for (int d = 0; d < DIM; ++d) s = __fmaf_rn((float)q[d], (float)k[t * kt + d], s);
+    }
+    float top = s;
+    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    top = fmaxf(top, m);
+    const float base = top == -INFINITY ? 0.f : top;
+    const float f = __builtin_amdgcn_exp2f(__fmul_rn(__fsub_rn(m, base), scale2));
+    const float p = t < sees ? __builtin_amdgcn_exp2f(__fmul_rn(__fsub_rn(s, base), scale2)) : 0.f;
+    m = top;
+    l = __fadd_rn(__fmul_rn(l, f), wave_sum_fixed(p));
+    for (int c = 0; c < C; ++c) o[c] = __fmul_rn(o[c], f);
+    for (int j = 0; j < min(64, sees - t0); ++j) {
+      const float pj = __shfl(p, j);
+      for (int c = 0; c < C; ++c) o[c] = __fmaf_rn(pj, (float)v[(t0 + j) * vt + lane + 64 * c], o[c]);
+    }
+  }
+  for (int c = 0; c < C; ++c) to[lane + 64 * c] = (T)__fdiv_rn(o[c], l == 0.f ? 1.f : l);
+}
+
+// The rows' outputs: lane (n, hh) holds channels 32 d + 8 i + 4 hh .. of its query; l is the row's
+// sum. Rows with their bit in `again` by plain_row.
+template <typename T, int DIM>
+__device__ __forceinline__ void store_rows(const Prompt& a, const Place& at, int row, float l, const v16f (&o)[DIM / 32],
+                                           uint32_t again) {
+  const float r = __fdiv_rn(1.f, l == 0.f ? 1.f : l);
+  T* to = (T*)a.out + ((int64_t)(at.start + row) * (a.heads * a.group) + at.head) * DIM + 4 * ((threadIdx.x >> 5) & 1);
+  if (row < at.len)
+#pragma unroll
+    for (int d = 0; d < DIM / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float y[4] = {__fmul_rn(o[d][4 * i], r), __fmul_rn(o[d][4 * i + 1], r), __fmul_rn(o[d][4 * i + 2], r),
+                          __fmul_rn(o[d][4 * i + 3], r)};
+      T* p = to + 32 * d + 8 * i;
+      if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(p) = make_float4(y[0], y[1], y[2], y[3]);
+      } else if constexpr (__is_same(T, __bf16)) {
+        *reinterpret_cast<uint2*>(p) = make_uint2(bf2(y[0], y[1]), bf2(y[2], y[3]));
+      } else {
+        typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<v4h*>(p) = v4h{(_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3]};
+      }
+    }
+  const int row0 = __builtin_amdgcn_readfirstlane(row), h = at.head / a.group;
+#pragma unroll 1
+  for (int i = 0; i < 32; ++i)
+    if ((again >> i) & 1) {
+      const int64_t q = at.start + row0 + i;
+      plain_row<T, DIM>((const T*)a.q + q * a.qt + at.head * a.qh, (const T*)a.k + (int64_t)at.start * a.kt + h * a.kh, a.kt,
+                        (const T*)a.v + (int64_t)at.start * a.vt + h * a.vh, a.vt,
+                        (T*)a.out + (q * (a.heads * a.group) + at.head) * DIM,
+                        a.causal ? min(at.len, row0 + i + 1) : at.len, a.scale2);
+    }
+}
+
+// Takes the values that are not finite out of a staged tile of v, which some query sees in part (they
+// would meet that query's weights of 0), and returns whether the lane's query sees one: it sees
+// the tile's first `sees` tokens. By the whole workgroup; found [KT].
+template <typename T, int DIM, int KT>
+__device__ __attribute__((noinline)) bool clear_values(unsigned char* v, int* found, int sees) {
+  constexpr int P = Kind<T>::P, PLANE = KT * DIM * 2;
+  constexpr uint32_t E = __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
+  if (threadIdx.x < KT) found[threadIdx.x] = 0;
+  wait_lds();
+  barrier();
+  for (int x = threadIdx.x; x < KT * DIM / 2; x += PROMPT_WAVES * 64) {  // two values
+    const int r = x / (DIM / 2), at = v_at<DIM>(r, x % (DIM / 2) / 4) + x % 4 * 4;
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(v + at);
+    const uint32_t keep = ((w & E) == E ? 0u : 0xffffu) | ((w & (E << 16)) == (E << 16) ? 0u : 0xffff0000u);
+    if (keep != ~0u) {
+      found[r] = 1;
+      for (int p = 0; p < P; ++p) *reinterpret_cast<uint32_t*>(v + p * PLANE + at) &= keep;
+    }
+  }
+  wait_lds();
+  barrier();
+  bool seen = false;
+  for (int r = 0; r < min(KT, sees); ++r) seen |= found[r] != 0;
+  wait_lds();
+  barrier();  // before `found` is cleared again
+  return seen;
+}
+
+// k's and v's planes of bf16 pieces, [piece][head][row][dim]: once a call, where
+// every workgroup would split its tiles again.
+template <int DIM>
+__global__ __launch_bounds__(256) void prompt_split_kernel(Prompt a) {
+  constexpr int LANES = DIM / 8;
+  const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int piece = x % LANES;
+  const uint32_t rest = (uint32_t)(x / LANES), i = rest / (uint32_t)(2 * a.heads);
+  const int w = rest - i * (2 * a.heads), h = w % a.heads;
+  if (i >= (uint32_t)a.n) return;
+  const bool is_v = w >= a.heads;
+  const float* p = is_v ? (const float*)a.v + i * a.vt + h * a.vh : (const float*)a.k + i * a.kt + h * a.kh;
+  const float4 y0 = *reinterpret_cast<const float4*>(p + 8 * piece), y1 = *reinterpret_cast<const float4*>(p + 8 * piece + 4);
+  const Split8 f = split8(y0, y1);
+  const size_t plane = (size_t)a.heads * a.n * DIM;
+  short* to = (short*)a.ws + (is_v ? 3 * plane : 0) + ((size_t)h * a.n + i) * DIM + 8 * piece;
+  *reinterpret_cast<v8bf*>(to) = f.p1;
+  *reinterpret_cast<v8bf*>(to + plane) = f.p2;
+  *reinterpret_cast<v8bf*>(to + 2 * plane) = f.p3;
+}
+
+// Tiles of KT keys and values come straight into LDS, rows past the sequence's end as zeros. The
+// 16-bit types hold two tiles, the next one's loads under this one's products, one barrier a tile.
+// f32 holds one (48 KB of planes at dim 128, so that two workgroups share a CU): the next keys load
+// under this tile's second product, the next values under the next tile's first, two barriers.
 template <typename T, int DIM>
 __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) {
-  using Tile = PromptTile<T, DIM>;
-  constexpr int P = Tile::P, KT = Tile::KT, STEPS = Tile::STEPS, VT = Tile::VT, PER = Tile::PER, SUB = KT / 32;
-  __shared__ __attribute__((aligned(16))) Tile tile;
-  const int heads = a.heads * a.group;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 31, hh = lane >> 5;
-
-  // this workgroup's head and place: places from the last down (the causal ones with most keys
-  // first); with a multiple of 8 heads each XCD (ids modulo 8) keeps to its own
-  int head = blockIdx.x % heads;
-  if (heads % 8 == 0) head = (head % 8) * (heads / 8) + head / 8;
-  int place = a.tiles - 1 - blockIdx.x / heads;
-  // the sequence: tiles of what lies before cu[0], of each sequence, of what lies past the last
-  // (those rows see nothing)
-  int start = 0, end = 0, kv = 0;
-  for (int base = 0; base < a.B + 2; base += 64) {
-    const int i = base + lane;
-    int s = 0, e = 0;
-    if (i <= a.B + 1) {
-      s = i == 0 ? 0 : min(max(a.cu[i - 1], 0), a.n);
-      e = i == a.B + 1 ? a.n : min(max(a.cu[i], 0), a.n);
-    }
-    const int mine = max(0, e - s + PROMPT_ROWS - 1) / PROMPT_ROWS;
-    int upto = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int y = __shfl_up(upto, d);
-      if (lane >= d) upto += y;
-    }
-    const uint64_t hit = __ballot(upto > place);
-    if (hit) {
-      const int at = __builtin_ctzll(hit);
-      place -= __shfl(upto - mine, at);
-      start = __shfl(s, at);
-      end = __shfl(e, at);
-      kv = base + at > 0 && base + at <= a.B;
-      break;
-    }
-    place -= __shfl(upto, 63);
-    if (base + 64 >= a.B + 2) return;  // fewer tiles than the grid has
-  }
-  const int len = end - start, q0 = place * PROMPT_ROWS;
+  constexpr int P = Kind<T>::P, KT = P == 3 ? 32 : 64, SUB = KT / 32, BUFS = P == 3 ? 1 : 2;
+  constexpr int STEPS = DIM / 16, VT = DIM / 32, PLANE = KT * DIM * 2;
+  constexpr int ROWS = 1024 / (DIM * 2);         // of a wave's load
+  constexpr int PER = KT / ROWS / PROMPT_WAVES;  // loads a wave and plane
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[BUFS * 2 * P * PLANE];
+  __shared__ int found[KT];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hh = lane >> 5;
+  Place at;
+  if (!place_of(a, &at)) return;
+  const int len = at.len, q0 = at.q0;
   const int qw = q0 + wave * 32, row = qw + n;  // the wave's first query, this lane's
-  const int h = head / a.group;
-  const T* q = (const T*)a.q + (int64_t)(start + row) * a.qt + head * a.qh;
-  const T* k = (const T*)a.k + (int64_t)start * a.kt + h * a.kh;
-  const T* v = (const T*)a.v + (int64_t)start * a.vt + h * a.vh;
+  const int h = at.head / a.group;
+  const int keys = !at.keys ? 0 : a.causal ? min(len, q0 + PROMPT_ROWS) : len;  // that the workgroup sees
+  const int wkeys = a.causal ? min(keys, qw + 32) : keys;                      // that the wave does
+  const int sees = a.causal ? min(len, row + 1) : len;                         // that the lane does
 
+  // k and v as loaded: the callers' rows, or the planes
+  const size_t plane = (size_t)a.heads * a.n * DIM * 2;
+  const int ktb = P == 3 ? DIM * 2 : (int)a.kt * 2, vtb = P == 3 ? DIM * 2 : (int)a.vt * 2;
+  const char *k, *v;
+  if constexpr (P == 3) {
+    k = (const char*)a.ws + ((size_t)h * a.n + at.start) * (DIM * 2);
+    v = k + 3 * plane;
+  } else {
+    k = (const char*)((const T*)a.k + (int64_t)at.start * a.kt + h * a.kh);
+    v = (const char*)((const T*)a.v + (int64_t)at.start * a.vt + h * a.vh);
+  }
+  // of this wave's loads: the lane's place in LDS is its own, the piece the one that lies there
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
+  uint32_t ko[PER], vo[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int r = (wave * PER + e) * ROWS + lane / (DIM / 8), slot = lane % (DIM / 8);
+    ko[e] = r * ktb + (k_at<DIM>(r, slot) & (DIM * 2 - 1));
+    vo[e] = r * vtb + (v_at<DIM>(r, slot) & (DIM * 2 - 1));
+  }
+  auto fetch = [&](const char* from, int stride, const uint32_t (&off)[PER], int t0, uint32_t to) {
+    const uint32_t bytes = (uint32_t)min((int64_t)(len - 1 - t0) * stride + DIM * 2, (int64_t)0x7fffffff);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const __amdgpu_buffer_rsrc_t r = make_rsrc(from + p * plane + (int64_t)t0 * stride, bytes);
+#pragma unroll
+      for (int e = 0; e < PER; ++e) dma16(r, off[e], to + p * PLANE + (wave * PER + e) * 1024);
+    }
+  };
   Frag<P> qf[STEPS];
+  const T* q = (const T*)a.q + (int64_t)(at.start + row) * a.qt + at.head * a.qh;
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) {
     Piece<T> x;
@@ -248,205 +373,130 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
     if (row < len) x.load(q + 16 * s + 8 * hh);
     qf[s] = x.frag();
   }
-  const int keys = !kv ? 0 : a.causal ? min(len, q0 + PROMPT_ROWS) : len;  // that the workgroup sees
-  const int wkeys = a.causal ? min(keys, qw + 32) : keys;                  // that the wave does
-  const int sees = a.causal ? min(len, row + 1) : len;                     // that the lane does
-  float m = -INFINITY, l = 0.f;
+  float m, l;
   v16f o[VT];
+  // Once; and where an output is not finite once more, with the values that are not out of the tiles
+  // that some query sees in part. Rows that see one, or are not finite then, go to plain_row: what a
+  // query does not see changes no bit of its output.
+  bool odd = false;
+  for (int again = 0;; again = 1) {
+    m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int d = 0; d < VT; ++d)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+    for (int d = 0; d < VT; ++d) o[d] = zeros16();
+    if (keys > 0) {
+      fetch(k, ktb, ko, 0, lds0);
+      if constexpr (BUFS == 2) fetch(v, vtb, vo, 0, lds0 + P * PLANE);
+    }
 
-  Piece<T> kr[PER], vr[PER];
-  auto fetch = [&](int t0) {
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const int x = threadIdx.x + e * PROMPT_WAVES * 64, r = x / (DIM / 8), c = x % (DIM / 8);
-      kr[e].clear();
-      vr[e].clear();
-      if (t0 + r < len) {
-        kr[e].load(k + (int64_t)(t0 + r) * a.kt + 8 * c);
-        vr[e].load(v + (int64_t)(t0 + r) * a.vt + 8 * c);
+    for (int t0 = 0, buf = 0; t0 < keys; t0 += KT, buf ^= BUFS - 1) {
+      wait_dma_all();
+      wait_lds();
+      barrier();  // the keys are there (both buffers: the values too), what is loaded over is read
+      const unsigned char *tk = lds + buf * 2 * P * PLANE, *tv = tk + P * PLANE;
+      auto middle = [&]() {  // f32: the values are there, the keys read
+        wait_dma_all();
+        wait_lds();
+        barrier();
+        if (t0 + KT < keys) fetch(k, ktb, ko, t0 + KT, lds0);
+      };
+      if constexpr (BUFS == 1) {
+        fetch(v, vtb, vo, t0, lds0 + P * PLANE);
+      } else if (t0 + KT < keys) {
+        const uint32_t to = lds0 + (buf ^ 1) * 2 * P * PLANE;
+        fetch(k, ktb, ko, t0 + KT, to);
+        fetch(v, vtb, vo, t0 + KT, to + P * PLANE);
       }
-    }
-  };
-  if (threadIdx.x < 2) tile.odd[threadIdx.x] = 0;
-  if (keys > 0) fetch(0);
-  for (int t0 = 0, turn = 0; t0 < keys; t0 += KT, turn ^= 1) {
-    __syncthreads();  // the last tile is read, its flag too
-    bool odd = false;
-    // f32 asks of every tile, the others of those that a query sees in part
-    const bool part = t0 + KT > len || (a.causal && t0 + KT > q0 + 1);
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const int x = threadIdx.x + e * PROMPT_WAVES * 64, r = x / (DIM / 8), c = x % (DIM / 8);
-      const Frag<P> kf = kr[e].frag(), vf = vr[e].frag();
-#pragma unroll
-      for (int p = 0; p < P; ++p) {
-        *reinterpret_cast<v8s*>(tile.k + p * Tile::PLANE + k_at<DIM>(r, c)) = kf.p[p];
-        *reinterpret_cast<v8s*>(tile.v + p * Tile::PLANE + v_at<DIM>(r, c)) = vf.p[p];
+      const bool clears = again && (t0 + KT > len || (a.causal && t0 + KT > q0 + 1));
+      if (t0 >= wkeys) {
+        if constexpr (BUFS == 1) middle();
+        if (clears) clear_values<T, DIM, KT>(const_cast<unsigned char*>(tv), found, 0);
+        continue;
       }
-      if (P == 3 || part) odd |= vr[e].odd();
-    }
-    if (threadIdx.x == 0) tile.odd[turn ^ 1] = 0;
-    if (odd) tile.odd[turn] = 1;
-    __syncthreads();
-    if (t0 + KT < keys) fetch(t0 + KT);
-    if (t0 >= wkeys) continue;
 
-    // S^T = k q^T
-    v16f s[SUB];
-#pragma unroll
-    for (int u = 0; u < SUB; ++u) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
-#pragma unroll
-      for (int e = 0; e < STEPS; ++e) {
-        Frag<P> kf;
-#pragma unroll
-        for (int p = 0; p < P; ++p)
-          kf.p[p] = *reinterpret_cast<const v8s*>(tile.k + p * Tile::PLANE + k_at<DIM>(32 * u + n, 2 * e + hh));
-        s[u] = product<T>(kf, qf[e], s[u]);
-      }
-    }
-    if constexpr (P == 3) {
+      // S^T = k q^T
+      v16f s[SUB];
 #pragma unroll
       for (int u = 0; u < SUB; ++u) {
-        float zero = 0.f;
+        s[u] = zeros16();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) zero = __fmaf_rn(s[u][i], 0.f, zero);
-        if (zero != 0.f && row < len) {
-          float x[16];
+        for (int e = 0; e < STEPS; ++e) {
+          Frag<P> kf;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] = s[u][i];
-          plain_scores((const float*)q, (const float*)k + (int64_t)(t0 + 32 * u) * a.kt, a.kt, DIM, len - t0 - 32 * u, hh, x);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[u][i] = x[i];
+          for (int p = 0; p < P; ++p)
+            kf.p[p] = *reinterpret_cast<const v8s*>(tk + p * PLANE + k_at<DIM>(32 * u + n, 2 * e + hh));
+          s[u] = product<T>(kf, qf[e], s[u]);
         }
       }
-    }
 
-    // softmax, one step
-    const bool edge = t0 + KT > len || (a.causal && t0 + KT > qw + 1);
-    if (edge)
+      // softmax, one step. The maximum that is subtracted lags by up to 2^8 (the weights' own size
+      // cancels in the quotient), so that most steps rescale nothing.
+      const bool edge = t0 + KT > len || (a.causal && t0 + KT > qw + 1);
+      if (edge)
 #pragma unroll
-      for (int u = 0; u < SUB; ++u)
+        for (int i = 0; i < 16 * SUB; ++i)
+          if (t0 + 32 * (i / 16) + 8 * (i % 16 / 4) + 4 * hh + i % 4 >= sees) s[i / 16][i % 16] = -INFINITY;
+      float top = s[0][0];
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (t0 + 32 * u + 8 * (i / 4) + 4 * hh + i % 4 >= sees) s[u][i] = -INFINITY;
-    float top = m;
+      for (int i = 1; i < 16 * SUB; ++i) top = fmaxf(top, s[i / 16][i % 16]);
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const bool grew = __fmul_rn(__fsub_rn(top, m), a.scale2) > 8.f;
+      if (__any(grew)) {
+        const float f = grew ? __builtin_amdgcn_exp2f(__fmul_rn(__fsub_rn(m, top), a.scale2)) : 1.f;
+        m = grew ? top : m;
+        l = __fmul_rn(l, f);
 #pragma unroll
-    for (int u = 0; u < SUB; ++u)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
-    top = fmaxf(top, __shfl_xor(top, 32));
-    const float base = top == -INFINITY ? 0.f : top;
-    if (__any(top > m)) {
-      const float f = __builtin_amdgcn_exp2f(__fmul_rn(__fsub_rn(m, base), a.scale2));
-      l = __fmul_rn(l, f);
-#pragma unroll
-      for (int d = 0; d < VT; ++d) o[d] *= f;
-      m = top;
-    }
-#pragma unroll
-    for (int u = 0; u < SUB; ++u)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[u][i] = __builtin_amdgcn_exp2f(__fmul_rn(__fsub_rn(s[u][i], base), a.scale2));
-        l = __fadd_rn(l, s[u][i]);
+        for (int d = 0; d < VT; ++d) o[d] *= f;
       }
+      const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int i = 0; i < 16 * SUB; ++i) {
+        const float p = __builtin_amdgcn_exp2f(__fmul_rn(__fsub_rn(s[i / 16][i % 16], base), a.scale2));
+        s[i / 16][i % 16] = p;
+        l = __fadd_rn(l, p);
+      }
+      if constexpr (BUFS == 1) middle();
 
-    // O^T += v^T p^T
-    const bool taint = tile.odd[turn] != 0;
+      if (clears) odd |= clear_values<T, DIM, KT>(const_cast<unsigned char*>(tv), found, sees - t0);
+
+      // O^T += v^T p^T
 #pragma unroll
-    for (int u = 0; u < SUB; ++u)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < 2 * SUB; ++e) {
         float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = s[u][8 * e + i];
+        for (int i = 0; i < 8; ++i) x[i] = s[e / 2][8 * (e % 2) + i];
         const Frag<P> pf = frag_of<T>(x);
-        if (!taint) {
 #pragma unroll
-          for (int d = 0; d < VT; ++d) o[d] = product<T>(tile.v_frag(d, 2 * u + e), pf, o[d]);
-        } else {
-          // Values that are not finite leave the product, where they would meet the zeros of
-          // tokens that a query does not see (and, in f32, pieces of either sign); what they come
-          // to is counted by products of ones: infinities that meet a weight, by sign, and NaN (a
-          // NaN that is seen, an infinity that meets a weight of 0).
-          constexpr short ONE = __is_same(T, _Float16) ? 0x3c00 : 0x3f80;
-          constexpr short E = __is_same(T, _Float16) ? 0x7c00 : 0x7f80;
-          v8s seen, met, none;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int t = t0 + 32 * u + 16 * e + 8 * (i / 4) + 4 * hh + i % 4;
-            seen[i] = t < sees ? ONE : 0;
-            met[i] = t < sees && x[i] > 0.f ? ONE : 0;
-            none[i] = t < sees && !(x[i] > 0.f) ? ONE : 0;
-          }
-#pragma unroll
-          for (int d = 0; d < VT; ++d) {
-            Frag<P> vf = tile.v_frag(d, 2 * u + e);
-            v8s plus, minus, nan, inf;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const short y = vf.p[0][i], mag = y & 0x7fff;
-              plus[i] = y == E ? ONE : 0;
-              minus[i] = mag == E && y != E ? ONE : 0;
-              inf[i] = mag == E ? ONE : 0;
-              nan[i] = mag > E ? ONE : 0;
-              if (mag >= E)
-#pragma unroll
-                for (int p = 0; p < P; ++p) vf.p[p][i] = 0;
-            }
-            o[d] = product<T>(vf, pf, o[d]);
-            v16f zero;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) zero[i] = 0.f;
-            const v16f cp = mma<T>(plus, met, zero), cm = mma<T>(minus, met, zero);
-            const v16f cn = mma<T>(inf, none, mma<T>(nan, seen, zero));
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              if (cp[i] > 0.f) o[d][i] = __fadd_rn(o[d][i], INFINITY);
-              if (cm[i] > 0.f) o[d][i] = __fadd_rn(o[d][i], -INFINITY);
-              if (cn[i] > 0.f) o[d][i] = NAN;
-            }
-          }
-        }
-      }
-  }
-
-  l = __fadd_rn(l, __shfl_xor(l, 32));
-  if (row >= len) return;
-  const float d1 = l == 0.f ? 1.f : l;
-  T* to = (T*)a.out + ((int64_t)(start + row) * heads + head) * DIM + 4 * hh;
-#pragma unroll
-  for (int d = 0; d < VT; ++d)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float y[4] = {__fdiv_rn(o[d][4 * i], d1), __fdiv_rn(o[d][4 * i + 1], d1), __fdiv_rn(o[d][4 * i + 2], d1),
-                          __fdiv_rn(o[d][4 * i + 3], d1)};
-      T* at = to + 32 * d + 8 * i;
-      if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float4*>(at) = make_float4(y[0], y[1], y[2], y[3]);
-      } else if constexpr (__is_same(T, __bf16)) {
-        *reinterpret_cast<uint2*>(at) = make_uint2(bf2(y[0], y[1]), bf2(y[2], y[3]));
-      } else {
-        typedef _Float16 v4h __attribute__((ext_vector_type(4)));
-        *reinterpret_cast<v4h*>(at) = v4h{(_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3]};
+        for (int d = 0; d < VT; ++d) o[d] = product<T>(v_frag<DIM, P>(tv, PLANE, d, e), pf, o[d]);
       }
     }
+    l = __fadd_rn(l, __shfl_xor(l, 32));
+    float zero = __fmul_rn(l, 0.f);  // NaN beside a value that is not finite
+#pragma unroll
+    for (int d = 0; d < VT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) zero = __fmaf_rn(o[d][i], 0.f, zero);
+    odd |= zero != 0.f;
+    odd = odd && row < len;
+    if (again || !__syncthreads_or(odd)) break;
+    odd = false;
+  }
+  const uint64_t who = __ballot(odd);
+  store_rows<T, DIM>(a, at, row, l, o, (uint32_t)(who | who >> 32));
 }
 
 }  // namespace bq
 
 using namespace bq;
 
+size_t bq_prompt_attention_ws_bytes(int type, int64_t n, int64_t heads, int64_t dim) {
+  if (type != 0 || n < 1 || heads < 1 || dim < 1) return 0;
+  return (size_t)12 * n * heads * dim;  // three planes of k and of v
+}
+
 int bq_prompt_attention(const void* q, const void* k, const void* v, int type, int64_t n, int64_t q_heads,
                         int64_t heads, int64_t dim, int64_t q_token, int64_t q_head, int64_t k_token, int64_t k_head,
                         int64_t v_token, int64_t v_head, const int32_t* cu, int64_t B, int causal, float scale,
-                        void* out, bq_stream_t stream) {
+                        void* out, void* ws, size_t ws_bytes, bq_stream_t stream) {
   const char* what = "bq_prompt_attention";
   if (type < 0 || type > 2) return set_error(BQ_ERR_ARG, "%s: type %d", what, type);
   if (dim != 64 && dim != 128)
@@ -463,14 +513,25 @@ int bq_prompt_attention(const void* q, const void* k, const void* v, int type, i
   if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) ||
       (q_token | q_head | k_token | k_head | v_token | v_head) * size % 16)
     return set_error(BQ_ERR_ARG, "%s: rows that are not 16-byte aligned", what);
+  if (k_token < 0 || v_token < 0 || k_token > 1 << 23 || v_token > 1 << 23)  // 64 rows within 32 bits
+    return set_error(BQ_ERR_UNSUPPORTED, "%s: rows of k or v too far apart", what);
   // whatever the lengths are: a full tile for every 128 rows and one begun for each sequence
   const int64_t tiles = n / PROMPT_ROWS + (B + 2 < n ? B + 2 : n);
   if (tiles * q_heads > 0x7fffffff) return set_error(BQ_ERR_ARG, "%s: size too large", what);
+  const size_t need = bq_prompt_attention_ws_bytes(type, n, heads, dim);
+  if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
+    return set_error(BQ_ERR_ARG, "%s: a workspace of %zu bytes, given %zu", what, need, ws ? ws_bytes : 0);
   const Prompt a = {q, k, v, out, q_token, q_head, k_token, k_head, v_token, v_head, cu, (int)n, (int)B, (int)heads,
-                    (int)(q_heads / heads), (int)tiles, causal ? 1 : 0, scale * 1.4426950408889634f};
+                    (int)(q_heads / heads), (int)tiles, causal ? 1 : 0, scale * 1.4426950408889634f, ws};
   const unsigned grid = (unsigned)(tiles * q_heads);
   hipStream_t st = (hipStream_t)stream;
   const bool wide = dim == 128;
+  if (need) {
+    const int64_t blocks = (n * 2 * heads * (dim / 8) + 255) / 256;
+    if (blocks > 0x7fffffff) return set_error(BQ_ERR_ARG, "%s: size too large", what);
+    if (wide) prompt_split_kernel<128><<<(unsigned)blocks, 256, 0, st>>>(a);
+    else prompt_split_kernel<64><<<(unsigned)blocks, 256, 0, st>>>(a);
+  }
 #define BQ_PROMPT(T)                                                                        \
   (wide ? prompt_kernel<T, 128><<<grid, PROMPT_WAVES * 64, 0, st>>>(a)                      \
         : prompt_kernel<T, 64><<<grid, PROMPT_WAVES * 64, 0, st>>>(a))

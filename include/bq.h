@@ -486,11 +486,14 @@ int bq_dequant_i8(const int8_t* q, int64_t N, int64_t K, const float* s, float* 
  * accumulation; f32 products as exact sums of bf16 pieces, to f32's accuracy (values below 2^-109
  * lose up to 2^-134); p rounded to the 16-bit types. What a query does not see never reaches its
  * output, infinities and NaN included. dim 64 or 128. Beside the path, as bq_attention_f32
- * (scaled_dot_product_attention, borch/_nn.py:2143-2170, with is_causal and enable_gqa). */
+ * (scaled_dot_product_attention, borch/_nn.py:2143-2170, with is_causal and enable_gqa). ws:
+ * bq_prompt_attention_ws_bytes bytes, 16-byte aligned (f32: the pieces of k and v; none for the 16-bit
+ * types, whose rows of k and v lie at most 2^23 elements apart). */
+size_t bq_prompt_attention_ws_bytes(int type, int64_t n, int64_t heads, int64_t dim);
 int bq_prompt_attention(const void* q, const void* k, const void* v, int type, int64_t n, int64_t q_heads,
                         int64_t heads, int64_t dim, int64_t q_token, int64_t q_head, int64_t k_token, int64_t k_head,
                         int64_t v_token, int64_t v_head, const int32_t* cu, int64_t B, int causal, float scale,
-                        void* out, bq_stream_t stream);
+                        void* out, void* ws, size_t ws_bytes, bq_stream_t stream);
 
 /* A key-value cache in pages of `page` tokens (a multiple of 32), for heads of dim 64 or 128. A
  * value is +-{0, 1/2, 1, 3/2, 2, 3, 4, 6} (4 bits: sign, two of exponent, one of mantissa) times the
