@@ -16,9 +16,12 @@
 // so are the rows of v^T (row m of product j is channel DIM / 16 m + j), both to load whole pieces.
 //
 // Each row keeps its running maximum, sum and output (one pass over the cache). A workgroup of four
-// waves takes a chunk of a sequence for one key-value head and 16 RT rows, and joins its waves in
-// LDS; where a sequence is cut into several chunks, they leave (maximum, sum, output) in the
-// workspace and a second kernel joins them. What the cached tokens received (the softmax weights
+// waves takes tokens of one sequence for one key-value head and 16 RT rows, and joins its waves in
+// LDS. Short caches: a workgroup a (sequence, head, rows). Long ones: all their units of 128 tokens
+// in one line, cut into equal shares for as many workgroups as the GPU holds at once (lengths are
+// the device's knowledge, and a share has one beginning and one end however unlike they are); a
+// (sequence, head, rows) that lies in several shares leaves (maximum, sum, output) of each in the
+// workspace, and a second kernel joins them. What the cached tokens received (the softmax weights
 // summed over the rows) needs the final maximum and sum of each row: a last kernel takes the scores
 // again, each token by one wave, so that sums are added without atomics, in one order.
 #include <math.h>
@@ -40,11 +43,12 @@ struct Attend {
   const int* lens;
   const void* q;
   int64_t qb, qt, qh;  // strides in elements: sequence, token, head
-  int tokens, group, rows, row_groups, max_len, chunk, splits;
+  int tokens, group, rows, row_groups, max_len, B;
+  int shares, least;  // workgroups of the line (0: one a sequence, head and rows), the least units a share
   FastDiv by_group;
   float scale2;  // scale * log2(e)
   void* out;     // [B][tokens][heads * group][DIM]
-  float *part, *stats;  // partial outputs [B heads][splits][rows][DIM + 2]; [B heads][rows][2]
+  float *part, *stats;  // shares' first and last parts [2 shares][16 RT][DIM + 2]; [B heads][rows][2]
   float* weights;
   int64_t wb, wh;
 };
@@ -230,208 +234,281 @@ __device__ __forceinline__ float weight_of(float s, float base, float c) {
 }
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
 
+constexpr int UNIT = 128;  // tokens: a block of 32 a wave
+
+__device__ __forceinline__ int len_of(const Attend& a, int b) { return max(0, min(a.lens[b], a.max_len)); }
+__device__ __forceinline__ int units_of(int len) { return max(1, (len + UNIT - 1) / UNIT); }  // an empty one writes zeros
+
+// The line of units, sequence after sequence, per_b (heads times row groups) runs of each: its
+// length, and for `upto` < B the place where that sequence's begin.
+__device__ __forceinline__ int line_of(const Attend& a, int per_b, int upto, int* begin) {
+  const int lane = threadIdx.x & 63;
+  int all = 0, before = 0;
+  for (int b = lane; b < a.B; b += 64) {
+    const int u = units_of(len_of(a, b)) * per_b;
+    all += u;
+    before += b < upto ? u : 0;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    all += __shfl_xor(all, d);
+    before += __shfl_xor(before, d);
+  }
+  *begin = __builtin_amdgcn_readfirstlane(before);
+  return __builtin_amdgcn_readfirstlane(all);
+}
+// The sequence in which place x of the line lies, and where its units begin.
+__device__ __forceinline__ int sequence_of(const Attend& a, int per_b, int x, int* begin) {
+  const int lane = threadIdx.x & 63;
+  int from = 0;
+  for (int b0 = 0;; b0 += 64) {
+    const int b = b0 + lane, mine = b < a.B ? units_of(len_of(a, b)) * per_b : 0;
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int y = __shfl_up(upto, d);
+      if (lane >= d) upto += y;
+    }
+    const uint64_t hit = __ballot(from + upto > x);
+    if (hit || b0 + 64 >= a.B) {
+      const int at = hit ? __builtin_ctzll(hit) : 0;
+      *begin = from + __builtin_amdgcn_readlane(upto - mine, at);
+      return min(b0 + at, a.B - 1);
+    }
+    from += __builtin_amdgcn_readlane(upto, 63);
+  }
+}
+__device__ __forceinline__ int share_of(const Attend& a, int line) { return max(a.least, (line + a.shares - 1) / a.shares); }
+
 template <typename T, int DIM, int RT>
-__global__ __launch_bounds__(256) void kv4_attend_kernel(Attend a) {
+__global__ __launch_bounds__(256, RT == 2 && DIM == 128 && !__is_same(T, __bf16) ? 1 : 2) void kv4_attend_kernel(Attend a) {
   constexpr int PP = P_PIECES<T>, NJ = DIM / 16, PITCH = DIM + 4;
   __shared__ __attribute__((aligned(16))) float so[4][16][PITCH];
   __shared__ float sm[4][16], sl[4][16];
-  const int split = blockIdx.x, h = blockIdx.y % a.c.heads, rg = blockIdx.y / a.c.heads, b = blockIdx.z;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-  const int len = max(0, min(a.lens[b], a.max_len));
-  const int t0 = split * a.chunk;
-  if (t0 >= len && split > 0) return;  // the first chunk of an empty sequence writes its zeros
-  const int t1 = min(len, t0 + a.chunk);
-  const int row0 = rg * 16 * RT;
-  const int sure = len - a.tokens + 1;  // tokens that every row sees
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+  const int per_b = a.c.heads * a.row_groups, bpp = a.c.page >> 5;
 
-  // this wave's blocks of 32 tokens: wave, wave + 4, ...; their pages, one a lane
-  const int blocks = (t1 - t0 + 31) >> 5;
-  const int first = (t0 >> 5) + wave;
-  const int bpp = a.c.page >> 5;
-  const int mine = blocks > wave ? (blocks - wave + 3) >> 2 : 0;
-  int pages = -1;
-  if (lane < mine) {
-    const int pi = fdiv(first + 4 * lane, a.c.by_blocks.mul, a.c.by_blocks.shift);
-    pages = kv4_page(a.c, b, pi);
+  // this workgroup's places x0 .. x1 of the line
+  int x0, x1, b, begin;
+  if (a.shares) {
+    const int line = line_of(a, per_b, 0, &begin), share = share_of(a, line);
+    x0 = blockIdx.x * share;
+    if (x0 >= line) return;
+    x1 = min(line, x0 + share);
+    b = sequence_of(a, per_b, x0, &begin);
+  } else {
+    b = blockIdx.x / per_b;
+    const int units = units_of(len_of(a, b));
+    begin = 0;
+    x0 = (blockIdx.x - b * per_b) * units;
+    x1 = x0 + units;
   }
+  for (int x = x0; x < x1;) {
+    const int len = len_of(a, b), units = units_of(len);
+    const int pair = (x - begin) / units, h = pair / a.row_groups, row0 = (pair - h * a.row_groups) * 16 * RT;
+    const int u0 = x - begin - pair * units, u1 = min(units, u0 + x1 - x);
+    const int sure = len - a.tokens + 1;  // tokens that every row sees
+    const int blocks = (len + 31) >> 5;
 
-  QFrag<T, DIM> q[RT];
-  int end[RT];  // what this lane's row sees
+    QFrag<T, DIM> q[RT];
+    int end[RT];  // what this lane's row sees
+    bool lost[RT];  // whether it sees a NaN value in its channels that left the products
+    float m[RT], l[RT];
+    v4f o[RT][NJ];
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    q[r].load(a, b, h, row0 + 16 * r);
-    const int t = fdiv(row0 + 16 * r + n, a.by_group.mul, a.by_group.shift);
-    end[r] = min(len, sure + t);
-  }
-  float m[RT], l[RT];
-  v4f o[RT][NJ];
+    for (int r = 0; r < RT; ++r) {
+      q[r].load(a, b, h, row0 + 16 * r);
+      const int t = fdiv(row0 + 16 * r + n, a.by_group.mul, a.by_group.shift);
+      end[r] = min(len, sure + t);
+      lost[r] = false;
+      m[r] = -INFINITY;
+      l[r] = 0.f;
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    m[r] = -INFINITY;
-    l[r] = 0.f;
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) o[r][j] = v4f{0.f, 0.f, 0.f, 0.f};
-  }
+      for (int j = 0; j < NJ; ++j) o[r][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
 
-  KBlock<DIM> kb, kn;
-  VBlock<DIM> vb, vn;
-  auto fetch = [&](int i, KBlock<DIM>& k, VBlock<DIM>& v) {
-    const int blk = first + 4 * i;
-    const int at = max(0, __builtin_amdgcn_readlane(pages, i));
-    const int off0 = (blk - fdiv(blk, a.c.by_blocks.mul, a.c.by_blocks.shift) * bpp) << 5;
-    k.load(a.c, at, h, off0);
-    v.load(a.c, at, h, off0);
-  };
-  if (mine > 0) fetch(0, kn, vn);
-  for (int i = 0; i < mine; ++i) {
-    kb = kn;
-    vb = vn;
-    if (i + 1 < mine) fetch(i + 1, kn, vn);
-    const int tok = (first + 4 * i) << 5;
-    if (__builtin_amdgcn_readlane(pages, i) < 0) continue;  // no page: nothing to see
-    float s[RT][8];
+    // 64 units at a time: this wave's block of each, their pages one a lane
+    for (int w0 = u0; w0 < u1; w0 += 64) {
+      const int first = 4 * w0 + wave;
+      const int mine = min(min(64, u1 - w0), blocks > first ? (blocks - first + 3) >> 2 : 0);
+      int pages = -1;
+      if (lane < mine) pages = kv4_page(a.c, b, fdiv(first + 4 * lane, a.c.by_blocks.mul, a.c.by_blocks.shift));
+      auto fetch = [&](int i, KBlock<DIM>& k, VBlock<DIM>& v) {
+        const int blk = first + 4 * i;
+        const int at = max(0, __builtin_amdgcn_readlane(pages, i));
+        const int off0 = (blk - fdiv(blk, a.c.by_blocks.mul, a.c.by_blocks.shift) * bpp) << 5;
+        k.load(a.c, at, h, off0);
+        v.load(a.c, at, h, off0);
+      };
+      auto body = [&](int i, const KBlock<DIM>& kb, VBlock<DIM>& vb) {
+        const int tok = (first + 4 * i) << 5;
+        if (__builtin_amdgcn_readlane(pages, i) < 0) return;  // no page: nothing to see
+        float s[RT][8];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) kb.template scores<T>(q[r], s[r]);
-    uint32_t lost = 0;  // bit e: token 8 g + e of this lane's slice is NaN and not seen by every row
-    const bool edge = tok + 32 > sure;
-    if (edge) {
+        for (int r = 0; r < RT; ++r) kb.template scores<T>(q[r], s[r]);
+        if (tok + 32 > sure) {
+          // The end: what a row does not see gets no weight, and no NaN of it (0 times NaN) may reach the
+          // row, so such values leave the products (bit e: token 8 g + e of this lane's slice); past
+          // the length everything does.
+          uint32_t nans = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int t = tok + 8 * g + e;
+          for (int e = 0; e < 8; ++e) {
+            const int t = tok + 8 * g + e;
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
-          if (t >= end[r]) s[r][e] = -INFINITY;
-        if (t >= sure && (t >= len || vb.byte(e) == 255)) {
-          if (t < len) lost |= 1u << e;
-          vb.clear(e);
+            for (int r = 0; r < RT; ++r)
+              if (t >= end[r]) s[r][e] = -INFINITY;
+            if (t >= sure && (t >= len || vb.byte(e) == 255)) {
+              if (t < len) nans |= 1u << e;
+              vb.clear(e);
+            }
+          }
+          if (__any(nans != 0)) {
+            // the rows that do see one get NaN in its 32 channels. Lane (n, g) of O holds channels DIM / 4 g ..,
+            // whose scale is that of v's slice 4 g, in the lanes of each token group u
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const uint64_t who = __ballot((nans >> e) & 1);
+              for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int r = 0; r < RT; ++r) lost[r] |= ((who >> (16 * u + 4 * g)) & 1) && tok + 8 * u + e < end[r];
+            }
+          }
+        }
+        Pieces<PP> p[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          float top = s[r][0];
+#pragma unroll
+          for (int e = 1; e < 8; ++e) top = fmaxf(top, s[r][e]);
+          top = fmaxf(top, __shfl_xor(top, 16));
+          top = fmaxf(top, __shfl_xor(top, 32));
+          // the maximum that is subtracted lags by up to 2^8 (the weights' own size cancels in the quotient)
+          const bool grew = __fmul_rn(__fsub_rn(top, m[r]), a.scale2) > 8.f;
+          if (__any(grew)) {
+            const float f = grew ? weight_of(m[r], top, a.scale2) : 1.f;
+            m[r] = grew ? top : m[r];
+            l[r] = __fmul_rn(l[r], f);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) o[r][j] *= f;
+          }
+          const float base = base_of(m[r]);
+          float w[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            w[e] = weight_of(s[r][e], base, a.scale2);
+            l[r] = __fadd_rn(l[r], w[e]);
+          }
+          p[r] = pieces_of<PP>(w);
+        }
+        auto product = [&]<int K>() {
+          v8bf f[2];
+          vb.template frags<K>(f[0], f[1]);
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int z = 0; z < 2; ++z)
+#pragma unroll
+              for (int k = PP - 1; k >= 0; --k)
+                o[r][2 * K + z] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[z], p[r].p[k], o[r][2 * K + z], 0, 0, 0);
+        };
+        product.template operator()<0>();
+        product.template operator()<1>();
+        if constexpr (DIM == 128) {
+          product.template operator()<2>();
+          product.template operator()<3>();
+        }
+      };
+      KBlock<DIM> k0, k1;
+      VBlock<DIM> v0, v1;
+      if (mine > 0) fetch(0, k0, v0);
+      for (int i = 0; i < mine; i += 2) {
+        if (i + 1 < mine) fetch(i + 1, k1, v1);
+        body(i, k0, v0);
+        if (i + 1 >= mine) break;
+        if (i + 2 < mine) fetch(i + 2, k0, v0);
+        body(i + 1, k1, v1);
+      }
+    }
+
+    // the four waves' rows together: lane (n, g) holds channels DIM / 4 g + DIM / 16 i + j of row n
+    const size_t bh = (size_t)b * a.c.heads + h;
+    const bool whole = u0 == 0 && u1 == units;
+    float* part = a.part + ((size_t)2 * blockIdx.x + (x != x0)) * (16 * RT) * (DIM + 2);
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      l[r] = __fadd_rn(l[r], __shfl_xor(l[r], 16));
+      l[r] = __fadd_rn(l[r], __shfl_xor(l[r], 32));
+      __syncthreads();  // the last rows are read
+      if (g == 0) {
+        sm[wave][n] = m[r];
+        sl[wave][n] = l[r];
+      }
+      const float nan = lost[r] ? NAN : 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; j += 4)
+          *reinterpret_cast<float4*>(&so[wave][n][DIM / 4 * g + NJ * i + j]) =
+              make_float4(__fadd_rn(o[r][j][i], nan), __fadd_rn(o[r][j + 1][i], nan), __fadd_rn(o[r][j + 2][i], nan),
+                          __fadd_rn(o[r][j + 3][i], nan));
+      __syncthreads();
+      constexpr int LANES = DIM / 4;  // threads a row, four channels each
+      for (int z = threadIdx.x; z < 16 * LANES; z += 256) {
+        const int rr = z / LANES, c4 = z % LANES * 4, row = row0 + 16 * r + rr;
+        if (row >= a.rows) continue;
+        const float top = fmaxf(fmaxf(sm[0][rr], sm[1][rr]), fmaxf(sm[2][rr], sm[3][rr])), base = base_of(top);
+        float sum = 0.f;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float f = weight_of(sm[w][rr], base, a.scale2);
+          const float4 v = *reinterpret_cast<const float4*>(&so[w][rr][c4]);
+          sum = __fmaf_rn(f, sl[w][rr], sum);
+          y.x = __fmaf_rn(f, v.x, y.x);
+          y.y = __fmaf_rn(f, v.y, y.y);
+          y.z = __fmaf_rn(f, v.z, y.z);
+          y.w = __fmaf_rn(f, v.w, y.w);
+        }
+        if (!whole) {
+          float* to = part + (16 * r + rr) * (DIM + 2);
+          *reinterpret_cast<float2*>(to + c4) = make_float2(y.x, y.y);
+          *reinterpret_cast<float2*>(to + c4 + 2) = make_float2(y.z, y.w);
+          if (c4 == 0) *reinterpret_cast<float2*>(to + DIM) = make_float2(top, sum);
+        } else {
+          const float d = sum == 0.f ? 1.f : sum;
+          const int t = fdiv(row, a.by_group.mul, a.by_group.shift), j = row - t * a.group;
+          T* to = (T*)a.out + (((size_t)b * a.tokens + t) * a.c.heads * a.group + h * a.group + j) * DIM + c4;
+          store4(to, __fdiv_rn(y.x, d), __fdiv_rn(y.y, d), __fdiv_rn(y.z, d), __fdiv_rn(y.w, d));
+          if (a.weights && c4 == 0) *reinterpret_cast<float2*>(a.stats + (bh * a.rows + row) * 2) = make_float2(top, d);
         }
       }
     }
-    Pieces<PP> p[RT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      float top = m[r];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, s[r][e]);
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      const float base = base_of(top);
-      if (__any(top > m[r])) {
-        const float f = weight_of(m[r], base, a.scale2);
-        l[r] = __fmul_rn(l[r], f);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) o[r][j] *= f;
-        m[r] = top;
-      }
-      float w[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        w[e] = weight_of(s[r][e], base, a.scale2);
-        l[r] = __fadd_rn(l[r], w[e]);
-      }
-      p[r] = pieces_of<PP>(w);
-    }
-    auto product = [&]<int K>() {
-      v8bf f[2];
-      vb.template frags<K>(f[0], f[1]);
-#pragma unroll
-      for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int z = 0; z < 2; ++z)
-#pragma unroll
-          for (int k = PP - 1; k >= 0; --k)
-            o[r][2 * K + z] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[z], p[r].p[k], o[r][2 * K + z], 0, 0, 0);
-    };
-    product.template operator()<0>();
-    product.template operator()<1>();
-    if constexpr (DIM == 128) {
-      product.template operator()<2>();
-      product.template operator()<3>();
-    }
-    if (edge && __any(lost != 0)) {
-      // NaN values that some rows see and others do not: they left the products; the rows that see
-      // them get NaN in the 32 channels that share the scale. Lane (n, g) of O holds channels
-      // DIM / 4 g .., of v's lanes those of slice 4 g (a token group u): its block's scale.
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint64_t who = __ballot((lost >> e) & 1);
-        for (int u = 0; u < 4; ++u)
-          if ((who >> (16 * u + 4 * g)) & 1)
-#pragma unroll
-            for (int r = 0; r < RT; ++r)
-              if (tok + 8 * u + e < end[r])
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) o[r][j] = v4f{NAN, NAN, NAN, NAN};
-      }
-    }
-  }
-
-  // the four waves' rows together: lane (n, g) holds channels DIM / 4 g + DIM / 16 i + j of row n
-  const size_t bh = (size_t)b * a.c.heads + h;
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    l[r] = __fadd_rn(l[r], __shfl_xor(l[r], 16));
-    l[r] = __fadd_rn(l[r], __shfl_xor(l[r], 32));
-    if (r) __syncthreads();
-    if (g == 0) {
-      sm[wave][n] = m[r];
-      sl[wave][n] = l[r];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < NJ; j += 4)
-        *reinterpret_cast<float4*>(&so[wave][n][DIM / 4 * g + NJ * i + j]) =
-            make_float4(o[r][j][i], o[r][j + 1][i], o[r][j + 2][i], o[r][j + 3][i]);
-    __syncthreads();
-    constexpr int LANES = DIM / 4;  // threads a row, four channels each
-    for (int x = threadIdx.x; x < 16 * LANES; x += 256) {
-      const int rr = x / LANES, c4 = x % LANES * 4, row = row0 + 16 * r + rr;
-      if (row >= a.rows) continue;
-      const float top = fmaxf(fmaxf(sm[0][rr], sm[1][rr]), fmaxf(sm[2][rr], sm[3][rr])), base = base_of(top);
-      float sum = 0.f;
-      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float f = weight_of(sm[w][rr], base, a.scale2);
-        const float4 z = *reinterpret_cast<const float4*>(&so[w][rr][c4]);
-        sum = __fmaf_rn(f, sl[w][rr], sum);
-        y.x = __fmaf_rn(f, z.x, y.x);
-        y.y = __fmaf_rn(f, z.y, y.y);
-        y.z = __fmaf_rn(f, z.z, y.z);
-        y.w = __fmaf_rn(f, z.w, y.w);
-      }
-      if (a.splits > 1) {
-        float* to = a.part + ((bh * a.splits + split) * a.rows + row) * (DIM + 2);
-        *reinterpret_cast<float2*>(to + c4) = make_float2(y.x, y.y);
-        *reinterpret_cast<float2*>(to + c4 + 2) = make_float2(y.z, y.w);
-        if (c4 == 0) *reinterpret_cast<float2*>(to + DIM) = make_float2(top, sum);
-      } else {
-        const float d = sum == 0.f ? 1.f : sum;
-        const int t = fdiv(row, a.by_group.mul, a.by_group.shift), j = row - t * a.group;
-        T* to = (T*)a.out + (((size_t)b * a.tokens + t) * a.c.heads * a.group + h * a.group + j) * DIM + c4;
-        store4(to, __fdiv_rn(y.x, d), __fdiv_rn(y.y, d), __fdiv_rn(y.z, d), __fdiv_rn(y.w, d));
-        if (a.weights && c4 == 0) *reinterpret_cast<float2*>(a.stats + (bh * a.rows + row) * 2) = make_float2(top, d);
-      }
+    x += u1 - u0;
+    if (x == begin + units * per_b) {  // the next sequence
+      begin = x;
+      ++b;
     }
   }
 }
 
-// The chunks of one row joined, a workgroup a row: four waves a quarter of the chunks each.
-template <typename T, int DIM>
+// The parts of one row joined, where its units lie in several shares: a workgroup a row, four waves
+// a quarter of the parts each.
+template <typename T, int DIM, int RT>
 __global__ __launch_bounds__(256) void kv4_join_kernel(Attend a) {
   __shared__ float sm[4], sl[4], so[4][DIM];
   const int row = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const size_t bh = (size_t)b * a.c.heads + h;
-  const int len = max(0, min(a.lens[b], a.max_len));
-  const int splits = max(1, (len + a.chunk - 1) / a.chunk);
-  const float* part = a.part + (bh * a.splits * a.rows + row) * (DIM + 2);
-  const size_t step = (size_t)a.rows * (DIM + 2);
+  const int rg = row / (16 * RT), units = units_of(len_of(a, b));
+  int begin;
+  const int share = share_of(a, line_of(a, a.c.heads * a.row_groups, b, &begin));
+  begin += (h * a.row_groups + rg) * units;
+  const int w0 = begin / share, w1 = (begin + units - 1) / share;
+  if (w0 == w1) return;  // whole in one share, and written there
+  const float* rows = a.part + (size_t)(row - rg * 16 * RT) * (DIM + 2);
   constexpr int C = DIM / 64;
   float top = -INFINITY, sum = 0.f, y[C] = {};
-  for (int s = wave; s < splits; s += 4) {
-    const float* p = part + s * step;
+  for (int w = w0 + wave; w <= w1; w += 4) {
+    const float* p = rows + ((size_t)2 * w + (w * share < begin)) * (16 * RT) * (DIM + 2);
     const float2 ms = *reinterpret_cast<const float2*>(p + DIM);
     float x[C];
 #pragma unroll
@@ -464,7 +541,8 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attend a) {
   T* to = (T*)a.out + (((size_t)b * a.tokens + t) * a.c.heads * a.group + h * a.group + j) * DIM + C * lane;
 #pragma unroll
   for (int c = 0; c < C; ++c) to[c] = (T)__fdiv_rn(y[c], d);
-  if (a.weights && lane == 0) *reinterpret_cast<float2*>(a.stats + (bh * a.rows + row) * 2) = make_float2(now, d);
+  if (a.weights && lane == 0)
+    *reinterpret_cast<float2*>(a.stats + (((size_t)b * a.c.heads + h) * a.rows + row) * 2) = make_float2(now, d);
 }
 
 // What each cached token received, added to its sum: the scores of 32 tokens a wave once more, each
@@ -512,27 +590,36 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(Attend a, int blocks) 
   }
 }
 
-// The tokens a chunk takes and how many chunks that makes of the longest sequence.
-static int chunk_of(int64_t B, int64_t heads, int64_t rows, int64_t max_len, int64_t* splits) {
-  const int64_t groups = B * heads * ((rows + 31) / 32);
-  int64_t chunk = 512;
-  while (chunk < 4096 && groups * ((max_len + 2 * chunk - 1) / (2 * chunk)) >= 4096) chunk *= 2;
-  while (chunk > 128 && groups * ((max_len + chunk - 1) / chunk) < 512) chunk /= 2;
-  *splits = (max_len + chunk - 1) / chunk;
-  if (*splits < 1) *splits = 1;
-  return (int)chunk;
+// How the work is cut: row tiles a workgroup (of 16), and the shares of the line, 0 for a workgroup a
+// (sequence, head, rows).
+struct Cut {
+  int tiles, row_groups, shares;
+};
+constexpr int LEAST_UNITS = 4;
+static Cut cut_of(int64_t B, int64_t heads, int64_t rows, int64_t max_len) {
+  Cut c;
+  c.tiles = rows <= 16 ? 1 : 2;
+  c.row_groups = (int)((rows + 16 * c.tiles - 1) / (16 * c.tiles));
+  const int64_t units = (max_len + UNIT - 1) / UNIT;
+  const int64_t line = B * heads * c.row_groups * units, most = 256 * 2;
+  c.shares = units <= LEAST_UNITS ? 0 : (int)(line < most ? line : most);
+  return c;
+}
+
+template <typename T, int DIM, int RT>
+static void launch_rows(const Attend& a, hipStream_t st) {
+  const unsigned grid = a.shares ? a.shares : a.B * a.c.heads * a.row_groups;
+  kv4_attend_kernel<T, DIM, RT><<<grid, 256, 0, st>>>(a);
+  if (a.shares) kv4_join_kernel<T, DIM, RT><<<dim3(a.rows, a.c.heads, a.B), 256, 0, st>>>(a);
 }
 
 template <typename T, int DIM>
-static int launch(const char* what, const Attend& a, int B, hipStream_t st) {
-  if (a.rows <= 16)
-    kv4_attend_kernel<T, DIM, 1><<<dim3(a.splits, a.c.heads, B), 256, 0, st>>>(a);
-  else
-    kv4_attend_kernel<T, DIM, 2><<<dim3(a.splits, a.c.heads * a.row_groups, B), 256, 0, st>>>(a);
-  if (a.splits > 1) kv4_join_kernel<T, DIM><<<dim3(a.rows, a.c.heads, B), 256, 0, st>>>(a);
+static int launch(const char* what, const Attend& a, int tiles, hipStream_t st) {
+  if (tiles == 1) launch_rows<T, DIM, 1>(a, st);
+  else launch_rows<T, DIM, 2>(a, st);
   if (a.weights && a.max_len > 0) {
     const int blocks = (a.max_len + 31) / 32;
-    kv4_weights_kernel<T, DIM><<<dim3((blocks + 3) / 4, a.c.heads, B), 256, 0, st>>>(a, blocks);
+    kv4_weights_kernel<T, DIM><<<dim3((blocks + 3) / 4, a.c.heads, a.B), 256, 0, st>>>(a, blocks);
   }
   return check_launch(what);
 }
@@ -543,10 +630,8 @@ using namespace bq;
 
 size_t bq_kv4_attend_ws_bytes(int64_t B, int64_t heads, int64_t rows, int64_t dim, int64_t max_len) {
   if (B < 1 || heads < 1 || rows < 1 || dim < 1 || max_len < 0) return 0;
-  int64_t splits;
-  chunk_of(B, heads, rows, max_len, &splits);
-  const size_t r = (size_t)B * heads * rows;
-  return r * 8 + (splits > 1 ? r * splits * (dim + 2) * 4 : 0);
+  const Cut c = cut_of(B, heads, rows, max_len);
+  return (size_t)B * heads * rows * 8 + (size_t)2 * c.shares * 16 * c.tiles * (dim + 2) * 4;
 }
 
 int bq_kv4_attend(const bq_kv4_cache* cache, const void* q, int type, int64_t tokens, int64_t q_heads, int64_t q_seq,
@@ -566,19 +651,19 @@ int bq_kv4_attend(const bq_kv4_cache* cache, const void* q, int type, int64_t to
   if (B == 0 || tokens == 0) return BQ_OK;
   const int64_t group = q_heads / cache->heads;
   if (tokens > 1 << 20 || group > 1 << 10 || B > 65535) return set_error(BQ_ERR_ARG, "%s: size too large", what);
-  const int64_t rows = tokens * group, row_groups = (rows + 31) / 32;
-  if (cache->heads * row_groups > 65535 || rows > 1 << 20) return set_error(BQ_ERR_ARG, "%s: size too large", what);
+  const int64_t rows = tokens * group;
+  if (rows > 1 << 20) return set_error(BQ_ERR_ARG, "%s: size too large", what);
+  const Cut cut = cut_of(B, cache->heads, rows, max_len);
+  if (B * cache->heads * cut.row_groups > 0x7fffffff / ((max_len + UNIT - 1) / UNIT + 1))
+    return set_error(BQ_ERR_ARG, "%s: size too large", what);
   if (!q || !lens || !out) return set_error(BQ_ERR_ARG, "%s: null pointer", what);
   const int64_t size = type == KV4_F32 ? 4 : 2;
   if ((((uintptr_t)q | (uintptr_t)out) & 15) || (q_seq | q_token | q_head) * size % 16)
     return set_error(BQ_ERR_ARG, "%s: rows that are not 16-byte aligned", what);
-  int64_t splits;
-  a.chunk = chunk_of(B, cache->heads, rows, max_len, &splits);
   const size_t need = bq_kv4_attend_ws_bytes(B, cache->heads, rows, cache->dim, max_len);
-  if ((weights || splits > 1) && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
+  if ((weights || cut.shares) && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
     return set_error(BQ_ERR_ARG, "%s: a workspace of %zu bytes, given %zu", what, need, ws ? ws_bytes : 0);
   const int64_t held = cache->pages ? width * cache->page : 0;  // tokens that a sequence's pages have room for
-  a.splits = (int)splits;
   a.lens = lens;
   a.q = q;
   a.qb = q_seq;
@@ -587,7 +672,10 @@ int bq_kv4_attend(const bq_kv4_cache* cache, const void* q, int type, int64_t to
   a.tokens = (int)tokens;
   a.group = (int)group;
   a.rows = (int)rows;
-  a.row_groups = (int)row_groups;
+  a.row_groups = cut.row_groups;
+  a.B = (int)B;
+  a.shares = cut.shares;
+  a.least = LEAST_UNITS;
   a.max_len = (int)(max_len < held ? max_len : held);
   a.by_group = fast_div((uint32_t)group);
   a.scale2 = scale * 1.4426950408889634f;
@@ -599,7 +687,7 @@ int bq_kv4_attend(const bq_kv4_cache* cache, const void* q, int type, int64_t to
   a.wh = w_head;
   hipStream_t st = (hipStream_t)stream;
   const bool wide = cache->dim == 128;
-  if (type == KV4_F32) return wide ? launch<float, 128>(what, a, (int)B, st) : launch<float, 64>(what, a, (int)B, st);
-  if (type == KV4_BF16) return wide ? launch<__bf16, 128>(what, a, (int)B, st) : launch<__bf16, 64>(what, a, (int)B, st);
-  return wide ? launch<_Float16, 128>(what, a, (int)B, st) : launch<_Float16, 64>(what, a, (int)B, st);
+  if (type == KV4_F32) return wide ? launch<float, 128>(what, a, cut.tiles, st) : launch<float, 64>(what, a, cut.tiles, st);
+  if (type == KV4_BF16) return wide ? launch<__bf16, 128>(what, a, cut.tiles, st) : launch<__bf16, 64>(what, a, cut.tiles, st);
+  return wide ? launch<_Float16, 128>(what, a, cut.tiles, st) : launch<_Float16, 64>(what, a, cut.tiles, st);
 }
