@@ -47,64 +47,78 @@ __device__ __forceinline__ v8f load8(const T* p) {
 // or below, read off its bits: 1.m 2^E fits for 1.m <= 1.5 with E - 2, else with E - 1. Scaling by
 // a power of two is exact (what underflows rounds to 0 either way), so the codes are the
 // hardware's rounding to nearest even of the exact quotient.
+// A workgroup takes 2048 / DIM tokens, whose places it looks up once, and PARTS of their 2 heads rows
+// (keys, then values), all loaded at once: with a row a thread the chain of lookups before each
+// row was most of the time (6237 tokens, 8 heads of 128: 15.5 us).
+constexpr int PARTS = 4;
 template <typename T, int DIM>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4 c, const T* __restrict__ nk, const T* __restrict__ nv,
-                                                         int64_t kt, int64_t kh, int64_t vt, int64_t vh, int first,
-                                                         uint32_t items, FastDiv per_token, const int* __restrict__ lens,
-                                                         const int* __restrict__ cu, int B) {
+                                                         int64_t kt, int64_t kh, int64_t vt, int64_t vh, int n, int groups,
+                                                         const int* __restrict__ lens, const int* __restrict__ cu, int B) {
   using At = Kv4At<DIM>;
   constexpr int P = DIM / 8;
-  const uint32_t id = blockIdx.x * 256u + threadIdx.x;
-  if (id >= items) return;  // whole rows: items is a multiple of P
-  int i = fdiv((int)id, per_token.mul, per_token.shift);
-  int rest = (int)id - i * (2 * c.heads * P);
-  i += first;
-  const int piece = rest % P;
-  rest /= P;
-  const bool is_v = rest >= c.heads;
-  const int h = is_v ? rest - c.heads : rest;
-  const v8f x = load8(is_v ? nv + i * vt + h * vh + 8 * piece : nk + i * kt + h * kh + 8 * piece);
+  const int tile = blockIdx.x / groups, part0 = (blockIdx.x - tile * groups) * PARTS;
+  const int i = tile * (256 / P) + threadIdx.x / P, piece = threadIdx.x % P;
+  if (i >= n) return;  // whole rows
+  v8f x[PARTS];
+#pragma unroll
+  for (int e = 0; e < PARTS; ++e) {
+    const int part = min(part0 + e, 2 * c.heads - 1);
+    const bool is_v = part >= c.heads;
+    const T* from = is_v ? nv + i * vt + (part - c.heads) * vh : nk + i * kt + part * kh;
+    x[e] = load8(from + 8 * piece);
+  }
   int lo = 0, hi = B;  // the sequence: the last b with cu[b] <= i
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
     if (cu[mid + 1] <= i) lo = mid + 1;
     else hi = mid;
   }
-  uint32_t peak = 0;  // |x| as integers: ordered as the values, NaN above infinity
-#pragma unroll
-  for (int e = 0; e < 8; ++e) peak = max(peak, __float_as_uint(x[e]) & 0x7fffffffu);
-  peak = max(peak, (uint32_t)__shfl_xor((int)peak, 1));
-  peak = max(peak, (uint32_t)__shfl_xor((int)peak, 2));
-  if (lo >= B) return;  // past the last sequence
-  const int64_t pos = (int64_t)lens[lo] - cu[lo + 1] + i;
-  if (pos < 0 || pos >= (int64_t)c.width * c.page) return;
-  const int pi = fdiv((int)pos, c.by_page.mul, c.by_page.shift);
-  const int at = kv4_page(c, lo, pi), off = (int)pos - pi * c.page;
-  if (at < 0) return;
-
-  const bool finite = peak < 0x7f800000u;
-  int byte = (int)((peak + 0x3fffffu) >> 23) - 2;  // E - 2, one more above 1.5 2^E
-  byte = finite ? max(byte, 1) : 255;
-  uint32_t code = 0;
-  if (finite) {
-    const float r = __uint_as_float((uint32_t)(254 - byte) << 23);  // 2^(127 - byte), byte <= 253
-    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, __fmul_rn(x[0], r), __fmul_rn(x[1], r), 1.0f, 0);
-    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, __fmul_rn(x[2], r), __fmul_rn(x[3], r), 1.0f, 1);
-    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, __fmul_rn(x[4], r), __fmul_rn(x[5], r), 1.0f, 2);
-    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, __fmul_rn(x[6], r), __fmul_rn(x[7], r), 1.0f, 3);
-  }
-  const size_t row = At::row(c, at, h, off);
-  if (is_v) {
-    if constexpr (DIM == 128) {
-      *reinterpret_cast<uint32_t*>(c.v + At::v(row, off, piece)) = code;
-    } else {
-      *reinterpret_cast<uint16_t*>(c.v + At::v(row, off, 2 * piece)) = (uint16_t)code;
-      *reinterpret_cast<uint16_t*>(c.v + At::v(row, off, 2 * piece + 1)) = (uint16_t)(code >> 16);
+  int at = -1, off = 0;
+  if (lo < B) {  // else past the last sequence
+    const int64_t pos = (int64_t)lens[lo] - cu[lo + 1] + i;
+    if (pos >= 0 && pos < (int64_t)c.width * c.page) {
+      const int pi = fdiv((int)pos, c.by_page.mul, c.by_page.shift);
+      at = kv4_page(c, lo, pi);
+      off = (int)pos - pi * c.page;
     }
-    if (piece % 4 == 0) c.vs[At::vs(row, off, piece / 4)] = (uint8_t)byte;
-  } else {
-    *reinterpret_cast<uint32_t*>(c.k + At::k(row) + 4 * piece) = code;
-    if (piece % 4 == 0) c.ks[At::ks(row, off, piece / 4)] = (uint8_t)byte;
+  }
+#pragma unroll
+  for (int e = 0; e < PARTS; ++e) {
+    uint32_t peak = 0;  // |x| as integers: ordered as the values, NaN above infinity
+#pragma unroll
+    for (int j = 0; j < 8; ++j) peak = max(peak, __float_as_uint(x[e][j]) & 0x7fffffffu);
+    peak = max(peak, (uint32_t)__builtin_amdgcn_mov_dpp((int)peak, 0xB1, 0xF, 0xF, false));
+    peak = max(peak, (uint32_t)__builtin_amdgcn_mov_dpp((int)peak, 0x4E, 0xF, 0xF, false));
+    if (at < 0 || part0 + e >= 2 * c.heads) continue;
+    const bool is_v = part0 + e >= c.heads, finite = peak < 0x7f800000u;
+    const int h = is_v ? part0 + e - c.heads : part0 + e;
+    int byte = (int)((peak + 0x3fffffu) >> 23) - 2;  // E - 2, one more above 1.5 2^E
+    byte = finite ? max(byte, 1) : 255;
+    uint32_t code = 0;
+    if (finite) {
+      const float r = __uint_as_float((uint32_t)(254 - byte) << 23);  // 2^(127 - byte), byte <= 253
+#define BQ_CODE(K) \
+  code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, __fmul_rn(x[e][2 * K], r), __fmul_rn(x[e][2 * K + 1], r), 1.0f, K)
+      BQ_CODE(0);
+      BQ_CODE(1);
+      BQ_CODE(2);
+      BQ_CODE(3);
+#undef BQ_CODE
+    }
+    const size_t row = At::row(c, at, h, off);
+    if (is_v) {
+      if constexpr (DIM == 128) {
+        *reinterpret_cast<uint32_t*>(c.v + At::v(row, off, piece)) = code;
+      } else {
+        *reinterpret_cast<uint16_t*>(c.v + At::v(row, off, 2 * piece)) = (uint16_t)code;
+        *reinterpret_cast<uint16_t*>(c.v + At::v(row, off, 2 * piece + 1)) = (uint16_t)(code >> 16);
+      }
+      if (piece % 4 == 0) c.vs[At::vs(row, off, piece / 4)] = (uint8_t)byte;
+    } else {
+      *reinterpret_cast<uint32_t*>(c.k + At::k(row) + 4 * piece) = code;
+      if (piece % 4 == 0) c.ks[At::ks(row, off, piece / 4)] = (uint8_t)byte;
+    }
   }
 }
 
@@ -159,151 +173,269 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4 c, const int* __restr
 
 // ---------------------------------------------------------------- eviction
 
-// A weight's place in the order: larger first as unsigned integers; -0 with 0, NaN above all.
+// A weight's place in the order, as unsigned integers, all above 0; -0 with 0, NaN above all.
 __device__ __forceinline__ uint32_t order_of(float w) {
-  if (__builtin_isnan(w)) return 0xffffffffu;
   const uint32_t u = __float_as_uint(__fadd_rn(w, 0.f));
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const uint32_t o = u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+  return __builtin_isnan(w) ? 0xffffffffu : o;
 }
+
+constexpr int EVICT_WAVES = 16, EVICT_THREADS = EVICT_WAVES * 64;
 
 // The sum of `v` over the workgroup's threads before this one; *all gets the sum of all.
 __device__ __forceinline__ int scan_before(int v, int* waves, int* all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, count = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int x = v;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
     const int y = __shfl_up(x, d);
     if (lane >= d) x += y;
   }
-  __syncthreads();
+  __syncthreads();  // the last scan's sums are read
   if (lane == 63) waves[wave] = x;
   __syncthreads();
   int before = 0, total = 0;
-  for (int i = 0; i < count; ++i) {
-    if (i < wave) before += waves[i];
-    total += waves[i];
+#pragma unroll
+  for (int i = 0; i < EVICT_WAVES; ++i) {
+    const int w = waves[i];
+    before += i < wave ? w : 0;
+    total += w;
   }
   *all = total;
   return before + x - v;
 }
 
 // Which tokens stay, one workgroup a (sequence, head): the `recent` last ones, and of the others
-// the keep - recent of largest weight, ties to the earlier token. A radix select from the top
-// byte of order_of finds the least weight that stays and how many of its equals do; a pass in
-// order then writes the places and weights.
-constexpr int EVICT_THREADS = 1024;
-__global__ __launch_bounds__(EVICT_THREADS) void kv4_select_kernel(const float* __restrict__ sums, int64_t sums_b,
-                                                                   int64_t sums_h, int most, int heads, const int* __restrict__ lens,
-                                                                   int keep, int recent, int* __restrict__ kept,
-                                                                   float* __restrict__ weights, int* __restrict__ left) {
-  __shared__ int hist[256], waves[EVICT_THREADS / 64], found[2];
-  const int bh = blockIdx.x, b = bh / heads, tid = threadIdx.x;
-  const int n = max(0, min(lens[b], most));
-  const float* w = sums + b * sums_b + (bh - b * heads) * sums_h;
-  kept += (size_t)bh * keep;
-  weights += (size_t)bh * keep;
-  if (bh % heads == 0 && tid == 0) left[b] = min(n, keep);
-  uint32_t least = 0;      // weights above this stay
+// the keep - recent of largest weight, ties to the earlier token.
+// A radix select over order_of finds the least weight that stays and how many of its equals do: 12,
+// 12 and 8 bits, a histogram in LDS each. The first digit spans sign, exponent and three bits of
+// the mantissa, so that weights of one size fall into eight counters and the lanes of a wave seldom
+// meet in one (with 8 bits they met in a few; and a thread that looked through the counters alone
+// took longer than the counting). A last pass writes places and weights in order: each wave counts,
+// by ballots, those that stay of its 256 tokens, and one scan sums the counts.
+// A span of 65536 weights is loaded once and stays in registers as order_of, 64 a thread: a pass is
+// then bound by its few instructions a weight on one CU. Longer rows load each span in each pass.
+constexpr int EVICT_LOADS = 16, EVICT_CHUNK = 256, EVICT_SPAN = EVICT_LOADS * EVICT_WAVES * EVICT_CHUNK;
+typedef float v4fu __attribute__((ext_vector_type(4), aligned(4)));
+
+// Chunk e of this wave in a span: 256 tokens, four a lane from token_of(span, e).
+__device__ __forceinline__ int chunk_of(int e) { return e * EVICT_WAVES + (threadIdx.x >> 6); }
+__device__ __forceinline__ int token_of(int s0, int e) { return s0 + chunk_of(e) * EVICT_CHUNK + 4 * (threadIdx.x & 63); }
+
+template <bool ONE>  // the row is one span
+__device__ __forceinline__ void select_row(const float* __restrict__ w, int n, int old, int keep, int recent,
+                                           int* __restrict__ kept, float* __restrict__ weights, int* hist, int* waves,
+                                           int* found) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  uint32_t u[EVICT_LOADS][4];  // order_of the span's weights; 0 from `old` on
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int e = 0; e < EVICT_LOADS; ++e) {
+      const int i = token_of(s0, e);
+      if (s0 + chunk_of(e) * EVICT_CHUNK >= old) break;
+      v4fu x = {0.f, 0.f, 0.f, 0.f};
+      if (i + 3 < old) {
+        x = *reinterpret_cast<const v4fu*>(w + i);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+          if (i + j < old) x[j] = w[i + j];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[e][j] = i + j < old ? order_of(x[j]) : 0u;
+    }
+  };
+  if constexpr (ONE) load(0);
+
+  uint32_t least = 0;       // weights above this stay
   int equals = 0x7fffffff;  // and so many that equal it
-  const int old = n > keep ? n - recent : n;
   if (n > keep) {
     int need = keep - recent;
     uint32_t prefix = 0, mask = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
+    for (int digit = 0; digit < 3; ++digit) {
+      const int shift = digit == 0 ? 20 : digit == 1 ? 8 : 0, count = digit == 2 ? 256 : 4096;
+      for (int i = tid; i < count; i += EVICT_THREADS) hist[i] = 0;
       __syncthreads();
-      for (int i = tid; i < old; i += EVICT_THREADS) {
-        const uint32_t u = order_of(w[i]);
-        if ((u & mask) == prefix) atomicAdd(&hist[(u >> shift) & 255], 1);
+      for (int s0 = 0; s0 < old; s0 += EVICT_SPAN) {
+        if constexpr (!ONE) load(s0);
+#pragma unroll
+        for (int e = 0; e < EVICT_LOADS; ++e) {
+          if (s0 + chunk_of(e) * EVICT_CHUNK >= old) break;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)  // a 0, of no weight, is counted under all others, where `need` never comes
+            if ((u[e][j] & mask) == prefix) atomicAdd(&hist[(u[e][j] >> shift) & (count - 1)], 1);
+        }
       }
       __syncthreads();
-      if (tid == 0) {  // from the largest digit down
-        int d = 255, rest = need;
-        while (d > 0 && hist[d] < rest) rest -= hist[d--];
-        found[0] = d;
-        found[1] = rest;
+      // the digit at which the counts from the largest down reach `need`: four counters a thread
+      int c4[4], sum = 0, all;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = count - 1 - 4 * tid - e;
+        c4[e] = d >= 0 ? hist[d] : 0;
+        sum += c4[e];
+      }
+      int above = scan_before(sum, waves, &all);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        // need = 0: the largest digit, of which none stays
+        if ((above < need && above + c4[e] >= need) || (need == 0 && tid == 0 && e == 0)) {
+          found[0] = count - 1 - 4 * tid - e;
+          found[1] = need - above;
+        }
+        above += c4[e];
       }
       __syncthreads();
       prefix |= (uint32_t)found[0] << shift;
-      mask |= 255u << shift;
+      mask |= (uint32_t)(count - 1) << shift;
       need = found[1];
       __syncthreads();
     }
     least = prefix;
     equals = need;
   }
-  int out = 0, same = 0;  // kept so far, equals of `least` met so far
-  for (int i0 = 0; i0 < n; i0 += EVICT_THREADS) {
-    const int i = i0 + tid;
-    int stays = 0;
-    float x = 0.f;
-    if (n <= keep) {
-      if (i < n) stays = 1, x = w[i];
-    } else {
-      uint32_t u = 0;
-      if (i < n) x = w[i], u = order_of(x);
-      int all;
-      const int eq = i < old && u == least;
-      const int rank = same + scan_before(eq, waves, &all);
-      same += all;
-      stays = i < n && (i >= old || u > least || (eq && rank < equals));
+  int out = 0, same = 0;  // kept before this span, equals of `least` met before it
+  for (int s0 = 0; s0 < old; s0 += EVICT_SPAN) {
+    if constexpr (!ONE) load(s0);
+    const int chunks = (min(EVICT_SPAN, old - s0) + EVICT_CHUNK - 1) / EVICT_CHUNK;  // at most 256
+    // hist: each chunk's tokens above `least` and, from 256 on, its equals of `least`
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < EVICT_LOADS; ++e) {
+      if (chunk_of(e) >= chunks) break;
+      int over = 0, eq = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        over += __popcll(__ballot(u[e][j] > least));
+        eq += __popcll(__ballot(u[e][j] == least));
+      }
+      if (lane == 0) {
+        hist[chunk_of(e)] = over;
+        hist[256 + chunk_of(e)] = eq;
+      }
     }
-    int all;
-    const int to = out + scan_before(stays, waves, &all);
+    __syncthreads();
+    int all_eq, all;
+    const int my_eq = tid < chunks ? hist[256 + tid] : 0, my_over = tid < chunks ? hist[tid] : 0;
+    const int eq_before = same + scan_before(my_eq, waves, &all_eq);
+    const int stay = my_over + max(0, min(my_eq, equals - eq_before));
+    const int before = out + scan_before(stay, waves, &all);
+    if (tid < chunks) {
+      hist[tid] = before;
+      hist[256 + tid] = eq_before;
+    }
+    same += all_eq;
     out += all;
-    if (stays && to < keep) {
-      kept[to] = i;
-      weights[to] = x;
+    __syncthreads();
+    const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+    for (int e = 0; e < EVICT_LOADS; ++e) {
+      if (chunk_of(e) >= chunks) break;
+      const int i = token_of(s0, e);
+      int rank = hist[256 + chunk_of(e)], to = hist[chunk_of(e)];  // of the lane's first token
+#pragma unroll
+      for (int j = 0; j < 4; ++j) rank += __popcll(__ballot(u[e][j] == least) & below);
+      bool stays[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool eq = u[e][j] == least;
+        stays[j] = u[e][j] > least || (eq && rank < equals);
+        rank += eq;
+        to += __popcll(__ballot(stays[j]) & below);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (stays[j] && to < keep) {
+          kept[to] = i + j;
+          weights[to] = w[i + j];
+        }
+        to += stays[j];
+      }
     }
   }
-  for (int i = out + tid; i < keep; i += EVICT_THREADS) {
-    kept[i] = -1;
-    weights[i] = 0.f;
+  for (int i = out + tid; i < keep; i += EVICT_THREADS) {  // the latest, and past the last
+    const int from = old + i - out;
+    kept[i] = from < n ? from : -1;
+    weights[i] = from < n ? w[from] : 0.f;
   }
 }
 
+__global__ __launch_bounds__(EVICT_THREADS) void kv4_select_kernel(const float* __restrict__ sums, int64_t sums_b,
+                                                                   int64_t sums_h, int most, int heads,
+                                                                   const int* __restrict__ lens, int keep, int recent,
+                                                                   int* __restrict__ kept, float* __restrict__ weights,
+                                                                   int* __restrict__ left) {
+  __shared__ int hist[4096], waves[EVICT_WAVES], found[2];
+  const int bh = blockIdx.x, b = bh / heads;
+  const int n = max(0, min(lens[b], most)), old = n > keep ? n - recent : 0;  // all stay: none is looked at
+  const float* w = sums + b * sums_b + (bh - b * heads) * sums_h;
+  kept += (size_t)bh * keep;
+  weights += (size_t)bh * keep;
+  if (bh % heads == 0 && threadIdx.x == 0) left[b] = min(n, keep);
+  if (old <= EVICT_SPAN) select_row<true>(w, n, old, keep, recent, kept, weights, hist, waves, found);
+  else select_row<false>(w, n, old, keep, recent, kept, weights, hist, waves, found);
+}
+
 // The kept tokens of each (sequence, head) to the new pages in order: codes and scales as they are.
+// A workgroup takes 4096 / DIM destinations, whose rows and sources' rows it looks up once; k's rows
+// move 16 bytes a thread, v's slices are put together where they go (a thread gathers one slice of a
+// block of tokens) and the scales in v_scales' order.
 template <int DIM>
 __global__ __launch_bounds__(256) void kv4_move_kernel(Kv4 c, Kv4 to, const int* __restrict__ kept, int keep,
                                                        int blocks) {
   using At = Kv4At<DIM>;
-  constexpr int P = DIM / 8, TOKENS = 256 / P;
-  const int bh = blockIdx.x / blocks, i = (blockIdx.x - bh * blocks) * TOKENS + threadIdx.x / P;
-  if (i >= keep) return;
-  const int b = bh / c.heads, h = bh - b * c.heads, piece = threadIdx.x % P;
-  const int src = kept[(size_t)bh * keep + i];
-  if (src < 0) return;
-  const int si = fdiv(src, c.by_page.mul, c.by_page.shift), di = fdiv(i, c.by_page.mul, c.by_page.shift);
-  const int sp = kv4_page(c, b, si), dp = kv4_page(to, b, di);
-  if (sp < 0 || dp < 0) return;
-  const int so = src - si * c.page, dof = i - di * c.page;
-  const size_t sr = At::row(c, sp, h, so), dr = At::row(c, dp, h, dof);
-  *reinterpret_cast<uint32_t*>(c.k + At::k(dr) + 4 * piece) = *reinterpret_cast<const uint32_t*>(c.k + At::k(sr) + 4 * piece);
-  if constexpr (DIM == 128) {
-    *reinterpret_cast<uint32_t*>(c.v + At::v(dr, dof, piece)) = *reinterpret_cast<const uint32_t*>(c.v + At::v(sr, so, piece));
-  } else {
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      *reinterpret_cast<uint16_t*>(c.v + At::v(dr, dof, 2 * piece + e)) =
-          *reinterpret_cast<const uint16_t*>(c.v + At::v(sr, so, 2 * piece + e));
+  constexpr int TB = At::TB, CB = At::CB, TOK = 4096 / DIM;
+  __shared__ long long from[TOK], dest[TOK];  // rows in the arrays; a source of -1: nothing to move
+  __shared__ int from_off[TOK], dest_off[TOK];
+  const int bh = blockIdx.x / blocks, t0 = (blockIdx.x - bh * blocks) * TOK;
+  const int b = bh / c.heads, h = bh - b * c.heads, tid = threadIdx.x;
+  if (tid < TOK) {
+    const int i = t0 + tid, src = i < keep ? kept[(size_t)bh * keep + i] : -1;
+    long long row = -1;
+    if (src >= 0) {
+      const int si = fdiv(src, c.by_page.mul, c.by_page.shift), di = fdiv(i, c.by_page.mul, c.by_page.shift);
+      const int sp = kv4_page(c, b, si), dp = kv4_page(to, b, di);
+      from_off[tid] = src - si * c.page;
+      dest_off[tid] = i - di * c.page;
+      if (sp >= 0 && dp >= 0) {
+        row = (long long)At::row(c, sp, h, from_off[tid]);
+        dest[tid] = (long long)At::row(c, dp, h, dest_off[tid]);
+      }
+    }
+    from[tid] = row;
   }
-  if (piece < DIM / 32) {
-    c.ks[At::ks(dr, dof, piece)] = c.ks[At::ks(sr, so, piece)];
-    c.vs[At::vs(dr, dof, piece)] = c.vs[At::vs(sr, so, piece)];
+  __syncthreads();
+  if (tid < 128) {  // k: 16 bytes
+    const int t = tid / (DIM / 32), q = tid % (DIM / 32);
+    if (from[t] >= 0)
+      *reinterpret_cast<uint4*>(c.k + At::k(dest[t]) + 16 * q) = *reinterpret_cast<const uint4*>(c.k + At::k(from[t]) + 16 * q);
+  } else {  // v: a slice of TB tokens, CB bytes each
+    const int t = (tid - 128) / 16 * TB, s = tid % 16;
+#pragma unroll
+    for (int e = 0; e < TB; ++e)
+      if (from[t + e] >= 0) {
+        const uint8_t* p = c.v + At::v(from[t + e], from_off[t + e], s);
+        uint8_t* at = c.v + At::v(dest[t + e], dest_off[t + e], s);
+        if constexpr (DIM == 128) *reinterpret_cast<uint32_t*>(at) = *reinterpret_cast<const uint32_t*>(p);
+        else *reinterpret_cast<uint16_t*>(at) = *reinterpret_cast<const uint16_t*>(p);
+      }
+  }
+  if (tid < TOK * CB) {
+    const int t = tid % TOK, s = tid / TOK;
+    if (from[t] >= 0) {
+      c.vs[At::vs(dest[t], dest_off[t], s)] = c.vs[At::vs(from[t], from_off[t], s)];
+      c.ks[At::ks(dest[t], dest_off[t], s)] = c.ks[At::ks(from[t], from_off[t], s)];
+    }
   }
 }
 
 template <typename T, int DIM>
 static void append_of(const Kv4& c, const void* nk, const void* nv, int64_t n, int64_t kt, int64_t kh, int64_t vt,
                       int64_t vh, const int* lens, const int* cu, int B, hipStream_t st) {
-  const int64_t per = 2 * (int64_t)c.heads * (DIM / 8);
-  const int64_t most = 0x70000000 / per;  // tokens a launch
-  const FastDiv by = fast_div((uint32_t)per);
-  for (int64_t first = 0; first < n; first += most) {
-    const int64_t items = (n - first < most ? n - first : most) * per;
-    kv4_append_kernel<T, DIM><<<(unsigned)((items + 255) / 256), 256, 0, st>>>(
-        c, (const T*)nk, (const T*)nv, kt, kh, vt, vh, (int)first, (uint32_t)items, by, lens, cu, B);
-  }
+  const int groups = (2 * c.heads + PARTS - 1) / PARTS;
+  const int64_t tiles = (n + 2048 / DIM - 1) / (2048 / DIM);
+  kv4_append_kernel<T, DIM><<<(unsigned)(tiles * groups), 256, 0, st>>>(c, (const T*)nk, (const T*)nv, kt, kh, vt, vh, (int)n,
+                                                                       groups, lens, cu, B);
 }
 
 }  // namespace bq
@@ -323,6 +455,8 @@ int bq_kv4_append(const bq_kv4_cache* cache, const void* new_k, const void* new_
   const int64_t size = type == KV4_F32 ? 4 : 2;
   if ((((uintptr_t)new_k | (uintptr_t)new_v) & 15) || (k_token | k_head | v_token | v_head) * size % 16)
     return set_error(BQ_ERR_ARG, "%s: rows that are not 16-byte aligned", what);
+  if ((n + 15) / 16 * ((2 * c.heads + PARTS - 1) / PARTS) > 0x7fffffff)
+    return set_error(BQ_ERR_ARG, "%s: size too large", what);
   hipStream_t st = (hipStream_t)stream;
   const bool wide = cache->dim == 128;
 #define BQ_APPEND(T)                                                                                            \
@@ -369,7 +503,7 @@ int bq_kv4_evict(const bq_kv4_cache* cache, const float* sums, int64_t sums_b, i
                      (long long)(new_width * c.page), (long long)keep);
   if (B == 0) return BQ_OK;
   if (!lens || !kept || !weights || !left || (most && !sums)) return set_error(BQ_ERR_ARG, "%s: null pointer", what);
-  const int64_t blocks = (keep + 255 / (cache->dim / 8)) / (256 / (cache->dim / 8));
+  const int64_t blocks = (keep + 4096 / cache->dim - 1) / (4096 / cache->dim);
   if (B * c.heads * blocks > 0x7fffffff) return set_error(BQ_ERR_ARG, "%s: size too large", what);
   hipStream_t st = (hipStream_t)stream;
   kv4_select_kernel<<<(unsigned)(B * c.heads), EVICT_THREADS, 0, st>>>(sums, sums_b, sums_h, (int)most, c.heads, lens, (int)keep,
