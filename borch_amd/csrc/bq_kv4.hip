@@ -210,42 +210,70 @@ __device__ __forceinline__ int scan_before(int v, int* waves, int* all) {
 // A radix select over order_of finds the least weight that stays and how many of its equals do: 12,
 // 12 and 8 bits, a histogram in LDS each. The first digit spans sign, exponent and three bits of
 // the mantissa, so that weights of one size fall into eight counters and the lanes of a wave seldom
-// meet in one (with 8 bits they met in a few; and a thread that looked through the counters alone
-// took longer than the counting). A last pass writes places and weights in order: each wave counts,
-// by ballots, those that stay of its 256 tokens, and one scan sums the counts.
-// A span of 65536 weights is loaded once and stays in registers as order_of, 64 a thread: a pass is
-// then bound by its few instructions a weight on one CU. Longer rows load each span in each pass.
-constexpr int EVICT_LOADS = 16, EVICT_CHUNK = 256, EVICT_SPAN = EVICT_LOADS * EVICT_WAVES * EVICT_CHUNK;
+// meet in one; the weights that share the digit found are then listed in LDS, where the other
+// digits take no time (a row with more such than the list holds is read again for each digit). Two
+// passes write places and weights in order: each wave counts, by ballots, those that stay of its 256
+// tokens, one scan sums the counts, and each lane knows its place.
+// The passes' loops stay rolled, the next loads under this step's work: with a row held in registers, 64
+// weights a thread, the straight code for them took longer to fetch than four more reads from L2
+// (64 rows of 4096: 30 us; 16 of 65536: 52).
+constexpr int EVICT_STEP = 4, EVICT_SPAN = 65536, EVICT_LIST = 8192;
 typedef float v4fu __attribute__((ext_vector_type(4), aligned(4)));
 
-// Chunk e of this wave in a span: 256 tokens, four a lane from token_of(span, e).
-__device__ __forceinline__ int chunk_of(int e) { return e * EVICT_WAVES + (threadIdx.x >> 6); }
-__device__ __forceinline__ int token_of(int s0, int e) { return s0 + chunk_of(e) * EVICT_CHUNK + 4 * (threadIdx.x & 63); }
+__global__ __launch_bounds__(EVICT_THREADS) void kv4_select_kernel(const float* __restrict__ sums, int64_t sums_b,
+                                                                   int64_t sums_h, int most, int heads,
+                                                                   const int* __restrict__ lens, int keep, int recent,
+                                                                   int* __restrict__ kept, float* __restrict__ weights,
+                                                                   int* __restrict__ left) {
+  __shared__ int hist[4096], waves[EVICT_WAVES], found[2], listed;
+  __shared__ uint32_t list[EVICT_LIST];
+  const int bh = blockIdx.x, b = bh / heads, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = max(0, min(lens[b], most)), old = n > keep ? n - recent : 0;  // all stay: none is looked at
+  const float* w = sums + b * sums_b + (bh - b * heads) * sums_h;
+  kept += (size_t)bh * keep;
+  weights += (size_t)bh * keep;
+  if (bh % heads == 0 && tid == 0) left[b] = min(n, keep);
 
-template <bool ONE>  // the row is one span
-__device__ __forceinline__ void select_row(const float* __restrict__ w, int n, int old, int keep, int recent,
-                                           int* __restrict__ kept, float* __restrict__ weights, int* hist, int* waves,
-                                           int* found) {
-  const int tid = threadIdx.x, lane = tid & 63;
-  uint32_t u[EVICT_LOADS][4];  // order_of the span's weights; 0 from `old` on
-  auto load = [&](int s0) {
+  // f(i, o) for tokens i .. i + 3 of the old ones from .. to, o order_of their weights, 0 past them; the
+  // threads side by side, a wave's 256 tokens or none
+  auto load = [&](int i0, int to, v4fu (&x)[EVICT_STEP]) {
 #pragma unroll
-    for (int e = 0; e < EVICT_LOADS; ++e) {
-      const int i = token_of(s0, e);
-      if (s0 + chunk_of(e) * EVICT_CHUNK >= old) break;
-      v4fu x = {0.f, 0.f, 0.f, 0.f};
-      if (i + 3 < old) {
-        x = *reinterpret_cast<const v4fu*>(w + i);
-      } else {
+    for (int e = 0; e < EVICT_STEP; ++e) {
+      const int c = i0 + (e * EVICT_WAVES + wave) * 256, i = c + 4 * lane;
+      if (c + 256 <= most) {
+        x[e] = *reinterpret_cast<const v4fu*>(w + i);
+      } else if (c < to) {
 #pragma unroll
-        for (int j = 0; j < 3; ++j)
-          if (i + j < old) x[j] = w[i + j];
+        for (int j = 0; j < 4; ++j) x[e][j] = w[min(i + j, old - 1)];
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) u[e][j] = i + j < old ? order_of(x[j]) : 0u;
     }
   };
-  if constexpr (ONE) load(0);
+  constexpr int STEP = EVICT_STEP * EVICT_THREADS * 4;  // tokens
+  auto each = [&](int from, int to, auto&& f, auto&& after) {  // after(i0): a step's tokens are done
+    v4fu now[EVICT_STEP] = {}, next[EVICT_STEP] = {};
+    load(from, to, now);
+#pragma unroll 1
+    for (int i0 = from; i0 < to; i0 += STEP) {
+      if (i0 + STEP < to) load(i0 + STEP, to, next);
+#pragma unroll
+      for (int e = 0; e < EVICT_STEP; ++e) {
+        const int c = i0 + (e * EVICT_WAVES + wave) * 256, i = c + 4 * lane;
+        if (c >= to) break;
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = order_of(now[e][j]);
+        if (c + 256 > to)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[j] = i + j < to ? o[j] : 0u;
+        f(i, o);
+      }
+      after(i0);
+#pragma unroll
+      for (int e = 0; e < EVICT_STEP; ++e) now[e] = next[e];
+    }
+  };
+  auto nothing = [](int) {};
 
   uint32_t least = 0;       // weights above this stay
   int equals = 0x7fffffff;  // and so many that equal it
@@ -255,17 +283,19 @@ __device__ __forceinline__ void select_row(const float* __restrict__ w, int n, i
     for (int digit = 0; digit < 3; ++digit) {
       const int shift = digit == 0 ? 20 : digit == 1 ? 8 : 0, count = digit == 2 ? 256 : 4096;
       for (int i = tid; i < count; i += EVICT_THREADS) hist[i] = 0;
+      if (tid == 0 && digit == 0) listed = 0;
       __syncthreads();
-      for (int s0 = 0; s0 < old; s0 += EVICT_SPAN) {
-        if constexpr (!ONE) load(s0);
+      // a 0, of no weight, is counted under all others, where `need` never comes
+      auto tally = [&](uint32_t o) {
+        if ((o & mask) == prefix) atomicAdd(&hist[(o >> shift) & (count - 1)], 1);
+      };
+      if (digit > 0 && listed <= EVICT_LIST)
+        for (int i = tid; i < listed; i += EVICT_THREADS) tally(list[i]);
+      else
+        each(0, old, [&](int, const uint32_t (&o)[4]) {
 #pragma unroll
-        for (int e = 0; e < EVICT_LOADS; ++e) {
-          if (s0 + chunk_of(e) * EVICT_CHUNK >= old) break;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)  // a 0, of no weight, is counted under all others, where `need` never comes
-            if ((u[e][j] & mask) == prefix) atomicAdd(&hist[(u[e][j] >> shift) & (count - 1)], 1);
-        }
-      }
+          for (int j = 0; j < 4; ++j) tally(o[j]);
+        }, nothing);
       __syncthreads();
       // the digit at which the counts from the largest down reach `need`: four counters a thread
       int c4[4], sum = 0, all;
@@ -289,6 +319,15 @@ __device__ __forceinline__ void select_row(const float* __restrict__ w, int n, i
       prefix |= (uint32_t)found[0] << shift;
       mask |= (uint32_t)(count - 1) << shift;
       need = found[1];
+      if (digit == 0)
+        each(0, old, [&](int, const uint32_t (&o)[4]) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if ((o[j] & mask) == prefix) {
+              const int at = atomicAdd(&listed, 1);
+              if (at < EVICT_LIST) list[at] = o[j];
+            }
+        }, nothing);
       __syncthreads();
     }
     least = prefix;
@@ -296,84 +335,86 @@ __device__ __forceinline__ void select_row(const float* __restrict__ w, int n, i
   }
   int out = 0, same = 0;  // kept before this span, equals of `least` met before it
   for (int s0 = 0; s0 < old; s0 += EVICT_SPAN) {
-    if constexpr (!ONE) load(s0);
-    const int chunks = (min(EVICT_SPAN, old - s0) + EVICT_CHUNK - 1) / EVICT_CHUNK;  // at most 256
-    // hist: each chunk's tokens above `least` and, from 256 on, its equals of `least`
+    const int end = min(old, s0 + EVICT_SPAN);
     __syncthreads();
-#pragma unroll
-    for (int e = 0; e < EVICT_LOADS; ++e) {
-      if (chunk_of(e) >= chunks) break;
+    // of each 256 tokens, those above `least` and, from 256 on, its equals
+    if (tid < 512) hist[tid] = 0;
+    __syncthreads();
+    each(s0, end, [&](int i, const uint32_t (&o)[4]) {
       int over = 0, eq = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        over += __popcll(__ballot(u[e][j] > least));
-        eq += __popcll(__ballot(u[e][j] == least));
+        over += (int)__popcll(__ballot(o[j] > least));
+        eq += (int)__popcll(__ballot(o[j] == least));
       }
       if (lane == 0) {
-        hist[chunk_of(e)] = over;
-        hist[256 + chunk_of(e)] = eq;
+        hist[(i - s0) >> 8] = over;
+        hist[256 + ((i - s0) >> 8)] = eq;
       }
-    }
+    }, nothing);
     __syncthreads();
     int all_eq, all;
-    const int my_eq = tid < chunks ? hist[256 + tid] : 0, my_over = tid < chunks ? hist[tid] : 0;
-    const int eq_before = same + scan_before(my_eq, waves, &all_eq);
-    const int stay = my_over + max(0, min(my_eq, equals - eq_before));
+    const int eq_here = tid < 256 ? hist[256 + tid] : 0;
+    const int eq_before = same + scan_before(eq_here, waves, &all_eq);
+    const int stay = (tid < 256 ? hist[tid] : 0) + max(0, min(eq_here, equals - eq_before));
     const int before = out + scan_before(stay, waves, &all);
-    if (tid < chunks) {
+    if (tid < 256) {
       hist[tid] = before;
-      hist[256 + tid] = eq_before;
+      hist[256 + tid] = equals - eq_before;  // so many of its equals stay
     }
+    int done = out;  // written
+    uint16_t* staged = reinterpret_cast<uint16_t*>(list);  // of one step: STEP entries
+    static_assert(STEP * 2 <= EVICT_LIST * 4 && EVICT_SPAN <= 65536, "staging");
     same += all_eq;
     out += all;
     __syncthreads();
-    const uint64_t below = (1ull << lane) - 1;
-#pragma unroll
-    for (int e = 0; e < EVICT_LOADS; ++e) {
-      if (chunk_of(e) >= chunks) break;
-      const int i = token_of(s0, e);
-      int rank = hist[256 + chunk_of(e)], to = hist[chunk_of(e)];  // of the lane's first token
-#pragma unroll
-      for (int j = 0; j < 4; ++j) rank += __popcll(__ballot(u[e][j] == least) & below);
+    auto below = [&](bool b) {  // lanes before this one with b
+      const uint64_t m = __ballot(b);
+      return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+    };
+    each(s0, end, [&](int i, const uint32_t (&o)[4]) {
+      const int at = __builtin_amdgcn_readfirstlane((i - s0) >> 8), cut = __builtin_amdgcn_readfirstlane(hist[256 + at]);
       bool stays[4];
+      if (cut <= 0 || cut >= 256) {  // no equal stays, or all
+        const uint32_t from = cut <= 0 ? least : least - 1;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool eq = u[e][j] == least;
-        stays[j] = u[e][j] > least || (eq && rank < equals);
-        rank += eq;
-        to += __popcll(__ballot(stays[j]) & below);
-      }
+        for (int j = 0; j < 4; ++j) stays[j] = o[j] > from;
+      } else {
+        int rank = 0;  // of the lane's first token among the equals
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (stays[j] && to < keep) {
-          kept[to] = i + j;
-          weights[to] = w[i + j];
+        for (int j = 0; j < 4; ++j) rank += below(o[j] == least);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          stays[j] = o[j] > least || (o[j] == least && rank < cut);
+          rank += o[j] == least;
         }
+      }
+      int to = hist[at] - done;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) to += below(stays[j]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (stays[j]) staged[to] = (uint16_t)(i + j - s0);
         to += stays[j];
       }
-    }
+    }, [&](int i0) {
+      // what stays of this step, from LDS: side by side, where each lane's own stores took most of the pass
+      const int next = (i0 - s0 + STEP) >> 8, upto = i0 + STEP < end ? hist[next] : out;
+      __syncthreads();
+      for (int x = tid; x < upto - done; x += EVICT_THREADS) {
+        const int i = s0 + staged[x];
+        kept[done + x] = i;
+        weights[done + x] = w[i];
+      }
+      __syncthreads();
+      done = upto;
+    });
   }
   for (int i = out + tid; i < keep; i += EVICT_THREADS) {  // the latest, and past the last
     const int from = old + i - out;
     kept[i] = from < n ? from : -1;
     weights[i] = from < n ? w[from] : 0.f;
   }
-}
-
-__global__ __launch_bounds__(EVICT_THREADS) void kv4_select_kernel(const float* __restrict__ sums, int64_t sums_b,
-                                                                   int64_t sums_h, int most, int heads,
-                                                                   const int* __restrict__ lens, int keep, int recent,
-                                                                   int* __restrict__ kept, float* __restrict__ weights,
-                                                                   int* __restrict__ left) {
-  __shared__ int hist[4096], waves[EVICT_WAVES], found[2];
-  const int bh = blockIdx.x, b = bh / heads;
-  const int n = max(0, min(lens[b], most)), old = n > keep ? n - recent : 0;  // all stay: none is looked at
-  const float* w = sums + b * sums_b + (bh - b * heads) * sums_h;
-  kept += (size_t)bh * keep;
-  weights += (size_t)bh * keep;
-  if (bh % heads == 0 && threadIdx.x == 0) left[b] = min(n, keep);
-  if (old <= EVICT_SPAN) select_row<true>(w, n, old, keep, recent, kept, weights, hist, waves, found);
-  else select_row<false>(w, n, old, keep, recent, kept, weights, hist, waves, found);
 }
 
 // The kept tokens of each (sequence, head) to the new pages in order: codes and scales as they are.
@@ -506,8 +547,8 @@ int bq_kv4_evict(const bq_kv4_cache* cache, const float* sums, int64_t sums_b, i
   const int64_t blocks = (keep + 4096 / cache->dim - 1) / (4096 / cache->dim);
   if (B * c.heads * blocks > 0x7fffffff) return set_error(BQ_ERR_ARG, "%s: size too large", what);
   hipStream_t st = (hipStream_t)stream;
-  kv4_select_kernel<<<(unsigned)(B * c.heads), EVICT_THREADS, 0, st>>>(sums, sums_b, sums_h, (int)most, c.heads, lens, (int)keep,
-                                                                       (int)recent, kept, weights, left);
+  kv4_select_kernel<<<(unsigned)(B * c.heads), EVICT_THREADS, 0, st>>>(sums, sums_b, sums_h, (int)most, c.heads, lens,
+                                                                       (int)keep, (int)recent, kept, weights, left);
   if (const int rc = check_launch(what)) return rc;
   const unsigned grid = (unsigned)(B * c.heads * blocks);
   if (c.pages == 0) return BQ_OK;
