@@ -117,7 +117,7 @@ SIGNATURES = {
     "bq_prompt_attention_ws_bytes": (_c_size, [_c_int, _c_i64, _c_i64, _c_i64]),
     "bq_kv4_append": (_c_int, [_c_p, _c_p, _c_p, _c_int, *[_c_i64] * 5, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p]),
     "bq_kv4_read": (_c_int, [_c_p, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_p]),
-    "bq_kv4_attend_ws_bytes": (_c_size, [_c_i64] * 5),
+    "bq_kv4_attend_ws_bytes": (_c_size, [*[_c_i64] * 5, _c_int]),
     "bq_kv4_attend": (_c_int, [_c_p, _c_p, _c_int, *[_c_i64] * 5, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_f, _c_p,
                                _c_p, _c_i64, _c_i64, _c_p, _c_size, _c_p]),
     "bq_kv4_evict": (_c_int, [_c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64,

@@ -5,7 +5,7 @@ It is the attention between a decoder's int8 projections when a prompt is read; 
 keys and values for the tokens that follow. Inference only: no gradient."""
 from __future__ import annotations
 
-import math
+from contextlib import nullcontext
 
 import torch
 
@@ -15,6 +15,13 @@ from .int8 import _stream
 __all__ = ["prompt_attention"]
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+SIZES = (4, 2, 2)
+_here = nullcontext()
+
+
+def on(index: int):
+    """The context in which a library call for device ``index`` runs (nothing to do on the current one)."""
+    return _here if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 def type_of(t: torch.Tensor, what: str) -> int:
@@ -24,29 +31,32 @@ def type_of(t: torch.Tensor, what: str) -> int:
     return code
 
 
-def rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` itself where its channels are contiguous and its rows 16-byte aligned, else a copy."""
-    size = t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
-            s * size % 16 == 0 for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+def rows(t: torch.Tensor, code: int):
+    """``t`` itself where its channels are contiguous and its rows 16-byte aligned, else a copy, and
+    the strides of all axes but the last (those of an axis of one count for nothing)."""
+    st = t.stride()
+    if st[-1] == 1:
+        every = t.data_ptr()
+        for s in st[:-1]:
+            every |= s * SIZES[code]
+        if not every & 15:
+            return t, st[:-1]
+        st = [s if n > 1 else 0 for s, n in zip(st[:-1], t.shape)]
+        if t.data_ptr() % 16 == 0 and not any(s * SIZES[code] % 16 for s in st):
+            return t, st
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride()[:-1]
 
 
-def strides(t: torch.Tensor):
-    """Strides of all axes but the last (0 for an axis of one)."""
-    return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)]
-
-
-def ints(t: torch.Tensor, n, what: str, device) -> torch.Tensor:
-    """An int32 index tensor of ``n`` entries on ``device``, contiguous."""
-    if t.dtype != torch.int32:
+def ints(t: torch.Tensor, shape, what: str, index: int) -> torch.Tensor:
+    """An int32 index tensor of ``shape`` on device ``index``, contiguous."""
+    if t.dtype is not torch.int32:
         raise TypeError(f"{what}: expected int32, got {t.dtype}")
-    if t.device != device:
-        raise RuntimeError(f"{what}: on {t.device}, the operands are on {device}")
-    if tuple(t.shape) != tuple(n):
-        raise RuntimeError(f"{what}: expected the shape {tuple(n)}, got {tuple(t.shape)}")
-    return t.contiguous()
+    if t.get_device() != index:
+        raise RuntimeError(f"{what}: on {t.device}, the operands are on cuda:{index}")
+    if t.shape != shape:
+        raise RuntimeError(f"{what}: expected the shape {tuple(shape)}, got {tuple(t.shape)}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, causal: bool = True,
@@ -59,30 +69,35 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
     zeros."""
     require_device(q.device)
     code = type_of(q, "prompt_attention")
-    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+    shape = q.shape
+    if len(shape) != 3 or k.dim() != 3:
         raise RuntimeError("prompt_attention: q, k and v are [tokens, heads, dim]")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    if k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise TypeError(f"prompt_attention: q is {q.dtype}, k {k.dtype}, v {v.dtype}")
-    if k.device != q.device or v.device != q.device:
+    index = q.get_device()
+    if k.get_device() != index or v.get_device() != index:
         raise RuntimeError(f"prompt_attention: q is on {q.device}, k on {k.device}, v on {v.device}")
-    n, hq, dim = q.shape
-    h = k.shape[1]
-    if k.shape != v.shape or k.shape[0] != n or k.shape[2] != dim:
+    n, hq, dim = shape
+    kn, h, kd = k.shape
+    if v.shape != k.shape or kn != n or kd != dim:
         raise RuntimeError(f"prompt_attention: shapes q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
     if h == 0 or hq % h:
         raise RuntimeError(f"prompt_attention: {hq} query heads over {h} key-value heads")
-    if cu.dim() != 1 or cu.shape[0] < 1:
+    B = cu.shape[0] - 1 if cu.dim() == 1 else -1
+    if B < 0:
         raise RuntimeError("prompt_attention: cu holds the sequences' first rows and the end")
-    cu = ints(cu, cu.shape, "cu", q.device)
-    out = torch.empty((n, hq, dim), dtype=q.dtype, device=q.device)
+    cu = ints(cu, (B + 1,), "cu", index)
+    out = torch.empty(shape, dtype=q.dtype, device=q.device)
     if n == 0 or hq == 0:
         return out
-    q, k, v = (x if max(strides(x)) <= 1 << 23 else x.contiguous() for x in (rows(q), rows(k), rows(v)))
-    need = lib().bq_prompt_attention_ws_bytes(code, n, h, dim)
+    (q, qs), (k, ks), (v, vs) = (rows(t, code) for t in (q, k, v))
+    if code and max(ks[0], vs[0]) > 1 << 23:
+        k, v = k.contiguous(), v.contiguous()
+        ks, vs = k.stride()[:2], v.stride()[:2]
+    need = lib().bq_prompt_attention_ws_bytes(code, n, h, dim) if code == 0 else 0
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    with torch.cuda.device(q.device):
-        check(lib().bq_prompt_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), code, n, hq, h, dim, *strides(q),
-                                        *strides(k), *strides(v), cu.data_ptr(), cu.shape[0] - 1, int(causal),
-                                        1.0 / math.sqrt(dim) if scale is None else scale, out.data_ptr(),
-                                        None if ws is None else ws.data_ptr(), need, _stream(q)))
+    with on(index):
+        check(lib().bq_prompt_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), code, n, hq, h, dim, *qs, *ks, *vs,
+                                        cu.data_ptr(), B, int(causal), dim ** -0.5 if scale is None else scale,
+                                        out.data_ptr(), ws.data_ptr() if need else None, need, _stream(q)))
     return out

@@ -122,6 +122,13 @@ __device__ __forceinline__ v8bf codes8(uint32_t w, float scale) {
   return v8bf{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+// 16 bytes of codes, read once a call: past the caches' other contents.
+__device__ __forceinline__ uint4 codes_at(const uint8_t* p) {
+  const v4u x = __builtin_nontemporal_load(reinterpret_cast<const v4u*>(p));
+  return make_uint4(x[0], x[1], x[2], x[3]);
+}
+
 // What a lane loads of 32 tokens' keys: of token 8 (n / 4) + 4 t + n % 4, its quarter g of the
 // channels (row n of score tile t), and the scale bytes of both tiles' tokens.
 template <int DIM>
@@ -135,7 +142,7 @@ struct KBlock {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       if constexpr (DIM == 128) {
-        const uint4 x = *reinterpret_cast<const uint4*>(p + t * 4 * (DIM / 2));
+        const uint4 x = codes_at(p + t * 4 * (DIM / 2));
         w[t][0] = x.x, w[t][1] = x.y, w[t][2] = x.z, w[t][3] = x.w;
       } else {
         const uint2 x = *reinterpret_cast<const uint2*>(p + t * 4 * (DIM / 2));
@@ -178,11 +185,11 @@ struct VBlock {
     if constexpr (DIM == 128) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const uint4 x = *reinterpret_cast<const uint4*>(p + (2 * g + e) * 256 + n * 16);
+        const uint4 x = codes_at(p + (2 * g + e) * 256 + n * 16);
         w[4 * e] = x.x, w[4 * e + 1] = x.y, w[4 * e + 2] = x.z, w[4 * e + 3] = x.w;
       }
     } else {
-      const uint4 x = *reinterpret_cast<const uint4*>(p + g * 256 + n * 16);
+      const uint4 x = codes_at(p + g * 256 + n * 16);
       w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
     }
     const uint2 y = *reinterpret_cast<const uint2*>(c.vs + row * (DIM / 32) + n * (DIM / 32) / 16 * 32 + 8 * g);
@@ -235,17 +242,20 @@ __device__ __forceinline__ float weight_of(float s, float base, float c) {
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
 
 constexpr int UNIT = 128;  // tokens: a block of 32 a wave
+// Places of the line that stand for the beginning and the end of a run (its queries, its pages, the
+// join of the waves): a share of many short runs is not longer than one of few long ones.
+constexpr int EDGE = 3;
 
 __device__ __forceinline__ int len_of(const Attend& a, int b) { return max(0, min(a.lens[b], a.max_len)); }
 __device__ __forceinline__ int units_of(int len) { return max(1, (len + UNIT - 1) / UNIT); }  // an empty one writes zeros
 
-// The line of units, sequence after sequence, per_b (heads times row groups) runs of each: its
-// length, and for `upto` < B the place where that sequence's begin.
+// The line, sequence after sequence, per_b (heads times row groups) runs of each, EDGE places and then
+// its units: its length, and for `upto` < B the place where that sequence's begin.
 __device__ __forceinline__ int line_of(const Attend& a, int per_b, int upto, int* begin) {
   const int lane = threadIdx.x & 63;
   int all = 0, before = 0;
   for (int b = lane; b < a.B; b += 64) {
-    const int u = units_of(len_of(a, b)) * per_b;
+    const int u = (EDGE + units_of(len_of(a, b))) * per_b;
     all += u;
     before += b < upto ? u : 0;
   }
@@ -257,12 +267,12 @@ __device__ __forceinline__ int line_of(const Attend& a, int per_b, int upto, int
   *begin = __builtin_amdgcn_readfirstlane(before);
   return __builtin_amdgcn_readfirstlane(all);
 }
-// The sequence in which place x of the line lies, and where its units begin.
+// The sequence in which place x of the line lies, and where its runs begin.
 __device__ __forceinline__ int sequence_of(const Attend& a, int per_b, int x, int* begin) {
   const int lane = threadIdx.x & 63;
   int from = 0;
   for (int b0 = 0;; b0 += 64) {
-    const int b = b0 + lane, mine = b < a.B ? units_of(len_of(a, b)) * per_b : 0;
+    const int b = b0 + lane, mine = b < a.B ? (EDGE + units_of(len_of(a, b))) * per_b : 0;
     int upto = mine;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -298,15 +308,23 @@ __global__ __launch_bounds__(256, RT == 2 && DIM == 128 && !__is_same(T, __bf16)
     b = sequence_of(a, per_b, x0, &begin);
   } else {
     b = blockIdx.x / per_b;
-    const int units = units_of(len_of(a, b));
+    const int run = EDGE + units_of(len_of(a, b));
     begin = 0;
-    x0 = (blockIdx.x - b * per_b) * units;
-    x1 = x0 + units;
+    x0 = (blockIdx.x - b * per_b) * run;
+    x1 = x0 + run;
   }
   for (int x = x0; x < x1;) {
     const int len = len_of(a, b), units = units_of(len);
-    const int pair = (x - begin) / units, h = pair / a.row_groups, row0 = (pair - h * a.row_groups) * 16 * RT;
-    const int u0 = x - begin - pair * units, u1 = min(units, u0 + x1 - x);
+    const int pair = (x - begin) / (EDGE + units), h = pair / a.row_groups, row0 = (pair - h * a.row_groups) * 16 * RT;
+    const int run = begin + pair * (EDGE + units) + EDGE;  // where this run's units begin
+    const int u0 = max(0, x - run), u1 = min(units, x1 - run);
+    x = run + units;  // the next run
+    const int seq = b;
+    if (x == begin + (EDGE + units) * per_b) {
+      begin = x;
+      ++b;
+    }
+    if (u0 >= u1) continue;  // its beginning only
     const int sure = len - a.tokens + 1;  // tokens that every row sees
     const int blocks = (len + 31) >> 5;
 
@@ -317,7 +335,7 @@ __global__ __launch_bounds__(256, RT == 2 && DIM == 128 && !__is_same(T, __bf16)
     v4f o[RT][NJ];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      q[r].load(a, b, h, row0 + 16 * r);
+      q[r].load(a, seq, h, row0 + 16 * r);
       const int t = fdiv(row0 + 16 * r + n, a.by_group.mul, a.by_group.shift);
       end[r] = min(len, sure + t);
       lost[r] = false;
@@ -332,7 +350,7 @@ __global__ __launch_bounds__(256, RT == 2 && DIM == 128 && !__is_same(T, __bf16)
       const int first = 4 * w0 + wave;
       const int mine = min(min(64, u1 - w0), blocks > first ? (blocks - first + 3) >> 2 : 0);
       int pages = -1;
-      if (lane < mine) pages = kv4_page(a.c, b, fdiv(first + 4 * lane, a.c.by_blocks.mul, a.c.by_blocks.shift));
+      if (lane < mine) pages = kv4_page(a.c, seq, fdiv(first + 4 * lane, a.c.by_blocks.mul, a.c.by_blocks.shift));
       auto fetch = [&](int i, KBlock<DIM>& k, VBlock<DIM>& v) {
         const int blk = first + 4 * i;
         const int at = max(0, __builtin_amdgcn_readlane(pages, i));
@@ -431,9 +449,9 @@ __global__ __launch_bounds__(256, RT == 2 && DIM == 128 && !__is_same(T, __bf16)
     }
 
     // the four waves' rows together: lane (n, g) holds channels DIM / 4 g + DIM / 16 i + j of row n
-    const size_t bh = (size_t)b * a.c.heads + h;
+    const size_t bh = (size_t)seq * a.c.heads + h;
     const bool whole = u0 == 0 && u1 == units;
-    float* part = a.part + ((size_t)2 * blockIdx.x + (x != x0)) * (16 * RT) * (DIM + 2);
+    float* part = a.part + ((size_t)2 * blockIdx.x + (x0 <= run)) * (16 * RT) * (DIM + 2);
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       l[r] = __fadd_rn(l[r], __shfl_xor(l[r], 16));
@@ -477,16 +495,11 @@ __global__ __launch_bounds__(256, RT == 2 && DIM == 128 && !__is_same(T, __bf16)
         } else {
           const float d = sum == 0.f ? 1.f : sum;
           const int t = fdiv(row, a.by_group.mul, a.by_group.shift), j = row - t * a.group;
-          T* to = (T*)a.out + (((size_t)b * a.tokens + t) * a.c.heads * a.group + h * a.group + j) * DIM + c4;
+          T* to = (T*)a.out + (((size_t)seq * a.tokens + t) * a.c.heads * a.group + h * a.group + j) * DIM + c4;
           store4(to, __fdiv_rn(y.x, d), __fdiv_rn(y.y, d), __fdiv_rn(y.z, d), __fdiv_rn(y.w, d));
           if (a.weights && c4 == 0) *reinterpret_cast<float2*>(a.stats + (bh * a.rows + row) * 2) = make_float2(top, d);
         }
       }
-    }
-    x += u1 - u0;
-    if (x == begin + units * per_b) {  // the next sequence
-      begin = x;
-      ++b;
     }
   }
 }
@@ -501,14 +514,14 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attend a) {
   const int rg = row / (16 * RT), units = units_of(len_of(a, b));
   int begin;
   const int share = share_of(a, line_of(a, a.c.heads * a.row_groups, b, &begin));
-  begin += (h * a.row_groups + rg) * units;
+  begin += (h * a.row_groups + rg) * (EDGE + units) + EDGE;
   const int w0 = begin / share, w1 = (begin + units - 1) / share;
   if (w0 == w1) return;  // whole in one share, and written there
   const float* rows = a.part + (size_t)(row - rg * 16 * RT) * (DIM + 2);
   constexpr int C = DIM / 64;
   float top = -INFINITY, sum = 0.f, y[C] = {};
   for (int w = w0 + wave; w <= w1; w += 4) {
-    const float* p = rows + ((size_t)2 * w + (w * share < begin)) * (16 * RT) * (DIM + 2);
+    const float* p = rows + ((size_t)2 * w + (w * share <= begin)) * (16 * RT) * (DIM + 2);
     const float2 ms = *reinterpret_cast<const float2*>(p + DIM);
     float x[C];
 #pragma unroll
@@ -590,24 +603,31 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(Attend a, int blocks) 
   }
 }
 
-// How the work is cut: row tiles a workgroup (of 16), and the shares of the line, 0 for a workgroup a
-// (sequence, head, rows).
+// How the work is cut: row tiles a workgroup (of 16), and the most shares of the line, 0 for a
+// workgroup a (sequence, head, rows): up to LEAST_UNITS units, where the line's second kernel costs more
+// than it saves (300 tokens: 10.3 us, 14.1 cut in shares).
 struct Cut {
   int tiles, row_groups, shares;
 };
+constexpr int MOST_SHARES = 256 * 3;
 constexpr int LEAST_UNITS = 4;
 static Cut cut_of(int64_t B, int64_t heads, int64_t rows, int64_t max_len) {
   Cut c;
   c.tiles = rows <= 16 ? 1 : 2;
   c.row_groups = (int)((rows + 16 * c.tiles - 1) / (16 * c.tiles));
   const int64_t units = (max_len + UNIT - 1) / UNIT;
-  const int64_t line = B * heads * c.row_groups * units, most = 256 * 2;
+  const int64_t line = B * heads * c.row_groups * (EDGE + units), most = MOST_SHARES;
   c.shares = units <= LEAST_UNITS ? 0 : (int)(line < most ? line : most);
   return c;
 }
 
+// As many shares as workgroups run at once: three a CU, two where the registers take more than a third
+// of the file (64 sequences of unlike lengths, bf16, 2 / 3 / 4 a CU: 75, 67, 82 us; two of 131072, f32,
+// 2 / 3 / 4: 66, 75, 76).
 template <typename T, int DIM, int RT>
-static void launch_rows(const Attend& a, hipStream_t st) {
+static void launch_rows(Attend a, hipStream_t st) {
+  constexpr int PER_CU = RT == 1 && (DIM == 64 || __is_same(T, __bf16)) ? 3 : 2;
+  if (a.shares > 256 * PER_CU) a.shares = 256 * PER_CU;
   const unsigned grid = a.shares ? a.shares : a.B * a.c.heads * a.row_groups;
   kv4_attend_kernel<T, DIM, RT><<<grid, 256, 0, st>>>(a);
   if (a.shares) kv4_join_kernel<T, DIM, RT><<<dim3(a.rows, a.c.heads, a.B), 256, 0, st>>>(a);
@@ -628,10 +648,10 @@ static int launch(const char* what, const Attend& a, int tiles, hipStream_t st) 
 
 using namespace bq;
 
-size_t bq_kv4_attend_ws_bytes(int64_t B, int64_t heads, int64_t rows, int64_t dim, int64_t max_len) {
+size_t bq_kv4_attend_ws_bytes(int64_t B, int64_t heads, int64_t rows, int64_t dim, int64_t max_len, int weights) {
   if (B < 1 || heads < 1 || rows < 1 || dim < 1 || max_len < 0) return 0;
   const Cut c = cut_of(B, heads, rows, max_len);
-  return (size_t)B * heads * rows * 8 + (size_t)2 * c.shares * 16 * c.tiles * (dim + 2) * 4;
+  return (weights ? (size_t)B * heads * rows * 8 : 0) + (size_t)2 * c.shares * 16 * c.tiles * (dim + 2) * 4;
 }
 
 int bq_kv4_attend(const bq_kv4_cache* cache, const void* q, int type, int64_t tokens, int64_t q_heads, int64_t q_seq,
@@ -654,14 +674,14 @@ int bq_kv4_attend(const bq_kv4_cache* cache, const void* q, int type, int64_t to
   const int64_t rows = tokens * group;
   if (rows > 1 << 20) return set_error(BQ_ERR_ARG, "%s: size too large", what);
   const Cut cut = cut_of(B, cache->heads, rows, max_len);
-  if (B * cache->heads * cut.row_groups > 0x7fffffff / ((max_len + UNIT - 1) / UNIT + 1))
+  if (B * cache->heads * cut.row_groups > 0x7fffffff / ((max_len + UNIT - 1) / UNIT + 1 + EDGE))
     return set_error(BQ_ERR_ARG, "%s: size too large", what);
   if (!q || !lens || !out) return set_error(BQ_ERR_ARG, "%s: null pointer", what);
   const int64_t size = type == KV4_F32 ? 4 : 2;
   if ((((uintptr_t)q | (uintptr_t)out) & 15) || (q_seq | q_token | q_head) * size % 16)
     return set_error(BQ_ERR_ARG, "%s: rows that are not 16-byte aligned", what);
-  const size_t need = bq_kv4_attend_ws_bytes(B, cache->heads, rows, cache->dim, max_len);
-  if ((weights || cut.shares) && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
+  const size_t need = bq_kv4_attend_ws_bytes(B, cache->heads, rows, cache->dim, max_len, weights != nullptr);
+  if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
     return set_error(BQ_ERR_ARG, "%s: a workspace of %zu bytes, given %zu", what, need, ws ? ws_bytes : 0);
   const int64_t held = cache->pages ? width * cache->page : 0;  // tokens that a sequence's pages have room for
   a.lens = lens;
@@ -675,13 +695,13 @@ int bq_kv4_attend(const bq_kv4_cache* cache, const void* q, int type, int64_t to
   a.row_groups = cut.row_groups;
   a.B = (int)B;
   a.shares = cut.shares;
-  a.least = LEAST_UNITS;
+  a.least = EDGE + LEAST_UNITS;
   a.max_len = (int)(max_len < held ? max_len : held);
   a.by_group = fast_div((uint32_t)group);
   a.scale2 = scale * 1.4426950408889634f;
   a.out = out;
   a.stats = (float*)ws;
-  a.part = a.stats + (size_t)B * cache->heads * rows * 2;
+  a.part = a.stats + (weights ? (size_t)B * cache->heads * rows * 2 : 0);
   a.weights = weights;
   a.wb = w_seq;
   a.wh = w_head;

@@ -7,15 +7,20 @@ of a token share: 4.25 bits a channel, 136 bytes for the keys and values of a to
 from __future__ import annotations
 
 import ctypes
-import math
+import functools
 
 import torch
 
 from ._lib import Kv4Desc, check, lib, require_device
-from .attention import ints, rows, strides, type_of
+from .attention import ints, on, rows, type_of
 from .int8 import _stream
 
 __all__ = ["Cache4"]
+
+
+@functools.lru_cache(maxsize=1024)
+def _attend_ws_bytes(*sizes) -> int:
+    return int(lib().bq_kv4_attend_ws_bytes(*sizes))
 
 
 class Cache4:
@@ -46,7 +51,7 @@ class Cache4:
                 raise RuntimeError(f"Cache4: {name}: expected the shape {(pages, heads, *want)}, got {tuple(t.shape)}")
         self.k, self.k_scales, self.v, self.v_scales = k, k_scales, v, v_scales
         self.pages, self.heads, self.page, self.dim = pages, heads, page, dim
-        self.device = k.device
+        self.device, self._index = k.device, k.get_device()
         self._desc = Kv4Desc(k.data_ptr(), k_scales.data_ptr(), v.data_ptr(), v_scales.data_ptr(), pages, heads, page,
                              dim)
         self._ref = ctypes.addressof(self._desc)
@@ -67,9 +72,10 @@ class Cache4:
         return cls(torch.zeros(k, **u8), torch.ones(ks, **u8), torch.zeros(v, **u8), torch.ones(vs, **u8))
 
     def _table(self, table, lens, what):
-        if table.dim() != 2:
+        shape = table.shape
+        if len(shape) != 2:
             raise RuntimeError(f"{what}: table is [sequences, pages]")
-        return ints(table, table.shape, "table", self.device), ints(lens, table.shape[:1], "lens", self.device)
+        return ints(table, shape, "table", self._index), ints(lens, shape[:1], "lens", self._index), *shape
 
     def append(self, new_k: torch.Tensor, new_v: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
                cu: torch.Tensor) -> None:
@@ -77,33 +83,34 @@ class Cache4:
         rows ``cu[b] .. cu[b + 1]``, the last ones of its ``lens[b]`` tokens (``lens`` counts them)."""
         require_device(self.device)
         code = type_of(new_k, "append")
-        if new_v.dtype != new_k.dtype:
+        if new_v.dtype is not new_k.dtype:
             raise TypeError(f"append: keys are {new_k.dtype}, values {new_v.dtype}")
-        if new_k.shape != new_v.shape or new_k.dim() != 3 or tuple(new_k.shape[1:]) != (self.heads, self.dim):
+        shape = new_k.shape
+        if new_v.shape != shape or shape[1:] != (self.heads, self.dim):
             raise RuntimeError(f"append: keys {tuple(new_k.shape)}, values {tuple(new_v.shape)}, "
                                f"the cache holds {self.heads} heads of {self.dim}")
-        if new_k.device != self.device or new_v.device != self.device:
+        if new_k.get_device() != self._index or new_v.get_device() != self._index:
             raise RuntimeError(f"append: the cache is on {self.device}, keys on {new_k.device}, values on {new_v.device}")
-        table, lens = self._table(table, lens, "append")
-        cu = ints(cu, (table.shape[0] + 1,), "cu", self.device)
-        new_k, new_v = rows(new_k), rows(new_v)
-        with torch.cuda.device(self.device):
-            check(lib().bq_kv4_append(self._ref, new_k.data_ptr(), new_v.data_ptr(), code, new_k.shape[0],
-                                      *strides(new_k), *strides(new_v), table.data_ptr(), *table.shape,
-                                      lens.data_ptr(), cu.data_ptr(), _stream(new_k)))
+        table, lens, B, width = self._table(table, lens, "append")
+        cu = ints(cu, (B + 1,), "cu", self._index)
+        (new_k, ks), (new_v, vs) = rows(new_k, code), rows(new_v, code)
+        with on(self._index):
+            check(lib().bq_kv4_append(self._ref, new_k.data_ptr(), new_v.data_ptr(), code, shape[0], *ks, *vs,
+                                      table.data_ptr(), B, width, lens.data_ptr(), cu.data_ptr(), _stream(new_k)))
 
     def read(self, table: torch.Tensor, lens: torch.Tensor, most: int):
         """The keys and values held, f32 ``[sequences, heads, most, dim]`` each, zeros from
         ``lens[b]`` on."""
         require_device(self.device)
-        table, lens = self._table(table, lens, "read")
+        table, lens, B, width = self._table(table, lens, "read")
         if most < 0:
             raise ValueError(f"read: {most} tokens")
-        shape = (table.shape[0], self.heads, most, self.dim)
-        k, v = (torch.empty(shape, dtype=torch.float32, device=self.device) for _ in range(2))
-        with torch.cuda.device(self.device):
-            check(lib().bq_kv4_read(self._ref, table.data_ptr(), *table.shape, lens.data_ptr(), most, k.data_ptr(),
-                                    v.data_ptr(), _stream(k)))
+        shape = (B, self.heads, most, self.dim)
+        k = torch.empty(shape, dtype=torch.float32, device=self.device)
+        v = torch.empty(shape, dtype=torch.float32, device=self.device)
+        with on(self._index):
+            check(lib().bq_kv4_read(self._ref, table.data_ptr(), B, width, lens.data_ptr(), most, k.data_ptr(), v.data_ptr(),
+                                    _stream(k)))
         return k, v
 
     def attend(self, q: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, max_len: int | None = None,
@@ -117,37 +124,39 @@ class Cache4:
         dim]`` of q's type."""
         require_device(self.device)
         code = type_of(q, "attend")
-        if q.dim() != 4 or q.shape[3] != self.dim or q.shape[2] % self.heads or q.shape[2] == 0:
+        shape = q.shape
+        if len(shape) != 4 or shape[3] != self.dim or shape[2] % self.heads or shape[2] == 0:
             raise RuntimeError(f"attend: q {tuple(q.shape)} is [sequences, tokens, query heads, dim] over "
                                f"{self.heads} key-value heads of {self.dim}")
-        if q.device != self.device:
+        if q.get_device() != self._index:
             raise RuntimeError(f"attend: the cache is on {self.device}, q on {q.device}")
-        table, lens = self._table(table, lens, "attend")
-        B, T, hq, dim = q.shape
-        if B != table.shape[0]:
-            raise RuntimeError(f"attend: {B} sequences of queries, {table.shape[0]} of pages")
-        held = table.shape[1] * self.page
+        table, lens, B, width = self._table(table, lens, "attend")
+        _, T, hq, dim = shape
+        if shape[0] != B:
+            raise RuntimeError(f"attend: {shape[0]} sequences of queries, {B} of pages")
+        held = width * self.page
         max_len = held if max_len is None else max_len
+        w, wb, wh = None, 0, 0
         if weights is not None:
-            if weights.dtype != torch.float32 or weights.device != self.device:
+            if weights.dtype is not torch.float32 or weights.get_device() != self._index:
                 raise TypeError(f"attend: weights are float32 on {self.device}, got {weights.dtype} on {weights.device}")
-            if weights.dim() != 3 or tuple(weights.shape[:2]) != (B, self.heads) or weights.shape[2] < min(max_len, held):
+            if weights.dim() != 3 or weights.shape[:2] != (B, self.heads) or weights.shape[2] < min(max_len, held):
                 raise RuntimeError(f"attend: weights {tuple(weights.shape)} for {B} sequences, {self.heads} heads and "
                                    f"{min(max_len, held)} tokens")
-            if weights.stride(2) != 1 and weights.shape[2] > 1:
+            wb, wh, ws = weights.stride()
+            if ws != 1 and weights.shape[2] > 1:
                 raise RuntimeError("attend: weights of one head have to be contiguous")
-        out = torch.empty((B, T, hq, dim), dtype=q.dtype, device=self.device)
-        if out.numel() == 0:
+            w = weights.data_ptr()
+        out = torch.empty(shape, dtype=q.dtype, device=self.device)
+        if B == 0 or T == 0:
             return out
-        q = rows(q)
-        need = lib().bq_kv4_attend_ws_bytes(B, self.heads, T * (hq // self.heads), dim, max_len)
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-        wb, wh = (weights.stride(0), weights.stride(1)) if weights is not None else (0, 0)
-        with torch.cuda.device(self.device):
-            check(lib().bq_kv4_attend(self._ref, q.data_ptr(), code, T, hq, *strides(q), table.data_ptr(), *table.shape,
-                                      lens.data_ptr(), max_len, 1.0 / math.sqrt(dim) if scale is None else scale,
-                                      out.data_ptr(), None if weights is None else weights.data_ptr(), wb, wh,
-                                      ws.data_ptr(), need, _stream(q)))
+        q, qs = rows(q, code)
+        need = _attend_ws_bytes(B, self.heads, T * (hq // self.heads), dim, max_len, int(w is not None))
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        with on(self._index):
+            check(lib().bq_kv4_attend(self._ref, q.data_ptr(), code, T, hq, *qs, table.data_ptr(), B, width,
+                                      lens.data_ptr(), max_len, dim ** -0.5 if scale is None else scale, out.data_ptr(),
+                                      w, wb, wh, ws.data_ptr() if need else None, need, _stream(q)))
         return out
 
     def evict(self, sums: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, new_table: torch.Tensor, keep: int,
@@ -159,23 +168,24 @@ class Cache4:
         Returns ``kept`` int32 ``[sequences, heads, keep]`` (their former places, -1 past the last),
         their ``weights`` (0 past the last) and ``left`` int32 ``[sequences]``, the new lengths."""
         require_device(self.device)
-        table, lens = self._table(table, lens, "evict")
-        if new_table.dim() != 2 or new_table.shape[0] != table.shape[0]:
-            raise RuntimeError(f"evict: new_table {tuple(new_table.shape)} for {table.shape[0]} sequences")
-        new_table = ints(new_table, new_table.shape, "new_table", self.device)
-        if sums.dtype != torch.float32 or sums.device != self.device:
+        table, lens, B, width = self._table(table, lens, "evict")
+        if new_table.dim() != 2 or new_table.shape[0] != B:
+            raise RuntimeError(f"evict: new_table {tuple(new_table.shape)} for {B} sequences")
+        new_table = ints(new_table, new_table.shape, "new_table", self._index)
+        if sums.dtype is not torch.float32 or sums.get_device() != self._index:
             raise TypeError(f"evict: sums are float32 on {self.device}, got {sums.dtype} on {sums.device}")
-        B = table.shape[0]
-        if sums.dim() != 3 or tuple(sums.shape[:2]) != (B, self.heads):
+        if sums.dim() != 3 or sums.shape[:2] != (B, self.heads):
             raise RuntimeError(f"evict: sums {tuple(sums.shape)} for {B} sequences and {self.heads} heads")
         if sums.stride(2) != 1 and sums.shape[2] > 1:
             sums = sums.contiguous()
-        kept = torch.empty((B, self.heads, max(keep, 0)), dtype=torch.int32, device=self.device)
-        weights = torch.empty((B, self.heads, max(keep, 0)), dtype=torch.float32, device=self.device)
+        if keep < 1:
+            raise ValueError(f"evict: keep {keep}")
+        kept = torch.empty((B, self.heads, keep), dtype=torch.int32, device=self.device)
+        weights = torch.empty((B, self.heads, keep), dtype=torch.float32, device=self.device)
         left = torch.empty(B, dtype=torch.int32, device=self.device)
-        with torch.cuda.device(self.device):
-            check(lib().bq_kv4_evict(self._ref, sums.data_ptr(), sums.stride(0), sums.stride(1), sums.shape[2],
-                                     table.data_ptr(), *table.shape, lens.data_ptr(), new_table.data_ptr(),
-                                     new_table.shape[1], keep, recent, kept.data_ptr(), weights.data_ptr(),
-                                     left.data_ptr(), _stream(kept)))
+        sb, sh, _ = sums.stride()
+        with on(self._index):
+            check(lib().bq_kv4_evict(self._ref, sums.data_ptr(), sb, sh, sums.shape[2], table.data_ptr(), B, width,
+                                     lens.data_ptr(), new_table.data_ptr(), new_table.shape[1], keep, recent,
+                                     kept.data_ptr(), weights.data_ptr(), left.data_ptr(), _stream(kept)))
         return kept, weights, left

@@ -523,8 +523,8 @@ int bq_kv4_append(const bq_kv4_cache* cache, const void* new_k, const void* new_
 int bq_kv4_read(const bq_kv4_cache* cache, const int32_t* table, int64_t B, int64_t width, const int32_t* lens,
                 int64_t most, float* k, float* v, bq_stream_t stream);
 
-/* Workspace bytes of bq_kv4_attend (rows = tokens * q_heads / heads). */
-size_t bq_kv4_attend_ws_bytes(int64_t B, int64_t heads, int64_t rows, int64_t dim, int64_t max_len);
+/* Workspace bytes of bq_kv4_attend (rows = tokens * q_heads / heads; weights: whether it gets any). */
+size_t bq_kv4_attend_ws_bytes(int64_t B, int64_t heads, int64_t rows, int64_t dim, int64_t max_len, int weights);
 
 /* Attention of each sequence's newest `tokens` tokens over the cache: q [B, tokens, q_heads, dim];
  * token t sees the first min(lens[b], max_len) - tokens + 1 + t cached tokens:

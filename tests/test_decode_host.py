@@ -72,9 +72,9 @@ def test_attend_and_evict_refusals():
     assert attend(q=None) == ARG and attend(q=24) == ARG
     assert attend(weights=16) == ARG and "workspace" in _lib.last_error()
     assert attend(tokens=2 ** 21) == ARG
-    need = lib.bq_kv4_attend_ws_bytes(1, 2, 2, 64, 100000)
+    need = lib.bq_kv4_attend_ws_bytes(1, 2, 2, 64, 100000, 0)
     assert need > 0 and attend(max_len=100000, ws=16, ws_bytes=need - 1) == ARG
-    assert lib.bq_kv4_attend_ws_bytes(0, 2, 2, 64, 100) == 0
+    assert lib.bq_kv4_attend_ws_bytes(0, 2, 2, 64, 100, 1) == 0
 
     def evict(keep=4, recent=0, most=8, new_width=1, ptr=None):
         return lib.bq_kv4_evict(r, ptr, 16, 8, most, 16, 1, 2, ptr, 16, new_width, keep, recent, ptr, ptr, ptr, None)
