@@ -95,21 +95,35 @@ __device__ __forceinline__ void load8f(const T* p, float x[8]) {
   }
 }
 
-// q's pieces as the score product's second operand: row 16 tile + n, step s, channels
-// DIM / 4 g + 8 s ..; rows past the last as zeros.
+// q's pieces as the score product's second operand: rows row0 .. + 15, step s, of lane (n, g) row
+// row0 + n, channels DIM / 4 g + 8 s ..; rows past the last as zeros.
 template <typename T, int DIM>
-struct QFrag {
-  Pieces<Q_PIECES<T>> s[DIM / 32];
-  __device__ __forceinline__ void load(const Attend& a, int b, int h, int row0) {
-    const int lane = threadIdx.x & 63, row = row0 + (lane & 15), g = lane >> 4;
-    const int t = fdiv(row, a.by_group.mul, a.by_group.shift), j = row - t * a.group;
-    const T* p = (const T*)a.q + b * a.qb + t * a.qt + (int64_t)(h * a.group + j) * a.qh + DIM / 4 * g;
+__device__ __forceinline__ Pieces<Q_PIECES<T>> q_frag(const Attend& a, int b, int h, int row0, int s) {
+  const int lane = threadIdx.x & 63, row = row0 + (lane & 15), g = lane >> 4;
+  const int t = fdiv(row, a.by_group.mul, a.by_group.shift), j = row - t * a.group;
+  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (row < a.rows)
+    load8f((const T*)a.q + b * a.qb + t * a.qt + (int64_t)(h * a.group + j) * a.qh + DIM / 4 * g + 8 * s, x);
+  return pieces_of<Q_PIECES<T>>(x);
+}
+// The operands of RT row tiles in LDS, once for the four waves (in registers they took a third of
+// them in f32, and a wave a SIMD): a lane reads its own 16 bytes.
+template <typename T, int DIM, int RT>
+struct QTile {
+  uint4 p[RT][DIM / 32][Q_PIECES<T>][64];
+  __device__ __forceinline__ void fill(const Attend& a, int b, int h, int row0) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-    for (int i = 0; i < DIM / 32; ++i) {
-      float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (row < a.rows) load8f(p + 8 * i, x);
-      s[i] = pieces_of<Q_PIECES<T>>(x);
+    for (int i = 0; i < (RT * (DIM / 32) + 3) / 4; ++i) {
+      const int x = 4 * i + wave, r = x / (DIM / 32), s = x % (DIM / 32);
+      if (x >= RT * (DIM / 32)) break;
+      const Pieces<Q_PIECES<T>> f = q_frag<T, DIM>(a, b, h, row0 + 16 * r, s);
+#pragma unroll
+      for (int k = 0; k < Q_PIECES<T>; ++k) p[r][s][k][lane] = __builtin_bit_cast(uint4, f.p[k]);
     }
+  }
+  __device__ __forceinline__ v8bf at(int r, int s, int k) const {
+    return __builtin_bit_cast(v8bf, p[r][s][k][threadIdx.x & 63]);
   }
 };
 
@@ -152,23 +166,27 @@ struct KBlock {
     scales = *reinterpret_cast<const uint16_t*>(c.ks + row * (DIM / 32) + ((n & 3) * (DIM / 32) + g * (DIM / 32) / 4) * 8 +
                                                 2 * (n >> 2));
   }
-  // The scores of 16 rows, before the scale: [4 t + i] is token 8 g + 4 t + i
-  template <typename T>
-  __device__ __forceinline__ void scores(const QFrag<T, DIM>& q, float s[8]) const {
-    constexpr int P = Q_PIECES<T>;
+  // The scores of 16 rows a tile, before the scale: [4 t + i] is token 8 g + 4 t + i
+  template <typename T, int RT>
+  __device__ __forceinline__ void scores(const QTile<T, DIM, RT>& q, float (&s)[RT][8]) const {
+    v8bf kf[2][DIM / 32];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const float f = scale_bits((scales >> (8 * t)) & 255);
-      v4f acc = {0.f, 0.f, 0.f, 0.f};
-      v8bf kf[DIM / 32];
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < DIM / 32; ++i) kf[i] = codes8(w[t][i], f);
+      for (int i = 0; i < DIM / 32; ++i) kf[t][i] = codes8(w[t][i], scale_bits((scales >> (8 * t)) & 255));
 #pragma unroll
-      for (int k = P - 1; k >= 0; --k)  // the smallest pieces first
+    for (int r = 0; r < RT; ++r) {
+      v4f acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-        for (int i = 0; i < DIM / 32; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i], q.s[i].p[k], acc, 0, 0, 0);
+      for (int k = Q_PIECES<T> - 1; k >= 0; --k)  // the smallest pieces first
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[4 * t + i] = acc[i];
+        for (int i = 0; i < DIM / 32; ++i) {
+          const v8bf f = q.at(r, i, k);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t][i], f, acc[t], 0, 0, 0);
+        }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[r][e] = acc[e / 4][e % 4];
     }
   }
 };
@@ -291,10 +309,11 @@ __device__ __forceinline__ int sequence_of(const Attend& a, int per_b, int x, in
 __device__ __forceinline__ int share_of(const Attend& a, int line) { return max(a.least, (line + a.shares - 1) / a.shares); }
 
 template <typename T, int DIM, int RT>
-__global__ __launch_bounds__(256, RT == 2 && DIM == 128 && !__is_same(T, __bf16) ? 1 : 2) void kv4_attend_kernel(Attend a) {
+__global__ __launch_bounds__(256, 2) void kv4_attend_kernel(Attend a) {
   constexpr int PP = P_PIECES<T>, NJ = DIM / 16, PITCH = DIM + 4;
   __shared__ __attribute__((aligned(16))) float so[4][16][PITCH];
   __shared__ float sm[4][16], sl[4][16];
+  __shared__ QTile<T, DIM, RT> q;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const int per_b = a.c.heads * a.row_groups, bpp = a.c.page >> 5;
 
@@ -328,14 +347,13 @@ __global__ __launch_bounds__(256, RT == 2 && DIM == 128 && !__is_same(T, __bf16)
     const int sure = len - a.tokens + 1;  // tokens that every row sees
     const int blocks = (len + 31) >> 5;
 
-    QFrag<T, DIM> q[RT];
-    int end[RT];  // what this lane's row sees
+    q.fill(a, seq, h, row0);  // every wave has left the last run's: the join's barriers
+    int end[RT];              // what this lane's row sees
     bool lost[RT];  // whether it sees a NaN value in its channels that left the products
     float m[RT], l[RT];
     v4f o[RT][NJ];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      q[r].load(a, seq, h, row0 + 16 * r);
       const int t = fdiv(row0 + 16 * r + n, a.by_group.mul, a.by_group.shift);
       end[r] = min(len, sure + t);
       lost[r] = false;
@@ -344,6 +362,8 @@ __global__ __launch_bounds__(256, RT == 2 && DIM == 128 && !__is_same(T, __bf16)
 #pragma unroll
       for (int j = 0; j < NJ; ++j) o[r][j] = v4f{0.f, 0.f, 0.f, 0.f};
     }
+
+    __syncthreads();
 
     // 64 units at a time: this wave's block of each, their pages one a lane
     for (int w0 = u0; w0 < u1; w0 += 64) {
@@ -362,8 +382,7 @@ __global__ __launch_bounds__(256, RT == 2 && DIM == 128 && !__is_same(T, __bf16)
         const int tok = (first + 4 * i) << 5;
         if (__builtin_amdgcn_readlane(pages, i) < 0) return;  // no page: nothing to see
         float s[RT][8];
-#pragma unroll
-        for (int r = 0; r < RT; ++r) kb.template scores<T>(q[r], s[r]);
+        kb.template scores<T, RT>(q, s);
         if (tok + 32 > sure) {
           // The end: what a row does not see gets no weight, and no NaN of it (0 times NaN) may reach the
           // row, so such values leave the products (bit e: token 8 g + e of this lane's slice); past
@@ -520,18 +539,37 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attend a) {
   const float* rows = a.part + (size_t)(row - rg * 16 * RT) * (DIM + 2);
   constexpr int C = DIM / 64;
   float top = -INFINITY, sum = 0.f, y[C] = {};
-  for (int w = w0 + wave; w <= w1; w += 4) {
-    const float* p = rows + ((size_t)2 * w + (w * share <= begin)) * (16 * RT) * (DIM + 2);
-    const float2 ms = *reinterpret_cast<const float2*>(p + DIM);
-    float x[C];
+  auto part_of = [&](int w) { return rows + ((size_t)2 * w + (w * share <= begin)) * (16 * RT) * (DIM + 2); };
+  // up to 64 of this wave's parts at a time: their maxima and sums a lane each, then their rows, whose
+  // loads wait for nothing
+  for (int f0 = w0 + wave; f0 <= w1; f0 += 256) {
+    const int mine = min(64, (w1 - f0) / 4 + 1);
+    float2 ms = make_float2(-INFINITY, 0.f);
+    if (lane < mine) ms = *reinterpret_cast<const float2*>(part_of(f0 + 4 * lane) + DIM);
+    float now = ms.x;
 #pragma unroll
-    for (int c = 0; c < C; ++c) x[c] = p[C * lane + c];
-    const float now = fmaxf(top, ms.x), base = base_of(now);
-    const float f = weight_of(top, base, a.scale2), e = weight_of(ms.x, base, a.scale2);
-    sum = __fmaf_rn(sum, f, __fmul_rn(ms.y, e));
-#pragma unroll
-    for (int c = 0; c < C; ++c) y[c] = __fmaf_rn(y[c], f, __fmul_rn(x[c], e));
+    for (int d = 1; d < 64; d *= 2) now = fmaxf(now, __shfl_xor(now, d));
+    now = fmaxf(now, top);
+    const float base = base_of(now), f = weight_of(top, base, a.scale2), e = weight_of(ms.x, base, a.scale2);
     top = now;
+    sum = __fmaf_rn(sum, f, wave_sum_fixed(__fmul_rn(ms.y, e)));
+#pragma unroll
+    for (int c = 0; c < C; ++c) y[c] = __fmul_rn(y[c], f);
+    for (int i0 = 0; i0 < mine; i0 += 8) {
+      float x[8][C];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float* p = part_of(f0 + 4 * min(i0 + i, mine - 1)) + C * lane;  // past the last: a weight of 0
+#pragma unroll
+        for (int c = 0; c < C; ++c) x[i][c] = p[c];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float ei = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(e), i0 + i));
+#pragma unroll
+        for (int c = 0; c < C; ++c) y[c] = __fmaf_rn(x[i][c], ei, y[c]);
+      }
+    }
   }
   if (lane == 0) sm[wave] = top, sl[wave] = sum;
 #pragma unroll
@@ -558,48 +596,70 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attend a) {
     *reinterpret_cast<float2*>(a.stats + (((size_t)b * a.c.heads + h) * a.rows + row) * 2) = make_float2(now, d);
 }
 
-// What each cached token received, added to its sum: the scores of 32 tokens a wave once more, each
-// row's weight from its final maximum and sum, rows in order.
-template <typename T, int DIM>
-__global__ __launch_bounds__(256) void kv4_weights_kernel(Attend a, int blocks) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  const int blk = blockIdx.x * 4 + wave, h = blockIdx.y, b = blockIdx.z;
-  const int len = max(0, min(a.lens[b], a.max_len)), tok = blk << 5;
-  if (tok >= len) return;
+// What each cached token received, added to its sum: the scores once more, each row's weight from its
+// final maximum and sum. A workgroup takes 32 tokens and its waves the row tiles in turn (several tiles),
+// or 128 tokens (one); the rows of a tile are added over lanes, the tiles of a wave and the waves in order.
+template <typename T, int DIM, bool ONE>
+__global__ __launch_bounds__(256) void kv4_weights_kernel(Attend a) {
+  __shared__ QTile<T, DIM, 1> qs[ONE ? 1 : 4];
+  __shared__ float sums[4][32];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int blk = ONE ? blockIdx.x * 4 + wave : blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int len = len_of(a, b), tok = blk << 5;
+  if ((ONE ? (int)blockIdx.x * 128 : tok) >= len) return;
   const int pi = fdiv(blk, a.c.by_blocks.mul, a.c.by_blocks.shift);
-  const int at = kv4_page(a.c, b, pi);
-  if (at < 0) return;
+  const int at = tok < len ? kv4_page(a.c, b, pi) : -1;
   const size_t bh = (size_t)b * a.c.heads + h;
-  KBlock<DIM> kb;
-  kb.load(a.c, at, h, (blk - pi * (a.c.page >> 5)) << 5);
+  KBlock<DIM> kb = {};
+  if (at >= 0) kb.load(a.c, at, h, (blk - pi * (a.c.page >> 5)) << 5);
+  if constexpr (ONE) {
+    qs[0].fill(a, b, h, 0);
+    __syncthreads();
+  }
   float total[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int row0 = 0; row0 < a.rows; row0 += 16) {
-    QFrag<T, DIM> q;
-    q.load(a, b, h, row0);
+#pragma unroll 1
+  for (int row0 = ONE ? 0 : 16 * wave; row0 < a.rows; row0 += 64) {
     const int row = row0 + n, t = fdiv(row, a.by_group.mul, a.by_group.shift);
     const int end = row < a.rows ? min(len, len - a.tokens + 1 + t) : 0;
     float2 st = make_float2(0.f, 1.f);
     if (row < a.rows) st = *reinterpret_cast<const float2*>(a.stats + (bh * a.rows + row) * 2);
-    float s[8];
-    kb.template scores<T>(q, s);
+    QTile<T, DIM, 1>& q = qs[ONE ? 0 : wave];
+    if constexpr (!ONE) {  // the wave's own
+#pragma unroll
+      for (int s = 0; s < DIM / 32; ++s) {
+        const Pieces<Q_PIECES<T>> f = q_frag<T, DIM>(a, b, h, row0, s);
+#pragma unroll
+        for (int k = 0; k < Q_PIECES<T>; ++k) q.p[0][s][k][lane] = __builtin_bit_cast(uint4, f.p[k]);
+      }
+    }
+    float s[1][8];
+    kb.template scores<T, 1>(q, s);
     const float base = base_of(st.x);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (tok + 8 * g + e < end)
-        total[e] = __fadd_rn(total[e], __fdiv_rn(weight_of(s[e], base, a.scale2), st.y));
+        total[e] = __fadd_rn(total[e], __fdiv_rn(weight_of(s[0][e], base, a.scale2), st.y));
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
 #pragma unroll
     for (int d = 1; d < 16; d *= 2) total[e] = __fadd_rn(total[e], __shfl_xor(total[e], d));
   }
-  float mine = total[0];  // lane n < 8 writes token 8 g + n
+  float mine = total[0];  // lane n < 8: token 8 g + n
 #pragma unroll
   for (int e = 1; e < 8; ++e) mine = n == e ? total[e] : mine;
   const int t = tok + 8 * g + n;
-  if (n < 8 && t < len) {
-    float* to = a.weights + b * a.wb + h * a.wh + t;
-    *to = __fadd_rn(*to, mine);
+  float* to = a.weights + b * a.wb + h * a.wh + t;
+  if constexpr (ONE) {
+    if (n < 8 && t < len && at >= 0) *to = __fadd_rn(*to, mine);
+  } else {
+    if (n < 8) sums[wave][8 * g + n] = mine;
+    __syncthreads();
+    if (wave == 0 && n < 8 && t < len && at >= 0) {
+      const float all = __fadd_rn(__fadd_rn(sums[0][8 * g + n], sums[1][8 * g + n]),
+                                  __fadd_rn(sums[2][8 * g + n], sums[3][8 * g + n]));
+      *to = __fadd_rn(*to, all);
+    }
   }
 }
 
@@ -609,7 +669,7 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(Attend a, int blocks) 
 struct Cut {
   int tiles, row_groups, shares;
 };
-constexpr int MOST_SHARES = 256 * 3;
+constexpr int MOST_SHARES = 256 * 4;
 constexpr int LEAST_UNITS = 4;
 static Cut cut_of(int64_t B, int64_t heads, int64_t rows, int64_t max_len) {
   Cut c;
@@ -621,12 +681,11 @@ static Cut cut_of(int64_t B, int64_t heads, int64_t rows, int64_t max_len) {
   return c;
 }
 
-// As many shares as workgroups run at once: three a CU, two where the registers take more than a third
-// of the file (64 sequences of unlike lengths, bf16, 2 / 3 / 4 a CU: 75, 67, 82 us; two of 131072, f32,
-// 2 / 3 / 4: 66, 75, 76).
+// As many shares as workgroups run at once, by the registers (64 sequences of unlike lengths, bf16,
+// 2 / 3 / 4 a CU: 77, 69, 80 us; two of 131072, f32: 70, 64, 75).
 template <typename T, int DIM, int RT>
 static void launch_rows(Attend a, hipStream_t st) {
-  constexpr int PER_CU = RT == 1 && (DIM == 64 || __is_same(T, __bf16)) ? 3 : 2;
+  constexpr int PER_CU = (RT == 1 ? 3 : 2) + (DIM == 64);
   if (a.shares > 256 * PER_CU) a.shares = 256 * PER_CU;
   const unsigned grid = a.shares ? a.shares : a.B * a.c.heads * a.row_groups;
   kv4_attend_kernel<T, DIM, RT><<<grid, 256, 0, st>>>(a);
@@ -638,8 +697,10 @@ static int launch(const char* what, const Attend& a, int tiles, hipStream_t st) 
   if (tiles == 1) launch_rows<T, DIM, 1>(a, st);
   else launch_rows<T, DIM, 2>(a, st);
   if (a.weights && a.max_len > 0) {
-    const int blocks = (a.max_len + 31) / 32;
-    kv4_weights_kernel<T, DIM><<<dim3((blocks + 3) / 4, a.c.heads, a.B), 256, 0, st>>>(a, blocks);
+    if (a.rows <= 16)
+      kv4_weights_kernel<T, DIM, true><<<dim3((a.max_len + 127) / 128, a.c.heads, a.B), 256, 0, st>>>(a);
+    else
+      kv4_weights_kernel<T, DIM, false><<<dim3((a.max_len + 31) / 32, a.c.heads, a.B), 256, 0, st>>>(a);
   }
   return check_launch(what);
 }
@@ -695,7 +756,7 @@ int bq_kv4_attend(const bq_kv4_cache* cache, const void* q, int type, int64_t to
   a.row_groups = cut.row_groups;
   a.B = (int)B;
   a.shares = cut.shares;
-  a.least = EDGE + LEAST_UNITS;
+  a.least = EDGE + 1;
   a.max_len = (int)(max_len < held ? max_len : held);
   a.by_group = fast_div((uint32_t)group);
   a.scale2 = scale * 1.4426950408889634f;
