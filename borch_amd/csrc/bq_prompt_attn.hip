@@ -12,9 +12,12 @@
 // 4 tokens each, which is what the transposing LDS read takes of v's rows.
 //
 // The 16-bit types multiply as they are and p is rounded to their type (half a step of 2^-8 or
-// 2^-11 on each term, where the output takes one as large). f32 operands are the exact sums of
+// 2^-11 on each term, where the output takes one as large). In f32 p and v are the exact sums of
 // three bf16 pieces (bq_bf16x3.h), of whose nine products the six of weight 2^-18 and above are
-// added. Outputs that do not come out finite are taken again in plain f32 (plain_row), so that
+// added: a small weight on a large value keeps its bits. In the scores only the sum over the channels
+// counts, so q and k are two fp16 pieces each, 22 bits below a power of two of their row (what a
+// channel 2^-14 of the row's largest loses is 2^-38 of that largest), and of the four products three
+// are added: half the matrix work of the bf16 pieces, each product within 3 2^-22. Outputs that do not come out finite are taken again in plain f32 (plain_row), so that
 // infinities and NaN act as f32 has them, and only on the queries that see them.
 #include <math.h>
 
@@ -38,7 +41,8 @@ struct Prompt {
   const int* cu;
   int n, B, heads, group, tiles, causal;
   float scale2;  // scale * log2(e)
-  void* ws;      // f32: the planes of k, then of v
+  void* ws;        // f32: the planes of k, then of v
+  int* exponents;  // and of each row of k
 };
 
 // A workgroup's head and queries.
@@ -86,7 +90,8 @@ __device__ __forceinline__ bool place_of(const Prompt& a, Place* out) {
 
 template <typename T>
 struct Kind {
-  static constexpr int P = sizeof(T) == 4 ? 3 : 1;  // pieces
+  static constexpr int P = sizeof(T) == 4 ? 3 : 1;   // pieces of v and p
+  static constexpr int PK = sizeof(T) == 4 ? 2 : 1;  // of k and q
 };
 
 template <int P>
@@ -113,6 +118,33 @@ __device__ __forceinline__ v16f product(const Frag<Kind<T>::P>& a, const Frag<Ki
   return mma<T>(a.p[0], b.p[0], c);
 }
 
+// The scores' product: two fp16 pieces, the smaller terms first, or one of the 16-bit types.
+template <typename T>
+__device__ __forceinline__ v16f score(const Frag<Kind<T>::PK>& k, const Frag<Kind<T>::PK>& q, v16f c) {
+  if constexpr (Kind<T>::PK == 2) {
+    c = mma<_Float16>(k.p[1], q.p[0], c);
+    c = mma<_Float16>(k.p[0], q.p[1], c);
+    return mma<_Float16>(k.p[0], q.p[0], c);
+  } else {
+    return mma<T>(k.p[0], q.p[0], c);
+  }
+}
+
+// The power of two that takes a row's largest magnitude (as bits) to [2^13, 2^14): its exponent. Rows
+// that are not finite get any; their products are not finite.
+__device__ __forceinline__ int row_exponent(uint32_t peak) { return max((int)(peak >> 23), 1) - 127 - 13; }
+// Two fp16 pieces of x 2^-e.
+__device__ __forceinline__ Frag<2> halves(const float x[8], int e) {
+  v8h hi, lo;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float y = __builtin_ldexpf(x[i], -e);
+    hi[i] = (_Float16)y;
+    lo[i] = (_Float16)__fsub_rn(y, (float)hi[i]);
+  }
+  return Frag<2>{{__builtin_bit_cast(v8s, hi), __builtin_bit_cast(v8s, lo)}};
+}
+
 // Eight floats as one operand.
 template <typename T>
 __device__ __forceinline__ Frag<Kind<T>::P> frag_of(const float x[8]) {
@@ -133,28 +165,12 @@ __device__ __forceinline__ Frag<Kind<T>::P> frag_of(const float x[8]) {
   return f;
 }
 
-// Eight elements as loaded.
+// Eight elements.
 template <typename T>
-struct Piece {
-  uint4 x[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T* p) {
-    x[0] = *reinterpret_cast<const uint4*>(p);
-    if constexpr (sizeof(T) == 4) x[1] = *reinterpret_cast<const uint4*>(p + 4);
-  }
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (uint4& v : x) v = make_uint4(0, 0, 0, 0);
-  }
-  __device__ __forceinline__ Frag<Kind<T>::P> frag() const {
-    if constexpr (sizeof(T) == 4) {
-      const float y[8] = {__uint_as_float(x[0].x), __uint_as_float(x[0].y), __uint_as_float(x[0].z), __uint_as_float(x[0].w),
-                          __uint_as_float(x[1].x), __uint_as_float(x[1].y), __uint_as_float(x[1].z), __uint_as_float(x[1].w)};
-      return frag_of<T>(y);
-    } else {
-      return Frag<1>{{__builtin_bit_cast(v8s, x[0])}};
-    }
-  }
-};
+__device__ __forceinline__ void load8(const T* p, float x[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
 
 // Where a 16-byte piece of a row lies in a staged tile. k's rows are read 16 at a time at one
 // piece, v's four at a time over four pieces (64 bytes): XORed so that either covers all 64 banks.
@@ -292,38 +308,51 @@ __device__ __attribute__((noinline)) bool clear_values(unsigned char* v, int* fo
   return seen;
 }
 
-// k's and v's planes of bf16 pieces, [piece][head][row][dim]: once a call, where
-// every workgroup would split its tiles again.
+// k's two planes and exponents and v's three planes, [piece][head][row][dim]: once a call, where every
+// workgroup would split its tiles again.
 template <int DIM>
 __global__ __launch_bounds__(256) void prompt_split_kernel(Prompt a) {
   constexpr int LANES = DIM / 8;
-  const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int piece = x % LANES;
-  const uint32_t rest = (uint32_t)(x / LANES), i = rest / (uint32_t)(2 * a.heads);
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int piece = id % LANES;
+  const uint32_t rest = (uint32_t)(id / LANES), i = rest / (uint32_t)(2 * a.heads);
   const int w = rest - i * (2 * a.heads), h = w % a.heads;
-  if (i >= (uint32_t)a.n) return;
+  if (i >= (uint32_t)a.n) return;  // whole rows
   const bool is_v = w >= a.heads;
-  const float* p = is_v ? (const float*)a.v + i * a.vt + h * a.vh : (const float*)a.k + i * a.kt + h * a.kh;
-  const float4 y0 = *reinterpret_cast<const float4*>(p + 8 * piece), y1 = *reinterpret_cast<const float4*>(p + 8 * piece + 4);
-  const Split8 f = split8(y0, y1);
-  const size_t plane = (size_t)a.heads * a.n * DIM;
-  short* to = (short*)a.ws + (is_v ? 3 * plane : 0) + ((size_t)h * a.n + i) * DIM + 8 * piece;
-  *reinterpret_cast<v8bf*>(to) = f.p1;
-  *reinterpret_cast<v8bf*>(to + plane) = f.p2;
-  *reinterpret_cast<v8bf*>(to + 2 * plane) = f.p3;
+  float x[8];
+  load8((is_v ? (const float*)a.v + i * a.vt + h * a.vh : (const float*)a.k + i * a.kt + h * a.kh) + 8 * piece, x);
+  uint32_t peak = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) peak = max(peak, __float_as_uint(x[j]) & 0x7fffffffu);
+#pragma unroll
+  for (int d = 1; d < LANES; d *= 2) peak = max(peak, (uint32_t)__shfl_xor((int)peak, d));
+  const size_t plane = (size_t)a.heads * a.n * DIM, row = (size_t)h * a.n + i;
+  short* to = (short*)a.ws + (is_v ? 2 * plane : 0) + row * DIM + 8 * piece;
+  if (is_v) {
+    const Frag<3> f = frag_of<float>(x);
+#pragma unroll
+    for (int e = 0; e < 3; ++e) *reinterpret_cast<v8s*>(to + e * plane) = f.p[e];
+  } else {
+    const int e = row_exponent(peak);
+    const Frag<2> f = halves(x, e);
+    *reinterpret_cast<v8s*>(to) = f.p[0];
+    *reinterpret_cast<v8s*>(to + plane) = f.p[1];
+    if (piece == 0) a.exponents[row] = e;
+  }
 }
 
 // Tiles of KT keys and values come straight into LDS, rows past the sequence's end as zeros. The
 // 16-bit types hold two tiles, the next one's loads under this one's products, one barrier a tile.
-// f32 holds one (48 KB of planes at dim 128, so that two workgroups share a CU): the next keys load
+// f32 holds one (40 KB of planes at dim 128, so that two workgroups share a CU): the next keys load
 // under this tile's second product, the next values under the next tile's first, two barriers.
 template <typename T, int DIM>
 __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) {
-  constexpr int P = Kind<T>::P, KT = P == 3 ? 32 : 64, SUB = KT / 32, BUFS = P == 3 ? 1 : 2;
+  constexpr int P = Kind<T>::P, PK = Kind<T>::PK, KT = P == 3 ? 32 : 64, SUB = KT / 32, BUFS = P == 3 ? 1 : 2;
   constexpr int STEPS = DIM / 16, VT = DIM / 32, PLANE = KT * DIM * 2;
   constexpr int ROWS = 1024 / (DIM * 2);         // of a wave's load
   constexpr int PER = KT / ROWS / PROMPT_WAVES;  // loads a wave and plane
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[BUFS * 2 * P * PLANE];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[BUFS * (PK + P) * PLANE];
+  __shared__ __attribute__((aligned(16))) int exponents[32];  // f32: of the tile's keys
   __shared__ int found[KT];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hh = lane >> 5;
   Place at;
@@ -341,7 +370,7 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
   const char *k, *v;
   if constexpr (P == 3) {
     k = (const char*)a.ws + ((size_t)h * a.n + at.start) * (DIM * 2);
-    v = k + 3 * plane;
+    v = k + 2 * plane;
   } else {
     k = (const char*)((const T*)a.k + (int64_t)at.start * a.kt + h * a.kh);
     v = (const char*)((const T*)a.v + (int64_t)at.start * a.vt + h * a.vh);
@@ -355,24 +384,44 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
     ko[e] = r * ktb + (k_at<DIM>(r, slot) & (DIM * 2 - 1));
     vo[e] = r * vtb + (v_at<DIM>(r, slot) & (DIM * 2 - 1));
   }
-  auto fetch = [&](const char* from, int stride, const uint32_t (&off)[PER], int t0, uint32_t to) {
+  auto fetch = [&](const char* from, int planes, int stride, const uint32_t (&off)[PER], int t0, uint32_t to) {
     const uint32_t bytes = (uint32_t)min((int64_t)(len - 1 - t0) * stride + DIM * 2, (int64_t)0x7fffffff);
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
+    for (int p = 0; p < planes; ++p) {
       const __amdgpu_buffer_rsrc_t r = make_rsrc(from + p * plane + (int64_t)t0 * stride, bytes);
 #pragma unroll
       for (int e = 0; e < PER; ++e) dma16(r, off[e], to + p * PLANE + (wave * PER + e) * 1024);
     }
   };
-  Frag<P> qf[STEPS];
-  const T* q = (const T*)a.q + (int64_t)(at.start + row) * a.qt + at.head * a.qh;
+  Frag<PK> qf[STEPS];
+  float c2 = a.scale2;  // f32: times the power of two of this lane's query, whose scores are in it
+  const T* q = (const T*)a.q + (int64_t)(at.start + row) * a.qt + at.head * a.qh + 8 * hh;
+  if constexpr (PK == 2) {
+    float x[STEPS][8];
+    uint32_t peak = 0;
 #pragma unroll
-  for (int s = 0; s < STEPS; ++s) {
-    Piece<T> x;
-    x.clear();
-    if (row < len) x.load(q + 16 * s + 8 * hh);
-    qf[s] = x.frag();
+    for (int s = 0; s < STEPS; ++s) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[s][i] = 0.f;
+      if (row < len) load8(q + 16 * s, x[s]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) peak = max(peak, __float_as_uint(x[s][i]) & 0x7fffffffu);
+    }
+    peak = max(peak, (uint32_t)__shfl_xor((int)peak, 32));
+    const int e = row_exponent(peak);
+    c2 = __builtin_ldexpf(a.scale2, e);
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) qf[s] = halves(x[s], e);
+  } else {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (row < len) x = *reinterpret_cast<const uint4*>(q + 16 * s);
+      qf[s].p[0] = __builtin_bit_cast(v8s, x);
+    }
   }
+  const int* row_e = PK == 2 ? a.exponents + (size_t)h * a.n + at.start : nullptr;
+  auto exponent = [&](int t0) { return PK == 2 && threadIdx.x < 32 && t0 + (int)threadIdx.x < len ? row_e[t0 + threadIdx.x] : 0; };
   float m, l;
   v16f o[VT];
   // Once; and where an output is not finite once more, with the values that are not out of the tiles
@@ -384,27 +433,32 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
 #pragma unroll
     for (int d = 0; d < VT; ++d) o[d] = zeros16();
     if (keys > 0) {
-      fetch(k, ktb, ko, 0, lds0);
-      if constexpr (BUFS == 2) fetch(v, vtb, vo, 0, lds0 + P * PLANE);
+      fetch(k, PK, ktb, ko, 0, lds0);
+      if constexpr (BUFS == 2) fetch(v, P, vtb, vo, 0, lds0 + PK * PLANE);
     }
 
+    int e_next = exponent(0);  // loaded with the keys, put in LDS when they are there
     for (int t0 = 0, buf = 0; t0 < keys; t0 += KT, buf ^= BUFS - 1) {
       wait_dma_all();
+      if (PK == 2 && threadIdx.x < 32) exponents[threadIdx.x] = e_next;
       wait_lds();
       barrier();  // the keys are there (both buffers: the values too), what is loaded over is read
-      const unsigned char *tk = lds + buf * 2 * P * PLANE, *tv = tk + P * PLANE;
+      const unsigned char *tk = lds + buf * (PK + P) * PLANE, *tv = tk + PK * PLANE;
       auto middle = [&]() {  // f32: the values are there, the keys read
         wait_dma_all();
         wait_lds();
         barrier();
-        if (t0 + KT < keys) fetch(k, ktb, ko, t0 + KT, lds0);
+        if (t0 + KT < keys) {
+          fetch(k, PK, ktb, ko, t0 + KT, lds0);
+          e_next = exponent(t0 + KT);
+        }
       };
       if constexpr (BUFS == 1) {
-        fetch(v, vtb, vo, t0, lds0 + P * PLANE);
+        fetch(v, P, vtb, vo, t0, lds0 + PK * PLANE);
       } else if (t0 + KT < keys) {
-        const uint32_t to = lds0 + (buf ^ 1) * 2 * P * PLANE;
-        fetch(k, ktb, ko, t0 + KT, to);
-        fetch(v, vtb, vo, t0 + KT, to + P * PLANE);
+        const uint32_t to = lds0 + (buf ^ 1) * (PK + P) * PLANE;
+        fetch(k, PK, ktb, ko, t0 + KT, to);
+        fetch(v, P, vtb, vo, t0 + KT, to + PK * PLANE);
       }
       const bool clears = again && (t0 + KT > len || (a.causal && t0 + KT > q0 + 1));
       if (t0 >= wkeys) {
@@ -420,11 +474,31 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
         s[u] = zeros16();
 #pragma unroll
         for (int e = 0; e < STEPS; ++e) {
-          Frag<P> kf;
+          Frag<PK> kf;
 #pragma unroll
-          for (int p = 0; p < P; ++p)
+          for (int p = 0; p < PK; ++p)
             kf.p[p] = *reinterpret_cast<const v8s*>(tk + p * PLANE + k_at<DIM>(32 * u + n, 2 * e + hh));
-          s[u] = product<T>(kf, qf[e], s[u]);
+          s[u] = score<T>(kf, qf[e], s[u]);
+        }
+      }
+
+      if constexpr (PK == 2) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);  // the next step's fragments under this one's products
+#pragma unroll
+        for (int i = 0; i < STEPS - 2; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int4 e = *reinterpret_cast<const int4*>(exponents + 8 * i + 4 * hh);
+          s[0][4 * i] = __builtin_ldexpf(s[0][4 * i], e.x);
+          s[0][4 * i + 1] = __builtin_ldexpf(s[0][4 * i + 1], e.y);
+          s[0][4 * i + 2] = __builtin_ldexpf(s[0][4 * i + 2], e.z);
+          s[0][4 * i + 3] = __builtin_ldexpf(s[0][4 * i + 3], e.w);
         }
       }
 
@@ -439,26 +513,26 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
 #pragma unroll
       for (int i = 1; i < 16 * SUB; ++i) top = fmaxf(top, s[i / 16][i % 16]);
       top = fmaxf(top, __shfl_xor(top, 32));
-      const bool grew = __fmul_rn(__fsub_rn(top, m), a.scale2) > 8.f;
+      const bool grew = __fmul_rn(__fsub_rn(top, m), c2) > 8.f;
       if (__any(grew)) {
         // the 16-bit types subtract the rounded product (below), and so does the factor between two
-        const float to = grew ? top : m, shift = -__fmul_rn(to, a.scale2);
+        const float to = grew ? top : m, shift = -__fmul_rn(to, c2);
         const float f = !grew ? 1.f
-                              : __builtin_amdgcn_exp2f(P == 3 ? __fmul_rn(__fsub_rn(m, top), a.scale2)
-                                                              : __fadd_rn(shift, __fmul_rn(m, a.scale2)));
+                              : __builtin_amdgcn_exp2f(P == 3 ? __fmul_rn(__fsub_rn(m, top), c2)
+                                                              : __fadd_rn(shift, __fmul_rn(m, c2)));
         m = to;
         l = __fmul_rn(l, f);
 #pragma unroll
         for (int d = 0; d < VT; ++d) o[d] *= f;
       }
-      const float base = m == -INFINITY ? 0.f : m, shift = -__fmul_rn(base, a.scale2);
+      const float base = m == -INFINITY ? 0.f : m, shift = -__fmul_rn(base, c2);
 #pragma unroll
       for (int i = 0; i < 16 * SUB; ++i) {
         float x = s[i / 16][i % 16];
         // f32 subtracts the maximum first. The 16-bit types take one FMA (8192 tokens 560 -> 547 us): the
         // rounding of `shift` is a factor common to the row, which cancels while it stays near 1; beyond
         // 2^24 (scores that large) the row is taken again.
-        x = P == 3 ? __fmul_rn(__fsub_rn(x, base), a.scale2) : __fmaf_rn(x, a.scale2, shift);
+        x = P == 3 ? __fmul_rn(__fsub_rn(x, base), c2) : __fmaf_rn(x, c2, shift);
         s[i / 16][i % 16] = x = __builtin_amdgcn_exp2f(x);
         l = __fadd_rn(l, x);
       }
@@ -476,6 +550,17 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
         const Frag<P> pf = frag_of<T>(x);
 #pragma unroll
         for (int d = 0; d < VT; ++d) o[d] = product<T>(v_frag<DIM, P>(tv, PLANE, d, e), pf, o[d]);
+      }
+      if constexpr (P == 3) {  // the same, the weights' splitting between
+        __builtin_amdgcn_sched_group_barrier(0x100, 12, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 80, 0);
+#pragma unroll
+        for (int i = 0; i < 6 * (2 * VT - 2); ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 12, 0);
       }
     }
     l = __fadd_rn(l, __shfl_xor(l, 32));
@@ -499,7 +584,7 @@ using namespace bq;
 
 size_t bq_prompt_attention_ws_bytes(int type, int64_t n, int64_t heads, int64_t dim) {
   if (type != 0 || n < 1 || heads < 1 || dim < 1) return 0;
-  return (size_t)12 * n * heads * dim;  // three planes of k and of v
+  return (size_t)n * heads * (10 * dim + 4);  // two planes of k, three of v, an exponent a row of k
 }
 
 int bq_prompt_attention(const void* q, const void* k, const void* v, int type, int64_t n, int64_t q_heads,
@@ -531,7 +616,8 @@ int bq_prompt_attention(const void* q, const void* k, const void* v, int type, i
   if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
     return set_error(BQ_ERR_ARG, "%s: a workspace of %zu bytes, given %zu", what, need, ws ? ws_bytes : 0);
   const Prompt a = {q, k, v, out, q_token, q_head, k_token, k_head, v_token, v_head, cu, (int)n, (int)B, (int)heads,
-                    (int)(q_heads / heads), (int)tiles, causal ? 1 : 0, scale * 1.4426950408889634f, ws};
+                    (int)(q_heads / heads), (int)tiles, causal ? 1 : 0, scale * 1.4426950408889634f, ws,
+                    (int*)((char*)ws + (size_t)10 * n * heads * dim)};
   const unsigned grid = (unsigned)(tiles * q_heads);
   hipStream_t st = (hipStream_t)stream;
   const bool wide = dim == 128;
