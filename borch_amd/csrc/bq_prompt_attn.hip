@@ -31,7 +31,6 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef short v8s __attribute__((ext_vector_type(8)));
 
-constexpr int PROMPT_ROWS = 128;  // queries a workgroup
 constexpr int PROMPT_WAVES = 4;
 
 struct Prompt {
@@ -55,6 +54,7 @@ struct Place {
 // side; with a multiple of 8 heads each XCD (ids modulo 8) keeps to its own. A place is a tile of
 // what lies before cu[0], of each sequence in turn, or of what lies past the last. False: the grid
 // has more workgroups than there are tiles.
+template <int ROWS>  // of a place
 __device__ __forceinline__ bool place_of(const Prompt& a, Place* out) {
   const int heads = a.heads * a.group, lane = threadIdx.x & 63;
   int head = blockIdx.x % heads;
@@ -67,7 +67,7 @@ __device__ __forceinline__ bool place_of(const Prompt& a, Place* out) {
       s = i == 0 ? 0 : min(max(a.cu[i - 1], 0), a.n);
       e = i == a.B + 1 ? a.n : min(max(a.cu[i], 0), a.n);
     }
-    const int mine = max(0, e - s + PROMPT_ROWS - 1) / PROMPT_ROWS;
+    const int mine = max(0, e - s + ROWS - 1) / ROWS;
     int upto = mine;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -80,7 +80,7 @@ __device__ __forceinline__ bool place_of(const Prompt& a, Place* out) {
       // one value for the wave, in scalar registers
       const int start = __builtin_amdgcn_readlane(s, at), end = __builtin_amdgcn_readlane(e, at);
       place -= __builtin_amdgcn_readlane(upto - mine, at);
-      *out = Place{head, start, end - start, place * PROMPT_ROWS, base + at > 0 && base + at <= a.B};
+      *out = Place{head, start, end - start, place * ROWS, base + at > 0 && base + at <= a.B};
       return true;
     }
     place -= __builtin_amdgcn_readlane(upto, 63);
@@ -345,9 +345,13 @@ __global__ __launch_bounds__(256) void prompt_split_kernel(Prompt a) {
 // 16-bit types hold two tiles, the next one's loads under this one's products, one barrier a tile.
 // f32 holds one (40 KB of planes at dim 128, so that two workgroups share a CU): the next keys load
 // under this tile's second product, the next values under the next tile's first, two barriers.
-template <typename T, int DIM>
+// PARTS = 2 (16-bit types): 64 queries a workgroup, and two waves take one half of each tile's keys each
+// for the same 32 queries, joined in LDS at the end: twice the workgroups, each half as long, where 128
+// queries a workgroup leave the GPU part empty.
+template <typename T, int DIM, int PARTS>
 __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) {
-  constexpr int P = Kind<T>::P, PK = Kind<T>::PK, KT = P == 3 ? 32 : 64, SUB = KT / 32, BUFS = P == 3 ? 1 : 2;
+  constexpr int P = Kind<T>::P, PK = Kind<T>::PK, KT = P == 3 ? 32 : 64, SUB = KT / 32 / PARTS, BUFS = P == 3 ? 1 : 2;
+  constexpr int ALL = 32 * PROMPT_WAVES / PARTS;  // queries a workgroup
   constexpr int STEPS = DIM / 16, VT = DIM / 32, PLANE = KT * DIM * 2;
   constexpr int ROWS = 1024 / (DIM * 2);         // of a wave's load
   constexpr int PER = KT / ROWS / PROMPT_WAVES;  // loads a wave and plane
@@ -356,11 +360,11 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
   __shared__ int found[KT];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hh = lane >> 5;
   Place at;
-  if (!place_of(a, &at)) return;
+  if (!place_of<ALL>(a, &at)) return;
   const int len = at.len, q0 = at.q0;
-  const int qw = q0 + wave * 32, row = qw + n;  // the wave's first query, this lane's
+  const int part = wave % PARTS, qw = q0 + wave / PARTS * 32, row = qw + n;  // the wave's first query, this lane's
   const int h = at.head / a.group;
-  const int keys = !at.keys ? 0 : a.causal ? min(len, q0 + PROMPT_ROWS) : len;  // that the workgroup sees
+  const int keys = !at.keys ? 0 : a.causal ? min(len, q0 + ALL) : len;  // that the workgroup sees
   const int wkeys = a.causal ? min(keys, qw + 32) : keys;                      // that the wave does
   const int sees = a.causal ? min(len, row + 1) : len;                         // that the lane does
 
@@ -394,7 +398,7 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
     }
   };
   Frag<PK> qf[STEPS];
-  float c2 = a.scale2;  // f32: times the power of two of this lane's query, whose scores are in it
+  int q_e = 0;  // f32: the exponent of this lane's query
   const T* q = (const T*)a.q + (int64_t)(at.start + row) * a.qt + at.head * a.qh + 8 * hh;
   if constexpr (PK == 2) {
     float x[STEPS][8];
@@ -408,10 +412,9 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
       for (int i = 0; i < 8; ++i) peak = max(peak, __float_as_uint(x[s][i]) & 0x7fffffffu);
     }
     peak = max(peak, (uint32_t)__shfl_xor((int)peak, 32));
-    const int e = row_exponent(peak);
-    c2 = __builtin_ldexpf(a.scale2, e);
+    q_e = row_exponent(peak);
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) qf[s] = halves(x[s], e);
+    for (int s = 0; s < STEPS; ++s) qf[s] = halves(x[s], q_e);
   } else {
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
@@ -461,11 +464,15 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
         fetch(v, P, vtb, vo, t0 + KT, to + PK * PLANE);
       }
       const bool clears = again && (t0 + KT > len || (a.causal && t0 + KT > q0 + 1));
-      if (t0 >= wkeys) {
+      const int tw = t0 + 32 * SUB * part;  // this wave's first key of the tile
+      if (tw >= wkeys) {
         if constexpr (BUFS == 1) middle();
         if (clears) clear_values<T, DIM, KT>(const_cast<unsigned char*>(tv), found, 0);
         continue;
       }
+
+      tk += part * 32 * SUB * DIM * 2;
+      tv += part * 32 * SUB * DIM * 2;
 
       // S^T = k q^T
       v16f s[SUB];
@@ -495,51 +502,51 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int4 e = *reinterpret_cast<const int4*>(exponents + 8 * i + 4 * hh);
-          s[0][4 * i] = __builtin_ldexpf(s[0][4 * i], e.x);
-          s[0][4 * i + 1] = __builtin_ldexpf(s[0][4 * i + 1], e.y);
-          s[0][4 * i + 2] = __builtin_ldexpf(s[0][4 * i + 2], e.z);
-          s[0][4 * i + 3] = __builtin_ldexpf(s[0][4 * i + 3], e.w);
+          s[0][4 * i] = __builtin_ldexpf(s[0][4 * i], e.x + q_e);
+          s[0][4 * i + 1] = __builtin_ldexpf(s[0][4 * i + 1], e.y + q_e);
+          s[0][4 * i + 2] = __builtin_ldexpf(s[0][4 * i + 2], e.z + q_e);
+          s[0][4 * i + 3] = __builtin_ldexpf(s[0][4 * i + 3], e.w + q_e);
         }
       }
 
       // softmax, one step. The maximum that is subtracted lags by up to 2^8 (the weights' own size
       // cancels in the quotient), so that most steps rescale nothing.
-      const bool edge = t0 + KT > len || (a.causal && t0 + KT > qw + 1);
+      const bool edge = tw + 32 * SUB > len || (a.causal && tw + 32 * SUB > qw + 1);
       if (edge)
 #pragma unroll
         for (int i = 0; i < 16 * SUB; ++i)
-          if (t0 + 32 * (i / 16) + 8 * (i % 16 / 4) + 4 * hh + i % 4 >= sees) s[i / 16][i % 16] = -INFINITY;
+          if (tw + 32 * (i / 16) + 8 * (i % 16 / 4) + 4 * hh + i % 4 >= sees) s[i / 16][i % 16] = -INFINITY;
       float top = s[0][0];
 #pragma unroll
       for (int i = 1; i < 16 * SUB; ++i) top = fmaxf(top, s[i / 16][i % 16]);
       top = fmaxf(top, __shfl_xor(top, 32));
-      const bool grew = __fmul_rn(__fsub_rn(top, m), c2) > 8.f;
+      const bool grew = __fmul_rn(__fsub_rn(top, m), a.scale2) > 8.f;
       if (__any(grew)) {
         // the 16-bit types subtract the rounded product (below), and so does the factor between two
-        const float to = grew ? top : m, shift = -__fmul_rn(to, c2);
+        const float to = grew ? top : m, shift = -__fmul_rn(to, a.scale2);
         const float f = !grew ? 1.f
-                              : __builtin_amdgcn_exp2f(P == 3 ? __fmul_rn(__fsub_rn(m, top), c2)
-                                                              : __fadd_rn(shift, __fmul_rn(m, c2)));
+                              : __builtin_amdgcn_exp2f(P == 3 ? __fmul_rn(__fsub_rn(m, top), a.scale2)
+                                                              : __fadd_rn(shift, __fmul_rn(m, a.scale2)));
         m = to;
         l = __fmul_rn(l, f);
 #pragma unroll
         for (int d = 0; d < VT; ++d) o[d] *= f;
       }
-      const float base = m == -INFINITY ? 0.f : m, shift = -__fmul_rn(base, c2);
+      const float base = m == -INFINITY ? 0.f : m, shift = -__fmul_rn(base, a.scale2);
 #pragma unroll
       for (int i = 0; i < 16 * SUB; ++i) {
         float x = s[i / 16][i % 16];
         // f32 subtracts the maximum first. The 16-bit types take one FMA (8192 tokens 560 -> 547 us): the
         // rounding of `shift` is a factor common to the row, which cancels while it stays near 1; beyond
         // 2^24 (scores that large) the row is taken again.
-        x = P == 3 ? __fmul_rn(__fsub_rn(x, base), c2) : __fmaf_rn(x, c2, shift);
+        x = P == 3 ? __fmul_rn(__fsub_rn(x, base), a.scale2) : __fmaf_rn(x, a.scale2, shift);
         s[i / 16][i % 16] = x = __builtin_amdgcn_exp2f(x);
         l = __fadd_rn(l, x);
       }
       if constexpr (P == 1) odd |= fabsf(shift) > 0x1p24f;
       if constexpr (BUFS == 1) middle();
 
-      if (clears) odd |= clear_values<T, DIM, KT>(const_cast<unsigned char*>(tv), found, sees - t0);
+      if (clears) odd |= clear_values<T, DIM, KT>(const_cast<unsigned char*>(tv) - part * 32 * SUB * DIM * 2, found, sees - t0);
 
       // O^T += v^T p^T
 #pragma unroll
@@ -563,6 +570,30 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
         __builtin_amdgcn_sched_group_barrier(0x008, 12, 0);
       }
     }
+    if constexpr (PARTS == 2) {  // the two halves' sums, in the place of the tiles
+      float* to = reinterpret_cast<float*>(lds) + (wave >> 1) * (16 * VT + 3) * 64 + lane;
+      wait_lds();
+      barrier();
+      if (part == 1) {
+        to[0] = m;
+        to[64] = l;
+        to[128] = odd ? 1.f : 0.f;
+#pragma unroll
+        for (int i = 0; i < 16 * VT; ++i) to[(3 + i) * 64] = o[i / 16][i % 16];
+      }
+      wait_lds();
+      barrier();
+      if (part == 0) {
+        const float m1 = to[0], now = fmaxf(m, m1), shift = -__fmul_rn(now, a.scale2);
+        const float f0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(__fadd_rn(shift, __fmul_rn(m, a.scale2)));
+        const float f1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(__fadd_rn(shift, __fmul_rn(m1, a.scale2)));
+        l = __fmaf_rn(l, f0, __fmul_rn(to[64], f1));
+        odd |= to[128] != 0.f;
+#pragma unroll
+        for (int i = 0; i < 16 * VT; ++i)
+          o[i / 16][i % 16] = __fmaf_rn(o[i / 16][i % 16], f0, __fmul_rn(to[(3 + i) * 64], f1));
+      }
+    }
     l = __fadd_rn(l, __shfl_xor(l, 32));
     float zero = __fmul_rn(l, 0.f);  // NaN beside a value that is not finite
 #pragma unroll
@@ -570,10 +601,11 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
 #pragma unroll
       for (int i = 0; i < 16; ++i) zero = __fmaf_rn(o[d][i], 0.f, zero);
     odd |= zero != 0.f;
-    odd = odd && row < len;
+    odd = odd && row < len && part == 0;
     if (again || !__syncthreads_or(odd)) break;
     odd = false;
   }
+  if (part) return;
   const uint64_t who = __ballot(odd);
   store_rows<T, DIM>(a, at, row, l, o, (uint32_t)(who | who >> 32));
 }
@@ -610,7 +642,12 @@ int bq_prompt_attention(const void* q, const void* k, const void* v, int type, i
   if (k_token < 0 || v_token < 0 || k_token > 1 << 23 || v_token > 1 << 23)  // 64 rows within 32 bits
     return set_error(BQ_ERR_UNSUPPORTED, "%s: rows of k or v too far apart", what);
   // whatever the lengths are: a full tile for every 128 rows and one begun for each sequence
-  const int64_t tiles = n / PROMPT_ROWS + (B + 2 < n ? B + 2 : n);
+  const int64_t begun = B + 2 < n ? B + 2 : n;
+  // 128 queries a workgroup would give at most two to a CU: half as many queries (PARTS). bf16, causal, us
+  // (128, 64): 2048 + 1111 tokens of 16 heads 57, 49; 1024 of 32: 28, 25; 2048 of 32: 57, 56; 3000 of
+  // 32: 87, 110; heads of 64: 2048 of 16: 34, 28
+  const bool halves = type != 0 && (n + 127) / 128 * q_heads <= 512;
+  const int64_t tiles = n / (halves ? 64 : 128) + begun;
   if (tiles * q_heads > 0x7fffffff) return set_error(BQ_ERR_ARG, "%s: size too large", what);
   const size_t need = bq_prompt_attention_ws_bytes(type, n, heads, dim);
   if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
@@ -627,12 +664,12 @@ int bq_prompt_attention(const void* q, const void* k, const void* v, int type, i
     if (wide) prompt_split_kernel<128><<<(unsigned)blocks, 256, 0, st>>>(a);
     else prompt_split_kernel<64><<<(unsigned)blocks, 256, 0, st>>>(a);
   }
-#define BQ_PROMPT(T)                                                                        \
-  (wide ? prompt_kernel<T, 128><<<grid, PROMPT_WAVES * 64, 0, st>>>(a)                      \
-        : prompt_kernel<T, 64><<<grid, PROMPT_WAVES * 64, 0, st>>>(a))
-  if (type == 0) BQ_PROMPT(float);
-  else if (type == 1) BQ_PROMPT(__bf16);
-  else BQ_PROMPT(_Float16);
+#define BQ_PROMPT(T, PARTS)                                                                   \
+  (wide ? prompt_kernel<T, 128, PARTS><<<grid, PROMPT_WAVES * 64, 0, st>>>(a)               \
+        : prompt_kernel<T, 64, PARTS><<<grid, PROMPT_WAVES * 64, 0, st>>>(a))
+  if (type == 0) BQ_PROMPT(float, 1);
+  else if (type == 1) halves ? BQ_PROMPT(__bf16, 2) : BQ_PROMPT(__bf16, 1);
+  else halves ? BQ_PROMPT(_Float16, 2) : BQ_PROMPT(_Float16, 1);
 #undef BQ_PROMPT
   return check_launch(what);
 }

@@ -150,6 +150,65 @@ def test_keys_that_are_not_finite(dev, kind, what):
     check(got, want, tol)
 
 
+def many_heads(x, heads):
+    """The 2 query heads and 1 key-value head of x with the query heads repeated to `heads`: enough
+    workgroups for the form that takes 128 queries each."""
+    return torch.cat([x[:, :2]] * (heads // 2) + [x[:, 2:]], 1)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("dim,causal", [(64, True), (128, True), (128, False)])
+def test_many_heads(dev, kind, dim, causal):
+    print(f"prompt many heads {kind} dim={dim} causal={causal}", flush=True)
+    x, cu = data([20, 385, 1, 130], 2, 1, dim, kind, 41)
+    want, tol = expected(x, cu, 2, 1, causal, kind)
+    got = run(dev, many_heads(x, 300), cu, 300, 1, causal)
+    for j in (0, 148, 298):
+        check(got[:, j:j + 2], want, tol)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("what,at", [(math.nan, 70), (math.inf, 149), (-math.inf, 3)])
+def test_many_heads_not_finite(dev, kind, what, at):
+    print(f"prompt many heads {kind} v[{at}]={what}", flush=True)
+    x, cu = data([20, 150, 30], 2, 1, 128, kind, 43)
+    clean = run(dev, many_heads(x, 600), cu, 600, 1, True)
+    x[20 + at, 3, 5] = what
+    x[20 + at, 3, 100] = -what
+    want, tol = expected(x, cu, 2, 1, True, kind)
+    got = run(dev, many_heads(x, 600), cu, 600, 1, True)
+    unseen = [i for i in range(200) if i < 20 + at or i >= 170]
+    assert torch.equal(got[unseen], clean[unseen])
+    check(got[:, 4:6], want, tol)
+
+
+@pytest.mark.parametrize("qs,ks", [(2.0 ** 100, 2.0 ** -98), (2.0 ** -120, 2.0 ** 118), (2.0 ** -140, 2.0 ** 30),
+                                   (2.0 ** -10, 2.0 ** 8)])
+def test_f32_rows_of_any_size(dev, qs, ks):
+    """Rows of q and k near f32's ends, rows of unlike size side by side, channels far below their row's
+    largest: the pieces follow each row."""
+    print(f"prompt f32 q * {qs} k * {ks}", flush=True)
+    x, cu = data([90, 140], 2, 1, 64, "f32", 47)
+    x[:, :2, 3] *= 2.0 ** -15
+    x[:, 2, 7] *= 2.0 ** -13
+    x[:, :2] *= qs * 2.0 ** torch.randint(-3, 1, (230, 1, 1), generator=torch.Generator().manual_seed(1))
+    x[:, 2] *= ks * 2.0 ** torch.randint(-3, 1, (230, 1), generator=torch.Generator().manual_seed(2))
+    want, tol = expected(x, cu, 2, 1, True, "f32")
+    check(run(dev, x, cu, 2, 1, True), want, tol)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_scores_beyond_the_rounded_shift(dev, kind):
+    """Scores so large that the product of the maximum and the scale is taken apart from its rounding."""
+    print(f"prompt large scores {kind}", flush=True)
+    size = 2.0 ** 16 if kind == "bf16" else 2.0 ** 14
+    x, cu = data([70, 40], 2, 1, 64, kind, 53)
+    x[:, :3] = (x[:, :3].float() * size).clamp(-60000, 60000).to(TYPES[kind]) if kind == "f16" else x[:, :3] * size
+    want, tol = expected(x, cu, 2, 1, True, kind)
+    check(run(dev, x, cu, 2, 1, True), want, tol)
+    check(run(dev, many_heads(x, 600), cu, 600, 1, True)[:, :2], want, tol)
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_graph_and_other_stream(dev, kind):
     print(f"prompt graph {kind}", flush=True)
