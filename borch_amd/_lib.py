@@ -121,7 +121,8 @@ SIGNATURES = {
     "bq_kv4_attend": (_c_int, [_c_p, _c_p, _c_int, *[_c_i64] * 5, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_f, _c_p,
                                _c_p, _c_i64, _c_i64, _c_p, _c_size, _c_p]),
     "bq_kv4_evict": (_c_int, [_c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64,
-                              _c_i64, _c_p, _c_p, _c_p, _c_p]),
+                              _c_i64, _c_p, _c_p, _c_p, _c_p, _c_size, _c_p]),
+    "bq_kv4_evict_ws_bytes": (_c_size, [_c_i64] * 4),
 }
 
 _lock = threading.Lock()

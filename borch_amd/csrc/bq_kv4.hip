@@ -205,59 +205,74 @@ __device__ __forceinline__ int scan_before(int v, int* waves, int* all) {
   return before + x - v;
 }
 
-// Which tokens stay, one workgroup a (sequence, head): the `recent` last ones, and of the others
-// the keep - recent of largest weight, ties to the earlier token.
+// Which tokens of a (sequence, head) stay: the `recent` last ones, and of the others (the old) the
+// keep - recent of largest weight, ties to the earlier token.
 // A radix select over order_of finds the least weight that stays and how many of its equals do: 12,
 // 12 and 8 bits, a histogram in LDS each. The first digit spans sign, exponent and three bits of
 // the mantissa, so that weights of one size fall into eight counters and the lanes of a wave seldom
-// meet in one; the weights that share the digit found are then listed in LDS, where the other
-// digits take no time (a row with more such than the list holds is read again for each digit). Two
-// passes write places and weights in order: each wave counts, by ballots, those that stay of its 256
-// tokens, one scan sums the counts, and each lane knows its place.
-// The passes' loops stay rolled, the next loads under this step's work: with a row held in registers, 64
-// weights a thread, the straight code for them took longer to fetch than four more reads from L2
-// (64 rows of 4096: 30 us; 16 of 65536: 52).
-constexpr int EVICT_STEP = 4, EVICT_SPAN = 65536, EVICT_LIST = 8192;
+// meet in one; the weights that share the digit found are then listed, and the other digits look at
+// the list alone (a row with more such than the list holds is read again for each). Places and weights
+// are written in order: each wave counts, by ballots, those that stay of its 256 tokens, one scan sums
+// the counts, and what stays is put side by side in LDS first.
+//
+// Rows of up to 16384 weights: one workgroup does it all (kv4_select_kernel<true>). Longer ones are
+// bound by instructions on one CU (16 rows of 65536: 47 us), so parts of 8192 weights take workgroups of
+// their own, in three launches: the first digit's counts of each part (kv4_tally_kernel), the list
+// (kv4_list_kernel), the rest (kv4_select_kernel<false>: every part resolves the list itself).
+constexpr int EVICT_STEP = 16384, EVICT_PART = 8192, EVICT_LIST = 8192;
+constexpr int EVICT_SOLO = EVICT_STEP;  // the longest row of one workgroup
 typedef float v4fu __attribute__((ext_vector_type(4), aligned(4)));
 
-__global__ __launch_bounds__(EVICT_THREADS) void kv4_select_kernel(const float* __restrict__ sums, int64_t sums_b,
-                                                                   int64_t sums_h, int most, int heads,
-                                                                   const int* __restrict__ lens, int keep, int recent,
-                                                                   int* __restrict__ kept, float* __restrict__ weights,
-                                                                   int* __restrict__ left) {
-  __shared__ int hist[4096], waves[EVICT_WAVES], found[2], listed;
-  __shared__ uint32_t list[EVICT_LIST];
-  const int bh = blockIdx.x, b = bh / heads, tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n = max(0, min(lens[b], most)), old = n > keep ? n - recent : 0;  // all stay: none is looked at
-  const float* w = sums + b * sums_b + (bh - b * heads) * sums_h;
-  kept += (size_t)bh * keep;
-  weights += (size_t)bh * keep;
-  if (bh % heads == 0 && tid == 0) left[b] = min(n, keep);
+struct Evict {
+  const float* sums;
+  int64_t sums_b, sums_h;
+  const int* lens;
+  int most, heads, keep, recent, parts;
+  int *kept, *left;
+  float* weights;
+  // long rows: a part's counts of the first digit [rows][parts][4096], its tokens above the digit found
+  // [rows][parts]; a row's list (order_of, token), its length, and the digit with what remains to keep
+  uint16_t* slots;
+  int* over;
+  uint2* list;
+  int* listed;
+  int2* found;
+};
 
-  // f(i, o) for tokens i .. i + 3 of the old ones from .. to, o order_of their weights, 0 past them; the
-  // threads side by side, a wave's 256 tokens or none
-  auto load = [&](int i0, int to, v4fu (&x)[EVICT_STEP]) {
+// A row's weights and lengths.
+struct Row {
+  const float* w;
+  int b, n, old;  // old: those before the latest, 0 where all stay
+  __device__ __forceinline__ Row(const Evict& a, int row) : b(row / a.heads) {
+    n = max(0, min(a.lens[b], a.most));
+    old = n > a.keep ? n - a.recent : 0;
+    w = a.sums + b * a.sums_b + (row - b * a.heads) * a.sums_h;
+  }
+  // f(i, o) for tokens i .. i + 3 of from .. to (at most `old`), o order_of their weights, 0 past `to`: the
+  // threads side by side, a wave's 256 tokens or none. The next loads under this step's work.
+  template <typename F>
+  __device__ __forceinline__ void each(int most, int from, int to, F&& f) const {
+    constexpr int LOADS = EVICT_STEP / (4 * EVICT_THREADS);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    auto load = [&](int i0, v4fu (&x)[LOADS]) {
 #pragma unroll
-    for (int e = 0; e < EVICT_STEP; ++e) {
-      const int c = i0 + (e * EVICT_WAVES + wave) * 256, i = c + 4 * lane;
-      if (c + 256 <= most) {
-        x[e] = *reinterpret_cast<const v4fu*>(w + i);
-      } else if (c < to) {
+      for (int e = 0; e < LOADS; ++e) {
+        const int c = i0 + (e * EVICT_WAVES + wave) * 256, i = c + 4 * lane;
+        if (c + 256 <= most) {
+          x[e] = *reinterpret_cast<const v4fu*>(w + i);
+        } else if (c < to) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[e][j] = w[min(i + j, old - 1)];
+          for (int j = 0; j < 4; ++j) x[e][j] = w[min(i + j, to - 1)];
+        }
       }
-    }
-  };
-  constexpr int STEP = EVICT_STEP * EVICT_THREADS * 4;  // tokens
-  auto each = [&](int from, int to, auto&& f, auto&& after) {  // after(i0): a step's tokens are done
-    v4fu now[EVICT_STEP] = {}, next[EVICT_STEP] = {};
-    load(from, to, now);
+    };
+    v4fu now[LOADS] = {}, next[LOADS] = {};
+    if (from < to) load(from, now);
 #pragma unroll 1
-    for (int i0 = from; i0 < to; i0 += STEP) {
-      if (i0 + STEP < to) load(i0 + STEP, to, next);
+    for (int i0 = from; i0 < to; i0 += EVICT_STEP) {
+      if (i0 + EVICT_STEP < to) load(i0 + EVICT_STEP, next);
 #pragma unroll
-      for (int e = 0; e < EVICT_STEP; ++e) {
+      for (int e = 0; e < LOADS; ++e) {
         const int c = i0 + (e * EVICT_WAVES + wave) * 256, i = c + 4 * lane;
         if (c >= to) break;
         uint32_t o[4];
@@ -268,152 +283,273 @@ __global__ __launch_bounds__(EVICT_THREADS) void kv4_select_kernel(const float* 
           for (int j = 0; j < 4; ++j) o[j] = i + j < to ? o[j] : 0u;
         f(i, o);
       }
-      after(i0);
 #pragma unroll
-      for (int e = 0; e < EVICT_STEP; ++e) now[e] = next[e];
+      for (int e = 0; e < LOADS; ++e) now[e] = next[e];
     }
-  };
-  auto nothing = [](int) {};
-
-  uint32_t least = 0;       // weights above this stay
-  int equals = 0x7fffffff;  // and so many that equal it
-  if (n > keep) {
-    int need = keep - recent;
-    uint32_t prefix = 0, mask = 0;
-    for (int digit = 0; digit < 3; ++digit) {
-      const int shift = digit == 0 ? 20 : digit == 1 ? 8 : 0, count = digit == 2 ? 256 : 4096;
-      for (int i = tid; i < count; i += EVICT_THREADS) hist[i] = 0;
-      if (tid == 0 && digit == 0) listed = 0;
-      __syncthreads();
-      // a 0, of no weight, is counted under all others, where `need` never comes
-      auto tally = [&](uint32_t o) {
-        if ((o & mask) == prefix) atomicAdd(&hist[(o >> shift) & (count - 1)], 1);
-      };
-      if (digit > 0 && listed <= EVICT_LIST)
-        for (int i = tid; i < listed; i += EVICT_THREADS) tally(list[i]);
-      else
-        each(0, old, [&](int, const uint32_t (&o)[4]) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) tally(o[j]);
-        }, nothing);
-      __syncthreads();
-      // the digit at which the counts from the largest down reach `need`: four counters a thread
-      int c4[4], sum = 0, all;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int d = count - 1 - 4 * tid - e;
-        c4[e] = d >= 0 ? hist[d] : 0;
-        sum += c4[e];
-      }
-      int above = scan_before(sum, waves, &all);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        // need = 0: the largest digit, of which none stays
-        if ((above < need && above + c4[e] >= need) || (need == 0 && tid == 0 && e == 0)) {
-          found[0] = count - 1 - 4 * tid - e;
-          found[1] = need - above;
-        }
-        above += c4[e];
-      }
-      __syncthreads();
-      prefix |= (uint32_t)found[0] << shift;
-      mask |= (uint32_t)(count - 1) << shift;
-      need = found[1];
-      if (digit == 0)
-        each(0, old, [&](int, const uint32_t (&o)[4]) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if ((o[j] & mask) == prefix) {
-              const int at = atomicAdd(&listed, 1);
-              if (at < EVICT_LIST) list[at] = o[j];
-            }
-        }, nothing);
-      __syncthreads();
-    }
-    least = prefix;
-    equals = need;
   }
-  int out = 0, same = 0;  // kept before this span, equals of `least` met before it
-  for (int s0 = 0; s0 < old; s0 += EVICT_SPAN) {
-    const int end = min(old, s0 + EVICT_SPAN);
-    __syncthreads();
-    // of each 256 tokens, those above `least` and, from 256 on, its equals
-    if (tid < 512) hist[tid] = 0;
-    __syncthreads();
-    each(s0, end, [&](int i, const uint32_t (&o)[4]) {
-      int over = 0, eq = 0;
+};
+
+// The digit at which hist's counts from the largest down reach `need`, and what then remains of it: four
+// counters a thread. need = 0: the largest digit, of which none stays. By the whole workgroup.
+__device__ __forceinline__ int2 find_digit(const int* hist, int count, int need, int* waves, int* found) {
+  const int tid = threadIdx.x;
+  int c4[4], sum = 0, all;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        over += (int)__popcll(__ballot(o[j] > least));
-        eq += (int)__popcll(__ballot(o[j] == least));
-      }
-      if (lane == 0) {
-        hist[(i - s0) >> 8] = over;
-        hist[256 + ((i - s0) >> 8)] = eq;
-      }
-    }, nothing);
-    __syncthreads();
-    int all_eq, all;
-    const int eq_here = tid < 256 ? hist[256 + tid] : 0;
-    const int eq_before = same + scan_before(eq_here, waves, &all_eq);
-    const int stay = (tid < 256 ? hist[tid] : 0) + max(0, min(eq_here, equals - eq_before));
-    const int before = out + scan_before(stay, waves, &all);
-    if (tid < 256) {
-      hist[tid] = before;
-      hist[256 + tid] = equals - eq_before;  // so many of its equals stay
+  for (int e = 0; e < 4; ++e) {
+    const int d = count - 1 - 4 * tid - e;
+    c4[e] = d >= 0 ? hist[d] : 0;
+    sum += c4[e];
+  }
+  int above = scan_before(sum, waves, &all);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if ((above < need && above + c4[e] >= need) || (need == 0 && tid == 0 && e == 0)) {
+      found[0] = count - 1 - 4 * tid - e;
+      found[1] = need - above;
     }
-    int done = out;  // written
-    uint16_t* staged = reinterpret_cast<uint16_t*>(list);  // of one step: STEP entries
-    static_assert(STEP * 2 <= EVICT_LIST * 4 && EVICT_SPAN <= 65536, "staging");
-    same += all_eq;
-    out += all;
+    above += c4[e];
+  }
+  __syncthreads();
+  const int2 r = make_int2(found[0], found[1]);
+  __syncthreads();
+  return r;
+}
+
+// Long rows, first: a part's counts of the first digit (a part has at most 8192).
+__global__ __launch_bounds__(EVICT_THREADS) void kv4_tally_kernel(Evict a) {
+  __shared__ int hist[4096];
+  const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts, tid = threadIdx.x, lo = part * EVICT_PART;
+  const Row r(a, row);
+  if (part == 0 && tid == 0) a.listed[row] = 0;
+  if (lo >= r.old) return;
+  for (int i = tid; i < 4096; i += EVICT_THREADS) hist[i] = 0;
+  __syncthreads();
+  r.each(a.most, lo, min(r.old, lo + EVICT_PART), [&](int, const uint32_t (&o)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (o[j]) atomicAdd(&hist[o[j] >> 20], 1);
+  });
+  __syncthreads();
+  uint2* to = reinterpret_cast<uint2*>(a.slots + ((size_t)row * a.parts + part) * 4096) + tid;
+  const int* h = hist + 4 * tid;
+  *to = make_uint2((uint32_t)h[0] | (uint32_t)h[1] << 16, (uint32_t)h[2] | (uint32_t)h[3] << 16);
+}
+
+// Then: the first digit from all parts' counts, this part's tokens above it counted and those of it listed.
+__global__ __launch_bounds__(EVICT_THREADS) void kv4_list_kernel(Evict a) {
+  __shared__ int hist[4096], waves[EVICT_WAVES], found[2], over, count, first;
+  __shared__ uint32_t keys[EVICT_PART];
+  __shared__ uint16_t tokens[EVICT_PART];
+  const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts, tid = threadIdx.x, lo = part * EVICT_PART;
+  const Row r(a, row);
+  if (lo >= r.old) return;
+  int c[4] = {0, 0, 0, 0};
+  const uint2* from = reinterpret_cast<const uint2*>(a.slots + (size_t)row * a.parts * 4096) + tid;
+  const int parts = (r.old + EVICT_PART - 1) / EVICT_PART;
+  for (int p0 = 0; p0 < parts; p0 += 8) {
+    uint2 x[8];
+#pragma unroll
+    for (int p = 0; p < 8; ++p) x[p] = from[(size_t)min(p0 + p, parts - 1) * 1024];
+#pragma unroll
+    for (int p = 0; p < 8; ++p)
+      if (p0 + p < parts) c[0] += x[p].x & 0xffff, c[1] += x[p].x >> 16, c[2] += x[p].y & 0xffff, c[3] += x[p].y >> 16;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) hist[4 * tid + e] = c[e];
+  if (tid == 0) over = count = 0;
+  __syncthreads();
+  const int2 digit = find_digit(hist, 4096, a.keep - a.recent, waves, found);
+  if (part == 0 && tid == 0) a.found[row] = digit;
+  int mine = 0;
+  r.each(a.most, lo, min(r.old, lo + EVICT_PART), [&](int i, const uint32_t (&o)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      mine += (int)(o[j] >> 20) > digit.x;
+      if (o[j] && (int)(o[j] >> 20) == digit.x) {
+        const int at = atomicAdd(&count, 1);
+        keys[at] = o[j];
+        tokens[at] = (uint16_t)(i + j - lo);
+      }
+    }
+  });
+  atomicAdd(&over, mine);
+  __syncthreads();
+  if (tid == 0) {
+    a.over[(size_t)row * a.parts + part] = over;
+    first = atomicAdd(&a.listed[row], count);  // the list's order does not matter
+  }
+  __syncthreads();
+  for (int x = tid; x < min(count, EVICT_LIST - first); x += EVICT_THREADS)
+    a.list[(size_t)row * EVICT_LIST + first + x] = make_uint2(keys[x], (uint32_t)(lo + tokens[x]));
+}
+
+template <bool SOLO>  // the row is one workgroup's
+__global__ __launch_bounds__(EVICT_THREADS) void kv4_select_kernel(Evict a) {
+  __shared__ int hist[4096], waves[EVICT_WAVES], found[2], listed;
+  __shared__ uint32_t list[EVICT_LIST];
+  __shared__ int tokens[SOLO ? 1 : EVICT_LIST];
+  const int row = SOLO ? blockIdx.x : blockIdx.x / a.parts, part = SOLO ? 0 : blockIdx.x - row * a.parts;
+  const int tid = threadIdx.x, lane = tid & 63, keep = a.keep;
+  const Row r(a, row);
+  const int lo = part * EVICT_PART, hi = SOLO ? r.n : min(r.n, lo + EVICT_PART);  // this workgroup's tokens
+  int* kept = a.kept + (size_t)row * keep;
+  float* weights = a.weights + (size_t)row * keep;
+  if (row % a.heads == 0 && part == 0 && tid == 0) a.left[r.b] = min(r.n, keep);
+  // the latest (or all), and past the last
+  for (int i = max(lo, r.old) + tid; i < hi; i += EVICT_THREADS) {
+    const int to = min(r.n, keep) - r.n + i;
+    kept[to] = i;
+    weights[to] = r.w[i];
+  }
+  for (int i = max(lo, r.n) + tid; i < (SOLO ? keep : min(keep, lo + EVICT_PART)); i += EVICT_THREADS) {
+    kept[i] = -1;
+    weights[i] = 0.f;
+  }
+  if (lo >= r.old) return;
+
+  uint32_t prefix = 0, mask = 0;  // weights of `prefix` in their bits of `mask` are still undecided
+  int need = keep - a.recent;     // and so many of them stay
+  bool fits = true;
+  if constexpr (!SOLO) {
+    const int2 digit = a.found[row];
+    prefix = (uint32_t)digit.x << 20;
+    mask = 0xfff00000u;
+    need = digit.y;
+    const int count = a.listed[row];
+    fits = count <= EVICT_LIST;
+    if (tid == 0) listed = min(count, EVICT_LIST);
+    for (int i = tid; i < min(count, EVICT_LIST); i += EVICT_THREADS) {
+      const uint2 x = a.list[(size_t)row * EVICT_LIST + i];
+      list[i] = x.x;
+      tokens[i] = (int)x.y;
+    }
+  } else if (tid == 0) {
+    listed = 0;
+  }
+  for (int digit = SOLO ? 0 : 1; digit < 3; ++digit) {
+    const int shift = digit == 0 ? 20 : digit == 1 ? 8 : 0, count = digit == 2 ? 256 : 4096;
+    for (int i = tid; i < count; i += EVICT_THREADS) hist[i] = 0;
     __syncthreads();
-    auto below = [&](bool b) {  // lanes before this one with b
-      const uint64_t m = __ballot(b);
-      return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+    auto tally = [&](uint32_t o) {
+      if (o && (o & mask) == prefix) atomicAdd(&hist[(o >> shift) & (count - 1)], 1);
     };
-    each(s0, end, [&](int i, const uint32_t (&o)[4]) {
-      const int at = __builtin_amdgcn_readfirstlane((i - s0) >> 8), cut = __builtin_amdgcn_readfirstlane(hist[256 + at]);
-      bool stays[4];
-      if (cut <= 0 || cut >= 256) {  // no equal stays, or all
-        const uint32_t from = cut <= 0 ? least : least - 1;
+    if (digit > 0 && fits)
+      for (int i = tid; i < listed; i += EVICT_THREADS) tally(list[i]);
+    else
+      r.each(a.most, 0, r.old, [&](int, const uint32_t (&o)[4]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) stays[j] = o[j] > from;
-      } else {
-        int rank = 0;  // of the lane's first token among the equals
+        for (int j = 0; j < 4; ++j) tally(o[j]);
+      });
+    __syncthreads();
+    const int2 d = find_digit(hist, count, need, waves, found);
+    prefix |= (uint32_t)d.x << shift;
+    mask |= (uint32_t)(count - 1) << shift;
+    need = d.y;
+    if (SOLO && digit == 0) {
+      r.each(a.most, 0, r.old, [&](int, const uint32_t (&o)[4]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) rank += below(o[j] == least);
+        for (int j = 0; j < 4; ++j)
+          if (o[j] && (o[j] & mask) == prefix) {
+            const int at = atomicAdd(&listed, 1);
+            if (at < EVICT_LIST) list[at] = o[j];
+          }
+      });
+      __syncthreads();
+      fits = listed <= EVICT_LIST;
+    }
+  }
+  const uint32_t least = prefix;  // weights above it stay
+  const int equals = need;        // and so many that equal it
+
+  // those that stay before this workgroup's tokens, and the equals among them
+  int out = 0, same = 0;
+  if (!SOLO && part > 0) {
+    int over = 0, eq = 0;
+    if (fits) {
+      for (int p = tid; p < part; p += EVICT_THREADS) over += a.over[(size_t)row * a.parts + p];
+      for (int i = tid; i < listed; i += EVICT_THREADS) {
+        over += tokens[i] < lo && list[i] > least;
+        eq += tokens[i] < lo && list[i] == least;
+      }
+    } else {
+      r.each(a.most, 0, lo, [&](int, const uint32_t (&o)[4]) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          stays[j] = o[j] > least || (o[j] == least && rank < cut);
-          rank += o[j] == least;
+          over += o[j] > least;
+          eq += o[j] == least;
         }
-      }
-      int to = hist[at] - done;
+      });
+    }
+    scan_before(over, waves, &out);
+    scan_before(eq, waves, &same);
+    out += min(same, equals);
+  }
+
+  const int end = min(hi, r.old);  // one step
+  __syncthreads();
+  // of each 256 tokens, those above `least` and, from 256 on, its equals
+  if (tid < 512) hist[tid] = 0;
+  __syncthreads();
+  r.each(a.most, lo, end, [&](int i, const uint32_t (&o)[4]) {
+    int over = 0, eq = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) to += below(stays[j]);
+    for (int j = 0; j < 4; ++j) {
+      over += (int)__popcll(__ballot(o[j] > least));
+      eq += (int)__popcll(__ballot(o[j] == least));
+    }
+    if (lane == 0) {
+      hist[(i - lo) >> 8] = over;
+      hist[256 + ((i - lo) >> 8)] = eq;
+    }
+  });
+  __syncthreads();
+  int all_eq, all;
+  const int eq_here = tid < 256 ? hist[256 + tid] : 0;
+  const int eq_before = same + scan_before(eq_here, waves, &all_eq);
+  const int stay = (tid < 256 ? hist[tid] : 0) + max(0, min(eq_here, equals - eq_before));
+  const int before = scan_before(stay, waves, &all);
+  if (tid < 256) {
+    hist[tid] = before;
+    hist[256 + tid] = equals - eq_before;  // so many of its equals stay
+  }
+  __syncthreads();
+  auto below = [&](bool x) {  // lanes before this one with x
+    const uint64_t m = __ballot(x);
+    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+  };
+  uint16_t* staged = reinterpret_cast<uint16_t*>(list);
+  static_assert(EVICT_STEP * 2 <= EVICT_LIST * 4 && EVICT_STEP <= 65536 && EVICT_PART <= EVICT_STEP, "staging");
+  r.each(a.most, lo, end, [&](int i, const uint32_t (&o)[4]) {
+    const int at = __builtin_amdgcn_readfirstlane((i - lo) >> 8), cut = __builtin_amdgcn_readfirstlane(hist[256 + at]);
+    bool stays[4];
+    if (cut <= 0 || cut >= 256) {  // no equal stays, or all
+      const uint32_t from = cut <= 0 ? least : least - 1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) stays[j] = o[j] > from;
+    } else {
+      int rank = 0;  // of the lane's first token among the equals
+#pragma unroll
+      for (int j = 0; j < 4; ++j) rank += below(o[j] == least);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (stays[j]) staged[to] = (uint16_t)(i + j - s0);
-        to += stays[j];
+        stays[j] = o[j] > least || (o[j] == least && rank < cut);
+        rank += o[j] == least;
       }
-    }, [&](int i0) {
-      // what stays of this step, from LDS: side by side, where each lane's own stores took most of the pass
-      const int next = (i0 - s0 + STEP) >> 8, upto = i0 + STEP < end ? hist[next] : out;
-      __syncthreads();
-      for (int x = tid; x < upto - done; x += EVICT_THREADS) {
-        const int i = s0 + staged[x];
-        kept[done + x] = i;
-        weights[done + x] = w[i];
-      }
-      __syncthreads();
-      done = upto;
-    });
-  }
-  for (int i = out + tid; i < keep; i += EVICT_THREADS) {  // the latest, and past the last
-    const int from = old + i - out;
-    kept[i] = from < n ? from : -1;
-    weights[i] = from < n ? w[from] : 0.f;
+    }
+    int to = hist[at];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) to += below(stays[j]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (stays[j]) staged[to] = (uint16_t)(i + j - lo);
+      to += stays[j];
+    }
+  });
+  __syncthreads();
+  for (int x = tid; x < all; x += EVICT_THREADS) {
+    const int i = lo + staged[x];
+    kept[out + x] = i;
+    weights[out + x] = r.w[i];
   }
 }
 
@@ -528,9 +664,21 @@ int bq_kv4_read(const bq_kv4_cache* cache, const int32_t* table, int64_t B, int6
   return check_launch(what);
 }
 
+// Parts a row is cut into, 0 for one workgroup.
+static int64_t evict_parts(int64_t most, int64_t keep) {
+  return most <= EVICT_SOLO ? 0 : ((most > keep ? most : keep) + EVICT_PART - 1) / EVICT_PART;
+}
+
+size_t bq_kv4_evict_ws_bytes(int64_t B, int64_t heads, int64_t most, int64_t keep) {
+  if (B < 1 || heads < 1) return 0;
+  const size_t parts = (size_t)evict_parts(most, keep), rows = (size_t)B * heads;
+  return parts ? rows * (parts * (4096 * 2 + 4) + EVICT_LIST * 8 + 8 + 4) : 0;
+}
+
 int bq_kv4_evict(const bq_kv4_cache* cache, const float* sums, int64_t sums_b, int64_t sums_h, int64_t most, const int32_t* table, int64_t B,
                  int64_t width, const int32_t* lens, const int32_t* new_table, int64_t new_width, int64_t keep,
-                 int64_t recent, int32_t* kept, float* weights, int32_t* left, bq_stream_t stream) {
+                 int64_t recent, int32_t* kept, float* weights, int32_t* left, void* ws, size_t ws_bytes,
+                 bq_stream_t stream) {
   const char* what = "bq_kv4_evict";
   Kv4 c, to;
   if (const int rc = kv4_of(what, cache, table, B, width, &c)) return rc;
@@ -547,8 +695,24 @@ int bq_kv4_evict(const bq_kv4_cache* cache, const float* sums, int64_t sums_b, i
   const int64_t blocks = (keep + 4096 / cache->dim - 1) / (4096 / cache->dim);
   if (B * c.heads * blocks > 0x7fffffff) return set_error(BQ_ERR_ARG, "%s: size too large", what);
   hipStream_t st = (hipStream_t)stream;
-  kv4_select_kernel<<<(unsigned)(B * c.heads), EVICT_THREADS, 0, st>>>(sums, sums_b, sums_h, (int)most, c.heads, lens,
-                                                                       (int)keep, (int)recent, kept, weights, left);
+  const int64_t rows = B * c.heads, parts = evict_parts(most, keep);
+  const size_t need = bq_kv4_evict_ws_bytes(B, c.heads, most, keep);
+  if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
+    return set_error(BQ_ERR_ARG, "%s: a workspace of %zu bytes, given %zu", what, need, ws ? ws_bytes : 0);
+  if (rows * parts > 0x7fffffff) return set_error(BQ_ERR_ARG, "%s: size too large", what);
+  Evict a = {sums, sums_b, sums_h, lens, (int)most, c.heads, (int)keep, (int)recent, (int)parts, kept, left, weights};
+  if (parts) {
+    a.slots = (uint16_t*)ws;
+    a.list = (uint2*)(a.slots + (size_t)rows * parts * 4096);
+    a.found = (int2*)(a.list + (size_t)rows * EVICT_LIST);
+    a.listed = (int*)(a.found + rows);
+    a.over = a.listed + rows;
+    kv4_tally_kernel<<<(unsigned)(rows * parts), EVICT_THREADS, 0, st>>>(a);
+    kv4_list_kernel<<<(unsigned)(rows * parts), EVICT_THREADS, 0, st>>>(a);
+    kv4_select_kernel<false><<<(unsigned)(rows * parts), EVICT_THREADS, 0, st>>>(a);
+  } else {
+    kv4_select_kernel<true><<<(unsigned)rows, EVICT_THREADS, 0, st>>>(a);
+  }
   if (const int rc = check_launch(what)) return rc;
   const unsigned grid = (unsigned)(B * c.heads * blocks);
   if (c.pages == 0) return BQ_OK;

@@ -184,8 +184,11 @@ class Cache4:
         weights = torch.empty((B, self.heads, keep), dtype=torch.float32, device=self.device)
         left = torch.empty(B, dtype=torch.int32, device=self.device)
         sb, sh, _ = sums.stride()
+        need = lib().bq_kv4_evict_ws_bytes(B, self.heads, sums.shape[2], keep)
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         with on(self._index):
             check(lib().bq_kv4_evict(self._ref, sums.data_ptr(), sb, sh, sums.shape[2], table.data_ptr(), B, width,
                                      lens.data_ptr(), new_table.data_ptr(), new_table.shape[1], keep, recent,
-                                     kept.data_ptr(), weights.data_ptr(), left.data_ptr(), _stream(kept)))
+                                     kept.data_ptr(), weights.data_ptr(), left.data_ptr(), ws.data_ptr() if need else None,
+                                     need, _stream(kept)))
         return kept, weights, left

@@ -544,11 +544,13 @@ int bq_kv4_attend(const bq_kv4_cache* cache, const void* q, int type, int64_t to
  * and sums_h elements; ties to the earlier token, NaN above all); the tokens that stay move in
  * order to the pages of new_table i32 [B, new_width], which are none of those in use.
  *   kept i32 [B, heads, keep]: their former places (-1 past the last); weights f32 [B, heads, keep]:
- *   their sums (0 past the last); left i32 [B]: min(lens[b], keep). lens beyond `most` are cut. */
+ *   their sums (0 past the last); left i32 [B]: min(lens[b], keep). lens beyond `most` are cut.
+ * ws: bq_kv4_evict_ws_bytes bytes (0 for short rows), 16-byte aligned, need not be cleared. */
+size_t bq_kv4_evict_ws_bytes(int64_t B, int64_t heads, int64_t most, int64_t keep);
 int bq_kv4_evict(const bq_kv4_cache* cache, const float* sums, int64_t sums_b, int64_t sums_h, int64_t most,
                  const int32_t* table, int64_t B, int64_t width, const int32_t* lens, const int32_t* new_table,
                  int64_t new_width, int64_t keep, int64_t recent, int32_t* kept, float* weights, int32_t* left,
-                 bq_stream_t stream);
+                 void* ws, size_t ws_bytes, bq_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -77,11 +77,13 @@ def test_attend_and_evict_refusals():
     assert lib.bq_kv4_attend_ws_bytes(0, 2, 2, 64, 100, 1) == 0
 
     def evict(keep=4, recent=0, most=8, new_width=1, ptr=None):
-        return lib.bq_kv4_evict(r, ptr, 16, 8, most, 16, 1, 2, ptr, 16, new_width, keep, recent, ptr, ptr, ptr, None)
+        return lib.bq_kv4_evict(r, ptr, 16, 8, most, 16, 1, 2, ptr, 16, new_width, keep, recent, ptr, ptr, ptr, None, 0, None)
 
     assert evict(keep=0) == ARG and evict(recent=5) == ARG and evict(recent=-1) == ARG
     assert evict(keep=33) == ARG and "hold" in _lib.last_error()
     assert evict(most=-1) == ARG and evict() == ARG
+    assert lib.bq_kv4_evict_ws_bytes(1, 2, 16384, 8) == 0 < lib.bq_kv4_evict_ws_bytes(1, 2, 16385, 8)
+    assert evict(most=20000, ptr=16) == ARG and "workspace" in _lib.last_error()
 
 
 def test_cpu_tensors_are_refused():

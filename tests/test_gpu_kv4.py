@@ -316,6 +316,46 @@ def test_evict_orders(dev, name):
     check_evict(dev, c, table, lens, sums, keep, recent)
 
 
+@pytest.mark.parametrize("name", ["spread", "ties", "equal", "one"])
+def test_evict_long_rows(dev, name):
+    """Rows of several parts: the list of one digit, one that does not hold them all, ties across the
+    parts' borders, rows that keep all or end early."""
+    print(f"kv4 evict long {name}", flush=True)
+    lens, keep, recent, dim = [30000, 17000, 900, 8193], 2500, 100, 64
+    table, pages = tables(lens, 1024, 3)
+    pages += 4 * 3
+    c = kv4.Cache4.zeros(pages, 1, 1024, dim, dev)
+    for t in (c.k, c.v):  # any codes: all are values
+        t.copy_(torch.randint(0, 256, t.shape, generator=torch.Generator().manual_seed(2), dtype=torch.uint8))
+    g = torch.Generator().manual_seed(6)
+    sums = torch.exp(2 * torch.randn(4, 1, 30000, generator=g))
+    if name == "ties":
+        sums = torch.round(sums * 2) / 2
+    elif name == "equal":
+        sums = torch.full_like(sums, 0.25)
+    elif name == "one":  # all in one digit, none equal
+        sums = 1.0 + torch.rand(sums.shape, generator=g) / 8
+    if name == "spread":
+        keep, recent = 2500, 2500  # none of the old stay
+    kept, weights, left = c.evict(sums.to(dev), table.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev),
+                                  torch.tensor(sorted(set(range(pages)) - set(table.flatten().tolist())),
+                                               dtype=torch.int32)[:12].reshape(4, 3).to(dev), keep, recent)
+    for b, n in enumerate(lens):
+        at = D.evict(sums[b, 0].tolist(), n, keep, recent)
+        want = torch.full((keep,), -1, dtype=torch.int32)
+        want[:len(at)] = torch.tensor(at, dtype=torch.int32)
+        assert torch.equal(kept[b, 0].cpu(), want), b
+        assert torch.equal(weights[b, 0, :len(at)].cpu(), sums[b, 0][at]) and not weights[b, 0, len(at):].any()
+    assert left.tolist() == [2500, 2500, 900, 2500]
+
+
+def test_evict_long_rows_moved(dev):
+    print("kv4 evict long moved", flush=True)
+    c, table = roomy(dev, [17500], 1, 64, 256, 600, 5)
+    sums = torch.exp(2 * torch.randn(1, 1, 17500, generator=torch.Generator().manual_seed(8)))
+    check_evict(dev, c, table, [17500], sums, 600, 50)
+
+
 def test_evict_strided_sums(dev):
     print("kv4 evict strided", flush=True)
     c, table = roomy(dev, [70, 80], 2, 64, 32, 32, 3)
