@@ -348,7 +348,8 @@ __global__ __launch_bounds__(256) void prompt_split_kernel(Prompt a) {
 // PARTS = 2 (16-bit types): 64 queries a workgroup, and two waves take one half of each tile's keys each
 // for the same 32 queries, joined in LDS at the end: twice the workgroups, each half as long, where 128
 // queries a workgroup leave the GPU part empty.
-template <typename T, int DIM, int PARTS>
+// DIRECT (f32, short prompts): the workgroup splits its tiles itself, and no launch goes before.
+template <typename T, int DIM, int PARTS, bool DIRECT>
 __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) {
   constexpr int P = Kind<T>::P, PK = Kind<T>::PK, KT = P == 3 ? 32 : 64, SUB = KT / 32 / PARTS, BUFS = P == 3 ? 1 : 2;
   constexpr int ALL = 32 * PROMPT_WAVES / PARTS;  // queries a workgroup
@@ -424,7 +425,7 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
     }
   }
   const int* row_e = PK == 2 ? a.exponents + (size_t)h * a.n + at.start : nullptr;
-  auto exponent = [&](int t0) { return PK == 2 && threadIdx.x < 32 && t0 + (int)threadIdx.x < len ? row_e[t0 + threadIdx.x] : 0; };
+  auto exponent = [&](int t0) { return PK == 2 && !DIRECT && threadIdx.x < 32 && t0 + (int)threadIdx.x < len ? row_e[t0 + threadIdx.x] : 0; };
   float m, l;
   v16f o[VT];
   // Once; and where an output is not finite once more, with the values that are not out of the tiles
@@ -435,7 +436,7 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
     m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int d = 0; d < VT; ++d) o[d] = zeros16();
-    if (keys > 0) {
+    if (!DIRECT && keys > 0) {
       fetch(k, PK, ktb, ko, 0, lds0);
       if constexpr (BUFS == 2) fetch(v, P, vtb, vo, 0, lds0 + PK * PLANE);
     }
@@ -443,11 +444,44 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
     int e_next = exponent(0);  // loaded with the keys, put in LDS when they are there
     for (int t0 = 0, buf = 0; t0 < keys; t0 += KT, buf ^= BUFS - 1) {
       wait_dma_all();
-      if (PK == 2 && threadIdx.x < 32) exponents[threadIdx.x] = e_next;
+      if constexpr (DIRECT) {
+        barrier();  // the last tile is read
+#pragma unroll
+        for (int e = 0; e < 2 * KT * DIM / 8 / (PROMPT_WAVES * 64); ++e) {
+          constexpr int HALF = KT * DIM / 8;  // pieces of eight of k, then of v
+          const int id = threadIdx.x + e * PROMPT_WAVES * 64, r = id % HALF / (DIM / 8), c = id % (DIM / 8);
+          const bool is_v = id >= HALF;
+          float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          if (t0 + r < len) {
+            const int64_t at_row = at.start + t0 + r;
+            load8((is_v ? (const float*)a.v + at_row * a.vt + h * a.vh : (const float*)a.k + at_row * a.kt + h * a.kh) + 8 * c, x);
+          }
+          if (is_v) {
+            const Frag<3> f = frag_of<float>(x);
+#pragma unroll
+            for (int p = 0; p < 3; ++p)
+              *reinterpret_cast<v8s*>(lds + (PK + p) * PLANE + v_at<DIM>(r, c)) = f.p[p];
+          } else {
+            uint32_t peak = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) peak = max(peak, __float_as_uint(x[j]) & 0x7fffffffu);
+#pragma unroll
+            for (int d = 1; d < DIM / 8; d *= 2) peak = max(peak, (uint32_t)__shfl_xor((int)peak, d));
+            const int ex = row_exponent(peak);
+            const Frag<2> f = halves(x, ex);
+#pragma unroll
+            for (int p = 0; p < 2; ++p) *reinterpret_cast<v8s*>(lds + p * PLANE + k_at<DIM>(r, c)) = f.p[p];
+            if (c == 0) exponents[r] = ex;
+          }
+        }
+      } else if (PK == 2 && threadIdx.x < 32) {
+        exponents[threadIdx.x] = e_next;
+      }
       wait_lds();
       barrier();  // the keys are there (both buffers: the values too), what is loaded over is read
       const unsigned char *tk = lds + buf * (PK + P) * PLANE, *tv = tk + PK * PLANE;
       auto middle = [&]() {  // f32: the values are there, the keys read
+        if constexpr (DIRECT) return;
         wait_dma_all();
         wait_lds();
         barrier();
@@ -456,9 +490,9 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
           e_next = exponent(t0 + KT);
         }
       };
-      if constexpr (BUFS == 1) {
+      if constexpr (BUFS == 1 && !DIRECT) {
         fetch(v, P, vtb, vo, t0, lds0 + PK * PLANE);
-      } else if (t0 + KT < keys) {
+      } else if (BUFS == 2 && t0 + KT < keys) {
         const uint32_t to = lds0 + (buf ^ 1) * (PK + P) * PLANE;
         fetch(k, PK, ktb, ko, t0 + KT, to);
         fetch(v, P, vtb, vo, t0 + KT, to + PK * PLANE);
@@ -614,8 +648,13 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
 
 using namespace bq;
 
+// f32 prompts of up to this many channels of a head (192 tokens of 64, 96 of 128) are split where they
+// are used. With a launch for it and without, us: 102 tokens, 12 heads of 64 16.1, 12.2; 256 tokens
+// 22.6, 21.9; 94 tokens, 16 heads of 128 20.1, 16.7; 128 tokens 20.3, 21.8; 512 tokens 43, 61.
+constexpr int64_t PROMPT_DIRECT = 12288;
+
 size_t bq_prompt_attention_ws_bytes(int type, int64_t n, int64_t heads, int64_t dim) {
-  if (type != 0 || n < 1 || heads < 1 || dim < 1) return 0;
+  if (type != 0 || n * dim <= PROMPT_DIRECT || heads < 1 || dim < 1) return 0;
   return (size_t)n * heads * (10 * dim + 4);  // two planes of k, three of v, an exponent a row of k
 }
 
@@ -650,6 +689,7 @@ int bq_prompt_attention(const void* q, const void* k, const void* v, int type, i
   const int64_t tiles = n / (halves ? 64 : 128) + begun;
   if (tiles * q_heads > 0x7fffffff) return set_error(BQ_ERR_ARG, "%s: size too large", what);
   const size_t need = bq_prompt_attention_ws_bytes(type, n, heads, dim);
+  const bool direct = type == 0 && !need;
   if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
     return set_error(BQ_ERR_ARG, "%s: a workspace of %zu bytes, given %zu", what, need, ws ? ws_bytes : 0);
   const Prompt a = {q, k, v, out, q_token, q_head, k_token, k_head, v_token, v_head, cu, (int)n, (int)B, (int)heads,
@@ -664,12 +704,12 @@ int bq_prompt_attention(const void* q, const void* k, const void* v, int type, i
     if (wide) prompt_split_kernel<128><<<(unsigned)blocks, 256, 0, st>>>(a);
     else prompt_split_kernel<64><<<(unsigned)blocks, 256, 0, st>>>(a);
   }
-#define BQ_PROMPT(T, PARTS)                                                                   \
-  (wide ? prompt_kernel<T, 128, PARTS><<<grid, PROMPT_WAVES * 64, 0, st>>>(a)               \
-        : prompt_kernel<T, 64, PARTS><<<grid, PROMPT_WAVES * 64, 0, st>>>(a))
-  if (type == 0) BQ_PROMPT(float, 1);
-  else if (type == 1) halves ? BQ_PROMPT(__bf16, 2) : BQ_PROMPT(__bf16, 1);
-  else halves ? BQ_PROMPT(_Float16, 2) : BQ_PROMPT(_Float16, 1);
+#define BQ_PROMPT(T, PARTS, DIRECT)                                                           \
+  (wide ? prompt_kernel<T, 128, PARTS, DIRECT><<<grid, PROMPT_WAVES * 64, 0, st>>>(a)         \
+        : prompt_kernel<T, 64, PARTS, DIRECT><<<grid, PROMPT_WAVES * 64, 0, st>>>(a))
+  if (type == 0) direct ? BQ_PROMPT(float, 1, true) : BQ_PROMPT(float, 1, false);
+  else if (type == 1) halves ? BQ_PROMPT(__bf16, 2, false) : BQ_PROMPT(__bf16, 1, false);
+  else halves ? BQ_PROMPT(_Float16, 2, false) : BQ_PROMPT(_Float16, 1, false);
 #undef BQ_PROMPT
   return check_launch(what);
 }

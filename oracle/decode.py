@@ -103,7 +103,8 @@ class Pages:
 
 def softmax_rows(q, k, v, seen, scale):
     """softmax(scale q k^T) v of q [r, d] over k, v [n, d], row i over seen[i] [n], in float64; zeros
-    for a row that sees nothing. Returns the output, the weights and sum_i p_i |v_i|."""
+    for a row that sees nothing, or only scores of -infinity. Returns the output, the weights and sum_i
+    p_i |v_i|."""
     q, k, v = q.double(), k.double(), v.double()
     out = torch.zeros(q.shape[0], v.shape[1], dtype=torch.float64)
     size = torch.zeros_like(out)
@@ -115,7 +116,7 @@ def softmax_rows(q, k, v, seen, scale):
         s = (k[at] * q[i]).sum(-1) * scale
         top = s.max()
         w = torch.exp(s - (top if torch.isfinite(top) else 0.0))
-        w = w / w.sum()
+        w = w / (w.sum() if w.sum() != 0 else 1.0)
         p[i, at] = w
         out[i] = (w[:, None] * v[at]).sum(0)
         size[i] = (w[:, None] * v[at].abs()).sum(0)

@@ -32,8 +32,9 @@ def test_prompt_refusals():
     assert call(n=0) == 0
     assert call(ptr=8) == ARG and "aligned" in _lib.last_error()
     assert call(ptr=16, strides=(255, 64, 128, 64, 128, 64)) == ARG
-    assert call(ptr=16) == ARG and "workspace" in _lib.last_error()
-    assert _lib.lib().bq_prompt_attention_ws_bytes(0, 4, 2, 64) > 0 == _lib.lib().bq_prompt_attention_ws_bytes(1, 4, 2, 64)
+    assert call(ptr=16, n=4000) == ARG and "workspace" in _lib.last_error()
+    ws = _lib.lib().bq_prompt_attention_ws_bytes
+    assert ws(0, 4000, 2, 64) > 0 == ws(1, 4000, 2, 64) == ws(0, 4, 2, 64)
     assert call(ptr=16, type=1, strides=(256, 64, 2 ** 23 + 8, 64, 128, 64)) == UNSUPPORTED
     assert call(ptr=16, n=2 ** 31 - 10000, hq=4096, h=2) == ARG and "large" in _lib.last_error()
 

@@ -182,6 +182,31 @@ def test_many_heads_not_finite(dev, kind, what, at):
     check(got[:, 4:6], want, tol)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("which", [2, 3])
+@pytest.mark.parametrize("what,at", [(math.nan, 40), (math.inf, 59), (-math.inf, 0)])
+def test_short_f32_not_finite(dev, dim, which, what, at):
+    """Short f32 prompts, whose tiles are split where they are used."""
+    print(f"prompt short dim={dim} operand {which}[{at}]={what}", flush=True)
+    x, cu = data([20, 60, 10], 2, 1, dim, "f32", 59)
+    clean = run(dev, x, cu, 2, 1, True)
+    x[20 + at, which, 5] = what
+    want, tol = expected(x, cu, 2, 1, True, "f32")
+    got = run(dev, x, cu, 2, 1, True)
+    unseen = [i for i in range(90) if i < 20 + at or i >= 80]
+    assert torch.equal(got[unseen], clean[unseen])
+    check(got, want, tol)
+
+
+@pytest.mark.parametrize("dim,n", [(64, 192), (64, 193), (128, 96), (128, 97)])
+def test_f32_either_side_of_the_split(dev, dim, n):
+    print(f"prompt f32 dim={dim} n={n}", flush=True)
+    x, cu = data([n - 33, 33], 6, 2, dim, "f32", n)
+    for causal in (True, False):
+        want, tol = expected(x, cu, 6, 2, causal, "f32")
+        check(run(dev, x, cu, 6, 2, causal), want, tol)
+
+
 @pytest.mark.parametrize("qs,ks", [(2.0 ** 100, 2.0 ** -98), (2.0 ** -120, 2.0 ** 118), (2.0 ** -140, 2.0 ** 30),
                                    (2.0 ** -10, 2.0 ** 8)])
 def test_f32_rows_of_any_size(dev, qs, ks):
