@@ -19,6 +19,10 @@
 // channel 2^-14 of the row's largest loses is 2^-38 of that largest), and of the four products three
 // are added: half the matrix work of the bf16 pieces, each product within 3 2^-22. Outputs that do not come out finite are taken again in plain f32 (plain_row), so that
 // infinities and NaN act as f32 has them, and only on the queries that see them.
+//
+// Bound by the MFMAs at the clock that they leave: 8192 tokens, 32 heads of 128 over 8, bf16, causal:
+// 520 to 575 us, 0.96 to 1.06 PFLOP/s, where the library's 8192^3 product reaches 1.21; 2048 and 1111
+// tokens, 16 heads of 128 over 4, f32: 146 us, nine 16-bit products for two.
 #include <math.h>
 
 #include "bq_bf16x3.h"

@@ -487,7 +487,7 @@ int bq_dequant_i8(const int8_t* q, int64_t N, int64_t K, const float* s, float* 
  * accumulation; f32 products as exact sums of bf16 pieces, to f32's accuracy (values below 2^-109
  * lose up to 2^-134); p rounded to the 16-bit types. What a query does not see never reaches its
  * output, infinities and NaN included. dim 64 or 128. Beside the path, as bq_attention_f32
- * (scaled_dot_product_attention, borch/_nn.py:2143-2170, with is_causal and enable_gqa). ws:
+ * (scaled_dot_product_attention, borch/_nn.py:2143-2170). ws:
  * bq_prompt_attention_ws_bytes bytes, 16-byte aligned (f32: the pieces of k and v, unless short; none for
  * the 16-bit types, whose rows of k and v lie at most 2^23 elements apart). */
 size_t bq_prompt_attention_ws_bytes(int type, int64_t n, int64_t heads, int64_t dim);

@@ -356,6 +356,18 @@ def test_evict_long_rows_moved(dev):
     check_evict(dev, c, table, [17500], sums, 600, 50)
 
 
+def test_evict_rows_of_odd_length(dev):
+    """Rows of weights that start at no multiple of 16 bytes, in one workgroup and in parts."""
+    print("kv4 evict odd rows", flush=True)
+    c, table = roomy(dev, [1001, 700], 2, 64, 32, 100, 13)
+    sums = torch.exp(2 * torch.randn(2, 2, 1001, generator=torch.Generator().manual_seed(2)))
+    check_evict(dev, c, table, [1001, 700], sums, 100, 7)
+    wide = torch.exp(2 * torch.randn(2, 2, 20003, generator=torch.Generator().manual_seed(3)))
+    wide[:, :, :1001] = sums
+    c, table = roomy(dev, [1001, 700], 2, 64, 32, 100, 13)
+    check_evict(dev, c, table, [1001, 700], wide, 100, 7)
+
+
 def test_evict_strided_sums(dev):
     print("kv4 evict strided", flush=True)
     c, table = roomy(dev, [70, 80], 2, 64, 32, 32, 3)
