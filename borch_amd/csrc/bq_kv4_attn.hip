@@ -271,44 +271,44 @@ constexpr int EDGE = 3;
 __device__ __forceinline__ int len_of(const Attend& a, int b) { return max(0, min(a.lens[b], a.max_len)); }
 __device__ __forceinline__ int units_of(int len) { return max(1, (len + UNIT - 1) / UNIT); }  // an empty one writes zeros
 
-// The line, sequence after sequence, per_b (heads times row groups) runs of each, EDGE places and then
-// its units: its length, and for `upto` < B the place where that sequence's begin.
-__device__ __forceinline__ int line_of(const Attend& a, int per_b, int upto, int* begin) {
+__device__ __forceinline__ int scan64(int v) {  // over the wave, this lane's with those before it
   const int lane = threadIdx.x & 63;
-  int all = 0, before = 0;
-  for (int b = lane; b < a.B; b += 64) {
-    const int u = (EDGE + units_of(len_of(a, b))) * per_b;
-    all += u;
-    before += b < upto ? u : 0;
-  }
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
-    all += __shfl_xor(all, d);
-    before += __shfl_xor(before, d);
+    const int y = __shfl_up(v, d);
+    if (lane >= d) v += y;
   }
-  *begin = __builtin_amdgcn_readfirstlane(before);
-  return __builtin_amdgcn_readfirstlane(all);
+  return v;
 }
-// The sequence in which place x of the line lies, and where its runs begin.
-__device__ __forceinline__ int sequence_of(const Attend& a, int per_b, int x, int* begin) {
+// The line: sequence after sequence, per_b (heads times row groups) runs of each, EDGE places and then
+// its units. Its length, and of the sequence `seq`, or of that in which place at(line) lies (seq < 0),
+// the number and the place where its runs begin. Up to 64 sequences are looked at once.
+template <typename F>
+__device__ __forceinline__ int line_of(const Attend& a, int per_b, int seq, F&& at, int* which, int* begin) {
   const int lane = threadIdx.x & 63;
-  int from = 0;
-  for (int b0 = 0;; b0 += 64) {
-    const int b = b0 + lane, mine = b < a.B ? (EDGE + units_of(len_of(a, b))) * per_b : 0;
-    int upto = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int y = __shfl_up(upto, d);
-      if (lane >= d) upto += y;
+  auto mine = [&](int b0) { return b0 + lane < a.B ? (EDGE + units_of(len_of(a, b0 + lane))) * per_b : 0; };
+  const int first = mine(0), upto0 = scan64(first);
+  int line = __builtin_amdgcn_readlane(upto0, 63);
+  for (int b0 = 64; b0 < a.B; b0 += 64) line += __builtin_amdgcn_readlane(scan64(mine(b0)), 63);
+  const int x = seq < 0 ? at(line) : 0;
+  int from = 0, u = first, upto = upto0;
+  *which = max(seq, 0);
+  *begin = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    if (b0) {
+      u = mine(b0);
+      upto = scan64(u);
     }
-    const uint64_t hit = __ballot(from + upto > x);
-    if (hit || b0 + 64 >= a.B) {
-      const int at = hit ? __builtin_ctzll(hit) : 0;
-      *begin = from + __builtin_amdgcn_readlane(upto - mine, at);
-      return min(b0 + at, a.B - 1);
+    const uint64_t hit = __ballot(seq < 0 ? from + upto > x : b0 + lane == seq);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      *which = b0 + l;
+      *begin = from + __builtin_amdgcn_readlane(upto - u, l);
+      break;
     }
     from += __builtin_amdgcn_readlane(upto, 63);
   }
+  return line;
 }
 __device__ __forceinline__ int share_of(const Attend& a, int line) { return max(a.least, (line + a.shares - 1) / a.shares); }
 
@@ -324,11 +324,10 @@ __global__ __launch_bounds__(256, 2) void kv4_attend_kernel(Attend a) {
   // this workgroup's places x0 .. x1 of the line
   int x0, x1, b, begin;
   if (a.shares) {
-    const int line = line_of(a, per_b, 0, &begin), share = share_of(a, line);
-    x0 = blockIdx.x * share;
+    const int line = line_of(a, per_b, -1, [&](int n) { return (int)blockIdx.x * share_of(a, n); }, &b, &begin);
+    x0 = blockIdx.x * share_of(a, line);
     if (x0 >= line) return;
-    x1 = min(line, x0 + share);
-    b = sequence_of(a, per_b, x0, &begin);
+    x1 = min(line, x0 + share_of(a, line));
   } else {
     b = blockIdx.x / per_b;
     const int run = EDGE + units_of(len_of(a, b));
@@ -351,9 +350,29 @@ __global__ __launch_bounds__(256, 2) void kv4_attend_kernel(Attend a) {
     const int sure = len - a.tokens + 1;  // tokens that every row sees
     const int blocks = (len + 31) >> 5;
 
+    // up to 64 units at a time: this wave's block of each, their pages one a lane; the first block's
+    // codes are on their way while the queries are split
+    int first, mine, pages;
+    KBlock<DIM> k0, k1;
+    VBlock<DIM> v0, v1;
+    auto fetch = [&](int i, KBlock<DIM>& k, VBlock<DIM>& v) {
+      const int blk = first + 4 * i;
+      const int at = max(0, __builtin_amdgcn_readlane(pages, i));
+      const int off0 = (blk - fdiv(blk, a.c.by_blocks.mul, a.c.by_blocks.shift) * bpp) << 5;
+      k.load(a.c, at, h, off0);
+      v.load(a.c, at, h, off0);
+    };
+    auto look = [&](int w0) {
+      first = 4 * w0 + wave;
+      mine = min(min(64, u1 - w0), blocks > first ? (blocks - first + 3) >> 2 : 0);
+      pages = -1;
+      if (lane < mine) pages = kv4_page(a.c, seq, fdiv(first + 4 * lane, a.c.by_blocks.mul, a.c.by_blocks.shift));
+      if (mine > 0) fetch(0, k0, v0);
+    };
+    look(u0);
     q.fill(a, seq, h, row0);  // every wave has left the last run's: the join's barriers
     int end[RT];              // what this lane's row sees
-    bool lost[RT];  // whether it sees a NaN value in its channels that left the products
+    bool lost[RT];            // whether it sees a NaN value in its channels that left the products
     float m[RT], l[RT];
     v4f o[RT][NJ];
 #pragma unroll
@@ -366,22 +385,10 @@ __global__ __launch_bounds__(256, 2) void kv4_attend_kernel(Attend a) {
 #pragma unroll
       for (int j = 0; j < NJ; ++j) o[r][j] = v4f{0.f, 0.f, 0.f, 0.f};
     }
-
     __syncthreads();
 
-    // 64 units at a time: this wave's block of each, their pages one a lane
     for (int w0 = u0; w0 < u1; w0 += 64) {
-      const int first = 4 * w0 + wave;
-      const int mine = min(min(64, u1 - w0), blocks > first ? (blocks - first + 3) >> 2 : 0);
-      int pages = -1;
-      if (lane < mine) pages = kv4_page(a.c, seq, fdiv(first + 4 * lane, a.c.by_blocks.mul, a.c.by_blocks.shift));
-      auto fetch = [&](int i, KBlock<DIM>& k, VBlock<DIM>& v) {
-        const int blk = first + 4 * i;
-        const int at = max(0, __builtin_amdgcn_readlane(pages, i));
-        const int off0 = (blk - fdiv(blk, a.c.by_blocks.mul, a.c.by_blocks.shift) * bpp) << 5;
-        k.load(a.c, at, h, off0);
-        v.load(a.c, at, h, off0);
-      };
+      if (w0 > u0) look(w0);
       auto body = [&](int i, const KBlock<DIM>& kb, VBlock<DIM>& vb) {
         const int tok = (first + 4 * i) << 5;
         if (__builtin_amdgcn_readlane(pages, i) < 0) return;  // no page: nothing to see
@@ -459,9 +466,6 @@ __global__ __launch_bounds__(256, 2) void kv4_attend_kernel(Attend a) {
           product.template operator()<3>();
         }
       };
-      KBlock<DIM> k0, k1;
-      VBlock<DIM> v0, v1;
-      if (mine > 0) fetch(0, k0, v0);
       for (int i = 0; i < mine; i += 2) {
         if (i + 1 < mine) fetch(i + 1, k1, v1);
         body(i, k0, v0);
@@ -535,8 +539,8 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attend a) {
   const int row = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int rg = row / (16 * RT), units = units_of(len_of(a, b));
-  int begin;
-  const int share = share_of(a, line_of(a, a.c.heads * a.row_groups, b, &begin));
+  int begin, seq;
+  const int share = share_of(a, line_of(a, a.c.heads * a.row_groups, b, [](int) { return 0; }, &seq, &begin));
   begin += (h * a.row_groups + rg) * (EDGE + units) + EDGE;
   const int w0 = begin / share, w1 = (begin + units - 1) / share;
   if (w0 == w1) return;  // whole in one share, and written there
@@ -638,11 +642,11 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(Attend a) {
     }
     float s[1][8];
     kb.template scores<T, 1>(q, s);
-    const float base = base_of(st.x);
+    const float base = base_of(st.x), part = __fdiv_rn(1.f, st.y);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (tok + 8 * g + e < end)
-        total[e] = __fadd_rn(total[e], __fdiv_rn(weight_of(s[0][e], base, a.scale2), st.y));
+        total[e] = __fmaf_rn(weight_of(s[0][e], base, a.scale2), part, total[e]);
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
