@@ -35,7 +35,6 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef short v8s __attribute__((ext_vector_type(8)));
 
-constexpr int PROMPT_WAVES = 4;
 
 struct Prompt {
   const void *q, *k, *v;
@@ -287,14 +286,14 @@ __device__ __forceinline__ void store_rows(const Prompt& a, const Place& at, int
 // Takes the values that are not finite out of a staged tile of v, which some query sees in part (they
 // would meet that query's weights of 0), and returns whether the lane's query sees one: it sees
 // the tile's first `sees` tokens. By the whole workgroup; found [KT].
-template <typename T, int DIM, int KT>
+template <typename T, int DIM, int KT, int WAVES>
 __device__ __attribute__((noinline)) bool clear_values(unsigned char* v, int* found, int sees) {
   constexpr int P = Kind<T>::P, PLANE = KT * DIM * 2;
   constexpr uint32_t E = __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
   if (threadIdx.x < KT) found[threadIdx.x] = 0;
   wait_lds();
   barrier();
-  for (int x = threadIdx.x; x < KT * DIM / 2; x += PROMPT_WAVES * 64) {  // two values
+  for (int x = threadIdx.x; x < KT * DIM / 2; x += WAVES * 64) {  // two values
     const int r = x / (DIM / 2), at = v_at<DIM>(r, x % (DIM / 2) / 4) + x % 4 * 4;
     const uint32_t w = *reinterpret_cast<const uint32_t*>(v + at);
     const uint32_t keep = ((w & E) == E ? 0u : 0xffffu) | ((w & (E << 16)) == (E << 16) ? 0u : 0xffff0000u);
@@ -349,21 +348,22 @@ __global__ __launch_bounds__(256) void prompt_split_kernel(Prompt a) {
 // 16-bit types hold two tiles, the next one's loads under this one's products, one barrier a tile.
 // f32 holds one (40 KB of planes at dim 128, so that two workgroups share a CU): the next keys load
 // under this tile's second product, the next values under the next tile's first, two barriers.
-// PARTS = 2 (16-bit types): 64 queries a workgroup, and two waves take one half of each tile's keys each
-// for the same 32 queries, joined in LDS at the end: twice the workgroups, each half as long, where 128
-// queries a workgroup leave the GPU part empty. Heads of 64 take tiles of 128 keys then, so that a wave
-// has as much of a tile as without (2048 tokens, 16 heads, f16: 29 -> 25 us).
+// PARTS = 2: two waves take one half of each tile's keys each for the same 32 queries, joined in LDS at
+// the end, where 128 queries a workgroup of four waves leave the GPU part empty. Four waves have 64
+// queries then, in twice the workgroups, each half as long. (Heads of 64 in 16 bits take tiles of 128 keys, so
+// that a wave has as much of a tile as without: 2048 tokens, 16 heads, f16: 29 -> 25 us.) f32 heads of 128,
+// whose tile of 64 keys fills half of LDS, take eight waves and 128 queries.
 // DIRECT (f32, short prompts): the workgroup splits its tiles itself, and no launch goes before.
-template <typename T, int DIM, int PARTS, bool DIRECT>
-__global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) {
-  constexpr int P = Kind<T>::P, PK = Kind<T>::PK, KT = P == 3 ? 32 : PARTS == 2 && DIM == 64 ? 128 : 64;
+template <typename T, int DIM, int PARTS, bool DIRECT, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
+  constexpr int P = Kind<T>::P, PK = Kind<T>::PK, KT = P == 3 ? 32 * PARTS : PARTS == 2 && DIM == 64 ? 128 : 64;
   constexpr int SUB = KT / 32 / PARTS, BUFS = P == 3 ? 1 : 2;
-  constexpr int ALL = 32 * PROMPT_WAVES / PARTS;  // queries a workgroup
+  constexpr int ALL = 32 * WAVES / PARTS;  // queries a workgroup
   constexpr int STEPS = DIM / 16, VT = DIM / 32, PLANE = KT * DIM * 2;
   constexpr int ROWS = 1024 / (DIM * 2);         // of a wave's load
-  constexpr int PER = KT / ROWS / PROMPT_WAVES;  // loads a wave and plane
+  constexpr int PER = KT / ROWS / WAVES;  // loads a wave and plane
   __shared__ __attribute__((aligned(1024))) unsigned char lds[BUFS * (PK + P) * PLANE];
-  __shared__ __attribute__((aligned(16))) int exponents[32];  // f32: of the tile's keys
+  __shared__ __attribute__((aligned(16))) int exponents[KT];  // f32: of the tile's keys
   __shared__ int found[KT];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hh = lane >> 5;
   Place at;
@@ -431,7 +431,7 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
     }
   }
   const int* row_e = PK == 2 ? a.exponents + (size_t)h * a.n + at.start : nullptr;
-  auto exponent = [&](int t0) { return PK == 2 && !DIRECT && threadIdx.x < 32 && t0 + (int)threadIdx.x < len ? row_e[t0 + threadIdx.x] : 0; };
+  auto exponent = [&](int t0) { return PK == 2 && !DIRECT && threadIdx.x < KT && t0 + (int)threadIdx.x < len ? row_e[t0 + threadIdx.x] : 0; };
   float m, l;
   v16f o[VT];
   // Once; and where an output is not finite once more, with the values that are not out of the tiles
@@ -453,9 +453,9 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
       if constexpr (DIRECT) {
         barrier();  // the last tile is read
 #pragma unroll
-        for (int e = 0; e < 2 * KT * DIM / 8 / (PROMPT_WAVES * 64); ++e) {
+        for (int e = 0; e < 2 * KT * DIM / 8 / (WAVES * 64); ++e) {
           constexpr int HALF = KT * DIM / 8;  // pieces of eight of k, then of v
-          const int id = threadIdx.x + e * PROMPT_WAVES * 64, r = id % HALF / (DIM / 8), c = id % (DIM / 8);
+          const int id = threadIdx.x + e * WAVES * 64, r = id % HALF / (DIM / 8), c = id % (DIM / 8);
           const bool is_v = id >= HALF;
           float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
           if (t0 + r < len) {
@@ -480,7 +480,7 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
             if (c == 0) exponents[r] = ex;
           }
         }
-      } else if (PK == 2 && threadIdx.x < 32) {
+      } else if (PK == 2 && threadIdx.x < KT) {
         exponents[threadIdx.x] = e_next;
       }
       wait_lds();
@@ -507,7 +507,7 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
       const int tw = t0 + 32 * SUB * part;  // this wave's first key of the tile
       if (tw >= wkeys) {
         if constexpr (BUFS == 1) middle();
-        if (clears) clear_values<T, DIM, KT>(const_cast<unsigned char*>(tv), found, 0);
+        if (clears) clear_values<T, DIM, KT, WAVES>(const_cast<unsigned char*>(tv), found, 0);
         continue;
       }
 
@@ -541,7 +541,7 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
         __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int4 e = *reinterpret_cast<const int4*>(exponents + 8 * i + 4 * hh);
+          const int4 e = *reinterpret_cast<const int4*>(exponents + 32 * SUB * part + 8 * i + 4 * hh);
           s[0][4 * i] = __builtin_ldexpf(s[0][4 * i], e.x + q_e);
           s[0][4 * i + 1] = __builtin_ldexpf(s[0][4 * i + 1], e.y + q_e);
           s[0][4 * i + 2] = __builtin_ldexpf(s[0][4 * i + 2], e.z + q_e);
@@ -586,7 +586,7 @@ __global__ __launch_bounds__(PROMPT_WAVES * 64, 2) void prompt_kernel(Prompt a) 
       if constexpr (P == 1) odd |= fabsf(shift) > 0x1p24f;
       if constexpr (BUFS == 1) middle();
 
-      if (clears) odd |= clear_values<T, DIM, KT>(const_cast<unsigned char*>(tv) - part * 32 * SUB * DIM * 2, found, sees - t0);
+      if (clears) odd |= clear_values<T, DIM, KT, WAVES>(const_cast<unsigned char*>(tv) - part * 32 * SUB * DIM * 2, found, sees - t0);
 
       // O^T += v^T p^T
 #pragma unroll
@@ -687,15 +687,22 @@ int bq_prompt_attention(const void* q, const void* k, const void* v, int type, i
   if (k_token < 0 || v_token < 0 || k_token > 1 << 23 || v_token > 1 << 23)  // a tile's rows within 32 bits
     return set_error(BQ_ERR_UNSUPPORTED, "%s: rows of k or v too far apart", what);
   // whatever the lengths are: a full tile for every 128 rows and one begun for each sequence
+  const bool direct = type == 0 && n * dim <= PROMPT_DIRECT;
   const int64_t begun = B + 2 < n ? B + 2 : n;
-  // 128 queries a workgroup would give at most two to a CU: half as many queries (PARTS). bf16, causal, us
-  // (128, 64): 2048 + 1111 tokens of 16 heads 57, 49; 1024 of 32: 28, 25; 2048 of 32: 57, 56; 3000 of
-  // 32: 87, 110; heads of 64: 2048 of 16: 34, 28
-  const bool halves = type != 0 && (n + 127) / 128 * q_heads <= 512;
+  // The form (prompt_kernel's PARTS), by the workgroups of 128 queries that there would be, two of
+  // which a CU holds at once. us in one part and in two, causal:
+  //   16 bits, up to 512: bf16, 128 channels, 2048 + 1111 tokens of 16 heads (400) 57, 49; 1024 of 32 (256)
+  //     28, 25; 2048 of 32 (512) 57, 56; 3000 of 32 (752) 87, 110; f16, 64 channels, 2048 of 16 (256) 34, 25
+  //   f32, up to 768: 64 channels, 2048 + 1111 of 16 (400) 119, 84; 2048 of 32 (512) 122, 97; 4096 of 32
+  //     (1024) 305, 318; 128 channels, and sequences of 256 tokens on average or more: 2048 + 1111 of 16
+  //     159, 137; 2048 of 32 176, 161; 5542 in 8 of 16 (704) 260, 249; 4096 of 32 556, 570; 30 of 130
+  //     tokens of 8 heads 40, 50
+  const int64_t groups = (n + 127) / 128 * q_heads;
+  const bool wide = dim == 128, two = type ? groups <= 512 : !direct && groups <= 768 && (!wide || n >= 256 * B);
+  const bool eight = two && !type && wide, halves = two && !eight;
   const int64_t tiles = n / (halves ? 64 : 128) + begun;
   if (tiles * q_heads > 0x7fffffff) return set_error(BQ_ERR_ARG, "%s: size too large", what);
   const size_t need = bq_prompt_attention_ws_bytes(type, n, heads, dim);
-  const bool direct = type == 0 && !need;
   if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
     return set_error(BQ_ERR_ARG, "%s: a workspace of %zu bytes, given %zu", what, need, ws ? ws_bytes : 0);
   const Prompt a = {q, k, v, out, q_token, q_head, k_token, k_head, v_token, v_head, cu, (int)n, (int)B, (int)heads,
@@ -703,19 +710,29 @@ int bq_prompt_attention(const void* q, const void* k, const void* v, int type, i
                     (int*)((char*)ws + (size_t)10 * n * heads * dim)};
   const unsigned grid = (unsigned)(tiles * q_heads);
   hipStream_t st = (hipStream_t)stream;
-  const bool wide = dim == 128;
   if (need) {
     const int64_t blocks = (n * 2 * heads * (dim / 8) + 255) / 256;
     if (blocks > 0x7fffffff) return set_error(BQ_ERR_ARG, "%s: size too large", what);
     if (wide) prompt_split_kernel<128><<<(unsigned)blocks, 256, 0, st>>>(a);
     else prompt_split_kernel<64><<<(unsigned)blocks, 256, 0, st>>>(a);
   }
-#define BQ_PROMPT(T, PARTS, DIRECT)                                                           \
-  (wide ? prompt_kernel<T, 128, PARTS, DIRECT><<<grid, PROMPT_WAVES * 64, 0, st>>>(a)         \
-        : prompt_kernel<T, 64, PARTS, DIRECT><<<grid, PROMPT_WAVES * 64, 0, st>>>(a))
-  if (type == 0) direct ? BQ_PROMPT(float, 1, true) : BQ_PROMPT(float, 1, false);
-  else if (type == 1) halves ? BQ_PROMPT(__bf16, 2, false) : BQ_PROMPT(__bf16, 1, false);
-  else halves ? BQ_PROMPT(_Float16, 2, false) : BQ_PROMPT(_Float16, 1, false);
+#define BQ_PROMPT(T, PARTS, DIRECT)                                                          \
+  do {                                                                                       \
+    if (wide) prompt_kernel<T, 128, PARTS, DIRECT, 4><<<grid, 256, 0, st>>>(a);              \
+    else prompt_kernel<T, 64, PARTS, DIRECT, 4><<<grid, 256, 0, st>>>(a);                    \
+  } while (0)
+  if (type == 0) {
+    if (direct) BQ_PROMPT(float, 1, true);
+    else if (eight) prompt_kernel<float, 128, 2, false, 8><<<grid, 512, 0, st>>>(a);
+    else if (halves) prompt_kernel<float, 64, 2, false, 4><<<grid, 256, 0, st>>>(a);
+    else BQ_PROMPT(float, 1, false);
+  } else if (type == 1) {
+    if (halves) BQ_PROMPT(__bf16, 2, false);
+    else BQ_PROMPT(__bf16, 1, false);
+  } else {
+    if (halves) BQ_PROMPT(_Float16, 2, false);
+    else BQ_PROMPT(_Float16, 1, false);
+  }
 #undef BQ_PROMPT
   return check_launch(what);
 }

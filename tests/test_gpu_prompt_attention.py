@@ -167,6 +167,24 @@ def test_many_heads(dev, kind, dim, causal):
         check(got[:, j:j + 2], want, tol)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("what", [None, math.nan, math.inf])
+@pytest.mark.parametrize("lens,causal", [([600, 450], True), ([333, 7, 500], False), ([64] * 8, True)])
+def test_f32_forms(dev, dim, what, lens, causal):
+    """f32 prompts of several tiles, long and short sequences on average: one wave or two a query."""
+    print(f"prompt f32 forms dim={dim} lens={lens} causal={causal} {what}", flush=True)
+    x, cu = data(lens, 2, 1, dim, "f32", 61)
+    if what is not None:
+        at = lens[0] // 2 + 5
+        clean = run(dev, x, cu, 2, 1, causal)
+        x[at, 3, 9] = what
+        unseen = [i for i in range(sum(lens)) if i >= lens[0] or (causal and i < at)]
+        got = run(dev, x, cu, 2, 1, causal)
+        assert torch.equal(got[unseen], clean[unseen])
+    want, tol = expected(x, cu, 2, 1, causal, "f32")
+    check(run(dev, x, cu, 2, 1, causal), want, tol)
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("what,at", [(math.nan, 70), (math.inf, 149), (-math.inf, 3)])
 def test_many_heads_not_finite(dev, kind, what, at):
