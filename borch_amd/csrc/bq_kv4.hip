@@ -677,10 +677,10 @@ size_t bq_kv4_evict_ws_bytes(int64_t B, int64_t heads, int64_t most, int64_t kee
   return parts ? rows * (parts * (4096 * 2 + 4) + EVICT_LIST * 8 + 8 + 4) : 0;
 }
 
-int bq_kv4_evict(const bq_kv4_cache* cache, const float* sums, int64_t sums_b, int64_t sums_h, int64_t most, const int32_t* table, int64_t B,
-                 int64_t width, const int32_t* lens, const int32_t* new_table, int64_t new_width, int64_t keep,
-                 int64_t recent, int32_t* kept, float* weights, int32_t* left, void* ws, size_t ws_bytes,
-                 bq_stream_t stream) {
+int bq_kv4_evict(const bq_kv4_cache* cache, const float* sums, int64_t sums_b, int64_t sums_h, int64_t most,
+                 const int32_t* table, int64_t B, int64_t width, const int32_t* lens, const int32_t* new_table,
+                 int64_t new_width, int64_t keep, int64_t recent, int32_t* kept, float* weights, int32_t* left,
+                 void* ws, size_t ws_bytes, bq_stream_t stream) {
   const char* what = "bq_kv4_evict";
   Kv4 c, to;
   if (const int rc = kv4_of(what, cache, table, B, width, &c)) return rc;

@@ -17,12 +17,14 @@
 // added: a small weight on a large value keeps its bits. In the scores only the sum over the channels
 // counts, so q and k are two fp16 pieces each, 22 bits below a power of two of their row (what a
 // channel 2^-14 of the row's largest loses is 2^-38 of that largest), and of the four products three
-// are added: half the matrix work of the bf16 pieces, each product within 3 2^-22. Outputs that do not come out finite are taken again in plain f32 (plain_row), so that
-// infinities and NaN act as f32 has them, and only on the queries that see them.
+// are added: half the matrix work of the bf16 pieces, each product within 3 2^-22. Outputs that do not
+// come out finite, or in f32 below 2^-109 (zero aside), where the up to 2^-134 that the pieces take from
+// such a value is more than a rounding, are taken again in plain f32 (plain_row): infinities and NaN act
+// as f32 has them, and only on the queries that see them.
 //
 // Bound by the MFMAs at the clock that they leave: 8192 tokens, 32 heads of 128 over 8, bf16, causal:
 // 520 to 575 us, 0.96 to 1.06 PFLOP/s, where the library's 8192^3 product reaches 1.21; 2048 and 1111
-// tokens, 16 heads of 128 over 4, f32: 146 us, nine 16-bit products for two.
+// tokens, 16 heads of 128 over 4, f32: 136 us, nine 16-bit products for two.
 #include <math.h>
 
 #include "bq_bf16x3.h"
@@ -35,14 +37,13 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef short v8s __attribute__((ext_vector_type(8)));
 
-
 struct Prompt {
   const void *q, *k, *v;
   void* out;
   int64_t qt, qh, kt, kh, vt, vh;  // strides in elements
   const int* cu;
   int n, B, heads, group, tiles, causal;
-  float scale2;  // scale * log2(e)
+  float scale2;    // scale * log2(e)
   void* ws;        // f32: the planes of k, then of v
   int* exponents;  // and of each row of k
 };
@@ -276,8 +277,9 @@ __device__ __forceinline__ void store_rows(const Prompt& a, const Place& at, int
   for (int i = 0; i < 32; ++i)
     if ((again >> i) & 1) {
       const int64_t q = at.start + row0 + i;
-      plain_row<T, DIM>((const T*)a.q + q * a.qt + at.head * a.qh, (const T*)a.k + (int64_t)at.start * a.kt + h * a.kh, a.kt,
-                        (const T*)a.v + (int64_t)at.start * a.vt + h * a.vh, a.vt,
+      const T* k = (const T*)a.k + (int64_t)at.start * a.kt + h * a.kh;
+      const T* v = (const T*)a.v + (int64_t)at.start * a.vt + h * a.vh;
+      plain_row<T, DIM>((const T*)a.q + q * a.qt + at.head * a.qh, k, a.kt, v, a.vt,
                         (T*)a.out + (q * (a.heads * a.group) + at.head) * DIM,
                         a.causal ? min(at.len, row0 + i + 1) : at.len, a.scale2);
     }
@@ -431,7 +433,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
     }
   }
   const int* row_e = PK == 2 ? a.exponents + (size_t)h * a.n + at.start : nullptr;
-  auto exponent = [&](int t0) { return PK == 2 && !DIRECT && threadIdx.x < KT && t0 + (int)threadIdx.x < len ? row_e[t0 + threadIdx.x] : 0; };
+  auto exponent = [&](int t0) {
+    const int t = t0 + threadIdx.x;
+    return PK == 2 && !DIRECT && threadIdx.x < KT && t < len ? row_e[t] : 0;
+  };
   float m, l;
   v16f o[VT];
   // Once; and where an output is not finite once more, with the values that are not out of the tiles
@@ -460,7 +465,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
           float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
           if (t0 + r < len) {
             const int64_t at_row = at.start + t0 + r;
-            load8((is_v ? (const float*)a.v + at_row * a.vt + h * a.vh : (const float*)a.k + at_row * a.kt + h * a.kh) + 8 * c, x);
+            const float* from = is_v ? (const float*)a.v + at_row * a.vt + h * a.vh
+                                     : (const float*)a.k + at_row * a.kt + h * a.kh;
+            load8(from + 8 * c, x);
           }
           if (is_v) {
             const Frag<3> f = frag_of<float>(x);
@@ -586,7 +593,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
       if constexpr (P == 1) odd |= fabsf(shift) > 0x1p24f;
       if constexpr (BUFS == 1) middle();
 
-      if (clears) odd |= clear_values<T, DIM, KT, WAVES>(const_cast<unsigned char*>(tv) - part * 32 * SUB * DIM * 2, found, sees - t0);
+      if (clears)
+        odd |= clear_values<T, DIM, KT, WAVES>(const_cast<unsigned char*>(tv) - part * 32 * SUB * DIM * 2, found, sees - t0);
 
       // O^T += v^T p^T
 #pragma unroll
@@ -641,6 +649,14 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) zero = __fmaf_rn(o[d][i], 0.f, zero);
     odd |= zero != 0.f;
+    if constexpr (P == 3) {
+      uint32_t least = ~0u;  // |o| as an integer, 0 as the largest
+#pragma unroll
+      for (int d = 0; d < VT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) least = min(least, (__float_as_uint(o[d][i]) << 1) - 1u);
+      odd |= least < (__float_as_uint(__fmul_rn(l, 0x1p-109f)) << 1) - 1u;
+    }
     odd = odd && row < len && part == 0;
     if (again || !__syncthreads_or(odd)) break;
     odd = false;

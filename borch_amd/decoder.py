@@ -135,6 +135,8 @@ class DecoderState:
 
     def evict(self, keep: int, recent: int = 0) -> None:
         """Every sequence down to ``keep`` tokens a head, in every layer (``Cache4.evict``)."""
+        if keep >= self.longest:
+            return
         width = -(-keep // self.page)
         fresh = [[self.free.pop() for _ in range(width)] for _ in range(self.sequences)]
         table = self._ints(fresh)

@@ -483,13 +483,12 @@ int bq_dequant_i8(const int8_t* q, int64_t N, int64_t K, const float* s, float* 
  * dim]; query head j attends with key-value head j / (q_heads / heads).
  *   out [n, q_heads, dim] (contiguous, of q's type) = softmax(scale q k^T) v
  * over the sequence's rows, causal: up to the query's own. Rows of no sequence, or whose scores are all
- * -infinity, get zeros. f32
- * accumulation; f32 products as exact sums of bf16 pieces, to f32's accuracy (values below 2^-109
- * lose up to 2^-134); p rounded to the 16-bit types. What a query does not see never reaches its
- * output, infinities and NaN included. dim 64 or 128. Beside the path, as bq_attention_f32
- * (scaled_dot_product_attention, borch/_nn.py:2143-2170). ws:
- * bq_prompt_attention_ws_bytes bytes, 16-byte aligned (f32: the pieces of k and v, unless short; none for
- * the 16-bit types, whose rows of k and v lie at most 2^23 elements apart). */
+ * -infinity, get zeros. f32 accumulation; f32 products as sums of 16-bit pieces, to f32's accuracy; p
+ * rounded to the 16-bit types. What a query does not see changes no bit of its output, infinities and
+ * NaN included; queries that see such values are computed again, so a call with them takes longer.
+ * dim 64 or 128. ws: bq_prompt_attention_ws_bytes bytes, 16-byte aligned (f32: the pieces of k and v,
+ * unless short; none for the 16-bit types, whose rows of k and v lie at most 2^23 elements apart).
+ * Beside the path, as bq_attention_f32 (scaled_dot_product_attention, borch/_nn.py:2143-2170). */
 size_t bq_prompt_attention_ws_bytes(int type, int64_t n, int64_t heads, int64_t dim);
 int bq_prompt_attention(const void* q, const void* k, const void* v, int type, int64_t n, int64_t q_heads,
                         int64_t heads, int64_t dim, int64_t q_token, int64_t q_head, int64_t k_token, int64_t k_head,

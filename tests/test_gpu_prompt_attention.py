@@ -225,6 +225,18 @@ def test_f32_either_side_of_the_split(dev, dim, n):
         check(run(dev, x, cu, 6, 2, causal), want, tol)
 
 
+@pytest.mark.parametrize("lens", [[40, 30], [400, 333]])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_f32_small_values(dev, dim, lens):
+    """Values that bf16 pieces cannot hold whole; flat scores, so that the tolerance is the sums' alone."""
+    print(f"prompt f32 small values dim={dim} lens={lens}", flush=True)
+    x, cu = data(lens, 2, 1, dim, "f32", 67)
+    x[:, :2] = 0
+    x[:, 3] *= 2.0 ** -119
+    want, tol = expected(x, cu, 2, 1, True, "f32")
+    check(run(dev, x, cu, 2, 1, True), want, tol)
+
+
 @pytest.mark.parametrize("qs,ks", [(2.0 ** 100, 2.0 ** -98), (2.0 ** -120, 2.0 ** 118), (2.0 ** -140, 2.0 ** 30),
                                    (2.0 ** -10, 2.0 ** 8)])
 def test_f32_rows_of_any_size(dev, qs, ks):
