@@ -77,7 +77,7 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4 c, const T* __restr
   int at = -1, off = 0;
   if (lo < B) {  // else past the last sequence
     const int64_t pos = (int64_t)lens[lo] - cu[lo + 1] + i;
-    if (pos >= 0 && pos < (int64_t)c.width * c.page) {
+    if (i >= cu[lo] && pos >= 0 && pos < (int64_t)c.width * c.page) {  // else before the first
       const int pi = fdiv((int)pos, c.by_page.mul, c.by_page.shift);
       at = kv4_page(c, lo, pi);
       off = (int)pos - pi * c.page;

@@ -512,9 +512,10 @@ typedef struct bq_kv4_cache {
 } bq_kv4_cache;
 
 /* New tokens into the cache: new_k, new_v [n, heads, dim], sequence b's the rows cu[b] .. cu[b + 1]
- * - 1, the last ones of its lens[b] tokens (lens counts them). Each 32 channels take the least
- * exponent (byte >= 1) that brings the largest magnitude to 6 or below, the codes round to nearest,
- * ties to even; a block with a value that is not finite gets byte 255. */
+ * - 1, the last ones of its lens[b] tokens (lens counts them); rows of no sequence are not written.
+ * Each 32 channels take the least exponent (byte >= 1) that brings the largest magnitude to 6 or
+ * below, the codes round to nearest, ties to even; a block with a value that is not finite gets byte
+ * 255. */
 int bq_kv4_append(const bq_kv4_cache* cache, const void* new_k, const void* new_v, int type, int64_t n,
                   int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, const int32_t* table, int64_t B,
                   int64_t width, const int32_t* lens, const int32_t* cu, bq_stream_t stream);

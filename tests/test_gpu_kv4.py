@@ -84,6 +84,19 @@ def test_append_and_read(dev, kind, dim, h, page, lens, new):
     assert torch.equal(k2.cpu(), k.cpu()[:, :, :2])
 
 
+def test_append_rows_of_no_sequence(dev):
+    """Rows before the first sequence and past the last one: what the cache held stays."""
+    print("kv4 append rows of no sequence", flush=True)
+    lens, h, dim, page = [40, 33, 70], 2, 64, 32
+    c, table, ln, _ = filled(dev, lens, h, dim, page, 37)
+    ref = D.Pages(c.k, c.k_scales, c.v, c.v_scales)
+    x = values(19, h, dim, "f32", 12)
+    cu = torch.tensor([6, 9, 9, 14], dtype=torch.int32)
+    c.append(x[:, :h].to(dev), x[:, h:].to(dev), table.to(dev), ln.to(dev), cu.to(dev))
+    ref.append(x[:, :h], x[:, h:], table, ln, cu)
+    same_pages(c, ref)
+
+
 def test_append_extremes(dev):
     """Rounding ties, signed zeros, exponents at both ends, blocks that are not finite."""
     print("kv4 extremes", flush=True)
