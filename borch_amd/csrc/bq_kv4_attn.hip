@@ -100,15 +100,38 @@ __device__ __forceinline__ void load8f(const T* p, float x[8]) {
 }
 
 // q's pieces as the score product's second operand: rows row0 .. + 15, step s, of lane (n, g) row
-// row0 + n, channels DIM / 4 g + 8 s ..; rows past the last as zeros.
+// row0 + n, channels DIM / 4 g + 8 s ..; rows past the last as zeros. An infinity stays one (inf - inf
+// left NaN in the second piece), and what f32 holds above bf16's largest value does not become one.
 template <typename T, int DIM>
 __device__ __forceinline__ Pieces<Q_PIECES<T>> q_frag(const Attend& a, int b, int h, int row0, int s) {
+  constexpr int P = Q_PIECES<T>;
   const int lane = threadIdx.x & 63, row = row0 + (lane & 15), g = lane >> 4;
   const int t = fdiv(row, a.by_group.mul, a.by_group.shift), j = row - t * a.group;
   float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (row < a.rows)
     load8f((const T*)a.q + b * a.qb + t * a.qt + (int64_t)(h * a.group + j) * a.qh + DIM / 4 * g + 8 * s, x);
-  return pieces_of<Q_PIECES<T>>(x);
+  Pieces<P> r = pieces_of<P>(x);
+  if constexpr (P > 1) {
+    constexpr float MOST = 0x1.fep127f;
+    float peak = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) peak = fmaxf(peak, fabsf(x[i]));
+    if (__any(peak > (P == 2 ? 65504.f : MOST))) {
+      float y[8], z[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool finite = fabsf(x[i]) < INFINITY;
+        y[i] = finite ? fminf(fmaxf(x[i], -MOST), MOST) : x[i];
+        y[i] = (float)(__bf16)y[i];
+        z[i] = finite ? __fsub_rn(x[i], y[i]) : 0.f;
+      }
+      r.p[0] = pieces_of<1>(y).p[0];
+      const Pieces<P - 1> rest = pieces_of<P - 1>(z);
+#pragma unroll
+      for (int k = 1; k < P; ++k) r.p[k] = rest.p[k - 1];
+    }
+  }
+  return r;
 }
 // The operands of RT row tiles in LDS, once for the four waves (in registers they took a third of
 // them in f32, and a wave a SIMD): a lane reads its own 16 bytes.
@@ -743,7 +766,8 @@ int bq_kv4_attend(const bq_kv4_cache* cache, const void* q, int type, int64_t to
   const int64_t rows = tokens * group;
   if (rows > 1 << 20) return set_error(BQ_ERR_ARG, "%s: size too large", what);
   const Cut cut = cut_of(B, cache->heads, rows, max_len);
-  if (B * cache->heads * cut.row_groups > 0x7fffffff / ((max_len + UNIT - 1) / UNIT + 1 + EDGE))
+  // the line and the places after its end that shares would begin at, within 32 bits
+  if (B * cache->heads * cut.row_groups > (0x7fffffff - 8 * MOST_SHARES) / ((max_len + UNIT - 1) / UNIT + 1 + EDGE))
     return set_error(BQ_ERR_ARG, "%s: size too large", what);
   if (!q || !lens || !out) return set_error(BQ_ERR_ARG, "%s: null pointer", what);
   const int64_t size = type == KV4_F32 ? 4 : 2;

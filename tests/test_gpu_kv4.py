@@ -258,6 +258,35 @@ def test_what_is_not_seen_does_not_count(dev, dim, which, bad):
     assert torch.equal(got[:, unseen], clean[:, unseen])
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attend_queries_at_the_ends(dev, kind, dim):
+    """The types' largest queries over small keys; infinite ones: all scores -infinity (zeros), else NaN."""
+    print(f"kv4 attend ends {kind} dim={dim}", flush=True)
+    n, top = 45, torch.finfo(TYPES[kind]).max
+    small = 2.0 ** -126 if kind != "f16" else 2.0 ** -14
+    x = values(n, 1, dim, "f32", 3)
+    x[:, 0] = torch.where(x[:, 0] < 0, -1.0, 1.0) * small * 2
+    x[:, 0, 5] = small * 2
+    table, pages = tables([n], 32, 2)
+    c = kv4.Cache4.zeros(pages, 1, 32, dim, dev)
+    ln = torch.tensor([n], dtype=torch.int32)
+    c.append(x[:, :1].to(dev), x[:, 1:].to(dev), table.to(dev), ln.to(dev), starts([n]).to(dev))
+    k, v, there = D.Pages(c.k, c.k_scales, c.v, c.v_scales).read(table, ln, n)
+    q = torch.zeros(1, 2, 2, dim)
+    q[0, 0, 0, 9], q[0, 0, 1, 40], q[0, 1, 0, 0], q[0, 1, 1, 5] = top, -top, top, top
+    q[0, 1, 0, 63] = top / 4
+    q = q.to(TYPES[kind])
+    check_attend(c.attend(q.to(dev), table.to(dev), ln.to(dev), scale=0.25), None, q, k, v, there, ln, n, kind, scale=0.25)
+    odd = torch.zeros(1, 1, 3, dim)
+    odd[0, 0, 0, 5], odd[0, 0, 1, 5], odd[0, 0, 2, 9] = -math.inf, math.inf, math.inf  # k of channel 5: all above 0
+    w = torch.zeros(1, 1, n, device=dev)
+    got = c.attend(odd.to(TYPES[kind]).to(dev)[:, :, :1], table.to(dev), ln.to(dev), max_len=n, weights=w).cpu()
+    assert not got.any() and not w.any()
+    got = c.attend(odd.to(TYPES[kind]).to(dev), table.to(dev), ln.to(dev)).cpu()
+    assert not got[:, :, 0].any() and bool(got[:, :, 1:].isnan().all())
+
+
 def check_evict(dev, c, table, lens, sums, keep, recent, spare_seed=5):
     B, h = len(lens), c.heads
     ln = torch.tensor(lens, dtype=torch.int32)
