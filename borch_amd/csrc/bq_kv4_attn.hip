@@ -154,6 +154,14 @@ struct QTile {
   }
 };
 
+// One row tile's in a wave's registers (the sums' kernel; f32, 128 rows over 16384 tokens: 61 -> 57 us
+// for the call, in LDS it took all of a CU's for 3 workgroups).
+template <typename T, int DIM>
+struct QRegs {
+  Pieces<Q_PIECES<T>> f[DIM / 32];
+  __device__ __forceinline__ v8bf at(int, int s, int k) const { return f[s].p[k]; }
+};
+
 __device__ __forceinline__ float scale_bits(uint32_t byte) { return __uint_as_float(byte << 23); }
 
 // Eight codes (one dword, low half byte first) times a scale, in bf16, exactly.
@@ -194,8 +202,8 @@ struct KBlock {
                                                 2 * (n >> 2));
   }
   // The scores of 16 rows a tile, before the scale: [4 t + i] is token 8 g + 4 t + i
-  template <typename T, int RT>
-  __device__ __forceinline__ void scores(const QTile<T, DIM, RT>& q, float (&s)[RT][8]) const {
+  template <typename T, int RT, typename Q>
+  __device__ __forceinline__ void scores(const Q& q, float (&s)[RT][8]) const {
     v8bf kf[2][DIM / 32];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -632,7 +640,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attend a) {
 // or 128 tokens (one); the rows of a tile are added over lanes, the tiles of a wave and the waves in order.
 template <typename T, int DIM, bool ONE>
 __global__ __launch_bounds__(256) void kv4_weights_kernel(Attend a) {
-  __shared__ QTile<T, DIM, 1> qs[ONE ? 1 : 4];
+  __shared__ QTile<T, ONE ? DIM : 32, 1> shared;  // one row tile: for the four waves; else unused
   __shared__ float sums[4][32];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int blk = ONE ? blockIdx.x * 4 + wave : blockIdx.x, h = blockIdx.y, b = blockIdx.z;
@@ -644,7 +652,7 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(Attend a) {
   KBlock<DIM> kb = {};
   if (at >= 0) kb.load(a.c, at, h, (blk - pi * (a.c.page >> 5)) << 5);
   if constexpr (ONE) {
-    qs[0].fill(a, b, h, 0);
+    shared.fill(a, b, h, 0);
     __syncthreads();
   }
   float total[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -654,17 +662,15 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(Attend a) {
     const int end = row < a.rows ? min(len, len - a.tokens + 1 + t) : 0;
     float2 st = make_float2(0.f, 1.f);
     if (row < a.rows) st = *reinterpret_cast<const float2*>(a.stats + (bh * a.rows + row) * 2);
-    QTile<T, DIM, 1>& q = qs[ONE ? 0 : wave];
-    if constexpr (!ONE) {  // the wave's own
-#pragma unroll
-      for (int s = 0; s < DIM / 32; ++s) {
-        const Pieces<Q_PIECES<T>> f = q_frag<T, DIM>(a, b, h, row0, s);
-#pragma unroll
-        for (int k = 0; k < Q_PIECES<T>; ++k) q.p[0][s][k][lane] = __builtin_bit_cast(uint4, f.p[k]);
-      }
-    }
     float s[1][8];
-    kb.template scores<T, 1>(q, s);
+    if constexpr (ONE) {
+      kb.template scores<T, 1>(shared, s);
+    } else {
+      QRegs<T, DIM> q;
+#pragma unroll
+      for (int i = 0; i < DIM / 32; ++i) q.f[i] = q_frag<T, DIM>(a, b, h, row0, i);
+      kb.template scores<T, 1>(q, s);
+    }
     const float base = base_of(st.x), part = __fdiv_rn(1.f, st.y);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
