@@ -706,13 +706,19 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(Attend a) {
 struct Cut {
   int tiles, row_groups, shares;
 };
+// Two row tiles read the codes once for 32 rows, one lets more workgroups run at once: one up to
+// ONE_TILE places of the line (us in one and in two, f16, heads of 128: 24 heads over 4, 16 tokens over
+// 1100 (288 places) 15.0, 18.6; 32 over 8, two of 4000, 16 tokens (2240) 21.5, 24.6; 32 over 4, two of
+// 65536, 4 tokens (8240) 40.2, 41.8; 32 over 8, four of 8192, 32 tokens (17152) 73.6, 70.9; sixteen of
+// 16384, 8 tokens (33536) 126, 114).
 constexpr int MOST_SHARES = 256 * 4;
 constexpr int LEAST_UNITS = 4;
+constexpr int ONE_TILE = 12 * 1024;
 static Cut cut_of(int64_t B, int64_t heads, int64_t rows, int64_t max_len) {
   Cut c;
-  c.tiles = rows <= 16 ? 1 : 2;
-  c.row_groups = (int)((rows + 16 * c.tiles - 1) / (16 * c.tiles));
-  const int64_t units = (max_len + UNIT - 1) / UNIT;
+  const int64_t units = (max_len + UNIT - 1) / UNIT, groups = (rows + 15) / 16;
+  c.tiles = groups == 1 || B * heads * groups <= ONE_TILE / (EDGE + units) ? 1 : 2;
+  c.row_groups = (int)((groups + c.tiles - 1) / c.tiles);
   const int64_t line = B * heads * c.row_groups * (EDGE + units), most = MOST_SHARES;
   c.shares = units <= LEAST_UNITS ? 0 : (int)(line < most ? line : most);
   return c;

@@ -260,6 +260,24 @@ def test_what_is_not_seen_does_not_count(dev, dim, which, bad):
 
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens,tokens,group,most", [([1500, 0, 777], 7, 5, 800000), ([300, 511], 878, 16, 512)])
+def test_attend_planned_for_much(dev, kind, dim, lens, tokens, group, most):
+    """Plans of many places, that take 32 rows a workgroup, in shares and without; rows that see nothing."""
+    print(f"kv4 attend planned {kind} dim={dim} lens={lens} tokens={tokens}", flush=True)
+    c, table, ln, _ = filled(dev, lens, 1, dim, 64, 31)
+    k, v = (x.cpu().double() for x in c.read(table.to(dev), ln.to(dev), max(lens)))
+    there = torch.arange(max(lens))[None] < ln[:, None]
+    q = torch.randn(len(lens), tokens, group, dim, generator=torch.Generator().manual_seed(7)).to(TYPES[kind])
+    wide = torch.full((len(lens), most // 64), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    w = torch.zeros(len(lens), 1, most, device=dev)
+    got = c.attend(q.to(dev), wide.to(dev), ln.to(dev), max_len=most, weights=w)
+    check_attend(got, w[:, :, :max(lens)], q, k, v, there, ln, max(lens), kind)
+    assert not w[:, :, max(lens):].any()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("dim", [64, 128])
 def test_attend_queries_at_the_ends(dev, kind, dim):
     """The types' largest queries over small keys; infinite ones: all scores -infinity (zeros), else NaN."""
     print(f"kv4 attend ends {kind} dim={dim}", flush=True)
