@@ -702,7 +702,9 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(Attend a) {
 
 // How the work is cut: row tiles a workgroup (of 16), and the most shares of the line, 0 for a
 // workgroup a (sequence, head, rows): up to LEAST_UNITS units, where the line's second kernel costs more
-// than it saves (300 tokens: 10.3 us, 14.1 cut in shares).
+// than it saves (us whole and cut, heads of 128: 300 tokens, f32 10.3, 14.1; 1000, 24 heads over 4, f32
+// 14.3, 14.9, bf16 11.1, 14.7; 100 sequences of 1000, 32 over 8, bf16 30, 38; 1500, f32 18.8, 14.8; ten of
+// 2000, bf16 23.4, 15.9).
 struct Cut {
   int tiles, row_groups, shares;
 };
@@ -712,7 +714,7 @@ struct Cut {
 // 65536, 4 tokens (8240) 40.2, 41.8; 32 over 8, four of 8192, 32 tokens (17152) 73.6, 70.9; sixteen of
 // 16384, 8 tokens (33536) 126, 114).
 constexpr int MOST_SHARES = 256 * 4;
-constexpr int LEAST_UNITS = 4;
+constexpr int LEAST_UNITS = 8;
 constexpr int ONE_TILE = 12 * 1024;
 static Cut cut_of(int64_t B, int64_t heads, int64_t rows, int64_t max_len) {
   Cut c;
