@@ -154,8 +154,8 @@ struct QTile {
   }
 };
 
-// One row tile's in a wave's registers (the sums' kernel; f32, 128 rows over 16384 tokens: 61 -> 57 us
-// for the call, in LDS it took all of a CU's for 3 workgroups).
+// One row tile's in a wave's registers, for the sums (f32, 16 tokens of 32 heads over 16384: 61 -> 57 us
+// for the call; in LDS there was room for three workgroups a CU).
 template <typename T, int DIM>
 struct QRegs {
   Pieces<Q_PIECES<T>> f[DIM / 32];
@@ -635,68 +635,110 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attend a) {
     *reinterpret_cast<float2*>(a.stats + (((size_t)b * a.c.heads + h) * a.rows + row) * 2) = make_float2(now, d);
 }
 
-// What each cached token received, added to its sum: the scores once more, each row's weight from its
-// final maximum and sum. A workgroup takes 32 tokens and its waves the row tiles in turn (several tiles),
-// or 128 tokens (one); the rows of a tile are added over lanes, the tiles of a wave and the waves in order.
-template <typename T, int DIM, bool ONE>
-__global__ __launch_bounds__(256) void kv4_weights_kernel(Attend a) {
-  __shared__ QTile<T, ONE ? DIM : 32, 1> shared;  // one row tile: for the four waves; else unused
-  __shared__ float sums[4][32];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  const int blk = ONE ? blockIdx.x * 4 + wave : blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-  const int len = len_of(a, b), tok = blk << 5;
-  if ((ONE ? (int)blockIdx.x * 128 : tok) >= len) return;
-  const int pi = fdiv(blk, a.c.by_blocks.mul, a.c.by_blocks.shift);
-  const int at = tok < len ? kv4_page(a.c, b, pi) : -1;
-  const size_t bh = (size_t)b * a.c.heads + h;
-  KBlock<DIM> kb = {};
-  if (at >= 0) kb.load(a.c, at, h, (blk - pi * (a.c.page >> 5)) << 5);
-  if constexpr (ONE) {
-    shared.fill(a, b, h, 0);
-    __syncthreads();
-  }
-  float total[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-  for (int row0 = ONE ? 0 : 16 * wave; row0 < a.rows; row0 += 64) {
-    const int row = row0 + n, t = fdiv(row, a.by_group.mul, a.by_group.shift);
-    const int end = row < a.rows ? min(len, len - a.tokens + 1 + t) : 0;
-    float2 st = make_float2(0.f, 1.f);
-    if (row < a.rows) st = *reinterpret_cast<const float2*>(a.stats + (bh * a.rows + row) * 2);
-    float s[1][8];
-    if constexpr (ONE) {
-      kb.template scores<T, 1>(shared, s);
-    } else {
-      QRegs<T, DIM> q;
-#pragma unroll
-      for (int i = 0; i < DIM / 32; ++i) q.f[i] = q_frag<T, DIM>(a, b, h, row0, i);
-      kb.template scores<T, 1>(q, s);
-    }
-    const float base = base_of(st.x), part = __fdiv_rn(1.f, st.y);
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (tok + 8 * g + e < end)
-        total[e] = __fmaf_rn(weight_of(s[0][e], base, a.scale2), part, total[e]);
-  }
+// Of 8 tokens' weights a lane, 16 rows: lane n < 8 of a group gets the sum of token n over the rows.
+__device__ __forceinline__ float over_rows(float (&total)[8]) {
+  const int n = threadIdx.x & 15;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
 #pragma unroll
     for (int d = 1; d < 16; d *= 2) total[e] = __fadd_rn(total[e], __shfl_xor(total[e], d));
   }
-  float mine = total[0];  // lane n < 8: token 8 g + n
+  float mine = total[0];
 #pragma unroll
   for (int e = 1; e < 8; ++e) mine = n == e ? total[e] : mine;
-  const int t = tok + 8 * g + n;
-  float* to = a.weights + b * a.wb + h * a.wh + t;
-  if constexpr (ONE) {
-    if (n < 8 && t < len && at >= 0) *to = __fadd_rn(*to, mine);
-  } else {
-    if (n < 8) sums[wave][8 * g + n] = mine;
-    __syncthreads();
-    if (wave == 0 && n < 8 && t < len && at >= 0) {
-      const float all = __fadd_rn(__fadd_rn(sums[0][8 * g + n], sums[1][8 * g + n]),
-                                  __fadd_rn(sums[2][8 * g + n], sums[3][8 * g + n]));
+  return mine;
+}
+
+// What each cached token received, added to its sum: the scores once more, each row's weight from its
+// final maximum and sum. A workgroup's waves take the row tiles in turn over the same 32 BLOCKS tokens;
+// the rows of a tile are added over lanes, the tiles of a wave and the waves in order.
+// Bound by the queries, which each workgroup loads and splits again: 64 tokens and two waves where the
+// work is cut in shares, 32 and four else, where latency counts (us for the call, f32, 32 heads of 128
+// over 8: 16 sequences of 8192, 8 tokens 144, 212; two of 1000, 16 tokens 25.9, 24.7).
+template <typename T, int DIM, int WAVES, int BLOCKS>
+__global__ __launch_bounds__(WAVES * 64) void kv4_weights_kernel(Attend a) {
+  __shared__ float sums[WAVES][32 * BLOCKS];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int blk = blockIdx.x * BLOCKS, h = blockIdx.y, b = blockIdx.z;
+  const int len = len_of(a, b), tok = blk << 5;
+  if (tok >= len) return;
+  const size_t bh = (size_t)b * a.c.heads + h;
+  KBlock<DIM> kb[BLOCKS] = {};
+  int at[BLOCKS];
+  float total[BLOCKS][8] = {};
+#pragma unroll
+  for (int z = 0; z < BLOCKS; ++z) {
+    const int pi = fdiv(blk + z, a.c.by_blocks.mul, a.c.by_blocks.shift);
+    at[z] = tok + 32 * z < len ? kv4_page(a.c, b, pi) : -1;
+    if (at[z] >= 0) kb[z].load(a.c, at[z], h, (blk + z - pi * (a.c.page >> 5)) << 5);
+  }
+#pragma unroll 1
+  for (int row0 = 16 * wave; row0 < a.rows; row0 += 16 * WAVES) {
+    const int row = row0 + n, t = fdiv(row, a.by_group.mul, a.by_group.shift);
+    const int end = row < a.rows ? min(len, len - a.tokens + 1 + t) : 0;
+    float2 st = make_float2(0.f, 1.f);
+    if (row < a.rows) st = *reinterpret_cast<const float2*>(a.stats + (bh * a.rows + row) * 2);
+    QRegs<T, DIM> q;
+#pragma unroll
+    for (int i = 0; i < DIM / 32; ++i) q.f[i] = q_frag<T, DIM>(a, b, h, row0, i);
+    const float base = base_of(st.x), part = __fdiv_rn(1.f, st.y);
+#pragma unroll
+    for (int z = 0; z < BLOCKS; ++z) {
+      float s[1][8];
+      kb[z].template scores<T, 1>(q, s);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (tok + 32 * z + 8 * g + e < end)
+          total[z][e] = __fmaf_rn(weight_of(s[0][e], base, a.scale2), part, total[z][e]);
+    }
+  }
+#pragma unroll
+  for (int z = 0; z < BLOCKS; ++z) {
+    const float mine = over_rows(total[z]);
+    if (n < 8) sums[wave][32 * z + 8 * g + n] = mine;
+  }
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int z = 0; z < BLOCKS; ++z) {
+    const int i = 32 * z + 8 * g + n;
+    if (n < 8 && tok + i < len && at[z] >= 0) {
+      float all = sums[0][i];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) all = __fadd_rn(all, sums[w][i]);
+      float* to = a.weights + b * a.wb + h * a.wh + tok + i;
       *to = __fadd_rn(*to, all);
     }
+  }
+}
+
+// The same of one row tile: a workgroup takes 128 tokens, its waves 32 each, the queries in LDS.
+template <typename T, int DIM>
+__global__ __launch_bounds__(256) void kv4_weights_one_kernel(Attend a) {
+  __shared__ QTile<T, DIM, 1> q;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+  const int blk = blockIdx.x * 4 + wave, h = blockIdx.y, b = blockIdx.z;
+  const int len = len_of(a, b), tok = blk << 5;
+  if ((int)blockIdx.x * 128 >= len) return;
+  const int pi = fdiv(blk, a.c.by_blocks.mul, a.c.by_blocks.shift);
+  const int at = tok < len ? kv4_page(a.c, b, pi) : -1;
+  KBlock<DIM> kb = {};
+  if (at >= 0) kb.load(a.c, at, h, (blk - pi * (a.c.page >> 5)) << 5);
+  q.fill(a, b, h, 0);
+  __syncthreads();
+  const int end = n < a.rows ? min(len, len - a.tokens + 1 + fdiv(n, a.by_group.mul, a.by_group.shift)) : 0;
+  float2 st = make_float2(0.f, 1.f);
+  if (n < a.rows) st = *reinterpret_cast<const float2*>(a.stats + (((size_t)b * a.c.heads + h) * a.rows + n) * 2);
+  float s[1][8], total[8];
+  kb.template scores<T, 1>(q, s);
+  const float base = base_of(st.x), part = __fdiv_rn(1.f, st.y);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) total[e] = tok + 8 * g + e < end ? __fmul_rn(weight_of(s[0][e], base, a.scale2), part) : 0.f;
+  const float mine = over_rows(total);
+  const int t = tok + 8 * g + n;
+  if (n < 8 && t < len && at >= 0) {
+    float* to = a.weights + b * a.wb + h * a.wh + t;
+    *to = __fadd_rn(*to, mine);
   }
 }
 
@@ -743,9 +785,11 @@ static int launch(const char* what, const Attend& a, int tiles, hipStream_t st) 
   else launch_rows<T, DIM, 2>(a, st);
   if (a.weights && a.max_len > 0) {
     if (a.rows <= 16)
-      kv4_weights_kernel<T, DIM, true><<<dim3((a.max_len + 127) / 128, a.c.heads, a.B), 256, 0, st>>>(a);
+      kv4_weights_one_kernel<T, DIM><<<dim3((a.max_len + 127) / 128, a.c.heads, a.B), 256, 0, st>>>(a);
+    else if (a.shares)
+      kv4_weights_kernel<T, DIM, 2, 2><<<dim3((a.max_len + 63) / 64, a.c.heads, a.B), 128, 0, st>>>(a);
     else
-      kv4_weights_kernel<T, DIM, false><<<dim3((a.max_len + 31) / 32, a.c.heads, a.B), 256, 0, st>>>(a);
+      kv4_weights_kernel<T, DIM, 4, 1><<<dim3((a.max_len + 31) / 32, a.c.heads, a.B), 256, 0, st>>>(a);
   }
   return check_launch(what);
 }

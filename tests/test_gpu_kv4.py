@@ -278,6 +278,24 @@ def test_attend_planned_for_much(dev, kind, dim, lens, tokens, group, most):
 
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page", [32, 96])
+def test_sums_over_pages(dev, kind, dim, page):
+    """What tokens received, of several row tiles: small pages, entries that are no page among them."""
+    print(f"kv4 sums over pages {kind} dim={dim} page={page}", flush=True)
+    lens = [1300, 1025, 33]
+    c, table, ln, _ = filled(dev, lens, 1, dim, page, 41)
+    table[0, 3], table[1, 0], table[2, 0] = -1, c.pages, -7
+    ref = D.Pages(c.k, c.k_scales, c.v, c.v_scales)
+    k, v, there = ref.read(table, ln, 1300)
+    q = torch.randn(3, 5, 7, dim, generator=torch.Generator().manual_seed(19)).to(TYPES[kind])
+    w0 = torch.rand(3, 1, 1301, generator=torch.Generator().manual_seed(20))
+    w = w0.to(dev)
+    got = c.attend(q.to(dev), table.to(dev), ln.to(dev), max_len=1300, weights=w)
+    check_attend(got, w, q, k, v, there, ln, 1300, kind, w0)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("dim", [64, 128])
 def test_attend_queries_at_the_ends(dev, kind, dim):
     """The types' largest queries over small keys; infinite ones: all scores -infinity (zeros), else NaN."""
     print(f"kv4 attend ends {kind} dim={dim}", flush=True)
