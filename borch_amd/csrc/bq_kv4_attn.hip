@@ -562,11 +562,11 @@ __global__ __launch_bounds__(256, 2) void kv4_attend_kernel(Attend a) {
   }
 }
 
-// The parts of one row joined, where its units lie in several shares: a workgroup a row, four waves
-// a quarter of the parts each.
-template <typename T, int DIM, int RT>
-__global__ __launch_bounds__(256) void kv4_join_kernel(Attend a) {
-  __shared__ float sm[4], sl[4], so[4][DIM];
+// The parts of one row joined, where its units lie in several shares: a workgroup a row, its waves the
+// parts in turn.
+template <typename T, int DIM, int RT, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void kv4_join_kernel(Attend a) {
+  __shared__ float sm[WAVES], sl[WAVES], so[WAVES][DIM];
   const int row = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int rg = row / (16 * RT), units = units_of(len_of(a, b));
@@ -581,10 +581,10 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attend a) {
   auto part_of = [&](int w) { return rows + ((size_t)2 * w + (w * share <= begin)) * (16 * RT) * (DIM + 2); };
   // up to 64 of this wave's parts at a time: their maxima and sums a lane each, then their rows, whose
   // loads wait for nothing
-  for (int f0 = w0 + wave; f0 <= w1; f0 += 256) {
-    const int mine = min(64, (w1 - f0) / 4 + 1);
+  for (int f0 = w0 + wave; f0 <= w1; f0 += 64 * WAVES) {
+    const int mine = min(64, (w1 - f0) / WAVES + 1);
     float2 ms = make_float2(-INFINITY, 0.f);
-    if (lane < mine) ms = *reinterpret_cast<const float2*>(part_of(f0 + 4 * lane) + DIM);
+    if (lane < mine) ms = *reinterpret_cast<const float2*>(part_of(f0 + WAVES * lane) + DIM);
     float now = ms.x;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) now = fmaxf(now, __shfl_xor(now, d));
@@ -598,7 +598,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attend a) {
       float x[8][C];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float* p = part_of(f0 + 4 * min(i0 + i, mine - 1)) + C * lane;  // past the last: a weight of 0
+        const float* p = part_of(f0 + WAVES * min(i0 + i, mine - 1)) + C * lane;  // past the last: a weight of 0
 #pragma unroll
         for (int c = 0; c < C; ++c) x[i][c] = p[c];
       }
@@ -615,12 +615,15 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attend a) {
   for (int c = 0; c < C; ++c) so[wave][C * lane + c] = y[c];
   __syncthreads();
   if (wave) return;
-  const float now = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), base = base_of(now);
+  float now = sm[0];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) now = fmaxf(now, sm[w]);
+  const float base = base_of(now);
   sum = 0.f;
 #pragma unroll
   for (int c = 0; c < C; ++c) y[c] = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < WAVES; ++w) {
     const float f = weight_of(sm[w], base, a.scale2);
     sum = __fmaf_rn(f, sl[w], sum);
 #pragma unroll
@@ -769,14 +772,20 @@ static Cut cut_of(int64_t B, int64_t heads, int64_t rows, int64_t max_len) {
 }
 
 // As many shares as workgroups run at once, by the registers (64 sequences of unlike lengths, bf16,
-// 2 / 3 / 4 a CU: 77, 69, 80 us; two of 131072, f32: 70, 64, 75).
+// 2 / 3 / 4 a CU: 77, 69, 80 us; two of 131072, f32: 70, 64, 75). A row is joined by two waves where it has
+// up to 16 parts on average, else by eight (us by two and by eight, heads of 128: 200 sequences of 2000,
+// 32 heads over 8, bf16 94, 110; two of 131072 and 100001, f32 62.8, 61.3; one of 131072, 8 over 1, f32
+// 23.4, 17.0).
 template <typename T, int DIM, int RT>
 static void launch_rows(Attend a, hipStream_t st) {
   constexpr int PER_CU = (RT == 1 ? 3 : 2) + (DIM == 64);
   if (a.shares > 256 * PER_CU) a.shares = 256 * PER_CU;
   const unsigned grid = a.shares ? a.shares : a.B * a.c.heads * a.row_groups;
   kv4_attend_kernel<T, DIM, RT><<<grid, 256, 0, st>>>(a);
-  if (a.shares) kv4_join_kernel<T, DIM, RT><<<dim3(a.rows, a.c.heads, a.B), 256, 0, st>>>(a);
+  if (!a.shares) return;
+  const dim3 rows(a.rows, a.c.heads, a.B);
+  if (a.B * a.c.heads * a.row_groups >= a.shares / 16) kv4_join_kernel<T, DIM, RT, 2><<<rows, 128, 0, st>>>(a);
+  else kv4_join_kernel<T, DIM, RT, 8><<<rows, 512, 0, st>>>(a);
 }
 
 template <typename T, int DIM>

@@ -231,6 +231,21 @@ def test_attend_long(dev, kind, dim, tokens):
     check_attend(got, None, q, k[:, :, :2048], v[:, :, :2048], there[:, :2048], ln, 2048, kind, scale=0.3)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("lens", [[300000], [3] * 31 + [100000] + [3] * 29])
+def test_attend_in_many_parts(dev, kind, lens):
+    """More parts of a row than the waves that join them take at once."""
+    print(f"kv4 attend many parts {kind} {len(lens)}", flush=True)
+    c, table, ln, _ = filled(dev, lens, 1, 64, 256, 43, "bf16")
+    most = max(lens)
+    q = torch.randn(len(lens), 1, 2, 64, generator=torch.Generator().manual_seed(5)).to(TYPES[kind])
+    got = c.attend(q.to(dev), table.to(dev), ln.to(dev), max_len=most)
+    for b in sorted({0, lens.index(most), len(lens) - 1}):
+        k, v = (x.cpu().double() for x in c.read(table[b:b + 1].to(dev), ln[b:b + 1].to(dev), lens[b]))
+        there = torch.ones(1, lens[b], dtype=torch.bool)
+        check_attend(got[b:b + 1], None, q[b:b + 1], k, v, there, ln[b:b + 1], lens[b], kind)
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("which", ["k", "v"])
 @pytest.mark.parametrize("bad", [0, 40, 97, 98, 99])
