@@ -96,6 +96,17 @@ __device__ __forceinline__ float wave_sum_fixed(float v) {
   return __fadd_rn(__fadd_rn(a, b), __fadd_rn(c, d));
 }
 
+// The larger of lanes l and l ^ 32 (l ^ 16), by exchange of half waves (of rows of 16) instead of
+// through LDS.
+__device__ __forceinline__ float max_xor32(float v) {
+  const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
+__device__ __forceinline__ float max_xor16(float v) {
+  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
+
 // The scale rule: float32(peak / 127), correctly rounded (HIP's f32 division is the IEEE
 // correctly rounded one; __fdiv_rn makes that explicit).
 __device__ __forceinline__ float scale_of(float peak) { return __fdiv_rn(peak, 127.0f); }

@@ -459,8 +459,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attend_kernel(Attend a) {
           float top = s[r][0];
 #pragma unroll
           for (int e = 1; e < 8; ++e) top = fmaxf(top, s[r][e]);
-          top = fmaxf(top, __shfl_xor(top, 16));
-          top = fmaxf(top, __shfl_xor(top, 32));
+          top = max_xor32(max_xor16(top));
           // the maximum that is subtracted lags by up to 2^8 (the weights' own size cancels in the quotient)
           const bool grew = __fmul_rn(__fsub_rn(top, m[r]), a.scale2) > 8.f;
           if (__any(grew)) {

@@ -566,7 +566,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
       float top = s[0][0];
 #pragma unroll
       for (int i = 1; i < 16 * SUB; ++i) top = fmaxf(top, s[i / 16][i % 16]);
-      top = fmaxf(top, __shfl_xor(top, 32));
+      top = max_xor32(top);
       const bool grew = __fmul_rn(__fsub_rn(top, m), a.scale2) > 8.f;
       if (__any(grew)) {
         // the 16-bit types subtract the rounded product (below), and so does the factor between two
