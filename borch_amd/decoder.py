@@ -87,7 +87,7 @@ class DecoderState:
     def __init__(self, model: Decoder, sequences: int, tokens: int, page: int = 64):
         p = next(model.parameters())
         width = -(-tokens // page)
-        self.page, self.sequences, self.tokens = page, sequences, tokens
+        self.page, self.sequences, self.tokens, self.context = page, sequences, tokens, model.context
         # twice the pages: those in use, and those that an eviction fills
         self.caches = [Cache4.zeros(2 * sequences * width, model.kv_heads, page, model.dim, p.device) for _ in model.layers]
         self.free = list(range(2 * sequences * width))
@@ -116,18 +116,26 @@ class DecoderState:
         self.table.copy_(self._ints([p + [-1] * (width - len(p)) for p in self.pages]))
         self.lens.copy_(self._ints(self.held))
 
+    def _in_context(self, places):
+        """Refuses texts that go on past the model's learned places, before anything changes: evictions keep
+        the caches short, not the texts."""
+        if max(places) > self.context:
+            raise RuntimeError(f"a text of {max(places)} tokens, the model has places for {self.context}")
+
     def begin(self, lens):
         """Room for the prompts; their first rows, packed, and the end."""
         if any(self.held):
             raise RuntimeError("the state holds tokens already")
         if len(lens) != self.sequences or min(lens) < 1:
             raise RuntimeError(f"{len(lens)} prompts of at least one token for {self.sequences} sequences")
+        self._in_context(lens)
         self._room(lens)
         self.next = list(lens)
         return torch.cumsum(self._ints([0] + list(lens)), 0, dtype=torch.int32)
 
     def grow(self):
         """Room for one more token a sequence; their rows, and their places in the text."""
+        self._in_context([n + 1 for n in self.next])
         self._room([n + 1 for n in self.held])
         at = torch.tensor(self.next, device=self.table.device)
         self.next = [n + 1 for n in self.next]
