@@ -58,6 +58,8 @@ class Decoder(tnn.Module):
     def prompt(self, state: "DecoderState", ids: torch.Tensor, lens) -> torch.Tensor:
         """Prompts packed one after another, ``ids [sum(lens)]``, into an empty ``state``; the logits of
         each one's last token ``[len(lens), vocab]``."""
+        if ids.shape != (sum(lens),):
+            raise RuntimeError(f"ids {tuple(ids.shape)} for prompts of {sum(lens)} tokens")
         cu = state.begin(lens)
         at = torch.cat([torch.arange(n, device=ids.device) for n in lens])
         x = self.embed(ids) + self.places(at)
@@ -70,6 +72,8 @@ class Decoder(tnn.Module):
     @torch.no_grad()
     def step(self, state: "DecoderState", ids: torch.Tensor) -> torch.Tensor:
         """One more token of each sequence, ``ids [sequences]``; its logits ``[sequences, vocab]``."""
+        if ids.shape != (state.sequences,):
+            raise RuntimeError(f"ids {tuple(ids.shape)} for {state.sequences} sequences")
         cu, at = state.grow()
         x = self.embed(ids) + self.places(at)
         for i, (layer, cache) in enumerate(zip(self.layers, state.caches)):

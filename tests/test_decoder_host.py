@@ -43,3 +43,19 @@ def test_a_short_cache_does_not_lengthen_the_text():
     assert s.held == [9, 7] and s.next == [64, 7]
     with pytest.raises(RuntimeError, match="65 tokens"):
         s.grow()
+
+
+def test_ids_that_do_not_fit():
+    """One id for several sequences would have been taken for each; a prompt's would have failed halfway."""
+    m, s = state_of(2)
+    before = books(s)
+    for ids in (torch.zeros(4, dtype=torch.long), torch.zeros(1, dtype=torch.long), torch.zeros(1, 5, dtype=torch.long)):
+        with pytest.raises(RuntimeError, match="prompts of 5"):
+            m.prompt(s, ids, [2, 3])
+    assert books(s) == before
+    s.begin([2, 3])
+    before = books(s)
+    for ids in (torch.zeros(1, dtype=torch.long), torch.zeros(3, dtype=torch.long), torch.zeros(2, 1, dtype=torch.long)):
+        with pytest.raises(RuntimeError, match="2 sequences"):
+            m.step(s, ids)
+    assert books(s) == before
