@@ -147,6 +147,8 @@ class DecoderState:
 
     def evict(self, keep: int, recent: int = 0) -> None:
         """Every sequence down to ``keep`` tokens a head, in every layer (``Cache4.evict``)."""
+        if keep < 1 or not 0 <= recent <= keep:
+            raise ValueError(f"evict: keep {keep}, the {recent} latest of them")
         if keep >= self.longest:
             return
         width = -(-keep // self.page)

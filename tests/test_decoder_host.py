@@ -59,3 +59,13 @@ def test_ids_that_do_not_fit():
         with pytest.raises(RuntimeError, match="2 sequences"):
             m.step(s, ids)
     assert books(s) == before
+
+
+@pytest.mark.parametrize("keep,recent", [(8, 9), (8, -1), (0, 0), (-5, 0)])
+def test_refused_evictions_lose_no_page(keep, recent):
+    _, s = state_of(2)
+    s.begin([60, 3])
+    before = books(s)
+    with pytest.raises(ValueError, match="evict"):
+        s.evict(keep, recent)
+    assert books(s) == before
