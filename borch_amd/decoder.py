@@ -4,9 +4,9 @@ of ``attention`` and ``kv4`` as a program uses them.
     model = Decoder(...).to("cuda").eval()
     quantize_for_int8(model)                      # the Linears, as in any other model
     state = DecoderState(model, sequences=2, tokens=4096)
-    logits = model.prompt(state, ids, [700, 33])  # packed prompts: attention over them, caches filled
-    logits = model.step(state, logits.argmax(-1)) # one token a sequence over the cache
-    state.evict(keep=512, recent=64)              # the tokens that received least leave
+    logits = model.prompt(state, ids, [700, 33], window=16)  # packed prompts: attention over them, caches filled
+    state.evict(keep=512, recent=64)                         # the tokens that received least leave
+    logits = model.step(state, logits.argmax(-1))            # one token a sequence over the cache
 
 Random weights and learned positions; the layers are pre-norm with GELU, the query heads grouped."""
 from __future__ import annotations
@@ -55,18 +55,27 @@ class Decoder(tnn.Module):
         self.kv_heads, self.dim, self.context = kv_heads, dim, context
 
     @torch.no_grad()
-    def prompt(self, state: "DecoderState", ids: torch.Tensor, lens) -> torch.Tensor:
+    def prompt(self, state: "DecoderState", ids: torch.Tensor, lens, window: int = 0) -> torch.Tensor:
         """Prompts packed one after another, ``ids [sum(lens)]``, into an empty ``state``; the logits of
-        each one's last token ``[len(lens), vocab]``."""
+        each one's last token ``[len(lens), vocab]``. What the cached tokens receive from the last ``window``
+        tokens of each prompt is added to their sums, which an eviction goes by (0: none of it)."""
+        if window < 0:
+            raise ValueError(f"prompt: a window of {window} tokens")
         if ids.shape != (sum(lens),):
             raise RuntimeError(f"ids {tuple(ids.shape)} for prompts of {sum(lens)} tokens")
         cu = state.begin(lens)
         at = torch.cat([torch.arange(n, device=ids.device) for n in lens])
+        window = min(window, state.longest)
+        # of a prompt shorter than the window the first rows see nothing, whichever they are
+        last = (cu[1:, None].long() - window + torch.arange(window, device=ids.device)).clamp_min(0)
         x = self.embed(ids) + self.places(at)
-        for layer, cache in zip(self.layers, state.caches):
+        for i, (layer, cache) in enumerate(zip(self.layers, state.caches)):
             q, k, v = layer.heads_of(x)
             cache.append(k, v, state.table, state.lens, cu)
+            if window:
+                cache.attend(q[last], state.table, state.lens, max_len=state.longest, weights=state.sums[i])
             x = layer.close(x, prompt_attention(q, k, v, cu))
+        state.scored = window > 0
         return self.head(self.ln(x[cu[1:].long() - 1]))
 
     @torch.no_grad()
@@ -81,6 +90,7 @@ class Decoder(tnn.Module):
             cache.append(k, v, state.table, state.lens, cu)
             o = cache.attend(q[:, None], state.table, state.lens, max_len=state.longest, weights=state.sums[i])
             x = layer.close(x, o[:, 0])
+        state.scored = True
         return self.head(self.ln(x))
 
 
@@ -100,6 +110,7 @@ class DecoderState:
         self.table = torch.full((sequences, width), -1, dtype=torch.int32, device=p.device)
         self.lens = torch.zeros(sequences, dtype=torch.int32, device=p.device)
         self.sums = [torch.zeros(sequences, model.kv_heads, width * page, device=p.device) for _ in model.layers]
+        self.scored = False  # whether the sums hold anything: steps add to them, prompts by their window
 
     @property
     def longest(self) -> int:
@@ -151,6 +162,8 @@ class DecoderState:
             raise ValueError(f"evict: keep {keep}, the {recent} latest of them")
         if keep >= self.longest:
             return
+        if not self.scored and recent < keep:
+            raise RuntimeError("evict: no cached token has received anything yet (prompt's window, or a step)")
         width = -(-keep // self.page)
         fresh = [[self.free.pop() for _ in range(width)] for _ in range(self.sequences)]
         table = self._ints(fresh)

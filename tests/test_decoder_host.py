@@ -69,3 +69,17 @@ def test_refused_evictions_lose_no_page(keep, recent):
     with pytest.raises(ValueError, match="evict"):
         s.evict(keep, recent)
     assert books(s) == before
+
+
+def test_evictions_with_nothing_to_go_by():
+    """Sums that are all 0 would have kept the earliest tokens as ties."""
+    m, s = state_of(2)
+    s.begin([60, 3])
+    before = books(s)
+    with pytest.raises(RuntimeError, match="received"):
+        s.evict(20, 8)
+    assert books(s) == before
+    s.evict(60, 8)  # nothing leaves
+    assert books(s) == before
+    with pytest.raises(ValueError, match="window"):
+        m.prompt(s, torch.zeros(5, dtype=torch.long), [2, 3], window=-1)
