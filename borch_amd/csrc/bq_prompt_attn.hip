@@ -632,9 +632,14 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
       wait_lds();
       barrier();
       if (part == 0) {
+        // as in the loop: f32 subtracts the maxima first, the 16-bit types their rounded products
         const float m1 = to[0], now = fmaxf(m, m1), shift = -__fmul_rn(now, a.scale2);
-        const float f0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(__fadd_rn(shift, __fmul_rn(m, a.scale2)));
-        const float f1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(__fadd_rn(shift, __fmul_rn(m1, a.scale2)));
+        auto factor = [&](float x) {
+          if (x == -INFINITY) return 0.f;
+          return __builtin_amdgcn_exp2f(P == 3 ? __fmul_rn(__fsub_rn(x, now), a.scale2)
+                                               : __fadd_rn(shift, __fmul_rn(x, a.scale2)));
+        };
+        const float f0 = factor(m), f1 = factor(m1);
         l = __fmaf_rn(l, f0, __fmul_rn(to[64], f1));
         odd |= to[128] != 0.f;
 #pragma unroll

@@ -1,0 +1,45 @@
+"""prompt_attention in f32 where the tolerance does not hide a lost bit: scores and values that are exact.
+
+A score is one channel's product, a whole number of sixteenths that two fp16 pieces hold; few keys carry
+weight, so that the sums are short. Tolerance of an output, relative to sum_i p_i |v_i|, for differences of scores
+d <= 4 from the row's largest and h keys within it (all others are 200 below: a weight of 0): the exponent's
+argument within 3 2^-24 of itself (log2(e) as a constant, its product with the scale, the product), 3 * 4 2^-24 in p
+and once more in its sum, the exponential's 2^-23 likewise, h additions in each of the sums, and 16 2^-24 for the
+six products of pieces (what the three others would add is below 2^-24), the joined parts and the quotient:
+(24 + 4 + 2 h + 16) 2^-24."""
+import pytest
+import torch
+
+from borch_amd import attention as A
+from oracle import decode as D
+
+pytestmark = pytest.mark.gpu
+
+HEAVY = [(3, 0.0), (17, -1.0), (36, -1.0), (61, -0.5), (64, -4.0), (100, -0.25), (130, -2.0), (190, -1.5), (239, 0.0),
+         (299, -3.0)]
+
+
+@pytest.mark.parametrize("dim,n,heads", [(64, 300, 2), (128, 300, 2), (64, 300, 600), (128, 300, 600), (64, 150, 2), (128, 96, 2)])
+@pytest.mark.parametrize("top", [0.0, 1000.0, 2.0 ** 14, -(2.0 ** 14), 2.0 ** 17])
+@pytest.mark.parametrize("causal", [True, False])
+def test_f32_weights_of_large_scores(dev, dim, n, heads, top, causal):
+    """Every form: one wave or two a query (their halves joined), tiles split where they are used. The weights
+    are of both halves of a tile and of several tiles, whose maxima differ."""
+    print(f"prompt f32 exact dim={dim} n={n} heads={heads} top={top} causal={causal}", flush=True)
+    g = torch.Generator().manual_seed(dim + n)
+    v = torch.randn(n, 1, dim, generator=g)
+    score = torch.full((n,), top - 200.0)
+    heavy = [(i, d) for i, d in HEAVY if i < n]
+    for i, d in heavy:
+        score[i] = top + d
+    q, k = torch.zeros(n, heads, dim), torch.zeros(n, 1, dim)
+    q[:, :, 5], k[:, 0, 5] = 1.0, score * 8.0
+    cu = torch.tensor([0, n], dtype=torch.int32)
+    got = A.prompt_attention(q.to(dev), k.to(dev), v.to(dev), cu.to(dev), causal=causal, scale=0.125).cpu().double()
+    seen = torch.ones(n, n, dtype=torch.bool)
+    want, _, size = D.softmax_rows(q[:, 0], k[:, 0], v[:, 0], seen.tril() if causal else seen, 0.125)
+    rows = slice(heavy[0][0], n)  # before: rows of flat scores, whose sums are long
+    tol = (44 + 2 * len(heavy)) * 2.0 ** -24
+    for j in sorted({0, 1, heads - 1}):
+        off = ((got[:, j] - want).abs() / size)[rows if causal else slice(None)].max()
+        assert float(off) <= tol, f"off by {float(off):.3g}, tolerance {tol:.3g}"
