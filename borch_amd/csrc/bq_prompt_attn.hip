@@ -11,16 +11,19 @@
 // the second operand of O^T = v^T p^T: its contracted index (tokens) is permuted to suit, groups of
 // 4 tokens each, which is what the transposing LDS read takes of v's rows.
 //
-// The 16-bit types multiply as they are and p is rounded to their type (half a step of 2^-8 or
-// 2^-11 on each term, where the output takes one as large). In f32 p and v are the exact sums of
-// three bf16 pieces (bq_bf16x3.h), of whose nine products the six of weight 2^-18 and above are
-// added: a small weight on a large value keeps its bits. In the scores only the sum over the channels
-// counts, so q and k are two fp16 pieces each, 22 bits below a power of two of their row (what a
-// channel 2^-14 of the row's largest loses is 2^-38 of that largest), and of the four products three
-// are added: half the matrix work of the bf16 pieces, each product within 3 2^-22. Outputs that do not
-// come out finite, or in f32 below 2^-109 (zero aside), where the up to 2^-134 that the pieces take from
-// such a value is more than a rounding, are taken again in plain f32 (plain_row): infinities and NaN act
-// as f32 has them, and only on the queries that see them.
+// The 16-bit types multiply as they are and p is rounded to their type: half a step of 2^-8 or 2^-11 on each
+// term, where the output takes one as large (bf16, 8192 tokens: 2.1e-3 from float64 in the mean, 1.6e-3 by the
+// output's rounding alone). p in two pieces would leave the output's rounding alone and take half as much
+// matrix work again (8192 tokens 544 -> 706 us, 2048 and 1111 48 -> 55, 4096 of 64 channels 88 -> 117).
+//
+// In f32 p and v are the exact sums of three bf16 pieces (bq_bf16x3.h), of whose nine products the six of
+// weight 2^-18 and above are added: a small weight on a large value keeps its bits. In the scores only
+// the sum over the channels counts, so q and k are two fp16 pieces each, 22 bits below a power of two of
+// their row (what a channel 2^-14 of the row's largest loses is 2^-38 of that largest), and of the four
+// products three are added: half the matrix work of the bf16 pieces, each product within 3 2^-22. Outputs
+// that do not come out finite, or in f32 below 2^-109 (zero aside), where the up to 2^-134 that the pieces
+// take from such a value is more than a rounding, are taken again in plain f32 (plain_row): infinities and
+// NaN act as f32 has them, and only on the queries that see them.
 //
 // Bound by the MFMAs at the clock that they leave: 8192 tokens, 32 heads of 128 over 8, bf16, causal:
 // 520 to 575 us, 0.96 to 1.06 PFLOP/s, where the library's 8192^3 product reaches 1.21; 2048 and 1111
@@ -96,6 +99,11 @@ template <typename T>
 struct Kind {
   static constexpr int P = sizeof(T) == 4 ? 3 : 1;   // pieces of v and p
   static constexpr int PK = sizeof(T) == 4 ? 2 : 1;  // of k and q
+  // The maximum that is subtracted lags by up to 2^LAG, and the row's largest weight is 2^LIFT or more. In fp16
+  // weights keep their 11 bits down to 2^-25 of the largest (at 2^0 those below 2^-14 were subnormal: where a
+  // first token of values near 0 leads by e^14, outputs were off by 0.3 of their size), and none passes 2^15.5.
+  // A lag of 2^4 costs nothing beside one of 2^8: 8192 tokens, 32 heads of 128, 569 and 571 us.
+  static constexpr float LAG = __is_same(T, _Float16) ? 4.f : 8.f, LIFT = __is_same(T, _Float16) ? 11.f : 0.f;
 };
 
 template <int P>
@@ -437,6 +445,12 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
     const int t = t0 + threadIdx.x;
     return PK == 2 && !DIRECT && threadIdx.x < KT && t < len ? row_e[t] : 0;
   };
+  // What is added to a score times the scale, for a maximum, and the factor from the weights of one maximum
+  // to those of another: f32 subtracts the maxima first, the 16-bit types what they add, rounded.
+  auto shift_of = [&](float x) { return __fsub_rn(Kind<T>::LIFT, __fmul_rn(x, a.scale2)); };
+  auto factor = [&](float from, float to) {
+    return __builtin_amdgcn_exp2f(P == 3 ? __fmul_rn(__fsub_rn(from, to), a.scale2) : __fsub_rn(shift_of(to), shift_of(from)));
+  };
   float m, l;
   v16f o[VT];
   // Once; and where an output is not finite once more, with the values that are not out of the tiles
@@ -556,8 +570,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
         }
       }
 
-      // softmax, one step. The maximum that is subtracted lags by up to 2^8 (the weights' own size
-      // cancels in the quotient), so that most steps rescale nothing.
+      // softmax, one step. The maximum that is subtracted lags (the weights' own size cancels in the
+      // quotient), so that most steps rescale nothing.
       const bool edge = tw + 32 * SUB > len || (a.causal && tw + 32 * SUB > qw + 1);
       if (edge)
 #pragma unroll
@@ -567,19 +581,15 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
 #pragma unroll
       for (int i = 1; i < 16 * SUB; ++i) top = fmaxf(top, s[i / 16][i % 16]);
       top = max_xor32(top);
-      const bool grew = __fmul_rn(__fsub_rn(top, m), a.scale2) > 8.f;
+      const bool grew = __fmul_rn(__fsub_rn(top, m), a.scale2) > Kind<T>::LAG;
       if (__any(grew)) {
-        // the 16-bit types subtract the rounded product (below), and so does the factor between two
-        const float to = grew ? top : m, shift = -__fmul_rn(to, a.scale2);
-        const float f = !grew ? 1.f
-                              : __builtin_amdgcn_exp2f(P == 3 ? __fmul_rn(__fsub_rn(m, top), a.scale2)
-                                                              : __fadd_rn(shift, __fmul_rn(m, a.scale2)));
-        m = to;
+        const float f = grew ? factor(m, top) : 1.f;
+        m = grew ? top : m;
         l = __fmul_rn(l, f);
 #pragma unroll
         for (int d = 0; d < VT; ++d) o[d] *= f;
       }
-      const float base = m == -INFINITY ? 0.f : m, shift = -__fmul_rn(base, a.scale2);
+      const float base = m == -INFINITY ? 0.f : m, shift = shift_of(base);
 #pragma unroll
       for (int i = 0; i < 16 * SUB; ++i) {
         float x = s[i / 16][i % 16];
@@ -632,14 +642,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
       wait_lds();
       barrier();
       if (part == 0) {
-        // as in the loop: f32 subtracts the maxima first, the 16-bit types their rounded products
-        const float m1 = to[0], now = fmaxf(m, m1), shift = -__fmul_rn(now, a.scale2);
-        auto factor = [&](float x) {
-          if (x == -INFINITY) return 0.f;
-          return __builtin_amdgcn_exp2f(P == 3 ? __fmul_rn(__fsub_rn(x, now), a.scale2)
-                                               : __fadd_rn(shift, __fmul_rn(x, a.scale2)));
-        };
-        const float f0 = factor(m), f1 = factor(m1);
+        const float m1 = to[0], now = fmaxf(m, m1);
+        const float f0 = m == -INFINITY ? 0.f : factor(m, now), f1 = m1 == -INFINITY ? 0.f : factor(m1, now);
         l = __fmaf_rn(l, f0, __fmul_rn(to[64], f1));
         odd |= to[128] != 0.f;
 #pragma unroll
