@@ -709,7 +709,8 @@ int bq_prompt_attention(const void* q, const void* k, const void* v, int type, i
   if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) ||
       (q_token | q_head | k_token | k_head | v_token | v_head) * size % 16)
     return set_error(BQ_ERR_ARG, "%s: rows that are not 16-byte aligned", what);
-  if (k_token < 0 || v_token < 0 || k_token > 1 << 23 || v_token > 1 << 23)  // a tile's rows within 32 bits
+  // a tile's rows within 32 bits, where the callers' own come into LDS (f32's are split first, or where used)
+  if (k_token < 0 || v_token < 0 || (type && (k_token > 1 << 23 || v_token > 1 << 23)))
     return set_error(BQ_ERR_UNSUPPORTED, "%s: rows of k or v too far apart", what);
   // whatever the lengths are: a full tile for every 128 rows and one begun for each sequence
   const bool direct = type == 0 && n * dim <= PROMPT_DIRECT;
