@@ -2,7 +2,7 @@
 different lengths packed one after another, grouped heads, causal or not, in f32, bf16 or f16.
 
 It is the attention between a decoder's int8 projections when a prompt is read; ``kv4`` holds the
-keys and values for the tokens that follow. Inference only: no gradient."""
+keys and values for the tokens that follow. Inference only: operands that require a gradient are refused."""
 from __future__ import annotations
 
 from contextlib import nullcontext
@@ -29,6 +29,13 @@ def type_of(t: torch.Tensor, what: str) -> int:
     if code is None:
         raise TypeError(f"{what}: takes float32, bfloat16 or float16, got {t.dtype}")
     return code
+
+
+def no_graph(what: str, *operands: torch.Tensor) -> None:
+    """Refuses operands that autograd would record: the kernels keep no graph, and a result without one would
+    drop their gradients in silence."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in operands):
+        raise RuntimeError(f"{what}: no gradient is computed, and an operand requires one (torch.no_grad() or detach())")
 
 
 def rows(t: torch.Tensor, code: int):
@@ -67,6 +74,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
     row sees the rows up to itself. ``scale`` defaults to ``dim ** -0.5``. Views of a fused
     projection's output are read in place. Returns ``[n, q_heads, dim]``; rows of no sequence are
     zeros."""
+    no_graph("prompt_attention", q, k, v)
     require_device(q.device)
     code = type_of(q, "prompt_attention")
     shape = q.shape

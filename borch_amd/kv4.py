@@ -12,7 +12,7 @@ import functools
 import torch
 
 from ._lib import Kv4Desc, check, lib, require_device
-from .attention import ints, on, rows, type_of
+from .attention import ints, no_graph, on, rows, type_of
 from .int8 import _stream
 
 __all__ = ["Cache4"]
@@ -27,7 +27,8 @@ class Cache4:
     """The pages of a 4-bit cache: ``k``, ``k_scales``, ``v``, ``v_scales`` uint8 with ``[pages,
     heads]`` first (``Cache4.zeros`` makes them). The caller keeps, on the device and in int32,
     ``table [sequences, width]`` (each sequence's pages in order) and ``lens [sequences]`` (its cached
-    tokens). An entry that is no page holds nothing: not written, read as zeros, not attended to."""
+    tokens). An entry that is no page holds nothing: not written, read as zeros, not attended to. Inference
+    only: operands that require a gradient are refused."""
 
     def __init__(self, k: torch.Tensor, k_scales: torch.Tensor, v: torch.Tensor, v_scales: torch.Tensor):
         for name, t in (("k", k), ("k_scales", k_scales), ("v", v), ("v_scales", v_scales)):
@@ -81,6 +82,7 @@ class Cache4:
                cu: torch.Tensor) -> None:
         """``new_k``, ``new_v [n, heads, dim]`` (f32, bf16 or f16) into the cache: sequence ``b``'s the
         rows ``cu[b] .. cu[b + 1]``, the last ones of its ``lens[b]`` tokens (``lens`` counts them)."""
+        no_graph("append", new_k, new_v)
         require_device(self.device)
         code = type_of(new_k, "append")
         if new_v.dtype is not new_k.dtype:
@@ -122,6 +124,7 @@ class Cache4:
         ``[sequences, heads, >= max_len]``: each cached token's softmax weights, summed over the
         queries of its key-value head, are added in place. Returns ``[sequences, tokens, q_heads,
         dim]`` of q's type."""
+        no_graph("attend", *((q,) if weights is None else (q, weights)))
         require_device(self.device)
         code = type_of(q, "attend")
         shape = q.shape
@@ -167,6 +170,7 @@ class Cache4:
         to the pages of ``new_table [sequences, >= keep / page]``, none of which is in use.
         Returns ``kept`` int32 ``[sequences, heads, keep]`` (their former places, -1 past the last),
         their ``weights`` (0 past the last) and ``left`` int32 ``[sequences]``, the new lengths."""
+        no_graph("evict", sums)
         require_device(self.device)
         table, lens, B, width = self._table(table, lens, "evict")
         if new_table.dim() != 2 or new_table.shape[0] != B:
