@@ -802,6 +802,16 @@ static int launch(const char* what, const Attend& a, int tiles, hipStream_t st) 
   return check_launch(what);
 }
 
+// Whether the weights of B sequences and `heads` heads, `most` each, share no place: the one axis' rows lie within
+// a step of the other.
+static bool rows_apart(int64_t B, int64_t seq, int64_t heads, int64_t head, int64_t most) {
+  auto nested = [&](int64_t n, int64_t step, int64_t outer_n, int64_t outer) {
+    const __int128 in = step < 0 ? -(__int128)step : step, out = outer < 0 ? -(__int128)outer : outer;
+    return (n < 2 || in >= most) && (outer_n < 2 || out >= (n - 1) * in + most);
+  };
+  return most == 0 || nested(heads, head, B, seq) || nested(B, seq, heads, head);
+}
+
 }  // namespace bq
 
 using namespace bq;
@@ -839,10 +849,13 @@ int bq_kv4_attend(const bq_kv4_cache* cache, const void* q, int type, int64_t to
   const int64_t size = type == KV4_F32 ? 4 : 2;
   if ((((uintptr_t)q | (uintptr_t)out) & 15) || (q_seq | q_token | q_head) * size % 16)
     return set_error(BQ_ERR_ARG, "%s: rows that are not 16-byte aligned", what);
+  const int64_t held = cache->pages ? width * cache->page : 0;  // tokens that a sequence's pages have room for
+  // several workgroups would add to one place
+  if (weights && !rows_apart(B, w_seq, cache->heads, w_head, max_len < held ? max_len : held))
+    return set_error(BQ_ERR_ARG, "%s: weights of sequences or heads overlap", what);
   const size_t need = bq_kv4_attend_ws_bytes(B, cache->heads, rows, cache->dim, max_len, weights != nullptr);
   if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
     return set_error(BQ_ERR_ARG, "%s: a workspace of %zu bytes, given %zu", what, need, ws ? ws_bytes : 0);
-  const int64_t held = cache->pages ? width * cache->page : 0;  // tokens that a sequence's pages have room for
   a.lens = lens;
   a.q = q;
   a.qb = q_seq;

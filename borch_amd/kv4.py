@@ -122,7 +122,8 @@ class Cache4:
         tokens; where it sees none its output is 0. ``max_len``: no sequence is longer (default: what
         the table's pages hold; the work is planned for it, longer ones are cut). ``weights`` f32
         ``[sequences, heads, >= max_len]``: each cached token's softmax weights, summed over the
-        queries of its key-value head, are added in place. Returns ``[sequences, tokens, q_heads,
+        queries of its key-value head, are added in place (rows that overlap, as an expanded view's, are
+        refused). Returns ``[sequences, tokens, q_heads,
         dim]`` of q's type."""
         no_graph("attend", *((q,) if weights is None else (q, weights)))
         require_device(self.device)

@@ -15,3 +15,19 @@ def test_rows_far_apart_are_the_16_bit_types_limit():
     assert call(1, far) == UNSUPPORTED and call(2, far) == UNSUPPORTED
     assert call(0, far) == ARG and "workspace" in _lib.last_error()
     assert call(0, (256, 64, -64, 64, 128, 64)) == UNSUPPORTED
+
+
+def test_weights_that_overlap():
+    """Rows of weights that share places (an expanded view's) would be added to by several workgroups."""
+    d = _lib.Kv4Desc(16, 16, 16, 16, 8, 3, 32, 64)
+
+    def call(w_seq, w_head, B=2, max_len=40, width=2):  # refused for its workspace where nothing else is wrong
+        rc = _lib.lib().bq_kv4_attend(ctypes.byref(d), 16, 0, 1, 3, 256, 256, 64, 16, B, width, 16, max_len, 0.1, 16, 16,
+                                      w_seq, w_head, None, 0, None)
+        assert rc == ARG
+        return "overlap" in _lib.last_error()
+
+    assert not call(120, 40) and not call(40, 80) and not call(1000, 64) and not call(-120, 40)
+    assert call(0, 40) and call(120, 0) and call(120, 39) and call(119, 40) and call(40, 79) and call(0, 0)
+    assert not call(0, 40, B=1)
+    assert not call(32, 64, width=1) and call(31, 64, width=1)  # 32 tokens are what a page has room for
