@@ -470,6 +470,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
     for (int t0 = 0, buf = 0; t0 < keys; t0 += KT, buf ^= BUFS - 1) {
       wait_dma_all();
       if constexpr (DIRECT) {
+        wait_lds();
         barrier();  // the last tile is read
 #pragma unroll
         for (int e = 0; e < 2 * KT * DIM / 8 / (WAVES * 64); ++e) {

@@ -43,3 +43,16 @@ def test_f32_weights_of_large_scores(dev, dim, n, heads, top, causal):
     for j in sorted({0, 1, heads - 1}):
         off = ((got[:, j] - want).abs() / size)[rows if causal else slice(None)].max()
         assert float(off) <= tol, f"off by {float(off):.3g}, tolerance {tol:.3g}"
+
+
+@pytest.mark.parametrize("dim,n", [(64, 192), (128, 96)])
+def test_tiles_split_where_they_are_used(dev, dim, n):
+    """Several tiles in one buffer, filled again by all waves: every head and every run the same bits."""
+    print(f"prompt f32 tiles in one buffer dim={dim}", flush=True)
+    g = torch.Generator().manual_seed(n)
+    q, k, v = (torch.randn(n, 1, dim, generator=g).to(dev) for _ in range(3))
+    cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+    base = A.prompt_attention(q, k, v, cu, causal=False)
+    for _ in range(5):
+        got = A.prompt_attention(q.expand(n, 512, dim), k, v, cu, causal=False)
+        assert torch.equal(got, base.expand(n, 512, dim))
