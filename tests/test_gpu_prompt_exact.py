@@ -56,3 +56,27 @@ def test_tiles_split_where_they_are_used(dev, dim, n):
     for _ in range(5):
         got = A.prompt_attention(q.expand(n, 512, dim), k, v, cu, causal=False)
         assert torch.equal(got, base.expand(n, 512, dim))
+
+
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("at", [0, 63, 64, 200])
+def test_scores_that_decide_a_row(dev, kind, dim, at):
+    """A key whose scores are NaN or +infinity leaves NaN in every channel of the rows that see it, though keys
+    of -infinity and values that are not finite follow; the same key with scores of -infinity leaves the rest."""
+    print(f"prompt deciding scores {kind} dim={dim} at={at}", flush=True)
+    g = torch.Generator().manual_seed(dim)
+    n = 260
+    q, k, v = (torch.randn(n, h, dim, generator=g) for h in (2, 1, 1))
+    q[:, 0, 3], q[:, 1, 3] = q[:, 0, 3].abs() + 0.1, -q[:, 1, 3].abs() - 0.1
+    k[at, 0, 3] = torch.inf  # head 0: +infinity, head 1: -infinity
+    k[at + 5, 0, 3] = -torch.inf if at else torch.inf
+    v[at + 7, 0, 9] = torch.inf
+    q, k, v = q.to(kind), k.to(kind), v.to(kind)
+    cu = torch.tensor([0, n], dtype=torch.int32)
+    got = A.prompt_attention(q.to(dev), k.to(dev), v.to(dev), cu.to(dev)).cpu()
+    seen = torch.ones(n, n, dtype=torch.bool).tril()
+    for j in range(2):
+        want = D.softmax_rows(q[:, j], k[:, 0], v[:, 0], seen, dim ** -0.5)[0]
+        assert torch.equal(got[:, j].isnan(), want.isnan()) and torch.equal(got[:, j].isposinf(), want.isposinf())
+        assert bool(got[at:, 0].isnan().all())
