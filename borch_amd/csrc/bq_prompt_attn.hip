@@ -20,10 +20,12 @@
 // weight 2^-18 and above are added: a small weight on a large value keeps its bits. In the scores only
 // the sum over the channels counts, so q and k are two fp16 pieces each, 22 bits below a power of two of
 // their row (what a channel 2^-14 of the row's largest loses is 2^-38 of that largest), and of the four
-// products three are added: half the matrix work of the bf16 pieces, each product within 3 2^-22. Outputs
-// that do not come out finite, or in f32 below 2^-109 (zero aside), where the up to 2^-134 that the pieces
-// take from such a value is more than a rounding, are taken again in plain f32 (plain_row): infinities and
-// NaN act as f32 has them, and only on the queries that see them.
+// products three are added: half the matrix work of the bf16 pieces, each product within 3 2^-22. Taken again
+// in plain f32 (plain_row) are outputs that do not come out finite, so that infinities and NaN act as f32 has
+// them, and only on the queries that see them; in f32 those below 2^-109 (zero aside), where the up to 2^-134
+// that the pieces take from such a value is more than a rounding, and those for whose scores the 2^-38 could
+// count: a channel far above its row over rows that are small there (2^20 in q alone made the scores' error
+// twelve times f32's own, 2^30 outputs worthless).
 //
 // Bound by the MFMAs at the clock that they leave: 8192 tokens, 32 heads of 128 over 8, bf16, causal:
 // 520 to 575 us, 0.96 to 1.06 PFLOP/s, where the library's 8192^3 product reaches 1.21; 2048 and 1111
@@ -95,6 +97,11 @@ __device__ __forceinline__ bool place_of(const Prompt& a, Place* out) {
   return false;
 }
 
+// f32 prompts of up to this many channels of a head (192 tokens of 64, 96 of 128) are split where they
+// are used. With a launch for it and without, us: 102 tokens, 12 heads of 64 16.1, 12.2; 256 tokens
+// 22.6, 21.9; 94 tokens, 16 heads of 128 20.1, 16.7; 128 tokens 20.3, 21.8; 512 tokens 43, 61.
+constexpr int64_t PROMPT_DIRECT = 12288;
+
 template <typename T>
 struct Kind {
   static constexpr int P = sizeof(T) == 4 ? 3 : 1;   // pieces of v and p
@@ -145,6 +152,7 @@ __device__ __forceinline__ v16f score(const Frag<Kind<T>::PK>& k, const Frag<Kin
 // The power of two that takes a row's largest magnitude (as bits) to [2^13, 2^14): its exponent. Rows
 // that are not finite get any; their products are not finite.
 __device__ __forceinline__ int row_exponent(uint32_t peak) { return max((int)(peak >> 23), 1) - 127 - 13; }
+constexpr int NO_ROW = -139;  // of a row of zeros
 // Two fp16 pieces of x 2^-e.
 __device__ __forceinline__ Frag<2> halves(const float x[8], int e) {
   v8h hi, lo;
@@ -395,7 +403,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
   constexpr int ROWS = 1024 / (DIM * 2);         // of a wave's load
   constexpr int PER = KT / ROWS / WAVES;  // loads a wave and plane
   __shared__ __attribute__((aligned(1024))) unsigned char lds[BUFS * (PK + P) * PLANE];
-  __shared__ __attribute__((aligned(16))) int exponents[KT];  // f32: of the tile's keys
+  __shared__ __attribute__((aligned(16))) int exponents[DIRECT ? PROMPT_DIRECT / DIM : KT];  // f32: of the tile's keys, or of all
+  __shared__ int tops[WAVES];
   __shared__ int found[KT];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hh = lane >> 5;
   Place at;
@@ -465,7 +474,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
   const int* row_e = PK == 2 ? a.exponents + (size_t)h * a.n + at.start : nullptr;
   auto exponent = [&](int t0) {
     const int t = t0 + threadIdx.x;
-    return PK == 2 && !DIRECT && threadIdx.x < KT && t < len ? row_e[t] : 0;
+    return PK == 2 && !DIRECT && threadIdx.x < KT && t < len ? row_e[t] : NO_ROW;
   };
   // What is added to a score times the scale, for a maximum, and the factor from the weights of one maximum
   // to those of another: f32 subtracts the maxima first, the 16-bit types what they add, rounded.
@@ -474,13 +483,14 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
     return __builtin_amdgcn_exp2f(P == 3 ? __fmul_rn(__fsub_rn(from, to), a.scale2) : __fsub_rn(shift_of(to), shift_of(from)));
   };
   float m, l;
+  int most_e;  // f32: the largest exponent among the keys that this thread put into LDS
   v16f o[VT];
   // Once; and where an output is not finite once more, with the values that are not out of the tiles
   // that some query sees in part. Rows that see one, or are not finite then, go to plain_row: what a
   // query does not see changes no bit of its output.
   bool odd = false;
   for (int again = 0;; again = 1) {
-    m = -INFINITY, l = 0.f;
+    m = -INFINITY, l = 0.f, most_e = NO_ROW;
 #pragma unroll
     for (int d = 0; d < VT; ++d) o[d] = zeros16();
     if (!DIRECT && keys > 0) {
@@ -491,6 +501,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
     int e_next = exponent(0);  // loaded with the keys, put in LDS when they are there
     for (int t0 = 0, buf = 0; t0 < keys; t0 += KT, buf ^= BUFS - 1) {
       wait_dma_all();
+      int* key_e = exponents + (DIRECT ? t0 : 0);
       if constexpr (DIRECT) {
         wait_lds();
         barrier();  // the last tile is read
@@ -521,11 +532,13 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
             const Frag<2> f = halves(x, ex);
 #pragma unroll
             for (int p = 0; p < 2; ++p) *reinterpret_cast<v8s*>(lds + p * PLANE + k_at<DIM>(r, c)) = f.p[p];
-            if (c == 0) exponents[r] = ex;
+            if (c == 0) key_e[r] = ex;
+            most_e = max(most_e, ex);
           }
         }
       } else if (PK == 2 && threadIdx.x < KT) {
-        exponents[threadIdx.x] = e_next;
+        key_e[threadIdx.x] = e_next;
+        most_e = max(most_e, e_next);
       }
       wait_lds();
       barrier();  // the keys are there (both buffers: the values too), what is loaded over is read
@@ -585,7 +598,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
         __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int4 e = *reinterpret_cast<const int4*>(exponents + 32 * SUB * part + 8 * i + 4 * hh);
+          const int4 e = *reinterpret_cast<const int4*>(key_e + 32 * SUB * part + 8 * i + 4 * hh);
           s[0][4 * i] = __builtin_ldexpf(s[0][4 * i], e.x + q_e);
           s[0][4 * i + 1] = __builtin_ldexpf(s[0][4 * i + 1], e.y + q_e);
           s[0][4 * i + 2] = __builtin_ldexpf(s[0][4 * i + 2], e.z + q_e);
@@ -688,6 +701,23 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) least = min(least, (__float_as_uint(o[d][i]) << 1) - 1u);
       odd |= least < (__float_as_uint(__fmul_rn(l, 0x1p-109f)) << 1) - 1u;
+      // What the scores lose of channels far below their row's largest: 2^-38 of either row's largest, below
+      // 2^(exponent + 14), times dim channels of the other's. First by all keys that were here, which seldom
+      // says more; then by those that the query sees.
+      const float most = fmaxf(0x1p-17f, __fmul_rn(__fmul_rn(fabsf(m), a.scale2), 0x1p-22f));
+      auto counts = [&](int e) { return __builtin_ldexpf(a.scale2, q_e + e + (DIM == 128 ? -2 : -3)) > most; };
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) most_e = max(most_e, __shfl_xor(most_e, d));
+      if (lane == 0) tops[wave] = most_e;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) most_e = max(most_e, tops[w]);
+      if (part == 0 && __any(row < len && counts(most_e))) {
+        const int* e = DIRECT ? exponents : row_e;
+        int seen = NO_ROW;
+        for (int t = 0; t < wkeys; ++t) seen = max(seen, t < sees ? e[t] : NO_ROW);
+        odd |= counts(seen);
+      }
     }
     odd = odd && row < len && part == 0;
     if (again || !__syncthreads_or(odd)) break;
@@ -701,11 +731,6 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
 }  // namespace bq
 
 using namespace bq;
-
-// f32 prompts of up to this many channels of a head (192 tokens of 64, 96 of 128) are split where they
-// are used. With a launch for it and without, us: 102 tokens, 12 heads of 64 16.1, 12.2; 256 tokens
-// 22.6, 21.9; 94 tokens, 16 heads of 128 20.1, 16.7; 128 tokens 20.3, 21.8; 512 tokens 43, 61.
-constexpr int64_t PROMPT_DIRECT = 12288;
 
 size_t bq_prompt_attention_ws_bytes(int type, int64_t n, int64_t heads, int64_t dim) {
   if (type != 0 || n * dim <= PROMPT_DIRECT || heads < 1 || dim < 1) return 0;

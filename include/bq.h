@@ -483,9 +483,12 @@ int bq_dequant_i8(const int8_t* q, int64_t N, int64_t K, const float* s, float* 
  * dim]; query head j attends with key-value head j / (q_heads / heads).
  *   out [n, q_heads, dim] (contiguous, of q's type) = softmax(scale q k^T) v
  * over the sequence's rows, causal: up to the query's own. Rows of no sequence, or whose scores are all
- * -infinity, get zeros. f32 accumulation; f32 products as sums of 16-bit pieces, to f32's accuracy; p
- * rounded to the 16-bit types. What a query does not see changes no bit of its output, infinities and
- * NaN included; queries that see such values are computed again, so a call with them takes longer.
+ * -infinity, get zeros. f32 accumulation. f32 products are sums of 16-bit pieces: those of p and v to f32's
+ * accuracy, a score's within 3 2^-22 of sum |q||k|. The 16-bit types round p to their type (half a step on
+ * each term, as the output). What a query does not see changes no bit of its output, infinities and NaN
+ * included. Queries that see such values are computed again in plain f32, and so are, in f32, those whose
+ * scores could be off by 2^-17 (and by 2^-22 of the largest) because a channel of a row is 2^14 and more
+ * below that row's largest and held to 2^-38 of it: a call with them takes longer.
  * dim 64 or 128. ws: bq_prompt_attention_ws_bytes bytes, 16-byte aligned (f32: the pieces of k and v,
  * unless short; none for the 16-bit types, whose rows of k and v lie at most 2^23 elements apart).
  * Beside the path, as bq_attention_f32 (scaled_dot_product_attention, borch/_nn.py:2143-2170). */

@@ -80,3 +80,48 @@ def test_scores_that_decide_a_row(dev, kind, dim, at):
         want = D.softmax_rows(q[:, j], k[:, 0], v[:, 0], seen, dim ** -0.5)[0]
         assert torch.equal(got[:, j].isnan(), want.isnan()) and torch.equal(got[:, j].isposinf(), want.isposinf())
         assert bool(got[at:, 0].isnan().all())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n,heads", [(90, 1), (300, 1), (300, 264)])
+@pytest.mark.parametrize("above", [2.0 ** 10, 2.0 ** 14, 2.0 ** 20, 2.0 ** 30, 2.0 ** 45])
+@pytest.mark.parametrize("which", ["q", "k"])
+def test_f32_channel_above_its_row(dev, dim, n, heads, above, which):
+    """A channel far above the others of its rows, over rows that are as small there (or 0). A score (times log2 e)
+    is within 3 2^-22 of sum |q||k| and 3 dim 2^-24 of it for the products' sums, and within 2^-17 or 2^-22 of the
+    row's largest for what small channels lose; twice the largest of them in the output, (n + 44) 2^-24 as above."""
+    print(f"prompt f32 channel above dim={dim} n={n} heads={heads} above={above} of {which}", flush=True)
+    g = torch.Generator().manual_seed(dim + n)
+    q, k, v = (torch.randn(n, 1, dim, generator=g) for _ in range(3))
+    high, low = (q, k) if which == "q" else (k, q)
+    high[..., 5] *= above
+    low[..., 5] /= above
+    low[::2, :, 5] = 0
+    cu = torch.tensor([0, n], dtype=torch.int32)
+    got = A.prompt_attention(q.expand(n, heads, dim).to(dev), k.to(dev), v.to(dev), cu.to(dev), causal=False, scale=0.125)
+    got = got[:, heads - 1].cpu().double()
+    want, _, size = D.softmax_rows(q[:, 0], k[:, 0], v[:, 0], torch.ones(n, n, dtype=torch.bool), 0.125)
+    top = (q[:, 0].double() @ k[:, 0].double().t().contiguous()).amax(1, keepdim=True).abs() * 0.125
+    each = (q[:, 0].double().abs() @ k[:, 0].double().abs().t().contiguous()).amax(1, keepdim=True) * 0.125
+    off = each * (3 * 2.0 ** -22 + 3 * dim * 2.0 ** -24) + torch.clamp_min(top * 2.0 ** -22, 2.0 ** -17)
+    tol = size * (2 * off + (n + 44) * 2.0 ** -24)
+    assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n,heads", [(90, 1), (300, 1), (300, 264)])
+def test_f32_channel_above_that_is_not_seen(dev, dim, n, heads):
+    """Keys and queries with such a channel change no bit of the rows before them, nor of the next sequence."""
+    print(f"prompt f32 channel above unseen dim={dim} n={n} heads={heads}", flush=True)
+    g = torch.Generator().manual_seed(dim + n)
+    q, k, v = (torch.randn(n, h, dim, generator=g) for h in (heads, 1, 1))
+    cu = torch.tensor([0, n - 20, n], dtype=torch.int32, device=dev)
+    clean = A.prompt_attention(q.to(dev), k.to(dev), v.to(dev), cu)
+    for at in (37, 66):
+        k[at, 0, 5] = 2.0 ** 40
+        got = A.prompt_attention(q.to(dev), k.to(dev), v.to(dev), cu)
+        assert torch.equal(got[:37], clean[:37]) and torch.equal(got[n - 20:], clean[n - 20:])
+        assert not torch.equal(got[at], clean[at])
+    q[40] *= 2.0 ** 60
+    got = A.prompt_attention(q.to(dev), k.to(dev), v.to(dev), cu)
+    assert torch.equal(got[:37], clean[:37]) and torch.equal(got[n - 20:], clean[n - 20:])
