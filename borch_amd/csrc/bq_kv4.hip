@@ -2,6 +2,8 @@
 // values it holds, and the eviction of the tokens that received least.
 #include <math.h>
 
+#include <type_traits>
+
 #include "bq_kv4.h"
 
 namespace bq {
@@ -564,46 +566,50 @@ __global__ __launch_bounds__(256) void kv4_move_kernel(Kv4 c, Kv4 to, const int*
                                                        int blocks) {
   using At = Kv4At<DIM>;
   constexpr int TB = At::TB, CB = At::CB, TOK = 4096 / DIM;
-  __shared__ long long from[TOK], dest[TOK];  // rows in the arrays; a source of -1: nothing to move
+  // rows in the arrays; a destination of -1: nothing to move; a source of -1: zeros (its entry is no page, and the
+  // new page may hold anything)
+  __shared__ long long from[TOK], dest[TOK];
   __shared__ int from_off[TOK], dest_off[TOK];
   const int bh = blockIdx.x / blocks, t0 = (blockIdx.x - bh * blocks) * TOK;
   const int b = bh / c.heads, h = bh - b * c.heads, tid = threadIdx.x;
   if (tid < TOK) {
     const int i = t0 + tid, src = i < keep ? kept[(size_t)bh * keep + i] : -1;
-    long long row = -1;
+    long long row = -1, to_row = -1;
     if (src >= 0) {
       const int si = fdiv(src, c.by_page.mul, c.by_page.shift), di = fdiv(i, c.by_page.mul, c.by_page.shift);
       const int sp = kv4_page(c, b, si), dp = kv4_page(to, b, di);
       from_off[tid] = src - si * c.page;
       dest_off[tid] = i - di * c.page;
-      if (sp >= 0 && dp >= 0) {
-        row = (long long)At::row(c, sp, h, from_off[tid]);
-        dest[tid] = (long long)At::row(c, dp, h, dest_off[tid]);
-      }
+      if (sp >= 0) row = (long long)At::row(c, sp, h, from_off[tid]);
+      if (dp >= 0) to_row = (long long)At::row(c, dp, h, dest_off[tid]);
     }
     from[tid] = row;
+    dest[tid] = to_row;
   }
   __syncthreads();
   if (tid < 128) {  // k: 16 bytes
     const int t = tid / (DIM / 32), q = tid % (DIM / 32);
-    if (from[t] >= 0)
-      *reinterpret_cast<uint4*>(c.k + At::k(dest[t]) + 16 * q) = *reinterpret_cast<const uint4*>(c.k + At::k(from[t]) + 16 * q);
+    if (dest[t] >= 0) {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (from[t] >= 0) x = *reinterpret_cast<const uint4*>(c.k + At::k(from[t]) + 16 * q);
+      *reinterpret_cast<uint4*>(c.k + At::k(dest[t]) + 16 * q) = x;
+    }
   } else {  // v: a slice of TB tokens, CB bytes each
     const int t = (tid - 128) / 16 * TB, s = tid % 16;
 #pragma unroll
     for (int e = 0; e < TB; ++e)
-      if (from[t + e] >= 0) {
-        const uint8_t* p = c.v + At::v(from[t + e], from_off[t + e], s);
-        uint8_t* at = c.v + At::v(dest[t + e], dest_off[t + e], s);
-        if constexpr (DIM == 128) *reinterpret_cast<uint32_t*>(at) = *reinterpret_cast<const uint32_t*>(p);
-        else *reinterpret_cast<uint16_t*>(at) = *reinterpret_cast<const uint16_t*>(p);
+      if (dest[t + e] >= 0) {
+        typedef std::conditional_t<DIM == 128, uint32_t, uint16_t> Slice;
+        Slice x = 0;
+        if (from[t + e] >= 0) x = *reinterpret_cast<const Slice*>(c.v + At::v(from[t + e], from_off[t + e], s));
+        *reinterpret_cast<Slice*>(c.v + At::v(dest[t + e], dest_off[t + e], s)) = x;
       }
   }
   if (tid < TOK * CB) {
     const int t = tid % TOK, s = tid / TOK;
-    if (from[t] >= 0) {
-      c.vs[At::vs(dest[t], dest_off[t], s)] = c.vs[At::vs(from[t], from_off[t], s)];
-      c.ks[At::ks(dest[t], dest_off[t], s)] = c.ks[At::ks(from[t], from_off[t], s)];
+    if (dest[t] >= 0) {
+      c.vs[At::vs(dest[t], dest_off[t], s)] = from[t] >= 0 ? c.vs[At::vs(from[t], from_off[t], s)] : (uint8_t)1;
+      c.ks[At::ks(dest[t], dest_off[t], s)] = from[t] >= 0 ? c.ks[At::ks(from[t], from_off[t], s)] : (uint8_t)1;
     }
   }
 }

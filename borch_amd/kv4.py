@@ -168,7 +168,8 @@ class Cache4:
         """Brings every (sequence, head) down to ``keep`` tokens: the ``recent`` last ones and, of the
         others, those of largest weight in ``sums`` f32 ``[sequences, heads, most]`` (what ``attend``
         added up; ties to the earlier token); a sequence of up to ``keep`` keeps all. They move in order
-        to the pages of ``new_table [sequences, >= keep / page]``, none of which is in use.
+        to the pages of ``new_table [sequences, >= keep / page]``, none of which is in use (zeros for one whose
+        entry is no page).
         Returns ``kept`` int32 ``[sequences, heads, keep]`` (their former places, -1 past the last),
         their ``weights`` (0 past the last) and ``left`` int32 ``[sequences]``, the new lengths."""
         no_graph("evict", sums)

@@ -508,7 +508,7 @@ int bq_prompt_attention(const void* q, const void* k, const void* v, int type, i
  *   v_scales  [page / 32][dim / 32][32]     token 32 a + b at [a][:][b]
  * Callers keep table i32 [B, width], each sequence's pages in order, and lens i32 [B], its cached
  * tokens. An entry that is no page (outside 0 .. pages - 1) holds nothing: tokens there are not
- * written, read as zeros, are not attended to and not moved. */
+ * written, read as zeros and are not attended to (an eviction that keeps one moves zeros). */
 typedef struct bq_kv4_cache {
   uint8_t *k, *k_scales, *v, *v_scales;
   int64_t pages, heads, page, dim;
