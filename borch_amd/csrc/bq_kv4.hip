@@ -664,7 +664,7 @@ int bq_kv4_read(const bq_kv4_cache* cache, const int32_t* table, int64_t B, int6
   if (!lens || !k || !v) return set_error(BQ_ERR_ARG, "%s: null pointer", what);
   if (((uintptr_t)k | (uintptr_t)v) & 15) return set_error(BQ_ERR_ARG, "%s: misaligned output", what);
   const int64_t blocks = (most + 31) / 32;
-  if (B * c.heads * blocks > 0x7fffffff) return set_error(BQ_ERR_ARG, "%s: size too large", what);
+  if (B * c.heads > 0x7fffffff / blocks) return set_error(BQ_ERR_ARG, "%s: size too large", what);  // within 64 bits
   hipStream_t st = (hipStream_t)stream;
   const unsigned grid = (unsigned)(B * c.heads * blocks);
   if (cache->dim == 128) kv4_read_kernel<128><<<grid, 256, 0, st>>>(c, lens, (int)most, (int)blocks, k, v);
@@ -701,7 +701,7 @@ int bq_kv4_evict(const bq_kv4_cache* cache, const float* sums, int64_t sums_b, i
   if (B == 0) return BQ_OK;
   if (!lens || !kept || !weights || !left || (most && !sums)) return set_error(BQ_ERR_ARG, "%s: null pointer", what);
   const int64_t blocks = (keep + 4096 / cache->dim - 1) / (4096 / cache->dim);
-  if (B * c.heads * blocks > 0x7fffffff) return set_error(BQ_ERR_ARG, "%s: size too large", what);
+  if (B * c.heads > 0x7fffffff / blocks) return set_error(BQ_ERR_ARG, "%s: size too large", what);  // within 64 bits
   hipStream_t st = (hipStream_t)stream;
   const int64_t rows = B * c.heads, parts = evict_parts(most, keep);
   const size_t need = bq_kv4_evict_ws_bytes(B, c.heads, most, keep);

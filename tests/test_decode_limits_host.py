@@ -31,3 +31,16 @@ def test_weights_that_overlap():
     assert call(0, 40) and call(120, 0) and call(120, 39) and call(119, 40) and call(40, 79) and call(0, 0)
     assert not call(0, 40, B=1)
     assert not call(32, 64, width=1) and call(31, 64, width=1)  # 32 tokens are what a page has room for
+
+
+def test_products_of_sizes_that_wrap():
+    """Sequences, heads and blocks whose product passes 64 bits are too large, not a small grid."""
+    lib = _lib.lib()
+    d = _lib.Kv4Desc(16, 16, 16, 16, 8, 65535, 32, 64)
+    most = 2 ** 31 - 8193
+    for B in (2 ** 22, 2 ** 23 - 1):
+        assert (B * 65535 * -(-most // 32) + 2 ** 63) % 2 ** 64 - 2 ** 63 < 2 ** 31  # as 64 bits have it
+        assert lib.bq_kv4_read(ctypes.byref(d), 16, B, 1, 16, most, 16, 16, None) == ARG and "large" in _lib.last_error()
+        keep = most // 2 // 32 * 32
+        rc = lib.bq_kv4_evict(ctypes.byref(d), 16, 8, 8, 8, 16, B, 1, 16, 16, keep // 32 + 1, keep, 0, 16, 16, 16, None, 0, None)
+        assert rc == ARG and "large" in _lib.last_error()
