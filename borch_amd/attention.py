@@ -34,8 +34,10 @@ def type_of(t: torch.Tensor, what: str) -> int:
 def no_graph(what: str, *operands: torch.Tensor) -> None:
     """Refuses operands that autograd would record: the kernels keep no graph, and a result without one would
     drop their gradients in silence."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in operands):
-        raise RuntimeError(f"{what}: no gradient is computed, and an operand requires one (torch.no_grad() or detach())")
+    if torch.is_grad_enabled():
+        for t in operands:
+            if t.requires_grad:
+                raise RuntimeError(f"{what}: no gradient is computed, and an operand requires one (torch.no_grad() or detach())")
 
 
 def rows(t: torch.Tensor, code: int):

@@ -125,7 +125,10 @@ class Cache4:
         queries of its key-value head, are added in place (rows that overlap, as an expanded view's, are
         refused). Returns ``[sequences, tokens, q_heads,
         dim]`` of q's type."""
-        no_graph("attend", *((q,) if weights is None else (q, weights)))
+        if weights is None:
+            no_graph("attend", q)
+        else:
+            no_graph("attend", q, weights)
         require_device(self.device)
         code = type_of(q, "attend")
         shape = q.shape
