@@ -153,6 +153,17 @@ __device__ __forceinline__ v16f score(const Frag<Kind<T>::PK>& k, const Frag<Kin
 // that are not finite get any; their products are not finite.
 __device__ __forceinline__ int row_exponent(uint32_t peak) { return max((int)(peak >> 23), 1) - 127 - 13; }
 constexpr int NO_ROW = -139;  // of a row of zeros
+// The largest over the wave.
+__device__ __forceinline__ int wave_max(int v) {
+  v = max(v, __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, false));   // lanes 1 apart
+  v = max(v, __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, false));   // 2
+  v = max(v, __builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, false));  // mirrored in 8
+  v = max(v, __builtin_amdgcn_mov_dpp(v, 0x140, 0xF, 0xF, false));  // and in 16
+  const auto x = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+  v = max((int)x[0], (int)x[1]);
+  const auto y = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+  return max((int)y[0], (int)y[1]);
+}
 // Two fp16 pieces of x 2^-e.
 __device__ __forceinline__ Frag<2> halves(const float x[8], int e) {
   v8h hi, lo;
@@ -706,8 +717,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(Prompt a) {
       // says more; then by those that the query sees.
       const float most = fmaxf(0x1p-17f, __fmul_rn(__fmul_rn(fabsf(m), a.scale2), 0x1p-22f));
       auto counts = [&](int e) { return __builtin_ldexpf(a.scale2, q_e + e + (DIM == 128 ? -2 : -3)) > most; };
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) most_e = max(most_e, __shfl_xor(most_e, d));
+      most_e = wave_max(most_e);
       if (lane == 0) tops[wave] = most_e;
       __syncthreads();
 #pragma unroll
