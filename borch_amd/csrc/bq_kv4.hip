@@ -560,7 +560,7 @@ __global__ __launch_bounds__(EVICT_THREADS) void kv4_select_kernel(Evict a) {
 // A workgroup takes 4096 / DIM destinations, whose rows and sources' rows it looks up once; k's rows
 // move 16 bytes a thread, v's slices are put together where they go (a thread gathers one slice of a
 // block of tokens) and the scales in v_scales' order. 2048 of 64 rows of 2500 on average, heads of 128:
-// 11 us; 16384 of 16 rows of 57768, heads of 64: 17 us, where nearly every block is touched (81 MB, 4.8 TB/s).
+// 12 us; 16384 of 16 rows of 57768, heads of 64: 17 us, where nearly every block is touched (81 MB, 4.8 TB/s).
 template <int DIM>
 __global__ __launch_bounds__(256) void kv4_move_kernel(Kv4 c, Kv4 to, const int* __restrict__ kept, int keep,
                                                        int blocks) {

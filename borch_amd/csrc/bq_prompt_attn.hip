@@ -29,7 +29,7 @@
 //
 // Bound by the MFMAs at the clock that they leave: 8192 tokens, 32 heads of 128 over 8, bf16, causal:
 // 520 to 575 us, 0.96 to 1.06 PFLOP/s, where the library's 8192^3 product reaches 1.21; 2048 and 1111
-// tokens, 16 heads of 128 over 4, f32: 136 us, nine 16-bit products for two.
+// tokens, 16 heads of 128 over 4, f32: 130 us, nine 16-bit products for two.
 #include <math.h>
 
 #include "bq_bf16x3.h"
