@@ -30,17 +30,9 @@
 // 4.3 TB/s. A streaming read of 4 GiB reaches 7.0 TB/s, a copy 4.75 (read and written).
 #include <math.h>
 
-#include "bq_bf16x3.h"
-#include "bq_kv4.h"
+#include "bq_kv4_pieces.h"
 
 namespace bq {
-
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-
-template <typename T>
-constexpr int Q_PIECES = __is_same(T, float) ? 3 : __is_same(T, _Float16) ? 2 : 1;
-template <typename T>
-constexpr int P_PIECES = __is_same(T, float) ? 3 : 2;
 
 struct Attend {
   Kv4 c;
@@ -57,51 +49,8 @@ struct Attend {
   int64_t wb, wh;
 };
 
-template <int P>
-struct Pieces {
-  v8bf p[P];
-};
-
-template <int P>
-__device__ __forceinline__ Pieces<P> pieces_of(const float x[8]) {
-  Pieces<P> r;
-  uint32_t w[P][4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float a = x[2 * i], b = x[2 * i + 1];
-#pragma unroll
-    for (int k = 0; k < P; ++k) {
-      w[k][i] = bf2(a, b);
-      if (k + 1 < P) {
-        a = __fsub_rn(a, __uint_as_float(w[k][i] << 16));
-        b = __fsub_rn(b, __uint_as_float(w[k][i] & 0xffff0000u));
-      }
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < P; ++k) r.p[k] = __builtin_bit_cast(v8bf, make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]));
-  return r;
-}
-
-template <typename T>
-__device__ __forceinline__ void load8f(const T* p, float x[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  } else if constexpr (__is_same(T, __bf16)) {
-    const v8bf a = *reinterpret_cast<const v8bf*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
-  } else {
-    const v8h a = *reinterpret_cast<const v8h*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
-  }
-}
-
 // q's pieces as the score product's second operand: rows row0 .. + 15, step s, of lane (n, g) row
-// row0 + n, channels DIM / 4 g + 8 s ..; rows past the last as zeros. An infinity stays one (inf - inf
-// left NaN in the second piece), and what f32 holds above bf16's largest value does not become one.
+// row0 + n, channels DIM / 4 g + 8 s ..; rows past the last as zeros.
 template <typename T, int DIM>
 __device__ __forceinline__ Pieces<Q_PIECES<T>> q_frag(const Attend& a, int b, int h, int row0, int s) {
   constexpr int P = Q_PIECES<T>;
@@ -110,28 +59,7 @@ __device__ __forceinline__ Pieces<Q_PIECES<T>> q_frag(const Attend& a, int b, in
   float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (row < a.rows)
     load8f((const T*)a.q + b * a.qb + t * a.qt + (int64_t)(h * a.group + j) * a.qh + DIM / 4 * g + 8 * s, x);
-  Pieces<P> r = pieces_of<P>(x);
-  if constexpr (P > 1) {
-    constexpr float MOST = 0x1.fep127f;
-    float peak = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) peak = fmaxf(peak, fabsf(x[i]));
-    if (__any(peak > (P == 2 ? 65504.f : MOST))) {
-      float y[8], z[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool finite = fabsf(x[i]) < INFINITY;
-        y[i] = finite ? fminf(fmaxf(x[i], -MOST), MOST) : x[i];
-        y[i] = (float)(__bf16)y[i];
-        z[i] = finite ? __fsub_rn(x[i], y[i]) : 0.f;
-      }
-      r.p[0] = pieces_of<1>(y).p[0];
-      const Pieces<P - 1> rest = pieces_of<P - 1>(z);
-#pragma unroll
-      for (int k = 1; k < P; ++k) r.p[k] = rest.p[k - 1];
-    }
-  }
-  return r;
+  return split_q<P>(x);
 }
 // The operands of RT row tiles in LDS, once for the four waves (in registers they took a third of
 // them in f32, and a wave a SIMD): a lane reads its own 16 bytes.
@@ -161,15 +89,6 @@ struct QRegs {
   Pieces<Q_PIECES<T>> f[DIM / 32];
   __device__ __forceinline__ v8bf at(int, int s, int k) const { return f[s].p[k]; }
 };
-
-__device__ __forceinline__ float scale_bits(uint32_t byte) { return __uint_as_float(byte << 23); }
-
-// Eight codes (one dword, low half byte first) times a scale, in bf16, exactly.
-__device__ __forceinline__ v8bf codes8(uint32_t w, float scale) {
-  const v2bf a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1),
-             c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3);
-  return v8bf{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
 
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 // 16 bytes of codes, read once a call: past the caches' other contents.
@@ -275,18 +194,6 @@ struct VBlock {
     odd = __builtin_bit_cast(v8bf, make_uint4(o[0], o[1], o[2], o[3]));
   }
 };
-
-template <typename T>
-__device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
-  } else if constexpr (__is_same(T, __bf16)) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(bf2(a, b), bf2(c, d));
-  } else {
-    typedef _Float16 v4h __attribute__((ext_vector_type(4)));
-    *reinterpret_cast<v4h*>(p) = v4h{(_Float16)a, (_Float16)b, (_Float16)c, (_Float16)d};
-  }
-}
 
 // exp2(c (s - m)) with an empty row's maximum, -infinity, taken as 0
 __device__ __forceinline__ float weight_of(float s, float base, float c) {

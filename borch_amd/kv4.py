@@ -1,5 +1,6 @@
 """A decoder's key-value cache held in 4 bits (``bq_kv4_*``, ``include/bq.h``): new tokens quantized
-into its pages, attention of the newest tokens over it, eviction of the tokens that received least.
+into its pages, attention of the newest tokens or of chunks of a prompt over it, eviction of the tokens that
+received least.
 
 A value is one of +-{0, 1/2, 1, 3/2, 2, 3, 4, 6} times the power of two that 32 neighbouring channels
 of a token share: 4.25 bits a channel, 136 bytes for the keys and values of a token and a head of
@@ -21,6 +22,11 @@ __all__ = ["Cache4"]
 @functools.lru_cache(maxsize=1024)
 def _attend_ws_bytes(*sizes) -> int:
     return int(lib().bq_kv4_attend_ws_bytes(*sizes))
+
+
+@functools.lru_cache(maxsize=1024)
+def _chunk_ws_bytes(*sizes) -> int:
+    return int(lib().bq_kv4_attend_chunk_ws_bytes(*sizes))
 
 
 class Cache4:
@@ -164,6 +170,41 @@ class Cache4:
             check(lib().bq_kv4_attend(self._ref, q.data_ptr(), code, T, hq, *qs, table.data_ptr(), B, width,
                                       lens.data_ptr(), max_len, dim ** -0.5 if scale is None else scale, out.data_ptr(),
                                       w, wb, wh, ws.data_ptr() if need else None, need, _stream(q)))
+        return out
+
+    def attend_chunk(self, q: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, cu: torch.Tensor,
+                     max_len: int | None = None, scale: float | None = None) -> torch.Tensor:
+        """Attention of chunks of new tokens over the cache, of another length for each sequence: ``q [n,
+        q_heads, dim]`` (f32, bf16 or f16), sequence ``b``'s the rows ``cu[b] .. cu[b + 1]`` (``cu`` int32 on
+        the device, ascending), the last ones of its ``lens[b]`` cached tokens, as ``append`` takes their
+        keys and values before. Row ``i`` is token ``lens[b] - cu[b + 1] + i`` and sees the cached tokens up
+        to itself; where it sees none its output is 0, and so are rows of no sequence. ``max_len``: no
+        sequence is longer (default: what the table's pages hold; the work is planned for it, longer ones
+        are cut). Returns ``[n, q_heads, dim]`` of q's type."""
+        no_graph("attend_chunk", q)
+        require_device(self.device)
+        code = type_of(q, "attend_chunk")
+        shape = q.shape
+        if len(shape) != 3 or shape[2] != self.dim or shape[1] % self.heads or shape[1] == 0:
+            raise RuntimeError(f"attend_chunk: q {tuple(q.shape)} is [tokens, query heads, dim] over {self.heads} "
+                               f"key-value heads of {self.dim}")
+        if q.get_device() != self._index:
+            raise RuntimeError(f"attend_chunk: the cache is on {self.device}, q on {q.device}")
+        table, lens, B, width = self._table(table, lens, "attend_chunk")
+        cu = ints(cu, (B + 1,), "cu", self._index)
+        n, hq, dim = shape
+        if max_len is None:
+            max_len = width * self.page
+        out = torch.empty(shape, dtype=q.dtype, device=self.device)
+        if n == 0:
+            return out
+        q, qs = rows(q, code)
+        need = _chunk_ws_bytes(n, B, hq, self.heads, dim, max_len)
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        with on(self._index):
+            check(lib().bq_kv4_attend_chunk(self._ref, q.data_ptr(), code, n, hq, *qs, table.data_ptr(), B, width,
+                                            lens.data_ptr(), cu.data_ptr(), max_len, dim ** -0.5 if scale is None else scale,
+                                            out.data_ptr(), ws.data_ptr() if need else None, need, _stream(q)))
         return out
 
     def evict(self, sums: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, new_table: torch.Tensor, keep: int,

@@ -544,6 +544,23 @@ int bq_kv4_attend(const bq_kv4_cache* cache, const void* q, int type, int64_t to
                   int64_t max_len, float scale, void* out, float* weights, int64_t w_seq, int64_t w_head, void* ws,
                   size_t ws_bytes, bq_stream_t stream);
 
+/* Workspace bytes of bq_kv4_attend_chunk (0 where the work is not cut). */
+size_t bq_kv4_attend_chunk_ws_bytes(int64_t n, int64_t B, int64_t q_heads, int64_t heads, int64_t dim, int64_t max_len);
+
+/* Attention of chunks of new tokens over the cache: q [n, q_heads, dim], sequence b's the rows cu[b] ..
+ * cu[b + 1] - 1 (cu i32 [B + 1], ascending), the last ones of its lens[b] cached tokens (lens counts them):
+ * row i is token lens[b] - cu[b + 1] + i and sees the tokens up to itself (of the first max_len):
+ *   out [n, q_heads, dim] (contiguous, of q's type) = softmax(scale q k^T) v
+ * over the values that the cache stands for, zeros where nothing is seen and in rows of no sequence; what a
+ * row does not see never reaches its output. f32 accumulation; f32 and f16 products to f32's accuracy, but
+ * f16's weights to 2^-17; bf16 rounds the weights to its type (half a step on each term, as the output). No
+ * atomics: the same bits in every run. ws: bq_kv4_attend_chunk_ws_bytes bytes, 16-byte aligned, need not be
+ * cleared. */
+int bq_kv4_attend_chunk(const bq_kv4_cache* cache, const void* q, int type, int64_t n, int64_t q_heads, int64_t q_token,
+                        int64_t q_head, const int32_t* table, int64_t B, int64_t width, const int32_t* lens,
+                        const int32_t* cu, int64_t max_len, float scale, void* out, void* ws, size_t ws_bytes,
+                        bq_stream_t stream);
+
 /* Eviction: of each (sequence, head) with more than `keep` cached tokens the `recent` last ones stay
  * and, of the others, the keep - recent of largest weight in sums f32 (`most` a row, rows at sums_b
  * and sums_h elements; ties to the earlier token, NaN above all); the tokens that stay move in
