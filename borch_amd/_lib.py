@@ -50,6 +50,12 @@ class Kv4Desc(ctypes.Structure):
                 ("heads", _c_i64), ("page", _c_i64), ("dim", _c_i64)]
 
 
+class PagesDesc(ctypes.Structure):
+    """``bq_pages`` (include/bq.h): page tables on the GPU."""
+    _fields_ = [("table", _c_p), ("lens", _c_p), ("refs", _c_p), ("sequences", _c_i64), ("width", _c_i64),
+                ("pages", _c_i64), ("page", _c_i64)]
+
+
 # name -> (restype, argtypes); mirrors include/bq.h one for one.
 SIGNATURES = {
     "bq_version": (_c_int, []),
@@ -116,6 +122,12 @@ SIGNATURES = {
                                    _c_size, _c_p]),
     "bq_prompt_attention_ws_bytes": (_c_size, [_c_int, _c_i64, _c_i64, _c_i64]),
     "bq_kv4_append": (_c_int, [_c_p, _c_p, _c_p, _c_int, *[_c_i64] * 5, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p]),
+    "bq_kv4_append_slots": (_c_int, [_c_p, _c_p, _c_p, _c_int, *[_c_i64] * 5, _c_p, _c_p]),
+    "bq_pages_cut": (_c_int, [_c_p, _c_p, _c_p]),
+    "bq_pages_fork": (_c_int, [_c_p, _c_p, _c_p]),
+    "bq_pages_grow_ws_bytes": (_c_size, [_c_i64]),
+    "bq_pages_grow": (_c_int, [_c_p, _c_p, _c_i64, *[_c_p] * 6, _c_size, _c_p]),
+    "bq_kv4_copy_pages": (_c_int, [_c_p, _c_i64, _c_p, _c_i64, _c_p]),
     "bq_kv4_read": (_c_int, [_c_p, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_p]),
     "bq_kv4_attend_ws_bytes": (_c_size, [*[_c_i64] * 5, _c_int]),
     "bq_kv4_attend": (_c_int, [_c_p, _c_p, _c_int, *[_c_i64] * 5, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_f, _c_p,

@@ -57,10 +57,10 @@ def rows(t: torch.Tensor, code: int):
     return t, t.stride()[:-1]
 
 
-def ints(t: torch.Tensor, shape, what: str, index: int) -> torch.Tensor:
-    """An int32 index tensor of ``shape`` on device ``index``, contiguous."""
-    if t.dtype is not torch.int32:
-        raise TypeError(f"{what}: expected int32, got {t.dtype}")
+def ints(t: torch.Tensor, shape, what: str, index: int, dtype: torch.dtype = torch.int32) -> torch.Tensor:
+    """An index tensor of ``shape`` and ``dtype`` on device ``index``, contiguous."""
+    if t.dtype is not dtype:
+        raise TypeError(f"{what}: expected {str(dtype)[6:]}, got {t.dtype}")
     if t.get_device() != index:
         raise RuntimeError(f"{what}: on {t.device}, the operands are on cuda:{index}")
     if t.shape != shape:

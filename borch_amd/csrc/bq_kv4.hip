@@ -51,12 +51,14 @@ __device__ __forceinline__ v8f load8(const T* p) {
 // hardware's rounding to nearest even of the exact quotient.
 // A workgroup takes 2048 / DIM tokens, whose places it looks up once, and PARTS of their 2 heads rows
 // (keys, then values), all loaded at once: with a row a thread the chain of lookups before each
-// row was most of the time (6237 tokens, 8 heads of 128, f32: 15.5 -> 13.4 us, 4.3 TB/s).
+// row was most of the time (6237 tokens, 8 heads of 128, f32: 15.5 -> 13.4 us, 4.3 TB/s). `slots`, where given,
+// are the places.
 constexpr int PARTS = 4;
 template <typename T, int DIM>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4 c, const T* __restrict__ nk, const T* __restrict__ nv,
                                                          int64_t kt, int64_t kh, int64_t vt, int64_t vh, int n, int groups,
-                                                         const int* __restrict__ lens, const int* __restrict__ cu, int B) {
+                                                         const int* __restrict__ lens, const int* __restrict__ cu, int B,
+                                                         const int64_t* __restrict__ slots) {
   using At = Kv4At<DIM>;
   constexpr int P = DIM / 8;
   const int tile = blockIdx.x / groups, part0 = (blockIdx.x - tile * groups) * PARTS;
@@ -70,14 +72,21 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4 c, const T* __restr
     const T* from = is_v ? nv + i * vt + (part - c.heads) * vh : nk + i * kt + part * kh;
     x[e] = load8(from + 8 * piece);
   }
-  int lo = 0, hi = B;  // the sequence: the last b with cu[b] <= i
+  int lo = 0, hi = slots ? 0 : B;  // the sequence: the last b with cu[b] <= i
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
     if (cu[mid + 1] <= i) lo = mid + 1;
     else hi = mid;
   }
   int at = -1, off = 0;
-  if (lo < B) {  // else past the last sequence
+  if (slots) {  // given
+    const int64_t slot = slots[i];
+    const int64_t p = slot >> 31 ? slot / c.page : fdiv((int)slot, c.by_page.mul, c.by_page.shift);
+    if (slot >= 0 && p < c.pages) {
+      at = (int)p;
+      off = (int)(slot - p * c.page);
+    }
+  } else if (lo < B) {  // else past the last sequence
     const int64_t pos = (int64_t)lens[lo] - cu[lo + 1] + i;
     if (i >= cu[lo] && pos >= 0 && pos < (int64_t)c.width * c.page) {  // else before the first
       const int pi = fdiv((int)pos, c.by_page.mul, c.by_page.shift);
@@ -616,11 +625,38 @@ __global__ __launch_bounds__(256) void kv4_move_kernel(Kv4 c, Kv4 to, const int*
 
 template <typename T, int DIM>
 static void append_of(const Kv4& c, const void* nk, const void* nv, int64_t n, int64_t kt, int64_t kh, int64_t vt,
-                      int64_t vh, const int* lens, const int* cu, int B, hipStream_t st) {
+                      int64_t vh, const int* lens, const int* cu, int B, const int64_t* slots, hipStream_t st) {
   const int groups = (2 * c.heads + PARTS - 1) / PARTS;
   const int64_t tiles = (n + 2048 / DIM - 1) / (2048 / DIM);
   kv4_append_kernel<T, DIM><<<(unsigned)(tiles * groups), 256, 0, st>>>(c, (const T*)nk, (const T*)nv, kt, kh, vt, vh, (int)n,
-                                                                       groups, lens, cu, B);
+                                                                       groups, lens, cu, B, slots);
+}
+
+// Tokens whose places come from lens and cu, or are given.
+static int append(const char* what, const bq_kv4_cache* cache, const void* new_k, const void* new_v, int type, int64_t n,
+                  int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, const int32_t* table, int64_t B,
+                  int64_t width, const int32_t* lens, const int32_t* cu, const int64_t* slots, bool given,
+                  hipStream_t st) {
+  Kv4 c;
+  if (const int rc = kv4_of(what, cache, table, B, width, &c)) return rc;
+  if (type < 0 || type > 2) return set_error(BQ_ERR_ARG, "%s: type %d", what, type);
+  if (n < 0 || n > 0x7fffffff) return set_error(BQ_ERR_ARG, "%s: %lld tokens", what, (long long)n);
+  if (n == 0 || (!given && (B == 0 || width == 0)) || c.pages == 0) return BQ_OK;
+  if (!new_k || !new_v || (given ? !slots : !lens || !cu)) return set_error(BQ_ERR_ARG, "%s: null pointer", what);
+  const int64_t size = type == KV4_F32 ? 4 : 2;
+  if ((((uintptr_t)new_k | (uintptr_t)new_v) & 15) || (k_token | k_head | v_token | v_head) * size % 16)
+    return set_error(BQ_ERR_ARG, "%s: rows that are not 16-byte aligned", what);
+  if ((n + 15) / 16 * ((2 * c.heads + PARTS - 1) / PARTS) > 0x7fffffff)
+    return set_error(BQ_ERR_ARG, "%s: size too large", what);
+  const bool wide = cache->dim == 128;
+#define BQ_APPEND(T)                                                                                            \
+  (wide ? append_of<T, 128>(c, new_k, new_v, n, k_token, k_head, v_token, v_head, lens, cu, (int)B, slots, st)  \
+        : append_of<T, 64>(c, new_k, new_v, n, k_token, k_head, v_token, v_head, lens, cu, (int)B, slots, st))
+  if (type == KV4_F32) BQ_APPEND(float);
+  else if (type == KV4_BF16) BQ_APPEND(__bf16);
+  else BQ_APPEND(_Float16);
+#undef BQ_APPEND
+  return check_launch(what);
 }
 
 }  // namespace bq
@@ -630,28 +666,15 @@ using namespace bq;
 int bq_kv4_append(const bq_kv4_cache* cache, const void* new_k, const void* new_v, int type, int64_t n,
                   int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, const int32_t* table, int64_t B,
                   int64_t width, const int32_t* lens, const int32_t* cu, bq_stream_t stream) {
-  const char* what = "bq_kv4_append";
-  Kv4 c;
-  if (const int rc = kv4_of(what, cache, table, B, width, &c)) return rc;
-  if (type < 0 || type > 2) return set_error(BQ_ERR_ARG, "%s: type %d", what, type);
-  if (n < 0 || n > 0x7fffffff) return set_error(BQ_ERR_ARG, "%s: %lld tokens", what, (long long)n);
-  if (n == 0 || B == 0 || width == 0 || c.pages == 0) return BQ_OK;
-  if (!new_k || !new_v || !lens || !cu) return set_error(BQ_ERR_ARG, "%s: null pointer", what);
-  const int64_t size = type == KV4_F32 ? 4 : 2;
-  if ((((uintptr_t)new_k | (uintptr_t)new_v) & 15) || (k_token | k_head | v_token | v_head) * size % 16)
-    return set_error(BQ_ERR_ARG, "%s: rows that are not 16-byte aligned", what);
-  if ((n + 15) / 16 * ((2 * c.heads + PARTS - 1) / PARTS) > 0x7fffffff)
-    return set_error(BQ_ERR_ARG, "%s: size too large", what);
-  hipStream_t st = (hipStream_t)stream;
-  const bool wide = cache->dim == 128;
-#define BQ_APPEND(T)                                                                                            \
-  (wide ? append_of<T, 128>(c, new_k, new_v, n, k_token, k_head, v_token, v_head, lens, cu, (int)B, st)         \
-        : append_of<T, 64>(c, new_k, new_v, n, k_token, k_head, v_token, v_head, lens, cu, (int)B, st))
-  if (type == KV4_F32) BQ_APPEND(float);
-  else if (type == KV4_BF16) BQ_APPEND(__bf16);
-  else BQ_APPEND(_Float16);
-#undef BQ_APPEND
-  return check_launch(what);
+  return append("bq_kv4_append", cache, new_k, new_v, type, n, k_token, k_head, v_token, v_head, table, B, width, lens,
+                cu, nullptr, false, (hipStream_t)stream);
+}
+
+int bq_kv4_append_slots(const bq_kv4_cache* cache, const void* new_k, const void* new_v, int type, int64_t n,
+                        int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, const int64_t* slots,
+                        bq_stream_t stream) {
+  return append("bq_kv4_append_slots", cache, new_k, new_v, type, n, k_token, k_head, v_token, v_head, nullptr, 0, 0,
+                nullptr, nullptr, slots, true, (hipStream_t)stream);
 }
 
 int bq_kv4_read(const bq_kv4_cache* cache, const int32_t* table, int64_t B, int64_t width, const int32_t* lens,

@@ -84,10 +84,14 @@ class Cache4:
             raise RuntimeError(f"{what}: table is [sequences, pages]")
         return ints(table, shape, "table", self._index), ints(lens, shape[:1], "lens", self._index), *shape
 
-    def append(self, new_k: torch.Tensor, new_v: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
-               cu: torch.Tensor) -> None:
+    def append(self, new_k: torch.Tensor, new_v: torch.Tensor, table: torch.Tensor | None = None,
+               lens: torch.Tensor | None = None, cu: torch.Tensor | None = None,
+               slots: torch.Tensor | None = None) -> None:
         """``new_k``, ``new_v [n, heads, dim]`` (f32, bf16 or f16) into the cache: sequence ``b``'s the
-        rows ``cu[b] .. cu[b + 1]``, the last ones of its ``lens[b]`` tokens (``lens`` counts them)."""
+        rows ``cu[b] .. cu[b + 1]``, the last ones of its ``lens[b]`` tokens (``lens`` counts them). Or, in
+        place of the three, ``slots`` int64 ``[n]``: row ``i`` into place ``slots[i] % page`` of page ``slots[i]
+        // page`` (``paging.Pages.grow`` gives them, for all layers at once); a slot in no page is not
+        written, and none is named twice."""
         no_graph("append", new_k, new_v)
         require_device(self.device)
         code = type_of(new_k, "append")
@@ -99,6 +103,17 @@ class Cache4:
                                f"the cache holds {self.heads} heads of {self.dim}")
         if new_k.get_device() != self._index or new_v.get_device() != self._index:
             raise RuntimeError(f"append: the cache is on {self.device}, keys on {new_k.device}, values on {new_v.device}")
+        if slots is not None:
+            if table is not None or lens is not None or cu is not None:
+                raise RuntimeError("append: slots, or table, lens and cu")
+            slots = ints(slots, shape[:1], "slots", self._index, torch.int64)
+            (new_k, ks), (new_v, vs) = rows(new_k, code), rows(new_v, code)
+            with on(self._index):
+                check(lib().bq_kv4_append_slots(self._ref, new_k.data_ptr(), new_v.data_ptr(), code, shape[0], *ks, *vs,
+                                                slots.data_ptr(), _stream(new_k)))
+            return
+        if table is None or lens is None or cu is None:
+            raise RuntimeError("append: slots, or table, lens and cu")
         table, lens, B, width = self._table(table, lens, "append")
         cu = ints(cu, (B + 1,), "cu", self._index)
         (new_k, ks), (new_v, vs) = rows(new_k, code), rows(new_v, code)

@@ -523,6 +523,12 @@ int bq_kv4_append(const bq_kv4_cache* cache, const void* new_k, const void* new_
                   int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, const int32_t* table, int64_t B,
                   int64_t width, const int32_t* lens, const int32_t* cu, bq_stream_t stream);
 
+/* bq_kv4_append of tokens whose places are known: row i into place slots[i] % page of page slots[i] / page
+ * (bq_pages_grow's slots); rows whose slot is in no page are not written. Slots that occur twice race. */
+int bq_kv4_append_slots(const bq_kv4_cache* cache, const void* new_k, const void* new_v, int type, int64_t n,
+                        int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, const int64_t* slots,
+                        bq_stream_t stream);
+
 /* The values held: k, v f32 [B, heads, most, dim], zeros from lens[b] on. */
 int bq_kv4_read(const bq_kv4_cache* cache, const int32_t* table, int64_t B, int64_t width, const int32_t* lens,
                 int64_t most, float* k, float* v, bq_stream_t stream);
@@ -573,6 +579,44 @@ int bq_kv4_evict(const bq_kv4_cache* cache, const float* sums, int64_t sums_b, i
                  const int32_t* table, int64_t B, int64_t width, const int32_t* lens, const int32_t* new_table,
                  int64_t new_width, int64_t keep, int64_t recent, int32_t* kept, float* weights, int32_t* left,
                  void* ws, size_t ws_bytes, bq_stream_t stream);
+
+/* ---- page tables on the GPU ----
+ *
+ * table i32 [sequences, width] names each sequence's pages in order, -1 past the last; lens i32 [sequences] its
+ * tokens; refs i32 [pages] how many entries name a page (0: it is free); page: tokens a page. Entries that are no
+ * page count nowhere. At most 8192 sequences and 2^24 pages. */
+typedef struct bq_pages {
+  int32_t *table, *lens, *refs;
+  int64_t sequences, width, pages, page;
+} bq_pages;
+
+/* Sequences cut back: lens[s] = min(lens[s], max(to[s], 0)), and the entries past the last page that is still
+ * needed leave the table and their pages' refs. */
+int bq_pages_cut(const bq_pages* pages, const int32_t* to, bq_stream_t stream);
+
+/* Every sequence becomes what its parent was (parents i32 [sequences]; none of them: empty): rows and lengths
+ * move, refs with them. */
+int bq_pages_fork(const bq_pages* pages, const int32_t* parents, bq_stream_t stream);
+
+/* Places for more[s] new tokens of each sequence s, of all or (ok i32 [1] = 0, nothing changes) of none: more and
+ * lens have to be 0 or above, the pages to fit `width` and what is free, the tokens, packed one sequence after
+ * another, `rows`. Free pages go to the sequences in ascending order of both. A last page that is partly filled
+ * and named by other entries too is replaced by a free one (before the sequence's others), save for the lowest of
+ * the sequences that share it so where all that name it grow.
+ *   cu i32 [sequences + 1]: their first rows and the end (all 0 if there is no room)
+ *   slots i64, at i32 [rows]: each token's place, page * pages->page + place in it, and its place in its
+ *     sequence; -1 past the last (and a slot of -1 where the table names no page)
+ *   moves i32 [3, sequences]: pages whose tokens have to move before more are written: from, to (-1: none) and
+ *     how many tokens (bq_kv4_copy_pages)
+ * ws: bq_pages_grow_ws_bytes bytes, 4-byte aligned, need not be cleared. */
+size_t bq_pages_grow_ws_bytes(int64_t pages);
+int bq_pages_grow(const bq_pages* pages, const int32_t* more, int64_t rows, int32_t* cu, int64_t* slots, int32_t* at,
+                  int32_t* moves, int32_t* ok, void* ws, size_t ws_bytes, bq_stream_t stream);
+
+/* The moves of bq_pages_grow in `count` caches (an array on the host): the first tokens, 32 at a time, of page
+ * moves[0][s] to page moves[1][s] of each. */
+int bq_kv4_copy_pages(const bq_kv4_cache* caches, int64_t count, const int32_t* moves, int64_t sequences,
+                      bq_stream_t stream);
 
 #ifdef __cplusplus
 }
