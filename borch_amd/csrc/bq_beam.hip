@@ -1,0 +1,261 @@
+// A beam search's selection: of each request's W beams and V tokens the W best continuations.
+//
+// A candidate's score is scores[b][w] + (x[b w][v] - lse), lse = m + log sum_v exp(x - m) over the beam's
+// logits x with their maximum m. Beams are compared with one another in 64 bits: two candidates whose scores
+// differ by less than f32 shows would else come out in an order that the sum's rounding decides. So the sum
+// and its exponentials are taken in 64 bits too, and everything else about a beam's own tokens goes by the logits
+// as they are: within a beam their order is that of the scores.
+//
+// Two launches. The first reads the logits once: a workgroup takes a part of a beam's tokens, and each of its
+// waves keeps the W best of what it reads, a candidate a lane in order (value and token as one 64-bit number,
+// so that equals go to the lower token); a logit that beats the last of them is rare after the first few
+// hundred, so the test of all 64 lanes at once is most of the cost. The second joins a request's parts and
+// beams.
+#include <math.h>
+
+#include "bq_common.h"
+
+namespace bq {
+
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+constexpr int MOST_BEAMS = 64, PART_WAVES = 4;
+
+struct Beam {
+  const void* x;
+  int64_t pitch;  // elements from beam to beam
+  const float* scores;
+  const uint8_t* done;  // nullable
+  int B, W, V, end, parts, per;  // per: tokens a part
+  uint64_t* best;  // [B W][parts][W] candidates in order
+  double2* sums;   // [B W][parts]: maximum, sum of exp(x - maximum)
+  float* out;
+  int *parents, *tokens;
+  uint8_t* ended;
+};
+
+// A logit and its token as one number: larger is better. -0 counts as 0; NaN does not come here.
+__device__ __forceinline__ uint64_t rank_of(float x, int token) {
+  const uint32_t u = __float_as_uint(__fadd_rn(x, 0.f));
+  const uint32_t o = u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+  return (uint64_t)o << 32 | (uint32_t)~token;
+}
+__device__ __forceinline__ float logit_of(uint64_t r) {
+  const uint32_t o = (uint32_t)(r >> 32);
+  return __uint_as_float(o ^ (o & 0x80000000u ? 0x80000000u : 0xffffffffu));
+}
+__device__ __forceinline__ int token_of(uint64_t r) { return (int)~(uint32_t)r; }
+
+// The best `W` so far, in order, lane i the i-th (0: none); `least` the W-th.
+struct List {
+  uint64_t mine, least;
+  int W;
+  __device__ __forceinline__ void clear(int w) { mine = 0, least = 0, W = w; }
+  // every lane's candidate that is good enough, one after another
+  __device__ __forceinline__ void add(uint64_t r) {
+    const int lane = threadIdx.x & 63;
+    uint64_t who = __ballot(r > least);
+    while (who) {
+      const int l = __builtin_ctzll(who);
+      const uint64_t x = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(r >> 32), l) << 32 |
+                         (uint32_t)__builtin_amdgcn_readlane((int)r, l);
+      const uint64_t up = __shfl_up(mine, 1);
+      mine = mine > x ? mine : lane == 0 || up > x ? x : up;
+      least = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), W - 1) << 32 |
+              (uint32_t)__builtin_amdgcn_readlane((int)mine, W - 1);
+      who &= who - 1;
+      who &= __ballot(r > least);
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ float at(const T* x, int i) {
+  return (float)x[i];
+}
+
+template <typename T>
+__global__ __launch_bounds__(PART_WAVES * 64) void beam_part_kernel(Beam a) {
+  __shared__ uint64_t lists[PART_WAVES][MOST_BEAMS];
+  __shared__ double sums[PART_WAVES];
+  __shared__ float tops[PART_WAVES];
+  const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
+  if (a.done && a.done[row]) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const T* x = (const T*)a.x + row * a.pitch;
+  const int lo = part * a.per, hi = min(a.V, lo + a.per);
+  // the maximum first, then the sum against it; NaN anywhere makes the sum NaN
+  float top = -INFINITY;
+  bool nan = false;
+  List best;
+  best.clear(a.W);
+  for (int i0 = lo + wave * 64; i0 < hi; i0 += PART_WAVES * 64) {
+    const int i = i0 + lane;
+    const float v = i < hi ? at(x, i) : -INFINITY;
+    nan |= v != v;
+    top = fmaxf(top, v);
+    best.add(i < hi && v == v ? rank_of(v, i) : 0);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  if (lane == 0) tops[wave] = top;
+  lists[wave][lane] = best.mine;
+  nan = __syncthreads_or(nan);
+#pragma unroll
+  for (int w = 0; w < PART_WAVES; ++w) top = fmaxf(top, tops[w]);
+  double sum = 0.0;
+  if (!nan && top > -INFINITY && top < INFINITY)
+    for (int i = lo + (int)threadIdx.x; i < hi; i += PART_WAVES * 64) sum += exp((double)at(x, i) - (double)top);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+  if (lane == 0) sums[wave] = sum;
+  __syncthreads();
+  if (wave) return;
+  for (int w = 1; w < PART_WAVES; ++w) best.add(lists[w][lane]);
+  const size_t slot = (size_t)row * a.parts + part;
+  if (lane < a.W) a.best[slot * a.W + lane] = best.mine;
+  if (lane == 0) {
+    double s = sums[0];
+    for (int w = 1; w < PART_WAVES; ++w) s += sums[w];
+    a.sums[slot] = make_double2(nan ? (double)NAN : (double)top, s);
+  }
+}
+
+// One request: each beam's parts joined, then the beams. Candidates are in order of (score, beam, place in the
+// beam's order), and a candidate's place among all is the number of those before it, beam by beam.
+__global__ __launch_bounds__(256) void beam_join_kernel(Beam a) {
+  extern __shared__ unsigned char lds[];
+  double* keys = reinterpret_cast<double*>(lds);             // [W][W]
+  int* toks = reinterpret_cast<int*>(keys + a.W * a.W);      // [W][W]
+  int* counts = toks + a.W * a.W;                            // [W]: a beam's candidates
+  const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, W = a.W, most = min(W, a.V);
+  for (int w = wave; w < W; w += 4) {
+    const int row = b * W + w;
+    const double score = (double)a.scores[row];
+    double key = -INFINITY;
+    int token = -1;
+    if (a.done && a.done[row]) {
+      key = score != score ? -INFINITY : score;
+      token = lane == 0 ? a.end : -1;
+    } else {
+      List best;
+      best.clear(W);
+      double top = -INFINITY, sum = 0.0;
+      bool nan = false;
+      for (int p0 = 0; p0 < a.parts; p0 += 64) {
+        const int p = p0 + lane;
+        double2 s = make_double2(-INFINITY, 0.0);
+        if (p < a.parts) s = a.sums[(size_t)row * a.parts + p];
+        nan |= s.x != s.x;
+        double now = s.x;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) now = fmax(now, __shfl_xor(now, d));
+        now = fmax(now, top);
+        double add = s.x > -INFINITY ? s.y * exp(s.x - now) : 0.0;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) add += __shfl_xor(add, d);
+        sum = (top > -INFINITY ? sum * exp(top - now) : 0.0) + add;
+        top = now;
+      }
+      for (int i0 = 0; i0 < a.parts * W; i0 += 64)
+        best.add(i0 + lane < a.parts * W ? a.best[(size_t)row * a.parts * W + i0 + lane] : 0);
+      const bool dead = __any(nan) || !(top > -INFINITY && top < INFINITY) || !(fabs(score) < INFINITY);
+      if (dead) {
+        token = lane;  // nothing tells its tokens apart
+      } else {
+        token = token_of(best.mine);
+        key = score + ((double)logit_of(best.mine) - (top + log(sum)));
+        if (key != key) key = -INFINITY;
+      }
+      if (lane >= most) token = -1;
+    }
+    if (lane < W) {
+      keys[w * W + lane] = key;
+      toks[w * W + lane] = token;
+    }
+    const uint64_t real = __ballot(lane < W && token >= 0);
+    if (lane == 0) counts[w] = __builtin_popcountll(real);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < W * W; i += 256) {
+    const int own = i / W, nth = i - own * W;
+    if (nth >= counts[own]) continue;
+    const double key = keys[i];
+    int place = nth;
+    for (int w = 0; w < W && place < W; ++w) {
+      if (w == own) continue;
+      int lo = 0, hi = counts[w];  // how many of w's come before
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        const double k = keys[w * W + mid];
+        if (k > key || (k == key && w < own)) lo = mid + 1;
+        else hi = mid;
+      }
+      place += lo;
+    }
+    if (place < W) {
+      const int row = b * W + own, to = b * W + place;
+      a.out[to] = (float)key;
+      a.parents[to] = row;
+      a.tokens[to] = toks[i];
+      if (a.ended) a.ended[to] = (a.done && a.done[row]) || toks[i] == a.end;
+    }
+  }
+}
+
+// The parts of a beam: enough workgroups for the GPU, of at least 1024 tokens each.
+static int64_t parts_of(int64_t rows, int64_t V) {
+  const int64_t want = (2048 + rows - 1) / rows, most = (V + 1023) / 1024;
+  const int64_t parts = want < most ? want : most;
+  return parts < 1 ? 1 : parts;
+}
+
+}  // namespace bq
+
+using namespace bq;
+
+size_t bq_beam_select_ws_bytes(int64_t B, int64_t W, int64_t V) {
+  if (B < 1 || W < 1 || W > MOST_BEAMS || V < 1) return 0;
+  return (size_t)(B * W * parts_of(B * W, V)) * (16 + 8 * W);
+}
+
+int bq_beam_select(const void* logits, int type, int64_t B, int64_t W, int64_t V, int64_t pitch, const float* scores,
+                   const uint8_t* done, int64_t end, float* out, int32_t* parents, int32_t* tokens, uint8_t* ended,
+                   void* ws, size_t ws_bytes, bq_stream_t stream) {
+  const char* what = "bq_beam_select";
+  if (type < 0 || type > 2) return set_error(BQ_ERR_ARG, "%s: type %d", what, type);
+  if (B < 0 || W < 1 || V < 1) return set_error(BQ_ERR_ARG, "%s: bad sizes", what);
+  if (W > MOST_BEAMS) return set_error(BQ_ERR_UNSUPPORTED, "%s: %lld beams (%d at most)", what, (long long)W, MOST_BEAMS);
+  if (V > 0x7fffffff - 8192 || B > 0x7fffff) return set_error(BQ_ERR_ARG, "%s: size too large", what);
+  if (done && (end < 0 || end > 0x7fffffff)) return set_error(BQ_ERR_ARG, "%s: end token %lld", what, (long long)end);
+  if (B == 0) return BQ_OK;
+  if (!logits || !scores || !out || !parents || !tokens) return set_error(BQ_ERR_ARG, "%s: null pointer", what);
+  const size_t need = bq_beam_select_ws_bytes(B, W, V);
+  if (!ws || ws_bytes < need || ((uintptr_t)ws & 15))
+    return set_error(BQ_ERR_ARG, "%s: a workspace of %zu bytes, given %zu", what, need, ws ? ws_bytes : 0);
+  Beam a;
+  a.x = logits;
+  a.pitch = pitch;
+  a.scores = scores;
+  a.done = done;
+  a.B = (int)B;
+  a.W = (int)W;
+  a.V = (int)V;
+  a.end = end < 0 || end > 0x7fffffff ? -1 : (int)end;
+  a.parts = (int)parts_of(B * W, V);
+  a.per = (int)((V + a.parts - 1) / a.parts);
+  a.sums = (double2*)ws;
+  a.best = (uint64_t*)(a.sums + B * W * a.parts);
+  a.out = out;
+  a.parents = parents;
+  a.tokens = tokens;
+  a.ended = ended;
+  hipStream_t st = (hipStream_t)stream;
+  const unsigned grid = (unsigned)(B * W * a.parts);
+  if (type == 0) beam_part_kernel<float><<<grid, PART_WAVES * 64, 0, st>>>(a);
+  else if (type == 1) beam_part_kernel<__bf16><<<grid, PART_WAVES * 64, 0, st>>>(a);
+  else beam_part_kernel<_Float16><<<grid, PART_WAVES * 64, 0, st>>>(a);
+  beam_join_kernel<<<(unsigned)B, 256, (size_t)W * W * 12 + W * 4, st>>>(a);
+  return check_launch(what);
+}

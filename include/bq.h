@@ -618,6 +618,23 @@ int bq_pages_grow(const bq_pages* pages, const int32_t* more, int64_t rows, int3
 int bq_kv4_copy_pages(const bq_kv4_cache* caches, int64_t count, const int32_t* moves, int64_t sequences,
                       bq_stream_t stream);
 
+/* ---- a beam search's selection ----
+ *
+ * Of each of B requests' W beams and V tokens the W best continuations: logits [B W, V] of `type` (rows at `pitch`
+ * elements), scores f32 [B, W]. A candidate's score is scores[b, w] + logits[b W + w, v] - log sum_v exp(logits[b W
+ * + w]), taken and compared in 64 bits, NaN as -infinity (and so all of a beam with a NaN or +infinity among its
+ * logits, none above -infinity, or an infinite score); a beam with done[b, w] (u8, nullable) has one candidate, the
+ * token `end` at its own score. Equals go to the lower beam; within a beam the order is that of its logits, then of
+ * the tokens.
+ *   out f32 [B, W]: the scores in order; parents i32 [B, W]: their beams, as b W + w; tokens i32 [B, W];
+ *   ended u8 [B, W] (nullable): the beam was done or the token is `end`
+ * W <= 64. None of the outputs is an input. The logits are read once (twice where they do not fit, from cache);
+ * no atomics. ws: bq_beam_select_ws_bytes bytes, 16-byte aligned, need not be cleared. */
+size_t bq_beam_select_ws_bytes(int64_t B, int64_t W, int64_t V);
+int bq_beam_select(const void* logits, int type, int64_t B, int64_t W, int64_t V, int64_t pitch, const float* scores,
+                   const uint8_t* done, int64_t end, float* out, int32_t* parents, int32_t* tokens, uint8_t* ended,
+                   void* ws, size_t ws_bytes, bq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
