@@ -8,6 +8,13 @@ of ``attention`` and ``kv4`` as a program uses them.
     state.evict(keep=512, recent=64)                         # the tokens that received least leave
     logits = model.step(state, logits.argmax(-1))            # one token a sequence over the cache
 
+Or with the page tables on the GPU: texts read in pieces of any length, and a beam search, whose steps never
+wait for the host.
+
+    state = PagedState(model, sequences=8, pages=256, width=8)
+    logits = model.read(state, ids, counts)              # the next pieces of up to 8 texts, packed
+    tokens, scores = model.search(state, ids, [700], beams=8, steps=32, end=0)
+
 Random weights and learned positions; the layers are pre-norm with GELU, the query heads grouped."""
 from __future__ import annotations
 
@@ -16,9 +23,11 @@ import torch.nn as tnn
 
 from . import nn
 from .attention import prompt_attention
+from .beams import beam_select
 from .kv4 import Cache4
+from .paging import Pages, copy_pages
 
-__all__ = ["Decoder", "DecoderState"]
+__all__ = ["Decoder", "DecoderState", "PagedState"]
 
 
 class DecoderLayer(tnn.Module):
@@ -92,6 +101,71 @@ class Decoder(tnn.Module):
             x = layer.close(x, o[:, 0])
         state.scored = True
         return self.head(self.ln(x))
+
+
+    @torch.no_grad()
+    def read(self, state: "PagedState", ids: torch.Tensor, counts: torch.Tensor) -> torch.Tensor:
+        """The next ``counts`` int32 ``[sequences]`` tokens of each sequence, packed, ``ids [sum(counts)]`` (or
+        more rows, past the last): a prompt's next piece, one token, or none. The logits of each one's last token
+        ``[sequences, vocab]``; those of a sequence without new tokens say nothing, and where not all tokens find
+        room (``state.ok`` 0) nothing changes and none do."""
+        got = state.pages.grow(counts, ids.shape[0])
+        copy_pages(state.caches, got.moves)
+        state.ok = got.ok
+        x = self.embed(ids) + self.places(got.at.clamp_min(0))
+        for layer, cache in zip(self.layers, state.caches):
+            q, k, v = layer.heads_of(x)
+            cache.append(k, v, slots=got.slots)
+            x = layer.close(x, cache.attend_chunk(q, state.pages.table, state.pages.lens, got.cu))
+        last = x[(got.cu[1:].long() - 1).clamp_min(0)]
+        return self.head(self.ln(last))
+
+    @torch.no_grad()
+    def search(self, state: "PagedState", ids: torch.Tensor, lens, beams: int, steps: int, end: int = 0):
+        """Beam search of ``steps`` tokens after each of the prompts ``ids [sum(lens)]``, packed, into an empty
+        ``state`` of ``len(lens) * beams`` sequences. ``tokens`` int32 ``[prompts, beams, steps]`` and ``scores``
+        f32 ``[prompts, beams]``, the best first; a beam that has ended goes on with ``end``."""
+        B, S, dev = len(lens), len(lens) * beams, ids.device
+        if state.pages.sequences != S or beams < 1 or steps < 1 or B < 1 or min(lens) < 1:
+            raise RuntimeError(f"search: {B} prompts of at least one token, {beams} beams and {steps} steps, in a state of "
+                               f"{state.pages.sequences} sequences")
+        if ids.shape != (sum(lens),):
+            raise RuntimeError(f"ids {tuple(ids.shape)} for prompts of {sum(lens)} tokens")
+        if max(lens) + steps - 1 > state.pages.width * state.pages.page:
+            raise RuntimeError(f"search: {max(lens)} tokens and {steps - 1} more in a state of "
+                               f"{state.pages.width * state.pages.page} a sequence")
+        counts = torch.zeros(B, beams, dtype=torch.int32, device=dev)
+        counts[:, 0] = torch.tensor(lens, dtype=torch.int32, device=dev)
+        scores = torch.full((B, beams), -torch.inf, device=dev)
+        scores[:, 0] = 0.0
+        done = torch.zeros(B, beams, dtype=torch.bool, device=dev)
+        tokens = torch.zeros(S, steps, dtype=torch.int32, device=dev)
+        logits = self.read(state, ids, counts.view(-1))
+        room, one = state.ok, torch.ones(S, dtype=torch.int32, device=dev)
+        for t in range(steps):
+            scores, parents, new, done = beam_select(logits, scores, done, end)
+            tokens = tokens[parents.view(-1)]
+            tokens[:, t] = new.view(-1)
+            if t + 1 < steps:
+                state.pages.fork(parents.view(-1))
+                logits = self.read(state, new.view(-1), one)
+                room = room * state.ok
+        if not room.item():
+            raise RuntimeError(f"search: the state's {state.pages.pages} pages are too few")
+        return tokens.view(B, beams, steps), scores
+
+
+class PagedState:
+    """The caches of ``sequences`` sequences of up to ``width`` pages each out of ``pages``, whose tables are kept
+    on the GPU (``paging.Pages``): ``pages.fork`` and ``pages.cut`` between the model's calls."""
+
+    def __init__(self, model: Decoder, sequences: int, pages: int, width: int, page: int = 64):
+        if width * page > model.context:
+            raise RuntimeError(f"sequences of {width * page} tokens, the model has places for {model.context}")
+        device = next(model.parameters()).device
+        self.caches = [Cache4.zeros(pages, model.kv_heads, page, model.dim, device) for _ in model.layers]
+        self.pages = Pages.zeros(sequences, width, pages, page, device)
+        self.ok = torch.ones(1, dtype=torch.int32, device=device)
 
 
 class DecoderState:
