@@ -30,28 +30,35 @@
 namespace bq {
 
 typedef float v16f __attribute__((ext_vector_type(16)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 struct Chunk {
   Kv4 c;
   const int *lens, *cu;
   const void* q;
   int64_t qt, qh;  // strides in elements: token, head
-  int n, group, B, max_len, tiles, upper, most;  // upper: units a share; most: shares a tile at most
+  int n, group, B, max_len;
+  int least;  // sequences of more rows than this take wide tiles
+  struct Kind {
+    int tiles, upper, most;  // that there can be; units a share; shares a tile at most
+  };
+  Kind wide, few;
   FastDiv by_group;
   float scale2;  // scale * log2(e)
   void* out;     // [n][heads * group][DIM]
   float *part, *stats;  // of each row, head and share: [n group][heads][most][DIM], [..][2]
 };
 
-constexpr int TILE = 128, KEYS = 64;  // rows a tile; keys a unit
-
+constexpr int WIDE = 128, FEW = 32, KEYS = 64;  // rows a tile, of sequences of many and of few; keys a unit
 // A tile's sequence and rows.
 struct Place {
   int b, start, rows, row0;  // b: -1 for rows of no sequence; the first row of q, the sequence's rows, the tile's first
   int base, len;             // the place in the cache of the sequence's first new token, and its tokens
 };
 
-// Tile `place` of what lies before cu[0], of each sequence in turn, or of what lies past the last.
+// Tile `place` of what lies before cu[0], of each sequence in turn, or of what lies past the last: of those that
+// tiles of TILE rows take.
+template <int TILE>
 __device__ __forceinline__ bool place_of(const Chunk& a, int place, Place* out) {
   const int lane = threadIdx.x & 63;
   for (int at = 0; at < a.B + 2; at += 64) {
@@ -61,7 +68,7 @@ __device__ __forceinline__ bool place_of(const Chunk& a, int place, Place* out) 
       s = i == 0 ? 0 : min(max(a.cu[i - 1], 0), a.n);
       e = i == a.B + 1 ? a.n : min(max(a.cu[i], 0), a.n);
     }
-    const int rows = max(0, e - s) * a.group, mine = (rows + TILE - 1) / TILE;
+    const int rows = max(0, e - s) * a.group, mine = (rows > a.least) == (TILE == WIDE) ? (rows + TILE - 1) / TILE : 0;
     int upto = mine;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -91,10 +98,25 @@ __device__ __forceinline__ int end_of(const Chunk& a, const Place& at, int row) 
   return max(0, min(at.len, at.base + fdiv(row, a.by_group.mul, a.by_group.shift) + 1));
 }
 // The units of the tile that holds `row`, and in how many shares they are cut.
+template <int TILE>
 __device__ __forceinline__ int units_of(const Chunk& a, const Place& at, int row0) {
   return (end_of(a, at, min(row0 + TILE, at.rows) - 1) + KEYS - 1) / KEYS;
 }
-__device__ __forceinline__ int shares_of(const Chunk& a, int units) { return max(1, (units + a.upper - 1) / a.upper); }
+__device__ __forceinline__ int shares_of(int upper, int units) { return max(1, (units + upper - 1) / upper); }
+__device__ __forceinline__ int64_t slot_of(const Chunk& a, const Place& at, int row, int h) {  // of a row's first share
+  return (((int64_t)at.start * a.group + row) * a.c.heads + h) * max(a.wide.most, a.few.most);
+}
+
+// Where 32 tokens lie: the first one's row in the cache's arrays, -1 where there is no page.
+__device__ __forceinline__ int64_t row_of(const Chunk& a, const Place& at, int h, int blk) {
+  const int i = fdiv(blk, a.c.by_blocks.mul, a.c.by_blocks.shift);
+  const int page = 32 * blk < at.len ? kv4_page(a.c, at.b, i) : -1;
+  return page < 0 ? -1 : ((int64_t)page * a.c.heads + h) * a.c.page + ((blk - i * (a.c.page >> 5)) << 5);
+}
+__device__ __forceinline__ int64_t of_lane(int64_t x, int lane) {
+  return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, lane) |
+         (int64_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32;
+}
 
 // A row's weights are relative to 2^ref, ref a whole number near its lagging maximum; or, where that
 // passes 2^20, to the maximum itself.
@@ -113,38 +135,48 @@ template <int DIM>
 __device__ __forceinline__ int k_at(int row, int piece) {
   return DIM == 128 ? row * 256 + ((piece ^ (row & 15)) << 4) : row * 128 + ((piece ^ ((row >> 1) & 7)) << 4);
 }
-__device__ __forceinline__ int v_at(int ch, int piece) { return ch * 128 + ((piece ^ (((ch >> 1) ^ (ch >> 3)) & 7)) << 4); }
+__device__ __forceinline__ int v_at(int ch, int piece) { return ch * 128 + ((piece ^ (((ch >> 1) ^ ((ch >> 4) & 3)) & 7)) << 4); }
 
 constexpr uint32_t HUGE = 253;  // scale bytes from here on may make codes infinite or NaN
+// Which of four bytes are: bits 7, 15, ... of the result.
+__device__ __forceinline__ uint32_t huge_of(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x03030303u) & w & 0x80808080u; }
+// Byte I of four as a scale of the expanding conversion, which takes a float's exponent and nothing else of it.
+template <int I>
+__device__ __forceinline__ float scale_byte(uint32_t w) {
+  return __uint_as_float(I < 3 ? w << (23 - 8 * I) : w >> 1);
+}
 
 // One of the 256 pieces of 64 tokens' codes: of token p / 4 a quarter of the keys' channels, of tokens
 // 4 (p / 16) .. + 3 channel slice p % 16 of the values. Pieces p / 128 lie in one block of 32 tokens.
 template <int DIM>
 struct Codes {
   uint32_t k[DIM / 32], v[DIM / 32], ks, vs;
-  __device__ __forceinline__ void load(const Kv4& c, int at, int h, int off0, int p) {
-    const size_t row = Kv4At<DIM>::row(c, at, h, off0);
-    const int t = (p & 127) >> 2, quarter = p & 3, four = (p & 127) >> 4, n = p & 15;
-    const uint8_t* kp = c.k + (row + t) * (DIM / 2) + quarter * (DIM / 8);
-    const uint8_t* vp = c.v + row * (DIM / 2);
-    if constexpr (DIM == 128) {
-      const uint4 x = *reinterpret_cast<const uint4*>(kp), y = *reinterpret_cast<const uint4*>(vp + four * 256 + n * 16);
-      k[0] = x.x, k[1] = x.y, k[2] = x.z, k[3] = x.w;
-      v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
-    } else {
-      const uint2 x = *reinterpret_cast<const uint2*>(kp);
-      const uint2 y = *reinterpret_cast<const uint2*>(vp + (four >> 1) * 256 + n * 16 + (four & 1) * 8);
-      k[0] = x.x, k[1] = x.y;
-      v[0] = y.x, v[1] = y.y;
-    }
+  // `row`: of the block's first token (uniform)
+  __device__ __forceinline__ void load_k(const Kv4& c, int64_t row, int p) {
     constexpr int CB = DIM / 32;
-    ks = c.ks[row * CB + (((t & 3) * CB + quarter * CB / 4) << 3) + (t >> 2)];
-    vs = *reinterpret_cast<const uint32_t*>(c.vs + row * CB + n * CB / 16 * 32 + 4 * four);
+    const int t = (p & 127) >> 2, quarter = p & 3;
+    const uint8_t* from = c.k + row * (DIM / 2) + (uint32_t)(t * (DIM / 2) + quarter * (DIM / 8));
+    if constexpr (DIM == 128) {
+      const uint4 x = *reinterpret_cast<const uint4*>(from);
+      k[0] = x.x, k[1] = x.y, k[2] = x.z, k[3] = x.w;
+    } else {
+      const uint2 x = *reinterpret_cast<const uint2*>(from);
+      k[0] = x.x, k[1] = x.y;
+    }
+    ks = (c.ks + row * CB)[(uint32_t)((((t & 3) * CB + quarter * CB / 4) << 3) + (t >> 2))];
   }
-  __device__ __forceinline__ void none() {
-#pragma unroll
-    for (int i = 0; i < DIM / 32; ++i) k[i] = v[i] = 0;
-    ks = 127, vs = 0x7f7f7f7fu;
+  __device__ __forceinline__ void load_v(const Kv4& c, int64_t row, int p) {
+    constexpr int CB = DIM / 32;
+    const int four = (p & 127) >> 4, n = p & 15;
+    const uint8_t* from = c.v + row * (DIM / 2);
+    if constexpr (DIM == 128) {
+      const uint4 x = *reinterpret_cast<const uint4*>(from + (uint32_t)(four * 256 + n * 16));
+      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+    } else {
+      const uint2 x = *reinterpret_cast<const uint2*>(from + (uint32_t)((four >> 1) * 256 + n * 16 + (four & 1) * 8));
+      v[0] = x.x, v[1] = x.y;
+    }
+    vs = *reinterpret_cast<const uint32_t*>(c.vs + row * CB + (uint32_t)(n * CB / 16 * 32 + 4 * four));
   }
   // Values of tokens from `len` on read as zeros; left: len minus the piece's first token.
   __device__ __forceinline__ void cut(int left) {
@@ -156,40 +188,39 @@ struct Codes {
         else v[i >> 1] &= i & 1 ? 0xffffu : 0xffff0000u;
       }
   }
-  __device__ __forceinline__ bool huge() const {
-    return max(max(vs & 255, (vs >> 8) & 255), max((vs >> 16) & 255, vs >> 24)) >= HUGE;
-  }
-  // Into a tile in LDS, as bf16. What is not finite among the values becomes 0 (it is added at the end).
-  __device__ __forceinline__ void expand(unsigned char* tk, unsigned char* tv, int p) const {
+  __device__ __forceinline__ bool huge() const { return huge_of(vs) != 0; }
+  // Into a tile in LDS, as bf16. CLEAR: what is not finite among the values becomes 0 (it is added at the end).
+  __device__ __forceinline__ void expand_k(unsigned char* tk, int p) const {
     const int t = p >> 2, row = (t & ~12) | ((t & 4) << 1) | ((t & 8) >> 1);
 #pragma unroll
     for (int i = 0; i < DIM / 32; ++i)
       *reinterpret_cast<v8bf*>(tk + k_at<DIM>(row, (p & 3) * (DIM / 32) + i)) = codes8(k[i], scale_bits(ks));
-    float s[4];
+  }
+  template <bool CLEAR, int K>
+  __device__ __forceinline__ void two(unsigned char* tv, int p, const float (&s)[4]) const {  // channels 2 K and + 1 of the slice
+    uint32_t x[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = scale_bits((vs >> (8 * i)) & 255);
-    const bool odd = huge();
-    auto two = [&]<int K>() {
-      uint32_t x[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (DIM == 128) x[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[i], s[i], K));
-        else if (i & 1) x[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[i >> 1], s[i], K + 2));
-        else x[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[i >> 1], s[i], K));
-        if (odd)
-          x[i] &= ((x[i] & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) | ((x[i] & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
-      }
-      const int ch = (p & 15) * (DIM / 16) + 2 * K, to = (p >> 4) >> 1, half = ((p >> 4) & 1) * 8;
-      *reinterpret_cast<uint2*>(tv + v_at(ch, to) + half) =
-          make_uint2(__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u));
-      *reinterpret_cast<uint2*>(tv + v_at(ch + 1, to) + half) =
-          make_uint2(__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u));
-    };
-    two.template operator()<0>();
-    two.template operator()<1>();
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DIM == 128) x[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[i], s[i], K));
+      else if (i & 1) x[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[i >> 1], s[i], K + 2));
+      else x[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[i >> 1], s[i], K));
+      if constexpr (CLEAR)
+        x[i] &= ((x[i] & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) | ((x[i] & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
+    }
+    const int ch = (p & 15) * (DIM / 16) + 2 * K, to = (p >> 4) >> 1, half = ((p >> 4) & 1) * 8;
+    *reinterpret_cast<uint2*>(tv + v_at(ch, to) + half) =
+        make_uint2(__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u));
+    *reinterpret_cast<uint2*>(tv + v_at(ch + 1, to) + half) =
+        make_uint2(__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u));
+  }
+  template <bool CLEAR>
+  __device__ __forceinline__ void expand_v(unsigned char* tv, int p) const {
+    const float s[4] = {scale_byte<0>(vs), scale_byte<1>(vs), scale_byte<2>(vs), scale_byte<3>(vs)};
+    two<CLEAR, 0>(tv, p, s);
+    two<CLEAR, 1>(tv, p, s);
     if constexpr (DIM == 128) {
-      two.template operator()<2>();
-      two.template operator()<3>();
+      two<CLEAR, 2>(tv, p, s);
+      two<CLEAR, 3>(tv, p, s);
     }
   }
 };
@@ -204,53 +235,42 @@ __device__ __forceinline__ v16f zeros16() {
 template <typename T>
 constexpr int W_PIECES = __is_same(T, float) ? 3 : __is_same(T, _Float16) ? 2 : 1;
 
-template <typename T, int DIM>
-__global__ __launch_bounds__(256, 2) void kv4_chunk_kernel(Chunk a) {
-  constexpr int QP = Q_PIECES<T>, PP = W_PIECES<T>, STEPS = DIM / 16, VT = DIM / 32;
-  constexpr int KB = KEYS * DIM * 2, BUF = 2 * KB;  // bytes of a tile's keys, as many of its values
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * BUF];
-  __shared__ int flags[2][4];  // of each buffer what its waves found: 1 the block is there, 2 values that are huge
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hh = lane >> 5;
-  const int h = blockIdx.x % a.c.heads, rest = blockIdx.x / a.c.heads, share = rest % a.most;
-  Place at;
-  if (!place_of(a, a.tiles - 1 - rest / a.most, &at)) return;
-  const int units = units_of(a, at, at.row0), shares = shares_of(a, units);
-  if (share >= shares) return;
-  const int u0 = (int)((int64_t)units * share / shares), u1 = (int)((int64_t)units * (share + 1) / shares);
-  const int rows = min(TILE, at.rows - at.row0);
-  const int parts = rows <= 32 ? 4 : rows <= 64 ? 2 : 1, part = wave & (parts - 1);
-  const int wrow = at.row0 + wave / parts * 32, row = wrow + n;  // the wave's first row and this lane's
-  const int last = at.rows - 1;
-  const int end = end_of(a, at, min(row, last));
-  const int sure = end_of(a, at, min(wrow, last)), most_end = end_of(a, at, min(wrow + 31, last));
-  const bool works = wrow <= last;
-  const int bpp = a.c.page >> 5, blocks = (at.len + 31) >> 5;
-
-  Pieces<QP> qf[STEPS];
-  {
-    const int t = fdiv(row, a.by_group.mul, a.by_group.shift), j = row - t * a.group;
-    const T* q = (const T*)a.q + (int64_t)(at.start + t) * a.qt + (int64_t)(h * a.group + j) * a.qh + 8 * hh;
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (row <= last && at.b >= 0) load8f(q + 16 * s, x);
-      qf[s] = split_q<QP>(x);
-    }
-  }
-  float m = -INFINITY, l = 0.f;
+// What a wave keeps of 32 rows of one key-value head: the queries' pieces, the running maxima and sums, the outputs.
+// Lane (n, hh) has row n; of the queries channels 16 s + 8 hh .. of step s, of the outputs 32 d + 8 i + 4 hh ...
+// With DIRECT the contracted channels of step s are DIM / 2 hh + 8 s .., the outputs VT (8 (i / 4) + 4 hh + i % 4) + d.
+template <typename T, int DIM, bool DIRECT>
+struct Rows {
+  static constexpr int QP = Q_PIECES<T>, PP = W_PIECES<T>, STEPS = DIM / 16, VT = DIM / 32;
+  Pieces<QP> q[STEPS];
+  float m, l;
   v16f o[VT];
+  int row, end, sure, most;  // this lane's row; what it sees; what all the wave's rows see, and any does
+
+  __device__ __forceinline__ void begin(const Chunk& a, const Place& at, int h, int first) {
+    const int n = threadIdx.x & 31, hh = (threadIdx.x >> 5) & 1, last = at.rows - 1;
+    row = first + n;
+    end = end_of(a, at, min(row, last));
+    sure = end_of(a, at, min(first, last));
+    most = first <= last ? end_of(a, at, min(first + 31, last)) : 0;
+    const int here = min(row, last);  // rows past the last are the last one's again, and not stored
+    const int t = fdiv(here, a.by_group.mul, a.by_group.shift), j = here - t * a.group;
+    const T* from = (const T*)a.q + (int64_t)(at.start + t) * a.qt + (int64_t)(h * a.group + j) * a.qh +
+                    (DIRECT ? DIM / 2 : 8) * hh;
+    float x[STEPS][8];
 #pragma unroll
-  for (int d = 0; d < VT; ++d) o[d] = zeros16();
+    for (int s = 0; s < STEPS; ++s) load8f(from + (DIRECT ? 8 : 16) * s, x[s]);
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) q[s] = split_q<QP>(x[s]);
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int d = 0; d < VT; ++d) o[d] = zeros16();
+  }
 
-  int huge = 0;  // whether there were values that may not be finite
-  auto page_of = [&](int blk) {
-    return blk < blocks ? kv4_page(a.c, at.b, fdiv(blk, a.c.by_blocks.mul, a.c.by_blocks.shift)) : -1;
-  };
-  auto off_of = [&](int blk) { return (blk - fdiv(blk, a.c.by_blocks.mul, a.c.by_blocks.shift) * bpp) << 5; };
-
-  // SUB times 32 keys from `tok`, in a tile's places from 32 sub on; there: a bit for each 32 that has a page
-  auto products = [&]<int SUB>(const unsigned char* tk, const unsigned char* tv, int sub, int tok, int there) {
-    v16f s[SUB];
+  // The scores of SUB times 32 keys, from row 32 sub of a tile on.
+  template <int SUB>
+  __device__ __forceinline__ void scores(const unsigned char* tk, int sub, v16f (&s)[SUB]) const {
+    const int n = threadIdx.x & 31, hh = (threadIdx.x >> 5) & 1;
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
       s[u] = zeros16();
@@ -258,18 +278,29 @@ __global__ __launch_bounds__(256, 2) void kv4_chunk_kernel(Chunk a) {
       for (int e = 0; e < STEPS; ++e) {
         const v8bf kf = *reinterpret_cast<const v8bf*>(tk + k_at<DIM>(32 * (sub + u) + n, 2 * e + hh));
 #pragma unroll
-        for (int p = QP - 1; p >= 0; --p) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[e].p[p], s[u], 0, 0, 0);
+        for (int p = QP - 1; p >= 0; --p) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[e].p[p], s[u], 0, 0, 0);
       }
     }
+  }
+
+  // What is not seen leaves them (keys from `tok`; there: a bit for each 32 that has a page), and the maximum
+  // follows. Returns what is subtracted.
+  template <int SUB>
+  __device__ __forceinline__ float raise(const Chunk& a, int tok, int there, v16f (&s)[SUB]) {
+    const int hh = (threadIdx.x >> 5) & 1;
     if (tok + 32 * SUB > sure || there != (1 << SUB) - 1)
 #pragma unroll
       for (int i = 0; i < 16 * SUB; ++i)
         if (tok + 32 * (i / 16) + 16 * (i % 16 / 8) + 8 * hh + i % 8 >= end || !((there >> (i / 16)) & 1))
           s[i / 16][i % 16] = -INFINITY;
-    float top = s[0][0];
+    float tops[4];  // four chains of maxima
 #pragma unroll
-    for (int i = 1; i < 16 * SUB; ++i) top = fmaxf(top, s[i / 16][i % 16]);
-    top = max_xor32(top);
+    for (int c = 0; c < 4; ++c) {
+      tops[c] = s[0][c];
+#pragma unroll
+      for (int i = c + 4; i < 16 * SUB; i += 4) tops[c] = fmaxf(tops[c], s[i / 16][i % 16]);
+    }
+    const float top = max_xor32(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
     const bool grew = __fmul_rn(__fsub_rn(top, m), a.scale2) > 8.f;
     if (__any(grew)) {
       const float f = grew ? factor(m, top, a.scale2) : 1.f;
@@ -278,197 +309,396 @@ __global__ __launch_bounds__(256, 2) void kv4_chunk_kernel(Chunk a) {
 #pragma unroll
       for (int d = 0; d < VT; ++d) o[d] *= f;
     }
-    const float ref = ref_of(m, a.scale2);
+    float ref = ref_of(m, a.scale2);
     const bool far = fabsf(ref) > FAR;
-    if (__any(far)) {
+    if (__any(far)) {  // such rows' differences are taken here, exactly as far as f32 goes
 #pragma unroll
-      for (int i = 0; i < 16 * SUB; ++i) {
-        float x = s[i / 16][i % 16];
-        x = far ? __fmul_rn(__fsub_rn(x, m), a.scale2) : __fmaf_rn(x, a.scale2, -ref);
-        s[i / 16][i % 16] = x = __builtin_amdgcn_exp2f(x);
-        l = __fadd_rn(l, x);
-      }
+      for (int i = 0; i < 16 * SUB; ++i)
+        if (far) s[i / 16][i % 16] = __fsub_rn(s[i / 16][i % 16], m);
+      if (far) ref = 0.f;
+    }
+    return ref;
+  }
+
+  // The weights of keys 16 e .. + 15, as the second product's operand, and their sum.
+  template <int SUB>
+  __device__ __forceinline__ Pieces<PP> weights(const Chunk& a, const v16f (&s)[SUB], float ref, int e, float* sum) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_exp2f(__fmaf_rn(s[e / 2][8 * (e % 2) + i], a.scale2, -ref));
+    const Pieces<PP> f = pieces_of<PP>(x);
+    if constexpr (PP == 1) {  // of the weights as rounded, two at a time
+      const uint4 w = __builtin_bit_cast(uint4, f.p[0]);
+      const v2bf one = {(__bf16)1.f, (__bf16)1.f};
+      float y = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w.x), one, 0.f, false);
+      y = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w.y), one, y, false);
+      y = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w.z), one, y, false);
+      *sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w.w), one, y, false);
+    } else {
+      *sum = __fadd_rn(__fadd_rn(__fadd_rn(x[0], x[1]), __fadd_rn(x[2], x[3])),
+                       __fadd_rn(__fadd_rn(x[4], x[5]), __fadd_rn(x[6], x[7])));
+    }
+    return f;
+  }
+
+  __device__ __forceinline__ void products(const unsigned char* tv, int sub, int e, const Pieces<PP>& f) {
+    const int n = threadIdx.x & 31, hh = (threadIdx.x >> 5) & 1;
+#pragma unroll
+    for (int d = 0; d < VT; ++d) {
+      const v8bf vf = *reinterpret_cast<const v8bf*>(tv + v_at(32 * d + n, 4 * sub + 2 * e + hh));
+#pragma unroll
+      for (int p = PP - 1; p >= 0; --p) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, f.p[p], o[d], 0, 0, 0);
+    }
+  }
+
+  // SUB times 32 keys from `tok`, in a tile's places from 32 sub on.
+  template <int SUB>
+  __device__ __forceinline__ void keys(const Chunk& a, const unsigned char* tk, const unsigned char* tv, int sub, int tok,
+                                       int there) {
+    v16f s[SUB];
+    scores<SUB>(tk, sub, s);
+    const float ref = raise<SUB>(a, tok, there, s);
+    float sums[2 * SUB];
+    if constexpr (PP == 1) {
+      Pieces<PP> f[2 * SUB];
+#pragma unroll
+      for (int e = 0; e < 2 * SUB; ++e) f[e] = weights<SUB>(a, s, ref, e, sums + e);
+#pragma unroll
+      for (int e = 0; e < 2 * SUB; ++e) products(tv, sub, e, f[e]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 16 * SUB; ++i) {
-        const float x = __builtin_amdgcn_exp2f(__fmaf_rn(s[i / 16][i % 16], a.scale2, -ref));
-        s[i / 16][i % 16] = x;
-        l = __fadd_rn(l, x);
-      }
+      for (int e = 0; e < 2 * SUB; ++e) products(tv, sub, e, weights<SUB>(a, s, ref, e, sums + e));
     }
-#pragma unroll
-    for (int e = 0; e < 2 * SUB; ++e) {
-      float x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = s[e / 2][8 * (e % 2) + i];
-      const Pieces<PP> pf = pieces_of<PP>(x);
-#pragma unroll
-      for (int d = 0; d < VT; ++d) {
-        const v8bf vf = *reinterpret_cast<const v8bf*>(tv + v_at(32 * d + n, 4 * sub + 2 * e + hh));
-#pragma unroll
-        for (int p = PP - 1; p >= 0; --p) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf.p[p], o[d], 0, 0, 0);
-      }
-    }
-  };
-
-  if (parts == 4) {  // each wave by itself: blocks of 32 keys 4 apart
-    unsigned char *tk = lds + (wave >> 1) * BUF, *tv = tk + KB;
-    const int sub = wave & 1, b1 = min(2 * u1, blocks), p0 = sub * 128 + lane;
-    Codes<DIM> now[2];
-    int page = -1, next_page = -1;
-    auto load = [&](int blk) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        if (page < 0) {
-          now[e].none();
-        } else {
-          now[e].load(a.c, page, h, off_of(blk), p0 + 64 * e);
-          if (32 * blk + 32 > at.len) now[e].cut(at.len - 32 * blk - 4 * (((p0 + 64 * e) & 127) >> 4));
-        }
-      }
-    };
-    int blk = 2 * u0 + wave;
-    if (blk < b1) {
-      page = page_of(blk);
-      next_page = page_of(blk + 4);
-      load(blk);
-    }
-    for (; blk < b1; blk += 4) {
-      // one wave's own part of LDS: its accesses there run in order
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      const bool there = page >= 0;
-      if (__any(now[0].huge() || now[1].huge())) huge = 1;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) now[e].expand(tk, tv, p0 + 64 * e);
-      page = next_page;
-      next_page = page_of(blk + 8);
-      if (blk + 4 < b1) load(blk + 4);
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      if (there) products.template operator()<1>(tk, tv, sub, 32 * blk, 1);
-    }
-  } else {
-    Codes<DIM> next;
-    const int p = threadIdx.x, mine = wave >> 1;  // which of a unit's two blocks
-    int page = -1, next_page = -1;
-    auto load = [&](int u) {
-      if (page < 0) {
-        next.none();
-      } else {
-        next.load(a.c, page, h, off_of(2 * u + mine), p);
-        if (KEYS * u + KEYS > at.len) next.cut(at.len - KEYS * u - 4 * (p >> 4));
-      }
-    };
-    auto expand = [&](int buf) {
-      const bool odd = __any(next.huge());
-      if (lane == 0) flags[buf][wave] = (page >= 0 ? 1 : 0) | (odd ? 2 : 0);
-      next.expand(lds + buf * BUF, lds + buf * BUF + KB, p);
-    };
-    if (u0 < u1) {
-      page = page_of(2 * u0 + mine);
-      next_page = page_of(2 * u0 + 2 + mine);
-      load(u0);
-      expand(0);
-      page = next_page;
-      if (u0 + 1 < u1) load(u0 + 1);
-    }
-    for (int u = u0, buf = 0; u < u1; ++u, buf ^= 1) {
-      wait_lds();
-      barrier();  // this unit is there, the last one is read
-      if (u + 1 < u1) {
-        next_page = page_of(2 * u + 4 + mine);
-        expand(buf ^ 1);
-        page = next_page;
-        if (u + 2 < u1) load(u + 2);
-      }
-      const unsigned char *tk = lds + buf * BUF, *tv = tk + KB;
-      const int f0 = flags[buf][0] | flags[buf][1], f1 = flags[buf][2] | flags[buf][3];
-      const int there = __builtin_amdgcn_readfirstlane((f0 & 1) | (f1 & 1) << 1);
-      huge |= __builtin_amdgcn_readfirstlane((f0 | f1) >> 1);
-      const int tok = KEYS * u + 32 * part;
-      if (!works || tok >= most_end) continue;
-      if (parts == 1) products.template operator()<2>(tk, tv, 0, tok, there);
-      else products.template operator()<1>(tk, tv, part, tok, (there >> part) & 1);
-    }
+    if constexpr (SUB == 2) l = __fadd_rn(l, __fadd_rn(__fadd_rn(sums[0], sums[1]), __fadd_rn(sums[2], sums[3])));
+    else l = __fadd_rn(l, __fadd_rn(sums[0], sums[1]));
   }
 
-  l = __fadd_rn(l, __shfl_xor(l, 32));
-  if (parts == 4) huge = __syncthreads_or(huge);  // each wave saw its own
-  if (parts > 1) {  // the waves of the same rows, in the place of the tiles
-    constexpr int WORDS = 16 * VT + 2;
-    float* all = reinterpret_cast<float*>(lds);
-    __syncthreads();
-    if (part) {
-      float* to = all + (wave - 1) * (WORDS * 64) + lane;
-      to[0] = m;
-      to[64] = l;
-#pragma unroll
-      for (int i = 0; i < 16 * VT; ++i) to[(2 + i) * 64] = o[i / 16][i % 16];
-    }
-    __syncthreads();
-    if (part) return;
-    for (int w = 1; w < parts; ++w) {
-      const float* from = all + (wave + w - 1) * (WORDS * 64) + lane;
-      const float m1 = from[0], now = fmaxf(m, m1);
-      const float f0 = m == now ? 1.f : factor(m, now, a.scale2), f1 = m1 == now ? 1.f : factor(m1, now, a.scale2);
-      m = now;
-      l = __fmaf_rn(l, f0, __fmul_rn(from[64], f1));
-#pragma unroll
-      for (int i = 0; i < 16 * VT; ++i)
-        o[i / 16][i % 16] = __fmaf_rn(o[i / 16][i % 16], f0, __fmul_rn(from[(2 + i) * 64], f1));
-    }
-  }
-  if (huge) {
-    // What was left out of the products is added to the outputs of the rows that see it, whatever its weight,
-    // and to no other's: lane (n, hh) holds channels 32 d + 8 i + 4 hh .. of its row.
-    for (int blk = 2 * u0; blk < min(2 * u1, blocks); ++blk) {
-      const int page = page_of(blk), off0 = off_of(blk);
-      if (page < 0) continue;
-      const size_t r0 = Kv4At<DIM>::row(a.c, page, h, off0);
+  // What was left out of the products is added to the outputs of the rows that see it, whatever its weight,
+  // and to no other's.
+  __device__ __forceinline__ void add_huge(const Chunk& a, const Place& at, int h, int blk0, int blk1) {
+    const int hh = (threadIdx.x >> 5) & 1;
+    for (int blk = blk0; blk < blk1; ++blk) {
+      const int64_t r0 = row_of(a, at, h, blk);
+      if (r0 < 0) continue;
 #pragma unroll 1
       for (int t = 0; t < 32; ++t) {
-        if (32 * blk + t >= most_end) break;
+        if (32 * blk + t >= most) break;
 #pragma unroll
-        for (int d = 0; d < VT; ++d) {
-          const uint32_t byte = a.c.vs[Kv4At<DIM>::vs(r0 + t, off0 + t, d)];
+        for (int i = 0; i < DIM / 8; ++i) {  // four channels at a time
+          const int ch = channel(4 * i, hh);
+          const uint32_t byte = a.c.vs[Kv4At<DIM>::vs(r0 + t, t, ch / 32)];
           if (byte < HUGE) continue;
+          const uint32_t w = *reinterpret_cast<const uint16_t*>(a.c.v + Kv4At<DIM>::v(r0 + t, t, ch / (DIM / 16)) +
+                                                                ch % (DIM / 16) / 2);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int ch = 32 * d + 8 * i + 4 * hh;
-            const uint32_t w = *reinterpret_cast<const uint16_t*>(
-                a.c.v + Kv4At<DIM>::v(r0 + t, off0 + t, ch / (DIM / 16)) + ch % (DIM / 16) / 2);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float y = (float)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w >> (8 * (e / 2)), scale_bits(byte), 0)[e & 1];
-              if (!(fabsf(y) < INFINITY) && 32 * blk + t < end) o[d][4 * i + e] = __fadd_rn(o[d][4 * i + e], y);
-            }
+          for (int e = 0; e < 4; ++e) {
+            const float y = (float)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w >> (8 * (e / 2)), scale_bits(byte), 0)[e & 1];
+            if (!(fabsf(y) < INFINITY) && 32 * blk + t < end) out(4 * i + e) = __fadd_rn(out(4 * i + e), y);
           }
         }
       }
     }
   }
-  if (row > last) return;
-  const int t = fdiv(row, a.by_group.mul, a.by_group.shift), j = row - t * a.group;
-  if (shares == 1) {
-    const float r = __fdiv_rn(1.f, l == 0.f ? 1.f : l);
-    T* to = (T*)a.out + ((int64_t)(at.start + t) * a.c.heads * a.group + h * a.group + j) * DIM + 4 * hh;
-#pragma unroll
-    for (int d = 0; d < VT; ++d)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        store4(to + 32 * d + 8 * i, __fmul_rn(o[d][4 * i], r), __fmul_rn(o[d][4 * i + 1], r), __fmul_rn(o[d][4 * i + 2], r),
-               __fmul_rn(o[d][4 * i + 3], r));
-  } else {
-    const int64_t slot = (((int64_t)at.start * a.group + row) * a.c.heads + h) * a.most + share;
-    float* to = a.part + slot * DIM + 4 * hh;
-#pragma unroll
-    for (int d = 0; d < VT; ++d)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<float4*>(to + 32 * d + 8 * i) = make_float4(o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]);
-    if (hh == 0) *reinterpret_cast<float2*>(a.stats + slot * 2) = make_float2(m, l);
+
+  // This lane's outputs in an order in which four at a time are neighbours: the x-th, and its channel.
+  __device__ __forceinline__ float& out(int x) { return DIRECT ? ((float*)&o[x % VT])[x / VT] : ((float*)&o[x / 16])[x % 16]; }
+  static __device__ __forceinline__ int channel(int x, int hh) {
+    if constexpr (DIRECT) {
+      const int i = x / VT;
+      return VT * (8 * (i / 4) + 4 * hh + i % 4) + x % VT;
+    } else {
+      return 32 * (x / 16) + 8 * (x % 16 / 4) + 4 * hh + x % 4;
+    }
   }
+
+  // Into the output, or as one of the shares of a row.
+  __device__ __forceinline__ void store(const Chunk& a, const Place& at, int h, int share, int shares) {
+    const int hh = (threadIdx.x >> 5) & 1;
+    if (row >= at.rows) return;
+    if (shares == 1) {
+      const int t = fdiv(row, a.by_group.mul, a.by_group.shift), j = row - t * a.group;
+      const float r = __fdiv_rn(1.f, l == 0.f ? 1.f : l);
+      T* to = (T*)a.out + ((int64_t)(at.start + t) * a.c.heads * a.group + h * a.group + j) * DIM;
+#pragma unroll
+      for (int x = 0; x < DIM / 2; x += 4)
+        store4(to + channel(x, hh), __fmul_rn(out(x), r), __fmul_rn(out(x + 1), r), __fmul_rn(out(x + 2), r),
+               __fmul_rn(out(x + 3), r));
+    } else {
+      const int64_t slot = slot_of(a, at, row, h) + share;
+      float* to = a.part + slot * DIM;
+#pragma unroll
+      for (int x = 0; x < DIM / 2; x += 4)
+        *reinterpret_cast<float4*>(to + channel(x, hh)) = make_float4(out(x), out(x + 1), out(x + 2), out(x + 3));
+      if (hh == 0) *reinterpret_cast<float2*>(a.stats + slot * 2) = make_float2(m, l);
+    }
+  }
+};
+
+// Which tile and share a workgroup has; false: none. Tiles from the last down (those with most keys first), the
+// key-value heads side by side.
+template <int TILE>
+__device__ __forceinline__ bool job_of(const Chunk& a, Place* at, int* h, int* share, int* shares, int* u0, int* u1) {
+  const Chunk::Kind& kind = TILE == WIDE ? a.wide : a.few;
+  *h = blockIdx.x % a.c.heads;
+  const int rest = blockIdx.x / a.c.heads;
+  *share = rest % kind.most;
+  if (!place_of<TILE>(a, kind.tiles - 1 - rest / kind.most, at)) return false;
+  const int units = units_of<TILE>(a, *at, at->row0);
+  *shares = shares_of(kind.upper, units);
+  if (*share >= *shares) return false;
+  *u0 = (int)((int64_t)units * *share / *shares);
+  *u1 = (int)((int64_t)units * (*share + 1) / *shares);
+  return true;
+}
+
+// Sequences of many rows: 32 rows a wave, tiles of 64 keys in LDS for all four.
+template <typename T, int DIM>
+__global__ __launch_bounds__(256, 2) void kv4_chunk_kernel(Chunk a) {
+  constexpr int KB = KEYS * DIM * 2, BUF = 2 * KB;  // bytes of a tile's keys, as many of its values
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * BUF];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Place at;
+  int h, share, shares, u0, u1;
+  if (!job_of<WIDE>(a, &at, &h, &share, &shares, &u0, &u1)) return;
+  Rows<T, DIM, false> r;
+  r.begin(a, at, h, at.row0 + 32 * wave);
+  Codes<DIM> next;
+  const int p = threadIdx.x, mine = wave >> 1;  // which of a unit's two blocks this wave's codes are of
+  // the rows of 64 units' two blocks, a unit a lane: looked up one by one, each waited for the codes on their way
+  int first = u0;
+  int64_t rows[2];
+  auto look = [&](int u) {
+    first = u;
+    rows[0] = row_of(a, at, h, 2 * (u + lane));
+    rows[1] = row_of(a, at, h, 2 * (u + lane) + 1);
+  };
+  look(u0);
+  int there = 0, loaded = 0;  // a bit for each block that has a page: of the unit expanded last, of the codes in `next`
+  bool huge = false;          // whether there were values that may not be finite
+  auto load = [&](int u) {
+    if (u - first == 64) look(u);
+    const int64_t r0 = of_lane(rows[0], u - first), r1 = of_lane(rows[1], u - first);
+    loaded = (r0 >= 0 ? 1 : 0) | (r1 >= 0 ? 2 : 0);
+    const int64_t row = max(mine ? r1 : r0, (int64_t)0);
+    next.load_k(a.c, row, p);
+    next.load_v(a.c, row, p);
+  };
+  auto expand = [&](int u, int buf) {
+    there = loaded;
+    // values that are not there are zeros; their scores are left out
+    const bool gone = !((loaded >> mine) & 1);
+    if (gone || KEYS * u + KEYS > at.len) next.cut(gone ? 0 : at.len - KEYS * u - 4 * (p >> 4));
+    unsigned char *tk = lds + buf * BUF, *tv = tk + KB;
+    next.expand_k(tk, p);
+    if (__any(next.huge())) {
+      huge = true;
+      next.template expand_v<true>(tv, p);
+    } else {
+      next.template expand_v<false>(tv, p);
+    }
+  };
+  if (u0 < u1) {
+    load(u0);
+    expand(u0, 0);
+    if (u0 + 1 < u1) load(u0 + 1);
+  }
+  for (int u = u0, buf = 0; u < u1; ++u, buf ^= 1) {
+    wait_lds();
+    barrier();  // this unit is there, the last one is read
+    const int now = there;
+    const unsigned char *tk = lds + buf * BUF, *tv = tk + KB;
+    if (u + 1 < u1) {
+      expand(u + 1, buf ^ 1);
+      if (u + 2 < u1) load(u + 2);
+    }
+    if constexpr (Q_PIECES<T> == 3 && DIM == 128) {  // as the registers allow
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (KEYS * u + 32 * e < r.most) r.template keys<1>(a, tk, tv, e, KEYS * u + 32 * e, (now >> e) & 1);
+    } else {
+      if (KEYS * u < r.most) r.template keys<2>(a, tk, tv, 0, KEYS * u, now);
+    }
+  }
+  if (__syncthreads_or(huge)) r.add_huge(a, at, h, 2 * u0, min(2 * u1, (at.len + 31) >> 5));
+  r.l = __fadd_rn(r.l, __shfl_xor(r.l, 32));
+  r.store(a, at, h, share, shares);
+}
+
+// Sequences of few rows, where the products are small beside the reading: each wave takes every fourth 32 keys for
+// the same 32 rows by itself, straight from memory into operands, without LDS and barriers: of the keys a lane
+// takes its token's half of the channels, of the values 8 tokens' codes of its VT neighbouring channels (the
+// loads hold twice that, and neighbouring lanes share them). The next keys load under the exponentials, the next
+// values under the next scores. The four waves are joined at the end.
+template <typename T, int DIM>
+__global__ __launch_bounds__(256, 2) void kv4_chunk_few_kernel(Chunk a) {
+  constexpr int VT = DIM / 32, CB = DIM / 32, PP = W_PIECES<T>;
+  constexpr int WORDS = 16 * VT + 2;
+  __shared__ float all[3 * WORDS * 64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hh = lane >> 5;
+  Place at;
+  int h, share, shares, u0, u1;
+  if (!job_of<FEW>(a, &at, &h, &share, &shares, &u0, &u1)) return;
+  Rows<T, DIM, true> r;
+  const int b1 = min(2 * u1, (at.len + 31) >> 5);
+  int blk = 2 * u0 + wave, first = 0;
+  int64_t rows;  // of 64 of this wave's blocks, one a lane
+  auto look = [&](int blk) {
+    first = blk;
+    rows = row_of(a, at, h, blk + 4 * lane);
+  };
+  // of the keys the lane's token (row n of the scores), of the values its channels
+  const int t = (n & ~12) | ((n & 4) << 1) | ((n & 8) >> 1);
+  const uint32_t k_off = t * (DIM / 2) + hh * (DIM / 4), ks_off = (((t & 3) * CB + hh * CB / 2) << 3) + (t >> 2);
+  const uint32_t v_off = (n >> 1) * 16 + hh * (DIM == 128 ? 512 : 256), vs_off = n * CB / 32 * 32 + 8 * hh;
+  const uint32_t v_take = DIM == 128 ? (n & 1 ? 0x07060302u : 0x05040100u) : (n & 1 ? 0x07050301u : 0x06040200u);
+  struct Block {
+    int64_t row;
+    uint32_t k[DIM / 16], ks[CB / 2], v[2][DIM / 16], vs[2][2];
+  } blocks[2];
+  auto load_k = [&](Block& c) {
+    const int64_t row = max(c.row, (int64_t)0);  // past the last block, or where there is no page, what is not looked at
+    const uint8_t *from = a.c.k + row * (DIM / 2), *bytes = a.c.ks + row * CB;
+#pragma unroll
+    for (int i = 0; i < DIM / 64; ++i) {
+      const v4u x = __builtin_nontemporal_load(reinterpret_cast<const v4u*>(from + k_off + 16 * i));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) c.k[4 * i + j] = x[j];
+      c.ks[i] = bytes[ks_off + 8 * i];
+    }
+  };
+  auto load_v = [&](Block& c) {
+    const int64_t row = max(c.row, (int64_t)0);
+    const uint8_t *from = a.c.v + row * (DIM / 2), *bytes = a.c.vs + row * CB;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {  // 8 tokens: two blocks of 4 (dim 128), or one
+#pragma unroll
+      for (int i = 0; i < DIM / 64; ++i) {
+        const uint4 x = *reinterpret_cast<const uint4*>(from + v_off + e * (8 * DIM) + 256 * i);
+        c.v[e][4 * i] = x.x, c.v[e][4 * i + 1] = x.y, c.v[e][4 * i + 2] = x.z, c.v[e][4 * i + 3] = x.w;
+      }
+      const uint2 y = *reinterpret_cast<const uint2*>(bytes + vs_off + 16 * e);
+      c.vs[e][0] = y.x, c.vs[e][1] = y.y;
+    }
+  };
+  auto find = [&](int blk) {  // blocks in turn
+    if (blk - first == 4 * 64) look(blk);
+    return blk < b1 ? of_lane(rows, (blk - first) >> 2) : -1;
+  };
+  look(blk);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    blocks[i].row = find(blk + 4 * i);
+    if (blk < b1) {
+      load_k(blocks[i]);
+      load_v(blocks[i]);
+    }
+  }
+  r.begin(a, at, h, at.row0);
+  bool huge = false;
+  auto body = [&](int blk, Block& c) {
+    const bool there = c.row >= 0;
+    c.row = find(blk + 8);
+    v16f s[1];
+    s[0] = zeros16();
+#pragma unroll
+    for (int e = 0; e < DIM / 16; ++e) {
+      const v8bf kf = codes8(c.k[e], scale_bits(c.ks[e * 8 / 32]));
+#pragma unroll
+      for (int p = Q_PIECES<T> - 1; p >= 0; --p) s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, r.q[e].p[p], s[0], 0, 0, 0);
+    }
+    load_k(c);
+    const float ref = r.template raise<1>(a, 32 * blk, there, s);
+    // values past the length, or of no page, read as zeros
+    if (!there || 32 * blk + 32 > at.len) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (!there || 32 * blk + 16 * e + 8 * hh + i >= at.len) {
+            if constexpr (DIM == 128) c.v[e][i] = 0;
+            else c.v[e][i / 2] &= i & 1 ? 0xffffu : 0xffff0000u;
+            c.vs[e][i / 4] = (c.vs[e][i / 4] & ~(255u << (8 * (i & 3)))) | (127u << (8 * (i & 3)));
+          }
+    }
+    const bool odd = __any((huge_of(c.vs[0][0]) | huge_of(c.vs[0][1]) | huge_of(c.vs[1][0]) | huge_of(c.vs[1][1])) != 0);
+    huge |= odd;
+    float sums[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const Pieces<PP> f = r.template weights<1>(a, s, ref, e, sums + e);
+      uint32_t x[8][VT / 2];  // token i's channels, two at a time
+      auto four = [&]<int Z>() {
+        const uint32_t b = c.vs[e][Z];
+        const float s0 = scale_byte<0>(b), s1 = scale_byte<1>(b), s2 = scale_byte<2>(b), s3 = scale_byte<3>(b);
+        if constexpr (DIM == 128) {  // the lane's halves of two tokens in one word
+          const uint32_t w0 = __builtin_amdgcn_perm(c.v[e][4 * Z + 1], c.v[e][4 * Z], v_take);
+          const uint32_t w1 = __builtin_amdgcn_perm(c.v[e][4 * Z + 3], c.v[e][4 * Z + 2], v_take);
+          x[4 * Z][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w0, s0, 0));
+          x[4 * Z][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w0, s0, 1));
+          x[4 * Z + 1][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w0, s1, 2));
+          x[4 * Z + 1][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w0, s1, 3));
+          x[4 * Z + 2][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w1, s2, 0));
+          x[4 * Z + 2][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w1, s2, 1));
+          x[4 * Z + 3][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w1, s3, 2));
+          x[4 * Z + 3][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w1, s3, 3));
+        } else {  // its bytes of four
+          const uint32_t w = __builtin_amdgcn_perm(c.v[e][2 * Z + 1], c.v[e][2 * Z], v_take);
+          x[4 * Z][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s0, 0));
+          x[4 * Z + 1][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s1, 1));
+          x[4 * Z + 2][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s2, 2));
+          x[4 * Z + 3][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s3, 3));
+        }
+      };
+      four.template operator()<0>();
+      four.template operator()<1>();
+      if (odd)  // what is not finite is added at the end
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int z = 0; z < VT / 2; ++z)
+            x[i][z] &= ((x[i][z] & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) |
+                       ((x[i][z] & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
+#pragma unroll
+      for (int d = 0; d < VT; ++d) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          w[i] = __builtin_amdgcn_perm(x[2 * i + 1][d / 2], x[2 * i][d / 2], d & 1 ? 0x07060302u : 0x05040100u);
+        const v8bf vf = __builtin_bit_cast(v8bf, make_uint4(w[0], w[1], w[2], w[3]));
+#pragma unroll
+        for (int p = PP - 1; p >= 0; --p) r.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, f.p[p], r.o[d], 0, 0, 0);
+      }
+    }
+    r.l = __fadd_rn(r.l, __fadd_rn(sums[0], sums[1]));
+    load_v(c);
+  };
+  for (; blk < b1; blk += 8) {
+    body(blk, blocks[0]);
+    if (blk + 4 < b1) body(blk + 4, blocks[1]);
+  }
+  r.l = __fadd_rn(r.l, __shfl_xor(r.l, 32));
+  huge = __syncthreads_or(huge);
+  if (wave) {
+    float* to = all + (wave - 1) * (WORDS * 64) + lane;
+    to[0] = r.m;
+    to[64] = r.l;
+#pragma unroll
+    for (int i = 0; i < 16 * VT; ++i) to[(2 + i) * 64] = r.o[i / 16][i % 16];
+  }
+  __syncthreads();
+  if (wave) return;
+  for (int w = 0; w < 3; ++w) {
+    const float* from = all + w * (WORDS * 64) + lane;
+    const float m1 = from[0], now_m = fmaxf(r.m, m1);
+    const float f0 = r.m == now_m ? 1.f : factor(r.m, now_m, a.scale2), f1 = m1 == now_m ? 1.f : factor(m1, now_m, a.scale2);
+    r.m = now_m;
+    r.l = __fmaf_rn(r.l, f0, __fmul_rn(from[64], f1));
+#pragma unroll
+    for (int i = 0; i < 16 * VT; ++i)
+      r.o[i / 16][i % 16] = __fmaf_rn(r.o[i / 16][i % 16], f0, __fmul_rn(from[(2 + i) * 64], f1));
+  }
+  if (huge) r.add_huge(a, at, h, 2 * u0, b1);
+  r.store(a, at, h, share, shares);
 }
 
 // The shares of each row joined: a wave a row and head.
@@ -494,21 +724,39 @@ __global__ __launch_bounds__(256) void kv4_chunk_join_kernel(Chunk a) {
   at.len = max(0, min(a.lens[lo], a.max_len));
   at.base = a.lens[lo] - (e - at.start);
   const int row = (i - at.start) * a.group + j;
-  const int shares = shares_of(a, units_of(a, at, row / TILE * TILE));
+  const int shares = at.rows > a.least ? shares_of(a.wide.upper, units_of<WIDE>(a, at, row / WIDE * WIDE))
+                                       : shares_of(a.few.upper, units_of<FEW>(a, at, row / FEW * FEW));
   if (shares == 1) return;
-  const int64_t slot = (((int64_t)at.start * a.group + row) * a.c.heads + h) * a.most;
+  const int64_t slot = slot_of(a, at, row, h);
   float m = -INFINITY, l = 0.f, y[C] = {};
-  for (int s = lane; s < shares; s += 64) m = fmaxf(m, a.stats[(slot + s) * 2]);
+  // up to 64 shares at a time: their maxima and sums a lane each, then their rows, whose loads wait for nothing
+  for (int s0 = 0; s0 < shares; s0 += 64) {
+    const int mine = min(64, shares - s0);
+    float2 st = make_float2(-INFINITY, 0.f);
+    if (lane < mine) st = *reinterpret_cast<const float2*>(a.stats + (slot + s0 + lane) * 2);
+    float now = st.x;
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
-  for (int s = 0; s < shares; ++s) {
-    const float2 st = *reinterpret_cast<const float2*>(a.stats + (slot + s) * 2);
-    const float f = st.x == m ? 1.f : factor(st.x, m, a.scale2);
-    l = __fmaf_rn(st.y, f, l);
+    for (int d = 1; d < 64; d *= 2) now = fmaxf(now, __shfl_xor(now, d));
+    now = fmaxf(now, m);
+    const float f = m == now ? 1.f : factor(m, now, a.scale2), e = st.x == now ? 1.f : factor(st.x, now, a.scale2);
+    m = now;
+    l = __fmaf_rn(l, f, wave_sum_fixed(__fmul_rn(st.y, e)));
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const float x = a.part[(slot + s) * DIM + C * lane + c];
-      y[c] = fabsf(x) < INFINITY ? __fmaf_rn(x, f, y[c]) : __fadd_rn(y[c], x);  // also where f is 0
+    for (int c = 0; c < C; ++c) y[c] = fabsf(y[c]) < INFINITY ? __fmul_rn(y[c], f) : y[c];
+    for (int i0 = 0; i0 < mine; i0 += 8) {
+      float x[8][C];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int c = 0; c < C; ++c) x[i][c] = a.part[(slot + s0 + min(i0 + i, mine - 1)) * DIM + C * lane + c];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float ei = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(e), min(i0 + i, mine - 1)));
+        if (i0 + i < mine)
+#pragma unroll
+          for (int c = 0; c < C; ++c)  // what is not finite stays so, also where its factor is 0
+            y[c] = fabsf(x[i][c]) < INFINITY ? __fmaf_rn(x[i][c], ei, y[c]) : __fadd_rn(y[c], x[i][c]);
+      }
     }
   }
   const float r = __fdiv_rn(1.f, l == 0.f ? 1.f : l);
@@ -517,25 +765,60 @@ __global__ __launch_bounds__(256) void kv4_chunk_join_kernel(Chunk a) {
   for (int c = 0; c < C; ++c) to[c] = (T)__fmul_rn(y[c], r);
 }
 
-// The tiles there can be, whatever the lengths are, the units of a share and the shares of a tile.
+// How the work is cut, whatever the lengths are.
+//
+// A sequence takes wide tiles from more than FEW_ROWS rows on, of which there are then few that are mostly empty; a
+// call of up to FEW_ALL rows takes narrow tiles alone, and one launch.
+//
+// Of the shares that a tile may be cut in that number is taken for which the workgroups, two a CU at once and all
+// as long as the longest sequence makes them, and what the join writes and reads cost least. (Taking sequences to
+// be half as long on average cut 64 equal ones of 4000 tokens too often: 62 -> 188 us.)
+constexpr int64_t FEW_ROWS = 64, FEW_ALL = 512, AT_ONCE = 512;
 struct Cut {
-  int64_t tiles;
-  int upper, most;
+  Chunk::Kind wide, few;
+  int64_t least;
 };
-static Cut cut_of(int64_t n, int64_t B, int64_t heads, int64_t group, int64_t max_len) {
+static Chunk::Kind kind_of(int64_t most_tiles, int64_t tiles, int64_t heads, int64_t units, double unit_us, double share_us) {
+  Chunk::Kind k = {(int)most_tiles, (int)units, 1};
+  double least = 0.0;
+  if (tiles < 1) tiles = 1;
+  for (int64_t m = 1; m <= 128 && m <= units; ++m) {
+    const int64_t all = tiles * heads * m, each = (units + m - 1) / m;
+    const double rounds = all <= AT_ONCE ? 1.0 : (double)all / AT_ONCE + 1.0;
+    const double us = rounds * each * unit_us + (m > 1 ? 4.0 + m * share_us : 0.0);
+    if (m == 1 || us < least) {
+      least = us;
+      k.upper = (int)each;
+      k.most = (int)((units + each - 1) / each);
+    }
+  }
+  return k;
+}
+static Cut cut_of(int type, int64_t n, int64_t B, int64_t heads, int64_t group, int64_t dim, int64_t max_len) {
+  const int64_t units = max_len > 0 ? (max_len + KEYS - 1) / KEYS : 1, begun = B + 2 < n ? B + 2 : n, rows = n * group;
+  const double share_us = (double)rows * heads * (2 * 4 * (dim + 2)) / 4e6;  // of all rows, written and read at 4 TB/s
+  // a unit's time in a workgroup of two a CU: 8192 tokens over themselves, 32 heads over 8, bf16 and f16, 4096 f32
+  const double unit_us = (type == 0 ? 5.5 : type == 1 ? 2.3 : 3.7) * (dim == 128 ? 1.0 : 0.6), FEW_UNIT_US = 2.0;
   Cut c;
-  const int64_t units = max_len > 0 ? (max_len + KEYS - 1) / KEYS : 1, begun = B + 2 < n ? B + 2 : n;
-  c.tiles = n * group / TILE + begun;
-  const int64_t want = (units * c.tiles * heads + 1023) / 1024;
-  c.upper = (int)(want < 8 ? 8 : want);
-  c.most = (int)((units + c.upper - 1) / c.upper);
+  c.least = rows <= FEW_ALL ? 0x7fffffff : FEW_ROWS;
+  if (rows <= FEW_ALL) {
+    const int64_t tiles = (rows + FEW - 1) / FEW, some = B < n ? B : n;
+    c.wide = {0, 1, 1};
+    c.few = kind_of(rows / FEW + begun, tiles > some ? tiles : some, heads, units, FEW_UNIT_US, share_us);
+  } else {
+    const int64_t many = rows / (FEW_ROWS + 1);  // sequences of more rows at most
+    c.wide = kind_of(rows / WIDE + (begun < many ? begun : many), rows / WIDE, heads, units, unit_us, share_us);
+    c.few = kind_of(begun * (FEW_ROWS / FEW), B < 1 ? 1 : B, heads, units, FEW_UNIT_US, share_us);
+  }
   return c;
 }
 
 template <typename T, int DIM>
 static int launch(const char* what, const Chunk& a, hipStream_t st) {
-  kv4_chunk_kernel<T, DIM><<<(unsigned)((int64_t)a.tiles * a.most * a.c.heads), 256, 0, st>>>(a);
-  if (a.most > 1) {
+  auto grid = [&](const Chunk::Kind& k) { return (unsigned)((int64_t)k.tiles * k.most * a.c.heads); };
+  if (a.wide.tiles) kv4_chunk_kernel<T, DIM><<<grid(a.wide), 256, 0, st>>>(a);
+  if (a.few.tiles) kv4_chunk_few_kernel<T, DIM><<<grid(a.few), 256, 0, st>>>(a);
+  if (a.wide.most > 1 || a.few.most > 1) {
     const int64_t rows = (int64_t)a.n * a.c.heads * a.group;
     kv4_chunk_join_kernel<T, DIM><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(a);
   }
@@ -546,10 +829,12 @@ static int launch(const char* what, const Chunk& a, hipStream_t st) {
 
 using namespace bq;
 
-size_t bq_kv4_attend_chunk_ws_bytes(int64_t n, int64_t B, int64_t q_heads, int64_t heads, int64_t dim, int64_t max_len) {
+size_t bq_kv4_attend_chunk_ws_bytes(int type, int64_t n, int64_t B, int64_t q_heads, int64_t heads, int64_t dim,
+                                    int64_t max_len) {
   if (n < 1 || B < 0 || heads < 1 || q_heads < heads || dim < 1 || max_len < 0) return 0;
-  const Cut c = cut_of(n, B, heads, q_heads / heads, max_len);
-  return c.most > 1 ? (size_t)n * q_heads * c.most * (dim + 2) * 4 : 0;
+  const Cut c = cut_of(type, n, B, heads, q_heads / heads, dim, max_len);
+  const int most = c.wide.most > c.few.most ? c.wide.most : c.few.most;
+  return most > 1 ? (size_t)n * q_heads * most * (dim + 2) * 4 : 0;
 }
 
 int bq_kv4_attend_chunk(const bq_kv4_cache* cache, const void* q, int type, int64_t n, int64_t q_heads, int64_t q_token,
@@ -569,14 +854,15 @@ int bq_kv4_attend_chunk(const bq_kv4_cache* cache, const void* q, int type, int6
   if (n == 0) return BQ_OK;
   const int64_t group = q_heads / cache->heads;
   if (n * group > 0x7fffffff - 8192) return set_error(BQ_ERR_ARG, "%s: size too large", what);
-  const Cut cut = cut_of(n, B, cache->heads, group, max_len);
-  if (cut.tiles * cut.most * cache->heads > 0x7fffffff || n * q_heads > 0x7fffffffll * 4)
+  const Cut cut = cut_of(type, n, B, cache->heads, group, cache->dim, max_len);
+  auto grid = [&](const Chunk::Kind& k) { return (int64_t)k.tiles * k.most * cache->heads; };
+  if (grid(cut.wide) > 0x7fffffff || grid(cut.few) > 0x7fffffff || n * q_heads > 0x7fffffffll * 4)
     return set_error(BQ_ERR_ARG, "%s: size too large", what);
   if (!q || !cu || !out || (B && !lens)) return set_error(BQ_ERR_ARG, "%s: null pointer", what);
   const int64_t size = type == KV4_F32 ? 4 : 2;
   if ((((uintptr_t)q | (uintptr_t)out) & 15) || (q_token | q_head) * size % 16)
     return set_error(BQ_ERR_ARG, "%s: rows that are not 16-byte aligned", what);
-  const size_t need = bq_kv4_attend_chunk_ws_bytes(n, B, q_heads, cache->heads, cache->dim, max_len);
+  const size_t need = bq_kv4_attend_chunk_ws_bytes(type, n, B, q_heads, cache->heads, cache->dim, max_len);
   if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
     return set_error(BQ_ERR_ARG, "%s: a workspace of %zu bytes, given %zu", what, need, ws ? ws_bytes : 0);
   const int64_t held = cache->pages ? width * cache->page : 0;  // tokens that a sequence's pages have room for
@@ -589,14 +875,14 @@ int bq_kv4_attend_chunk(const bq_kv4_cache* cache, const void* q, int type, int6
   a.group = (int)group;
   a.B = (int)B;
   a.max_len = (int)(max_len < held ? max_len : held);
-  a.tiles = (int)cut.tiles;
-  a.upper = cut.upper;
-  a.most = cut.most;
+  a.wide = cut.wide;
+  a.few = cut.few;
+  a.least = (int)cut.least;
   a.by_group = fast_div((uint32_t)group);
   a.scale2 = scale * 1.4426950408889634f;
   a.out = out;
   a.part = (float*)ws;
-  a.stats = a.part + (need ? (size_t)n * q_heads * cut.most * cache->dim : 0);
+  a.stats = a.part + (need ? need / (cache->dim + 2) / 4 * cache->dim : 0);
   hipStream_t st = (hipStream_t)stream;
   const bool wide = cache->dim == 128;
   if (type == KV4_F32) return wide ? launch<float, 128>(what, a, st) : launch<float, 64>(what, a, st);
