@@ -8,9 +8,13 @@
 //
 // Two launches. The first reads the logits once: a workgroup takes a part of a beam's tokens, and each of its
 // waves keeps the W best of what it reads, a candidate a lane in order (value and token as one 64-bit number,
-// so that equals go to the lower token); a logit that beats the last of them is rare after the first few
-// hundred, so the test of all 64 lanes at once is most of the cost. The second joins a request's parts and
-// beams.
+// so that equals go to the lower token). A logit that beats the last of them is rare: the W-th largest of the 64
+// lanes' maxima over the first 2048 or 1024 tokens bounds it from below before any is looked at alone, and then
+// one test of 64 lanes' maxima over 16 bytes each says that there is none. The exponentials need no maximum: f64
+// holds e^x for every logit within +-600, and parts with others are summed again against their maximum. The second
+// launch joins a request's parts and beams.
+//
+// Bound by the exponentials, 14 operations in f64 a logit, beside the reading.
 #include <math.h>
 
 #include "bq_common.h"
@@ -29,7 +33,7 @@ struct Beam {
   const uint8_t* done;  // nullable
   int B, W, V, end, parts, per;  // per: tokens a part
   uint64_t* best;  // [B W][parts][W] candidates in order
-  double2* sums;   // [B W][parts]: maximum, sum of exp(x - maximum)
+  double2* sums;   // [B W][parts]: what the exponents are relative to, their sum (NaN where a logit is)
   float* out;
   int *parents, *tokens;
   uint8_t* ended;
@@ -47,6 +51,9 @@ __device__ __forceinline__ float logit_of(uint64_t r) {
 }
 __device__ __forceinline__ int token_of(uint64_t r) { return (int)~(uint32_t)r; }
 
+// The value of the lane before (wave_shr:1); the first lane's is not looked at.
+__device__ __forceinline__ int lane_below(int v) { return __builtin_amdgcn_mov_dpp(v, 0x138, 0xF, 0xF, false); }
+
 // The best `W` so far, in order, lane i the i-th (0: none); `least` the W-th.
 struct List {
   uint64_t mine, least;
@@ -60,7 +67,7 @@ struct List {
       const int l = __builtin_ctzll(who);
       const uint64_t x = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(r >> 32), l) << 32 |
                          (uint32_t)__builtin_amdgcn_readlane((int)r, l);
-      const uint64_t up = __shfl_up(mine, 1);
+      const uint64_t up = (uint64_t)(uint32_t)lane_below((int)(mine >> 32)) << 32 | (uint32_t)lane_below((int)mine);
       mine = mine > x ? mine : lane == 0 || up > x ? x : up;
       least = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), W - 1) << 32 |
               (uint32_t)__builtin_amdgcn_readlane((int)mine, W - 1);
@@ -70,46 +77,123 @@ struct List {
   }
 };
 
-template <typename T>
-__device__ __forceinline__ float at(const T* x, int i) {
-  return (float)x[i];
+// e^x in f64 for |x| <= 740: 2^n times a polynomial for 2^f, f within 1/2 of 0 (interpolated at Chebyshev's nodes;
+// within 1.1e-12 of itself). NaN stays.
+__device__ __forceinline__ double exp_of(double x) {
+  constexpr double ROUND = 0x1.8p52;  // a sum with it is a whole number in its low bits
+  const double k = __builtin_fma(x, 0x1.71547652b82fep0, ROUND), n = k - ROUND;
+  const double f = __builtin_fma(x, 0x1.71547652b82fep0, -n);
+  double p = __builtin_fma(f, 0x1.63cf7dec51603p-20, 0x1.00dc48dc4d96cp-16);
+  p = __builtin_fma(f, p, 0x1.4308ae274a207p-13);
+  p = __builtin_fma(f, p, 0x1.5d8745a95d2d4p-10);
+  p = __builtin_fma(f, p, 0x1.3b2ab71725c04p-7);
+  p = __builtin_fma(f, p, 0x1.c6b08dd6fb6b1p-5);
+  p = __builtin_fma(f, p, 0x1.ebfbdff824847p-3);
+  p = __builtin_fma(f, p, 0x1.62e42fef84cf7p-1);
+  p = __builtin_fma(f, p, 0x1.ffffffffffffdp-1);
+  return __builtin_amdgcn_ldexp(p, (int)__builtin_bit_cast(uint64_t, k));
 }
+constexpr float WITHIN = 600.f, LEAST = -740.f;  // parts whose maximum is within +-WITHIN; logits below LEAST add nothing
 
 template <typename T>
 __global__ __launch_bounds__(PART_WAVES * 64) void beam_part_kernel(Beam a) {
+  constexpr int E = 16 / sizeof(T), U = 4;  // logits a load, loads on their way
+  typedef T Vec __attribute__((ext_vector_type(E)));
   __shared__ uint64_t lists[PART_WAVES][MOST_BEAMS];
   __shared__ double sums[PART_WAVES];
   __shared__ float tops[PART_WAVES];
   const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
   if (a.done && a.done[row]) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const T* x = (const T*)a.x + row * a.pitch;
-  const int lo = part * a.per, hi = min(a.V, lo + a.per);
-  // the maximum first, then the sum against it; NaN anywhere makes the sum NaN
-  float top = -INFINITY;
-  bool nan = false;
+  const int lo = min(part * a.per, a.V), hi = min(a.V, lo + a.per);
+  // 16-byte pieces from the first aligned one on; what lies before and behind them is the first wave's
+  const int head = min(hi - lo, (int)((E - ((uintptr_t)(x + lo) / sizeof(T)) % E) % E));
+  const int pieces = (hi - lo - head) / E, tail = lo + head + pieces * E;
+  float top = -INFINITY, bar = -INFINITY;  // bar: what a logit has to reach
+  double sum[2] = {0.0, 0.0};
   List best;
   best.clear(a.W);
-  for (int i0 = lo + wave * 64; i0 < hi; i0 += PART_WAVES * 64) {
-    const int i = i0 + lane;
-    const float v = i < hi ? at(x, i) : -INFINITY;
-    nan |= v != v;
+  auto add = [&](float v, int token) {
+    const float y = v < LEAST ? LEAST : v;  // NaN stays
+    sum[token & 1] += exp_of((double)y);
+  };
+  if (wave == 0) {
+    const int i = lane < head ? lo + lane : lane >= 32 && tail + lane - 32 < hi ? tail + lane - 32 : -1;
+    const float v = i >= 0 ? (float)x[i] : -INFINITY;
+    if (i >= 0) add(v, i);
     top = fmaxf(top, v);
-    best.add(i < hi && v == v ? rank_of(v, i) : 0);
+    best.add(i >= 0 && v == v ? rank_of(v, i) : 0);
+  }
+  // the list's last as a logit: later pieces hold later tokens, so they have to pass it (the odd ones before and
+  // behind do not count: they are of any place)
+  const Vec* from = reinterpret_cast<const Vec*>(x + lo + head);
+  bool begun = false;
+  for (int b0 = wave * 64; b0 < pieces; b0 += U * PART_WAVES * 64) {
+    Vec now[U];
+    bool there[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = b0 + u * PART_WAVES * 64 + lane;
+      there[u] = i < pieces;
+      now[u] = __builtin_nontemporal_load(from + min(i, pieces - 1));
+    }
+    float most[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      most[u] = -INFINITY;
+      if (there[u]) {
+        const int i = lo + head + (b0 + u * PART_WAVES * 64 + lane) * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          add((float)now[u][e], e);
+          most[u] = fmaxf(most[u], (float)now[u][e]);
+        }
+      }
+      top = fmaxf(top, most[u]);
+    }
+    if (!begun) {
+      begun = true;
+      float lane_most = most[0];
+#pragma unroll
+      for (int u = 1; u < U; ++u) lane_most = fmaxf(lane_most, most[u]);
+      for (int w = 0; w < a.W; ++w) {
+        bar = wave_max(lane_most);
+        const uint64_t who = __ballot(lane_most == bar);
+        if (who && lane == __builtin_ctzll(who)) lane_most = -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (!__any(there[u] && most[u] >= bar)) continue;
+      const int i = lo + head + (b0 + u * PART_WAVES * 64 + lane) * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float v = (float)now[u][e];
+        const bool may = there[u] && v >= bar;
+        if (__any(may)) best.add(may ? rank_of(v, i + e) : 0);
+      }
+      if (best.least) bar = fmaxf(bar, logit_of(best.least));
+    }
   }
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
   if (lane == 0) tops[wave] = top;
   lists[wave][lane] = best.mine;
-  nan = __syncthreads_or(nan);
+  __syncthreads();
 #pragma unroll
   for (int w = 0; w < PART_WAVES; ++w) top = fmaxf(top, tops[w]);
-  double sum = 0.0;
-  if (!nan && top > -INFINITY && top < INFINITY)
-    for (int i = lo + (int)threadIdx.x; i < hi; i += PART_WAVES * 64) sum += exp((double)at(x, i) - (double)top);
+  double all = sum[0] + sum[1], base = 0.0;
+  if (fabsf(top) > WITHIN) {  // sums against the maximum; of one that is not finite a NaN is kept, the rest is the join's
+    base = (double)top;
+    if (fabsf(top) < INFINITY) {
+      all = 0.0;
+      for (int i = lo + (int)threadIdx.x; i < hi; i += PART_WAVES * 64) all += exp((double)(float)x[i] - base);
+    }
+  }
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
-  if (lane == 0) sums[wave] = sum;
+  for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
+  if (lane == 0) sums[wave] = all;
   __syncthreads();
   if (wave) return;
   for (int w = 1; w < PART_WAVES; ++w) best.add(lists[w][lane]);
@@ -118,7 +202,7 @@ __global__ __launch_bounds__(PART_WAVES * 64) void beam_part_kernel(Beam a) {
   if (lane == 0) {
     double s = sums[0];
     for (int w = 1; w < PART_WAVES; ++w) s += sums[w];
-    a.sums[slot] = make_double2(nan ? (double)NAN : (double)top, s);
+    a.sums[slot] = make_double2(base, s);
   }
 }
 
@@ -147,7 +231,7 @@ __global__ __launch_bounds__(256) void beam_join_kernel(Beam a) {
         const int p = p0 + lane;
         double2 s = make_double2(-INFINITY, 0.0);
         if (p < a.parts) s = a.sums[(size_t)row * a.parts + p];
-        nan |= s.x != s.x;
+        nan |= s.y != s.y;
         double now = s.x;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) now = fmax(now, __shfl_xor(now, d));

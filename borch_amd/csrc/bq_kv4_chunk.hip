@@ -437,10 +437,10 @@ struct Rows {
 // Which tile and share a workgroup has; false: none. Tiles from the last down (those with most keys first), the
 // key-value heads side by side.
 template <int TILE>
-__device__ __forceinline__ bool job_of(const Chunk& a, Place* at, int* h, int* share, int* shares, int* u0, int* u1) {
+__device__ __forceinline__ bool job_of(const Chunk& a, int id, Place* at, int* h, int* share, int* shares, int* u0, int* u1) {
   const Chunk::Kind& kind = TILE == WIDE ? a.wide : a.few;
-  *h = blockIdx.x % a.c.heads;
-  const int rest = blockIdx.x / a.c.heads;
+  *h = id % a.c.heads;
+  const int rest = id / a.c.heads;
   *share = rest % kind.most;
   if (!place_of<TILE>(a, kind.tiles - 1 - rest / kind.most, at)) return false;
   const int units = units_of<TILE>(a, *at, at->row0);
@@ -453,13 +453,12 @@ __device__ __forceinline__ bool job_of(const Chunk& a, Place* at, int* h, int* s
 
 // Sequences of many rows: 32 rows a wave, tiles of 64 keys in LDS for all four.
 template <typename T, int DIM>
-__global__ __launch_bounds__(256, 2) void kv4_chunk_kernel(Chunk a) {
+__device__ __forceinline__ void wide_tile(const Chunk& a, int id, unsigned char* lds) {
   constexpr int KB = KEYS * DIM * 2, BUF = 2 * KB;  // bytes of a tile's keys, as many of its values
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * BUF];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Place at;
   int h, share, shares, u0, u1;
-  if (!job_of<WIDE>(a, &at, &h, &share, &shares, &u0, &u1)) return;
+  if (!job_of<WIDE>(a, id, &at, &h, &share, &shares, &u0, &u1)) return;
   Rows<T, DIM, false> r;
   r.begin(a, at, h, at.row0 + 32 * wave);
   Codes<DIM> next;
@@ -530,14 +529,14 @@ __global__ __launch_bounds__(256, 2) void kv4_chunk_kernel(Chunk a) {
 // loads hold twice that, and neighbouring lanes share them). The next keys load under the exponentials, the next
 // values under the next scores. The four waves are joined at the end.
 template <typename T, int DIM>
-__global__ __launch_bounds__(256, 2) void kv4_chunk_few_kernel(Chunk a) {
+__device__ __forceinline__ void narrow_tile(const Chunk& a, int id, float* all) {
   constexpr int VT = DIM / 32, CB = DIM / 32, PP = W_PIECES<T>;
   constexpr int WORDS = 16 * VT + 2;
-  __shared__ float all[3 * WORDS * 64];
+  constexpr int DEPTH = sizeof(T) == 4 && DIM == 128 ? 1 : 2;  // blocks on their way, as the registers allow
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hh = lane >> 5;
   Place at;
   int h, share, shares, u0, u1;
-  if (!job_of<FEW>(a, &at, &h, &share, &shares, &u0, &u1)) return;
+  if (!job_of<FEW>(a, id, &at, &h, &share, &shares, &u0, &u1)) return;
   Rows<T, DIM, true> r;
   const int b1 = min(2 * u1, (at.len + 31) >> 5);
   int blk = 2 * u0 + wave, first = 0;
@@ -554,7 +553,7 @@ __global__ __launch_bounds__(256, 2) void kv4_chunk_few_kernel(Chunk a) {
   struct Block {
     int64_t row;
     uint32_t k[DIM / 16], ks[CB / 2], v[2][DIM / 16], vs[2][2];
-  } blocks[2];
+  } blocks[DEPTH];
   auto load_k = [&](Block& c) {
     const int64_t row = max(c.row, (int64_t)0);  // past the last block, or where there is no page, what is not looked at
     const uint8_t *from = a.c.k + row * (DIM / 2), *bytes = a.c.ks + row * CB;
@@ -586,7 +585,7 @@ __global__ __launch_bounds__(256, 2) void kv4_chunk_few_kernel(Chunk a) {
   };
   look(blk);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < DEPTH; ++i) {
     blocks[i].row = find(blk + 4 * i);
     if (blk < b1) {
       load_k(blocks[i]);
@@ -597,7 +596,7 @@ __global__ __launch_bounds__(256, 2) void kv4_chunk_few_kernel(Chunk a) {
   bool huge = false;
   auto body = [&](int blk, Block& c) {
     const bool there = c.row >= 0;
-    c.row = find(blk + 8);
+    c.row = find(blk + 4 * DEPTH);
     v16f s[1];
     s[0] = zeros16();
 #pragma unroll
@@ -672,9 +671,9 @@ __global__ __launch_bounds__(256, 2) void kv4_chunk_few_kernel(Chunk a) {
     r.l = __fadd_rn(r.l, __fadd_rn(sums[0], sums[1]));
     load_v(c);
   };
-  for (; blk < b1; blk += 8) {
+  for (; blk < b1; blk += 4 * DEPTH) {
     body(blk, blocks[0]);
-    if (blk + 4 < b1) body(blk + 4, blocks[1]);
+    if (DEPTH == 2 && blk + 4 < b1) body(blk + 4, blocks[DEPTH - 1]);
   }
   r.l = __fadd_rn(r.l, __shfl_xor(r.l, 32));
   huge = __syncthreads_or(huge);
@@ -699,6 +698,22 @@ __global__ __launch_bounds__(256, 2) void kv4_chunk_few_kernel(Chunk a) {
   }
   if (huge) r.add_huge(a, at, h, 2 * u0, b1);
   r.store(a, at, h, share, shares);
+}
+
+// Both in one launch, the wide tiles first.
+template <typename T, int DIM, bool WIDES, bool FEWS>
+__global__ __launch_bounds__(256, 2) void kv4_chunk_kernel(Chunk a) {
+  constexpr int BYTES = WIDES ? 4 * KEYS * DIM * 2 : 3 * (DIM / 2 + 2) * 256;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[BYTES];
+  const int wides = a.wide.tiles * a.wide.most * a.c.heads;
+  if constexpr (WIDES && FEWS) {
+    if ((int)blockIdx.x < wides) wide_tile<T, DIM>(a, blockIdx.x, lds);
+    else narrow_tile<T, DIM>(a, blockIdx.x - wides, reinterpret_cast<float*>(lds));
+  } else if constexpr (WIDES) {
+    wide_tile<T, DIM>(a, blockIdx.x, lds);
+  } else {
+    narrow_tile<T, DIM>(a, blockIdx.x, reinterpret_cast<float*>(lds));
+  }
 }
 
 // The shares of each row joined: a wave a row and head.
@@ -770,21 +785,22 @@ __global__ __launch_bounds__(256) void kv4_chunk_join_kernel(Chunk a) {
 // A sequence takes wide tiles from more than FEW_ROWS rows on, of which there are then few that are mostly empty; a
 // call of up to FEW_ALL rows takes narrow tiles alone, and one launch.
 //
-// Of the shares that a tile may be cut in that number is taken for which the workgroups, two a CU at once and all
-// as long as the longest sequence makes them, and what the join writes and reads cost least. (Taking sequences to
+// Of the shares that a tile may be cut in that number is taken for which the workgroups that run at once, all as
+// long as the longest sequence makes them, and what the join writes and reads cost least. (Taking sequences to
 // be half as long on average cut 64 equal ones of 4000 tokens too often: 62 -> 188 us.)
-constexpr int64_t FEW_ROWS = 64, FEW_ALL = 512, AT_ONCE = 512;
+constexpr int64_t FEW_ROWS = 64, FEW_ALL = 512;
 struct Cut {
   Chunk::Kind wide, few;
   int64_t least;
 };
-static Chunk::Kind kind_of(int64_t most_tiles, int64_t tiles, int64_t heads, int64_t units, double unit_us, double share_us) {
+static Chunk::Kind kind_of(int64_t most_tiles, int64_t tiles, int64_t heads, int64_t units, int64_t at_once, double unit_us,
+                           double share_us) {
   Chunk::Kind k = {(int)most_tiles, (int)units, 1};
   double least = 0.0;
   if (tiles < 1) tiles = 1;
   for (int64_t m = 1; m <= 128 && m <= units; ++m) {
     const int64_t all = tiles * heads * m, each = (units + m - 1) / m;
-    const double rounds = all <= AT_ONCE ? 1.0 : (double)all / AT_ONCE + 1.0;
+    const double rounds = all <= at_once ? 1.0 : (double)all / at_once + 1.0;
     const double us = rounds * each * unit_us + (m > 1 ? 4.0 + m * share_us : 0.0);
     if (m == 1 || us < least) {
       least = us;
@@ -797,18 +813,20 @@ static Chunk::Kind kind_of(int64_t most_tiles, int64_t tiles, int64_t heads, int
 static Cut cut_of(int type, int64_t n, int64_t B, int64_t heads, int64_t group, int64_t dim, int64_t max_len) {
   const int64_t units = max_len > 0 ? (max_len + KEYS - 1) / KEYS : 1, begun = B + 2 < n ? B + 2 : n, rows = n * group;
   const double share_us = (double)rows * heads * (2 * 4 * (dim + 2)) / 4e6;  // of all rows, written and read at 4 TB/s
-  // a unit's time in a workgroup of two a CU: 8192 tokens over themselves, 32 heads over 8, bf16 and f16, 4096 f32
-  const double unit_us = (type == 0 ? 5.5 : type == 1 ? 2.3 : 3.7) * (dim == 128 ? 1.0 : 0.6), FEW_UNIT_US = 2.0;
+  // workgroups that run at once (two a CU, three where the registers allow), and a unit's time in one of them then
+  const int64_t at_once = dim == 64 && type ? 768 : 512;
+  const double unit_us = dim == 64 ? (type == 0 ? 3.3 : type == 1 ? 2.0 : 2.4) : type == 0 ? 5.5 : type == 1 ? 2.3 : 3.7;
+  constexpr double FEW_UNIT_US = 2.0;
   Cut c;
   c.least = rows <= FEW_ALL ? 0x7fffffff : FEW_ROWS;
   if (rows <= FEW_ALL) {
     const int64_t tiles = (rows + FEW - 1) / FEW, some = B < n ? B : n;
     c.wide = {0, 1, 1};
-    c.few = kind_of(rows / FEW + begun, tiles > some ? tiles : some, heads, units, FEW_UNIT_US, share_us);
+    c.few = kind_of(rows / FEW + begun, tiles > some ? tiles : some, heads, units, at_once, FEW_UNIT_US, share_us);
   } else {
     const int64_t many = rows / (FEW_ROWS + 1);  // sequences of more rows at most
-    c.wide = kind_of(rows / WIDE + (begun < many ? begun : many), rows / WIDE, heads, units, unit_us, share_us);
-    c.few = kind_of(begun * (FEW_ROWS / FEW), B < 1 ? 1 : B, heads, units, FEW_UNIT_US, share_us);
+    c.wide = kind_of(rows / WIDE + (begun < many ? begun : many), rows / WIDE, heads, units, at_once, unit_us, share_us);
+    c.few = kind_of(begun * (FEW_ROWS / FEW), B < 1 ? 1 : B, heads, units, at_once, FEW_UNIT_US, share_us);
   }
   return c;
 }
@@ -816,8 +834,8 @@ static Cut cut_of(int type, int64_t n, int64_t B, int64_t heads, int64_t group, 
 template <typename T, int DIM>
 static int launch(const char* what, const Chunk& a, hipStream_t st) {
   auto grid = [&](const Chunk::Kind& k) { return (unsigned)((int64_t)k.tiles * k.most * a.c.heads); };
-  if (a.wide.tiles) kv4_chunk_kernel<T, DIM><<<grid(a.wide), 256, 0, st>>>(a);
-  if (a.few.tiles) kv4_chunk_few_kernel<T, DIM><<<grid(a.few), 256, 0, st>>>(a);
+  if (a.wide.tiles) kv4_chunk_kernel<T, DIM, true, true><<<grid(a.wide) + grid(a.few), 256, 0, st>>>(a);
+  else kv4_chunk_kernel<T, DIM, false, true><<<grid(a.few), 256, 0, st>>>(a);
   if (a.wide.most > 1 || a.few.most > 1) {
     const int64_t rows = (int64_t)a.n * a.c.heads * a.group;
     kv4_chunk_join_kernel<T, DIM><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(a);
@@ -856,7 +874,7 @@ int bq_kv4_attend_chunk(const bq_kv4_cache* cache, const void* q, int type, int6
   if (n * group > 0x7fffffff - 8192) return set_error(BQ_ERR_ARG, "%s: size too large", what);
   const Cut cut = cut_of(type, n, B, cache->heads, group, cache->dim, max_len);
   auto grid = [&](const Chunk::Kind& k) { return (int64_t)k.tiles * k.most * cache->heads; };
-  if (grid(cut.wide) > 0x7fffffff || grid(cut.few) > 0x7fffffff || n * q_heads > 0x7fffffffll * 4)
+  if (grid(cut.wide) + grid(cut.few) > 0x7fffffff || n * q_heads > 0x7fffffffll * 4)
     return set_error(BQ_ERR_ARG, "%s: size too large", what);
   if (!q || !cu || !out || (B && !lens)) return set_error(BQ_ERR_ARG, "%s: null pointer", what);
   const int64_t size = type == KV4_F32 ? 4 : 2;

@@ -1,7 +1,8 @@
 """A beam search's selection against the oracle's: parents, tokens and ends exactly, scores to f32's rounding.
 
-Tolerance of the scores: the kernel's f64 sum is within 1e-13 of its size, so an f32 score is the exact one rounded
-once, half a step of 2^-24, and both sides' f64 errors (below 2^-40 of the score's parts) beside it. The inputs
+Tolerance of the scores: each f64 exponential is within 1.1e-12 < 2^-39 of itself, so the sum is and its logarithm within
+2^-39, and an f32 score is that rounded
+once, half a step of 2^-24 (the oracle's and the other f64 errors are far below). The inputs
 of the exact comparisons have no two candidates of different beams within 1e-9 of one another, other than equals."""
 import math
 
@@ -27,7 +28,7 @@ def check(dev, logits, scores, done=None, end=-1):
         assert got.tokens[b].tolist() == [c[2] for c in want], b
         assert got.done[b].tolist() == [c[3] for c in want], b
         for mine, (key, w, v, _) in zip(got.scores[b].tolist(), want):
-            assert mine == key or abs(mine - key) <= abs(key) * 2.0 ** -24 + 2.0 ** -149 + 2.0 ** -40, (b, mine, key)
+            assert mine == key or abs(mine - key) <= abs(key) * 2.0 ** -24 + 2.0 ** -149 + 2.0 ** -39, (b, mine, key)
     return got
 
 
@@ -189,3 +190,24 @@ def test_select_refusals(dev):
         beams.beam_select(torch.zeros(65, 9, device=dev), torch.zeros(1, 65, device=dev))
     with pytest.raises(RuntimeError, match="gradient"):
         beams.beam_select(logits.requires_grad_(), scores)
+
+
+def test_select_parts_of_nothing_but(dev):
+    """A part of the vocabulary that is all NaN, all -infinity, or all beyond what f64's exponentials hold, beside
+    ordinary ones; logits that start and end anywhere in 16 bytes."""
+    print("beams parts", flush=True)
+    V = 9001
+    logits, scores = random_case(1, 6, V, "f32", 11)
+    logits[0, 4096:] = math.nan
+    logits[1, 4096:] = -math.inf
+    logits[2, :6000] = -5000.0
+    logits[3, 5000:] += 2000.0
+    logits[4] = -3.0e4 + logits[4]
+    check(dev, logits, scores)
+    for off in range(9):
+        for kind in ("f32", "bf16"):
+            wide = random_case(1, 3, 2100, kind, off)[0]
+            x = wide.to(dev)[:, off:off + 2050 + off]
+            got = beams.beam_select(x, torch.zeros(1, 3, device=dev))
+            want = O.select(wide[:, off:off + 2050 + off].double().tolist(), [0.0] * 3, [False] * 3, -1)
+            assert got.tokens.tolist() == [[c[2] for c in want]] and got.parents.tolist() == [[c[1] for c in want]], (off, kind)
