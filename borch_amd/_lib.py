@@ -125,7 +125,7 @@ SIGNATURES = {
     "bq_kv4_append_slots": (_c_int, [_c_p, _c_p, _c_p, _c_int, *[_c_i64] * 5, _c_p, _c_p]),
     "bq_pages_cut": (_c_int, [_c_p, _c_p, _c_p]),
     "bq_pages_fork": (_c_int, [_c_p, _c_p, _c_p]),
-    "bq_pages_grow_ws_bytes": (_c_size, [_c_i64]),
+    "bq_pages_grow_ws_bytes": (_c_size, [_c_i64] * 2),
     "bq_pages_grow": (_c_int, [_c_p, _c_p, _c_i64, *[_c_p] * 6, _c_size, _c_p]),
     "bq_kv4_copy_pages": (_c_int, [_c_p, _c_i64, _c_p, _c_i64, _c_p]),
     "bq_kv4_read": (_c_int, [_c_p, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_p]),

@@ -40,28 +40,43 @@ __global__ __launch_bounds__(256) void pages_cut_kernel(Tables a, const int* __r
   if (lane == 0) a.lens[s] = keep;  // this wave has read it
 }
 
-// Every row of the table becomes its parent's: a workgroup takes `columns` columns of all rows through LDS,
-// the last one the lengths.
-constexpr int FORK_ENTRIES = 16384;
-__global__ __launch_bounds__(256) void pages_fork_kernel(Tables a, const int* __restrict__ parents, int columns) {
+// Every row of the table becomes its parent's: a workgroup takes 2^`shift` columns of all rows through LDS,
+// the last one the lengths. Few columns where there are few rows, for more workgroups.
+constexpr int FORK_ENTRIES = 16384, FORK_THREADS = 512, FORK_EACH = 4 * FORK_THREADS;
+__global__ __launch_bounds__(FORK_THREADS) void pages_fork_kernel(Tables a, const int* __restrict__ parents, int shift) {
   extern __shared__ int old[];
   const bool lengths = blockIdx.x == gridDim.x - 1;
-  const int c0 = blockIdx.x * columns, n = lengths ? 1 : min(columns, a.width - c0);
-  int* from = lengths ? a.lens : a.table + c0;
+  const int column = blockIdx.x << shift, count = a.S << (lengths ? 0 : shift), bits = lengths ? 0 : shift;
+  int* from = lengths ? a.lens : a.table;
   const size_t pitch = lengths ? 1 : a.width;
-  for (int i = threadIdx.x; i < a.S * n; i += 256) old[i] = from[i / n * pitch + i % n];
+  const int c0 = lengths ? 0 : column, c1 = lengths ? 1 : a.width;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < count; i += FORK_THREADS) {
+    const int s = i >> bits, c = c0 + (i & ((1 << bits) - 1));
+    old[i] = from[s * pitch + min(c, c1 - 1)];
+  }
   __syncthreads();
-  for (int i = threadIdx.x; i < a.S * n; i += 256) {
-    const int s = i / n, p = parents[s], was = old[i];
-    const int now = (unsigned)p < (unsigned)a.S ? old[p * n + i % n] : lengths ? 0 : -1;
-    if (now == was) continue;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < count; i += FORK_THREADS) {
+    const int s = i >> bits, e = i & ((1 << bits) - 1), p = parents[s], was = old[i];
+    const int now = (unsigned)p < (unsigned)a.S ? old[(p << bits) + e] : lengths ? 0 : -1;
+    if (now == was || c0 + e >= c1) continue;
     if (!lengths) {
       add_ref(a, was, -1);
       add_ref(a, now, 1);
     }
-    from[s * pitch + i % n] = now;
+    from[s * pitch + c0 + e] = now;
   }
 }
+
+// Growing. BLOCK pages' free ones are found as 64 words of 64 bits, a lane's word each. Up to SOLO_PAGES pages the
+// plan's waves read refs themselves, beyond it a launch before it writes the words down. One workgroup plans, since
+// the tables change only where all find room; it also hands out the pages and writes the places, but those of many
+// tokens (SOLO_ROWS) are launches of their own.
+constexpr int BLOCK = 4096, PLAN_THREADS = 1024, PLAN_WAVES = PLAN_THREADS / 64;
+constexpr int MOST_SEQUENCES = 8192, MOST_BLOCKS = 4096;
+constexpr int64_t SOLO_PAGES = (int64_t)BLOCK * PLAN_WAVES;
+constexpr int SOLO_ROWS = 8192;
 
 struct Grow {
   Tables t;
@@ -70,67 +85,105 @@ struct Grow {
   int* cu;
   int64_t* slots;
   int *at, *moves, *ok;
-  const int* counts;  // free pages in each BLOCK of them, or null
+  uint64_t* words;  // the workspace, or null: free pages; in each BLOCK, then before it; wanted pages before a sequence
+  int *counts, *upto;
+  bool solo;  // the plan hands out and writes the places
 };
 
-constexpr int BLOCK = 4096, PLAN_THREADS = 1024, PLAN_WAVES = PLAN_THREADS / 64;
-constexpr int MOST_SEQUENCES = 8192, MOST_BLOCKS = 4096;
-constexpr int64_t SOLO_PAGES = (int64_t)BLOCK * PLAN_WAVES;  // a wave of the plan counts a block itself
-constexpr int SOLO_ROWS = 8192;                             // places that the plan writes itself
-
-// The free pages of block b by one wave: f(page, rank) in ascending order, from `rank` on until it says no.
-template <typename F>
-__device__ __forceinline__ int each_free(const Tables& a, int b, int rank, F&& f) {
-  const int lane = threadIdx.x & 63, end = min(a.pages, (b + 1) * BLOCK);
-  const uint64_t before = (1ull << lane) - 1;
-  for (int i = b * BLOCK; i < end; i += 512) {
-    int refs[8];
+// Up to 64 words of free pages by one wave, the first for the pages from 64 `w0` on, lane l's the l-th.
+__device__ __forceinline__ uint64_t free_words(const Tables& a, int w0, int n) {
+  const int lane = threadIdx.x & 63;
+  uint64_t mine = 0;
+  for (int i = 0; i < n && (w0 + i) * 64 < a.pages; i += 16) {
+    int refs[16];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) refs[e] = a.refs[min(i + 64 * e + lane, end - 1)];
+    for (int e = 0; e < 16; ++e) refs[e] = a.refs[min((w0 + i + e) * 64 + lane, a.pages - 1)];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int p = i + 64 * e + lane;
-      const uint64_t free = __ballot(p < end && refs[e] == 0);
-      if ((free >> lane) & 1) f(p, rank + __builtin_popcountll(free & before));
-      rank += __builtin_popcountll(free);
+    for (int e = 0; e < 16; ++e) {
+      const uint64_t free = __ballot((w0 + i + e) * 64 + lane < a.pages && refs[e] == 0);
+      if (lane == i + e && i + e < n) mine = free;
     }
   }
-  return rank;
+  return mine;
 }
 
-__global__ __launch_bounds__(256) void pages_count_kernel(Tables a, int* counts) {
-  const int b = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if ((int64_t)b * BLOCK >= a.pages) return;
-  const int n = each_free(a, b, 0, [](int, int) {});
-  if ((threadIdx.x & 63) == 0) counts[b] = n;
+// The sum of the lanes' values up to this one's own; what passes 32 bits stays at their largest.
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ uint32_t plus_lanes(uint32_t v) {
+  return __builtin_elementwise_add_sat(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CONTROL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ uint32_t wave_upto(uint32_t v) {
+  v = plus_lanes<0x111, 0xF>(v);  // from the lanes 1, 2, 4 and 8 before in a row of 16,
+  v = plus_lanes<0x112, 0xF>(v);
+  v = plus_lanes<0x114, 0xF>(v);
+  v = plus_lanes<0x118, 0xF>(v);
+  v = plus_lanes<0x142, 0xA>(v);  // the last of the row before into the second and fourth,
+  return plus_lanes<0x143, 0xC>(v);  // lane 31's into the upper half
 }
 
-// The sum over the workgroup's threads before this one, and of all.
-__device__ __forceinline__ int64_t scan_all(int64_t v, int64_t* waves, int64_t* all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t x = v;
+// A wave's words' free pages in ascending order: f(page, k), k from `rank` on and below `limit`.
+template <typename F>
+__device__ __forceinline__ void each_free(uint64_t word, int w0, int rank, int limit, F&& f) {
+  const int lane = threadIdx.x & 63, upto = (int)wave_upto(__builtin_popcountll(word));
+  const int before = upto - __builtin_popcountll(word), n = min(__shfl(upto, 63), limit - rank);
+  for (int j0 = 0; j0 < n; j0 += 64) {
+    const int j = j0 + lane;
+    int l = 0;
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int64_t y = __shfl_up(x, d);
-    if (lane >= d) x += y;
+    for (int d = 32; d; d /= 2) l += __shfl(before, l + d) <= j ? d : 0;
+    int nth = j - __shfl(before, l), bit = 0;
+    uint64_t w = (uint64_t)(uint32_t)__shfl((int)(word >> 32), l) << 32 | (uint32_t)__shfl((int)word, l);
+#pragma unroll
+    for (int d = 32; d; d /= 2) {
+      const int low = __builtin_popcountll(w & ((1ull << d) - 1));
+      const bool above = nth >= low;
+      nth -= above ? low : 0;
+      bit += above ? d : 0;
+      w >>= above ? d : 0;
+    }
+    if (j < n) f((w0 + l) * 64 + bit, rank + j);
   }
+}
+
+__global__ __launch_bounds__(256) void pages_count_kernel(Grow g) {
+  __shared__ int of[4];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, w0 = blockIdx.x * 64 + wave * 16;
+  const uint64_t word = free_words(g.t, w0, 16);
+  if (lane < 16) g.words[w0 + lane] = word;
+  const int n = (int)wave_upto(__builtin_popcountll(word));
+  if (lane == 63) of[wave] = n;
+  __syncthreads();
+  if (threadIdx.x == 0) g.counts[blockIdx.x] = of[0] + of[1] + of[2] + of[3];
+}
+
+// The sums over the workgroup's threads before this one, and of all (at 32 bits' largest where they pass it, which
+// is more than any caller has room for).
+struct Pair {
+  uint32_t pages, tokens;
+};
+__device__ __forceinline__ Pair plus(Pair a, Pair b) {
+  return {__builtin_elementwise_add_sat(a.pages, b.pages), __builtin_elementwise_add_sat(a.tokens, b.tokens)};
+}
+__device__ __forceinline__ Pair scan_all(Pair v, Pair* waves, Pair* all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Pair x = {wave_upto(v.pages), wave_upto(v.tokens)};
   __syncthreads();  // the last scan's sums are read
   if (lane == 63) waves[wave] = x;
   __syncthreads();
-  int64_t before = 0, total = 0;
+  Pair before = {0, 0}, total = {0, 0};
 #pragma unroll
   for (int i = 0; i < PLAN_WAVES; ++i) {
-    const int64_t w = waves[i];
-    before += i < wave ? w : 0;
-    total += w;
+    if (i == wave) before = total;
+    total = plus(total, waves[i]);
   }
   *all = total;
-  return before + x - v;
+  const uint32_t p = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x.pages, 0x138, 0xF, 0xF, false);  // the lane before
+  const uint32_t t = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x.tokens, 0x138, 0xF, 0xF, false);
+  return plus(before, {p, t});
 }
 
-// The first i of n whose running sum upto[i] (without i itself) passes k, less one: where k lies.
-__device__ __forceinline__ int holder_of(const int* upto, int n, int k) {
-  int lo = 0, hi = n - 1;
+// Where k lies among the running sums upto[0] = 0, ...: the last i in [lo, hi] with upto[i] <= k.
+__device__ __forceinline__ int holder_of(const int* upto, int lo, int hi, int k) {
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (upto[mid] <= k) lo = mid;
@@ -148,20 +201,39 @@ __device__ __forceinline__ void put_place(const Grow& g, int i, int s, int64_t l
   g.slots[i] = (unsigned)page < (unsigned)a.pages ? (int64_t)page * a.page + (at - c * a.page) : -1;
 }
 
+// A free page to sequence s as its `nth` new one; `share`: the page that the first takes the place of, or -1.
+template <int SCOPE>
+__device__ __forceinline__ void give(const Grow& g, int page, int s, int nth, int len, int share) {
+  const Tables& a = g.t;
+  const int c = pages_of(a, len) + nth - (share >= 0 ? 1 : 0);
+  if (share >= 0 && nth == 0) {
+    __hip_atomic_fetch_add(a.refs + share, -1, __ATOMIC_RELAXED, SCOPE);
+    g.moves[a.S + s] = page;
+  }
+  a.table[(size_t)s * a.width + c] = page;
+  a.refs[page] = 1;
+}
+
 // What each sequence wants, one workgroup: nothing is written before it is known that all find room.
 __global__ __launch_bounds__(PLAN_THREADS) void pages_grow_kernel(Grow g) {
-  __shared__ int upto[MOST_SEQUENCES + 1], first[MOST_SEQUENCES + 1], share[MOST_SEQUENCES];  // pages, tokens before; the shared page
+  // pages and tokens before a sequence, its tokens, the page that it shares; pages free before a block. The first
+  // three hold the shared pages' hash table before that: the page, the lowest sequence, how many.
+  __shared__ int upto[MOST_SEQUENCES + 1], first[MOST_SEQUENCES + 1], held[MOST_SEQUENCES], share[MOST_SEQUENCES];
   __shared__ int blocks[MOST_BLOCKS + 1];
-  __shared__ int64_t waves[PLAN_WAVES];
+  __shared__ Pair waves[PLAN_WAVES];
   const Tables& a = g.t;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  // the first of this thread's sequences, and refs if they are read here: on their way together
+  const int mine = min(tid, a.S - 1), len0 = mine < 0 ? 0 : a.lens[mine], more0 = mine < 0 ? 0 : g.more[mine];
+  int count = PLAN_WAVES, each = ((a.pages + 63) / 64 + PLAN_WAVES - 1) / PLAN_WAVES;  // words a block, 64 at most
+  const uint64_t word = g.words ? 0 : free_words(a, wave * each, each);
   // the last page of each that grows, if it is partly filled and named elsewhere too
   bool bad = false, any = false;
   for (int s = tid; s < a.S; s += PLAN_THREADS) {
-    const int len = a.lens[s], more = g.more[s];
+    const int len = s == tid ? len0 : a.lens[s], more = s == tid ? more0 : g.more[s];
     const int c = fdiv(max(len, 0), a.by_page.mul, a.by_page.shift);
-    const int64_t after = ((int64_t)len + more + a.page - 1) / a.page;
-    bad |= more < 0 || len < 0 || after > a.width;
+    // width pages are fewer than 2^31 tokens
+    bad |= more < 0 || len < 0 || (int64_t)len + more > (int64_t)a.width * a.page;
     int page = -1;
     if (len > 0 && more > 0 && c < a.width && len != c * a.page) {
       page = a.table[(size_t)s * a.width + c];
@@ -170,121 +242,169 @@ __global__ __launch_bounds__(PLAN_THREADS) void pages_grow_kernel(Grow g) {
     share[s] = page;
     any |= page >= 0;
   }
-  const bool shares = __syncthreads_or(any);
   // of those that share a page and grow the lowest keeps it where they are all that name it
-  int64_t pages = 0, tokens = 0;
+  if (__syncthreads_or(any)) {
+    int bits = 6;
+    while (1 << bits < 2 * a.S && 1 << bits < MOST_SEQUENCES) ++bits;  // as many slots as sequences at least
+    const int mask = (1 << bits) - 1;
+    for (int i = tid; i <= mask; i += PLAN_THREADS) upto[i] = -1, first[i] = MOST_SEQUENCES, held[i] = 0;
+    __syncthreads();
+    for (int s = tid; s < a.S; s += PLAN_THREADS) {
+      const int page = share[s];
+      if (page < 0) continue;
+      int h = (int)((uint32_t)page * 0x9E3779B1u >> (32 - bits));
+      for (;; h = (h + 1) & mask) {
+        const int was = atomicCAS(upto + h, -1, page);
+        if (was == -1 || was == page) break;
+      }
+      atomicMin(first + h, s);
+      atomicAdd(held + h, 1);
+    }
+    __syncthreads();
+    for (int s = tid; s < a.S; s += PLAN_THREADS) {
+      const int page = share[s];
+      if (page < 0) continue;
+      int h = (int)((uint32_t)page * 0x9E3779B1u >> (32 - bits));
+      while (upto[h] != page) h = (h + 1) & mask;
+      if (first[h] == s && held[h] == a.refs[page]) share[s] = -1;
+    }
+    __syncthreads();
+  }
+  Pair total = {0, 0};
   for (int s0 = 0; s0 < a.S; s0 += PLAN_THREADS) {
     const int s = s0 + tid;
-    int64_t want = 0, more = 0;
+    Pair want = {0, 0}, all;
     if (s < a.S) {
-      bool own = false;
-      if (shares && share[s] >= 0) {
-        const int page = share[s];
-        int same = 0, lower = 0;
-        for (int i = 0; i < a.S; ++i) {
-          const int hit = share[i] == page;
-          same += hit;
-          lower += i < s ? hit : 0;
-        }
-        own = lower > 0 || same != a.refs[page];
-      }
-      const int64_t len = max(a.lens[s], 0);
-      more = max(g.more[s], 0);
-      want = (len + more + a.page - 1) / a.page - (len + a.page - 1) / a.page + own;
-      if (own) want |= 1ll << 40;
+      const int len = max(s0 == 0 ? len0 : a.lens[s], 0), more = max(s0 == 0 ? more0 : g.more[s], 0);
+      want.tokens = more;  // what does not fit is refused, whatever its pages
+      want.pages = max(pages_of(a, (int)min((uint32_t)len + more, 0x7fffffffu)) - pages_of(a, len), 0) + (share[s] >= 0);
+      held[s] = len;
     }
-    const bool own = (want >> 40) & 1;
-    want &= (1ll << 40) - 1;
-    int64_t all, all_more;
-    const int64_t w = pages + scan_all(want, waves, &all), m = tokens + scan_all(more, waves, &all_more);
+    const Pair before = scan_all(want, waves, &all);
     if (s < a.S) {
-      upto[s] = (int)min(w, (int64_t)0x7fffffff);
-      first[s] = (int)min(m, (int64_t)0x7fffffff);
-      g.moves[s] = own ? 0 : -1;  // read again below
+      const Pair from = plus(total, before);
+      upto[s] = (int)min(from.pages, 0x7fffffffu);
+      first[s] = (int)min(from.tokens, 0x7fffffffu);
     }
-    pages += all;
-    tokens += all_more;
+    total = plus(total, all);
   }
-  bad |= tokens > g.rows || pages > a.pages;
+  bad |= total.tokens > (uint32_t)g.rows || total.pages > (uint32_t)a.pages;
   // the free pages, where any are wanted
-  const int count = (int)(((int64_t)a.pages + BLOCK - 1) / BLOCK);
   bool good = !__syncthreads_or(bad);
-  if (good && pages > 0) {
-    if (!g.counts) {
-      if (wave < count) {
-        const int n = each_free(a, wave, 0, [](int, int) {});
-        if (lane == 0) blocks[wave] = n;
-      }
+  const int wanted = good ? (int)total.pages : 0;
+  if (wanted > 0) {
+    Pair all;
+    int free = 0;  // 2^24 at most
+    if (!g.words) {
+      const Pair before = scan_all({(uint32_t)__builtin_popcountll(word), 0}, waves, &all);
+      if (lane == 0) blocks[wave] = (int)before.pages;
+      free = (int)all.pages;
     } else {
-      for (int b = tid; b < count; b += PLAN_THREADS) blocks[b] = g.counts[b];
+      each = 64;
+      count = (a.pages + BLOCK - 1) / BLOCK;
+      for (int b0 = 0; b0 < count; b0 += PLAN_THREADS) {
+        const int b = b0 + tid;
+        const Pair before = scan_all({b < count ? (uint32_t)g.counts[b] : 0, 0}, waves, &all);
+        if (b < count) blocks[b] = free + (int)before.pages;
+        free += (int)all.pages;
+      }
     }
+    good = free >= wanted;
     __syncthreads();
-    int64_t free = 0;
-    for (int b0 = 0; b0 < count; b0 += PLAN_THREADS) {
-      const int b = b0 + tid, n = b < count ? blocks[b] : 0;
-      int64_t all;
-      const int64_t w = free + scan_all(n, waves, &all);
-      if (b < count) blocks[b] = (int)w;
-      free += all;
-    }
-    good = free >= pages;
-    __syncthreads();
-    if (good) {
-      for (int b = wave; b < count && blocks[b] < pages; b += PLAN_WAVES)
-        each_free(a, b, blocks[b], [&](int page, int k) {
-          if (k >= pages) return;
-          const int s = holder_of(upto, a.S, k), len = a.lens[s];
-          const bool own = g.moves[s] == 0;
-          const int nth = k - upto[s];
-          int c = pages_of(a, len) + nth - (own ? 1 : 0);
-          if (own && nth == 0) {
-            add_ref(a, share[s], -1);
-            g.moves[a.S + s] = page;
-          }
-          a.table[(size_t)s * a.width + c] = page;
-          a.refs[page] = 1;
+    if (good && g.words && !g.solo) {  // a launch of its own hands them out
+      for (int b = tid; b < count; b += PLAN_THREADS) g.counts[b] = blocks[b];
+      for (int s = tid; s < a.S; s += PLAN_THREADS) g.upto[s] = upto[s];
+    } else if (good) {
+      for (int b = wave; b < count && blocks[b] < wanted; b += PLAN_WAVES)
+        each_free(g.words ? g.words[b * 64 + lane] : word, b * each, blocks[b], wanted, [&](int page, int k) {
+          const int s = holder_of(upto, 0, a.S - 1, k);
+          give<__HIP_MEMORY_SCOPE_WORKGROUP>(g, page, s, k - upto[s], held[s], share[s]);
         });
     }
   }
+  if (g.words && tid == 0) g.upto[a.S] = good ? wanted : 0;
   __syncthreads();
   for (int s = tid; s < a.S; s += PLAN_THREADS) {
-    const int len = a.lens[s];
-    const bool own = good && g.moves[s] == 0;
+    const int len = held[s];
+    const bool own = good && share[s] >= 0;
     g.moves[s] = own ? share[s] : -1;
     if (!own) g.moves[a.S + s] = -1;
     g.moves[2 * a.S + s] = own ? len - fdiv(len, a.by_page.mul, a.by_page.shift) * a.page : 0;
     g.cu[s] = good ? first[s] : 0;
+    if (good) a.lens[s] = len + (s == tid ? more0 : g.more[s]);
   }
   if (tid == 0) {
-    g.cu[a.S] = good ? (int)tokens : 0;
+    g.cu[a.S] = good ? (int)total.tokens : 0;
     g.ok[0] = good ? 1 : 0;
   }
-  if (g.rows <= SOLO_ROWS)
+  if (g.solo)
     for (int i = tid; i < g.rows; i += PLAN_THREADS) {
-      if (!good || i >= tokens) {
+      if (!good || i >= (int)total.tokens) {
         g.at[i] = -1;
         g.slots[i] = -1;
       } else {
-        const int s = holder_of(first, a.S, i);
-        put_place(g, i, s, a.lens[s], first[s]);
+        const int s = holder_of(first, 0, a.S - 1, i);
+        put_place(g, i, s, held[s], first[s]);
       }
     }
-  __syncthreads();
-  if (good)
-    for (int s = tid; s < a.S; s += PLAN_THREADS) a.lens[s] += g.more[s];
 }
 
-// The places of many new tokens, after the plan.
-__global__ __launch_bounds__(256) void pages_places_kernel(Grow g) {
-  const int i = blockIdx.x * 256 + threadIdx.x, S = g.t.S;
-  if (i >= g.rows) return;
-  if (i >= g.cu[S]) {
-    g.at[i] = -1;
-    g.slots[i] = -1;
-    return;
+// The pages of many new tokens, after the plan: a workgroup a block, a wave four of its words.
+__global__ __launch_bounds__(1024) void pages_give_kernel(Grow g) {
+  extern __shared__ int upto[];
+  const Tables& a = g.t;
+  const int lane = threadIdx.x & 63, w0 = threadIdx.x >> 6 << 2, b = blockIdx.x;
+  const int wanted = g.upto[a.S], rank = g.counts[b];
+  if (rank >= wanted) return;
+  const uint64_t all = g.words[b * 64 + lane], mine = g.words[b * 64 + w0 + (lane & 3)];
+  for (int s = threadIdx.x; s < a.S; s += 1024) upto[s] = g.upto[s];
+  __syncthreads();
+  const int n = __builtin_popcountll(all), before = rank + __shfl((int)wave_upto(n) - n, w0);
+  if (before >= wanted) return;
+  each_free(lane < 4 ? mine : 0, b * 64 + w0, before, wanted, [&](int page, int k) {
+    const int s = holder_of(upto, 0, a.S - 1, k);
+    give<__HIP_MEMORY_SCOPE_AGENT>(g, page, s, k - upto[s], a.lens[s] - (g.cu[s + 1] - g.cu[s]), g.moves[s]);
+  });
+}
+
+// The last s with cu[s] <= k by one wave, 64 at a time.
+__device__ __forceinline__ int wave_holder(const int* cu, int S, int k) {
+  int lo = 0, n = S;
+  while (n > 1) {
+    const int step = (n + 63) >> 6, i = (int)(threadIdx.x & 63) * step;
+    const int below = __builtin_popcountll(__ballot(i < n && cu[lo + min(i, n - 1)] <= k)) - 1;  // cu[lo] <= k
+    lo += below * step;
+    n = min(step, n - below * step);
   }
-  const int s = holder_of(g.cu, S, i);
-  put_place(g, i, s, (int64_t)g.t.lens[s] - (g.cu[s + 1] - g.cu[s]), g.cu[s]);
+  return lo;
+}
+
+// The places of many new tokens, after their pages: a wave takes 256.
+__global__ __launch_bounds__(256) void pages_places_kernel(Grow g) {
+  const int lane = threadIdx.x & 63, S = g.t.S, all = S ? g.cu[S] : 0;
+  const int64_t i0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 256;
+  if (i0 >= g.rows) return;
+  int lo = 0, hi = 0;
+  if (i0 < all) {
+    const int last = (int)min(i0 + 255, (int64_t)all - 1);
+    lo = wave_holder(g.cu, S, (int)i0);
+    hi = g.cu[lo + 1] > last ? lo : lo + wave_holder(g.cu + lo, S - lo, last);
+  }
+  int s[4], first[4], end[4], len[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) s[e] = lo;
+  if (lo < hi)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] = holder_of(g.cu, lo, hi, (int)min(i0 + e * 64 + lane, (int64_t)all - 1));
+  if (i0 < all)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) first[e] = g.cu[s[e]], end[e] = g.cu[s[e] + 1], len[e] = g.t.lens[s[e]];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int64_t at = i0 + e * 64 + lane;
+    if (at < all && at < g.rows) put_place(g, (int)at, s[e], (int64_t)len[e] - (end[e] - first[e]), first[e]);
+    else if (at < g.rows) g.at[at] = -1, g.slots[at] = -1;
+  }
 }
 
 // The tokens of pages that go over to others, in up to CACHES caches: a workgroup a cache, move and head
@@ -351,15 +471,16 @@ int bq_pages_fork(const bq_pages* pages, const int32_t* parents, bq_stream_t str
   if (const int rc = tables_of(what, pages, &a)) return rc;
   if (a.S == 0) return BQ_OK;
   if (!parents) return set_error(BQ_ERR_ARG, "%s: null pointer", what);
-  int columns = 16;
-  while (columns * a.S > FORK_ENTRIES) columns /= 2;  // S <= 8192: two at least
-  const int tiles = (a.width + columns - 1) / columns;
-  pages_fork_kernel<<<tiles + 1, 256, (size_t)columns * a.S * 4, (hipStream_t)stream>>>(a, parents, columns);
+  int shift = 4;
+  while (shift > 1 && (a.S << shift) > (shift > 3 ? FORK_EACH : FORK_ENTRIES)) --shift;  // S <= 8192: two columns at least
+  const int tiles = (a.width + (1 << shift) - 1) >> shift;
+  pages_fork_kernel<<<tiles + 1, FORK_THREADS, ((size_t)a.S << shift) * 4, (hipStream_t)stream>>>(a, parents, shift);
   return check_launch(what);
 }
 
-size_t bq_pages_grow_ws_bytes(int64_t pages) {
-  return pages > SOLO_PAGES ? (size_t)((pages + BLOCK - 1) / BLOCK) * 4 : 0;
+size_t bq_pages_grow_ws_bytes(int64_t sequences, int64_t pages) {
+  if (sequences < 0 || sequences > MOST_SEQUENCES || pages <= SOLO_PAGES || pages > (int64_t)MOST_BLOCKS * BLOCK) return 0;
+  return (size_t)((pages + BLOCK - 1) / BLOCK) * (64 * 8 + 4) + (sequences + 1) * 4;
 }
 
 int bq_pages_grow(const bq_pages* pages, const int32_t* more, int64_t rows, int32_t* cu, int64_t* slots, int32_t* at,
@@ -370,9 +491,10 @@ int bq_pages_grow(const bq_pages* pages, const int32_t* more, int64_t rows, int3
   if (rows < 0 || rows > 0x7fffffff - 8192) return set_error(BQ_ERR_ARG, "%s: %lld rows", what, (long long)rows);
   if (!cu || !ok || (rows && (!slots || !at)) || (g.t.S && (!more || !moves)))
     return set_error(BQ_ERR_ARG, "%s: null pointer", what);
-  const size_t need = bq_pages_grow_ws_bytes(g.t.pages);
-  if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 3)))
+  const size_t need = bq_pages_grow_ws_bytes(g.t.S, g.t.pages);
+  if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 7)))
     return set_error(BQ_ERR_ARG, "%s: a workspace of %zu bytes, given %zu", what, need, ws ? ws_bytes : 0);
+  const int blocks = (g.t.pages + BLOCK - 1) / BLOCK;
   g.more = more;
   g.rows = (int)rows;
   g.cu = cu;
@@ -380,14 +502,15 @@ int bq_pages_grow(const bq_pages* pages, const int32_t* more, int64_t rows, int3
   g.at = at;
   g.moves = moves;
   g.ok = ok;
-  g.counts = need ? (const int*)ws : nullptr;
+  g.words = need ? (uint64_t*)ws : nullptr;
+  g.counts = need ? (int*)(g.words + (size_t)blocks * 64) : nullptr;
+  g.upto = need ? g.counts + blocks : nullptr;
+  g.solo = rows <= SOLO_ROWS;
   hipStream_t st = (hipStream_t)stream;
-  if (need) {
-    const int blocks = (g.t.pages + BLOCK - 1) / BLOCK;
-    pages_count_kernel<<<(blocks + 3) / 4, 256, 0, st>>>(g.t, (int*)ws);
-  }
+  if (need) pages_count_kernel<<<blocks, 256, 0, st>>>(g);
   pages_grow_kernel<<<1, PLAN_THREADS, 0, st>>>(g);
-  if (rows > SOLO_ROWS) pages_places_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(g);
+  if (need && !g.solo) pages_give_kernel<<<blocks, 1024, (size_t)g.t.S * 4, st>>>(g);
+  if (!g.solo) pages_places_kernel<<<(unsigned)((rows + 1023) / 1024), 256, 0, st>>>(g);
   return check_launch(what);
 }
 

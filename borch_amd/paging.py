@@ -101,7 +101,7 @@ class Pages:
         i32 = dict(dtype=torch.int32, device=self.device)
         got = Grown(torch.empty(S + 1, **i32), torch.empty(rows, dtype=torch.int64, device=self.device),
                     torch.empty(rows, **i32), torch.empty((3, S), **i32), torch.empty(1, **i32))
-        need = lib().bq_pages_grow_ws_bytes(self.pages)
+        need = lib().bq_pages_grow_ws_bytes(S, self.pages)
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         with on(self._index):
             check(lib().bq_pages_grow(self._ref, more.data_ptr(), rows, got.cu.data_ptr(), got.slots.data_ptr(),

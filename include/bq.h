@@ -609,8 +609,8 @@ int bq_pages_fork(const bq_pages* pages, const int32_t* parents, bq_stream_t str
  *     sequence; -1 past the last (and a slot of -1 where the table names no page)
  *   moves i32 [3, sequences]: pages whose tokens have to move before more are written: from, to (-1: none) and
  *     how many tokens (bq_kv4_copy_pages)
- * ws: bq_pages_grow_ws_bytes bytes, 4-byte aligned, need not be cleared. */
-size_t bq_pages_grow_ws_bytes(int64_t pages);
+ * ws: bq_pages_grow_ws_bytes bytes, 8-byte aligned, need not be cleared. */
+size_t bq_pages_grow_ws_bytes(int64_t sequences, int64_t pages);
 int bq_pages_grow(const bq_pages* pages, const int32_t* more, int64_t rows, int32_t* cu, int64_t* slots, int32_t* at,
                   int32_t* moves, int32_t* ok, void* ws, size_t ws_bytes, bq_stream_t stream);
 

@@ -104,6 +104,37 @@ def test_many_rows(dev, rows):
     b.grow([0, rows, 0, 0, 0], rows)
 
 
+@pytest.mark.parametrize("pages", [9000, 65536, 70001])
+def test_scattered_pages(dev, pages):
+    """Free pages strewn among taken ones, shared last pages among those that grow, for many tokens and for few."""
+    print(f"pages scattered {pages}", flush=True)
+    r = random.Random(pages)
+    sequences, page = 70, 8
+    b = Both(dev, sequences, 300, pages, page)
+    b.grow([r.randint(0, 100) for _ in range(sequences)], 7000)
+    b.fork([s if r.random() < 0.5 else r.randrange(sequences) for s in range(sequences)])
+    held = torch.tensor([n == 0 and r.random() < 0.7 for n in b.ref.refs], device=dev)
+    b.gpu.refs += held.int()  # pages that others than these sequences hold
+    b.ref.refs = b.gpu.refs.tolist()
+    free = b.ref.refs.count(0)
+    long = min(free // 20 * page, 1000)
+    assert b.grow([r.choice([0, 1, page, long]) for _ in range(sequences)], 70000).ok.item() == 1
+    b.fork([s if r.random() < 0.5 else r.randrange(sequences) for s in range(sequences)])
+    assert b.grow([r.choice([0, 0, 1, 3 * page]) for _ in range(sequences)], 2000).ok.item() == 1
+
+
+def test_most_sequences(dev):
+    """As many sequences as there may be, most of them sharing pages that are partly filled."""
+    print("pages of 8192 sequences", flush=True)
+    r = random.Random(5)
+    b = Both(dev, 8192, 3, 20000, 32)
+    b.grow([r.randint(0, 40) for _ in range(8192)], 8192 * 40)
+    b.fork([s if r.random() < 0.3 else r.randrange(8192) for s in range(8192)])
+    assert b.grow([r.randint(0, 1) for _ in range(8192)], 8192).ok.item() == 1
+    b.fork([r.randrange(3) if s % 2 else s for s in range(8192)])
+    assert b.grow([1] * 8192, 8192).ok.item() == 1
+
+
 def test_shared_pages(dev):
     """Who keeps a shared page: the lowest where all that share it grow; nobody where one does not, or has
     filled it."""

@@ -43,8 +43,8 @@ def test_grow_is_checked():
     assert call(rows=-1) == ARG and call(rows=2 ** 31) == ARG
     for name in ("more", "cu", "slots", "at", "moves", "ok"):
         assert call(**{name: None}) == ARG, name
-    need = lib.bq_pages_grow_ws_bytes(70000)
-    assert need > 0 == lib.bq_pages_grow_ws_bytes(65536)
+    need = lib.bq_pages_grow_ws_bytes(2, 70000)
+    assert need > 0 == lib.bq_pages_grow_ws_bytes(2, 65536)
     assert call(desc(pages=70000)) == ARG and "workspace" in _lib.last_error()
     assert call(desc(pages=70000), ws=16, size=need - 1) == ARG and call(desc(pages=70000), ws=18, size=need) == ARG
 
