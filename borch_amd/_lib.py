@@ -135,7 +135,7 @@ SIGNATURES = {
     "bq_kv4_attend_chunk_ws_bytes": (_c_size, [_c_int, *[_c_i64] * 6]),
     "bq_kv4_attend_chunk": (_c_int, [_c_p, _c_p, _c_int, *[_c_i64] * 4, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_f,
                                      _c_p, _c_p, _c_size, _c_p]),
-    "bq_beam_select_ws_bytes": (_c_size, [_c_i64] * 3),
+    "bq_beam_select_ws_bytes": (_c_size, [_c_int, *[_c_i64] * 3]),
     "bq_beam_select": (_c_int, [_c_p, _c_int, *[_c_i64] * 4, _c_p, _c_p, _c_i64, *[_c_p] * 5, _c_size, _c_p]),
     "bq_kv4_evict": (_c_int, [_c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64,
                               _c_i64, _c_p, _c_p, _c_p, _c_p, _c_size, _c_p]),

@@ -60,7 +60,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, done: torch.Tensor |
     if B == 0:
         return out
     V = logits.shape[1]
-    need = lib().bq_beam_select_ws_bytes(B, W, V)
+    need = lib().bq_beam_select_ws_bytes(code, B, W, V)
     ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
     with on(index):
         check(lib().bq_beam_select(logits.data_ptr(), code, B, W, V, logits.stride(0), scores.data_ptr(),

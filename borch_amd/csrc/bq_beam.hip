@@ -8,13 +8,15 @@
 //
 // Two launches. The first reads the logits once: a workgroup takes a part of a beam's tokens, and each of its
 // waves keeps the W best of what it reads, a candidate a lane in order (value and token as one 64-bit number,
-// so that equals go to the lower token). A logit that beats the last of them is rare: the W-th largest of the 64
-// lanes' maxima over the first 2048 or 1024 tokens bounds it from below before any is looked at alone, and then
-// one test of 64 lanes' maxima over 16 bytes each says that there is none. The exponentials need no maximum: f64
-// holds e^x for every logit within +-600, and parts with others are summed again against their maximum. The second
-// launch joins a request's parts and beams.
+// so that equals go to the lower token). Which logits are looked at alone is known from maxima: the W-th largest of a
+// wave's 64 lanes' maxima is reached by W logits at least, so that less than the largest such bar of the four waves
+// is never among the W best of the part, and only the 16 bytes whose maximum reaches it are read again. The
+// exponentials need no maximum: f64 holds e^x for every logit within +-600, and parts with others are summed again
+// against their maximum. The second launch joins a request's parts and beams.
 //
-// Bound by the exponentials, 14 operations in f64 a logit, beside the reading.
+// Bound by the exponentials, 10 operations in f64 and as many in 32 bits a logit, beside the reading: 64 requests of
+// 8 beams and 128000 tokens in bf16 (131 MB) take 50 us for the first launch (the vector units busy for two thirds of
+// it) and 9 for the second. 4 beams of 32000 in f32: 6 us each, latency.
 #include <math.h>
 
 #include "bq_common.h"
@@ -25,6 +27,7 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int MOST_BEAMS = 64, PART_WAVES = 4;
+constexpr int PIECES = 16, PART_BYTES = PIECES * PART_WAVES * 64 * 16;  // 16 bytes each of a lane; of a part
 
 struct Beam {
   const void* x;
@@ -77,23 +80,21 @@ struct List {
   }
 };
 
-// e^x in f64 for |x| <= 740: 2^n times a polynomial for 2^f, f within 1/2 of 0 (interpolated at Chebyshev's nodes;
-// within 1.1e-12 of itself). NaN stays.
-__device__ __forceinline__ double exp_of(double x) {
-  constexpr double ROUND = 0x1.8p52;  // a sum with it is a whole number in its low bits
-  const double k = __builtin_fma(x, 0x1.71547652b82fep0, ROUND), n = k - ROUND;
-  const double f = __builtin_fma(x, 0x1.71547652b82fep0, -n);
-  double p = __builtin_fma(f, 0x1.63cf7dec51603p-20, 0x1.00dc48dc4d96cp-16);
-  p = __builtin_fma(f, p, 0x1.4308ae274a207p-13);
-  p = __builtin_fma(f, p, 0x1.5d8745a95d2d4p-10);
-  p = __builtin_fma(f, p, 0x1.3b2ab71725c04p-7);
-  p = __builtin_fma(f, p, 0x1.c6b08dd6fb6b1p-5);
-  p = __builtin_fma(f, p, 0x1.ebfbdff824847p-3);
-  p = __builtin_fma(f, p, 0x1.62e42fef84cf7p-1);
-  p = __builtin_fma(f, p, 0x1.ffffffffffffdp-1);
-  return __builtin_amdgcn_ldexp(p, (int)__builtin_bit_cast(uint64_t, k));
+// e^x in f64 for |x| <= 700: 2^(n / 32) from a table of n's low bits and n's others as its exponent, times a
+// polynomial for 2^(f / 32), f within 1/2 of 0 (interpolated at Chebyshev's nodes; within 8e-14 of itself). NaN stays.
+// The table's 32 entries are the 64 banks of LDS once each, so lanes read any of them without conflict.
+__device__ __forceinline__ double exp_of(double x, const double* table) {
+  constexpr double ROUND = 0x1.8p52, C = 0x1.71547652b82fep5;  // a sum with ROUND is a whole number in its low bits
+  const double k = __builtin_fma(x, C, ROUND), f = __builtin_fma(x, C, -(k - ROUND));
+  const int n = (int)__builtin_bit_cast(uint64_t, k);
+  const uint64_t at = __builtin_bit_cast(uint64_t, table[n & 31]) + ((uint64_t)(uint32_t)((n >> 5) << 20) << 32);
+  double p = __builtin_fma(f, 0x1.3b2b13640caa1p-27, 0x1.c6b167e0c48a8p-20);
+  p = __builtin_fma(f, p, 0x1.ebfbdff8198e6p-13);
+  p = __builtin_fma(f, p, 0x1.62e42fef6d05bp-6);
+  p = __builtin_fma(f, p, 1.0);
+  return p * __builtin_bit_cast(double, at);
 }
-constexpr float WITHIN = 600.f, LEAST = -740.f;  // parts whose maximum is within +-WITHIN; logits below LEAST add nothing
+constexpr float WITHIN = 600.f, LEAST = -700.f;  // parts whose maximum is within +-WITHIN; logits below LEAST add nothing
 
 template <typename T>
 __global__ __launch_bounds__(PART_WAVES * 64) void beam_part_kernel(Beam a) {
@@ -101,9 +102,12 @@ __global__ __launch_bounds__(PART_WAVES * 64) void beam_part_kernel(Beam a) {
   typedef T Vec __attribute__((ext_vector_type(E)));
   __shared__ uint64_t lists[PART_WAVES][MOST_BEAMS];
   __shared__ double sums[PART_WAVES];
-  __shared__ float tops[PART_WAVES];
+  __shared__ float tops[PART_WAVES], bars[PART_WAVES], mosts[PIECES][PART_WAVES * 64];
+  __shared__ double table[32];
   const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
   if (a.done && a.done[row]) return;
+  if (threadIdx.x < 32) table[threadIdx.x] = exp2(threadIdx.x / 32.0);
+  __syncthreads();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const T* x = (const T*)a.x + row * a.pitch;
   const int lo = min(part * a.per, a.V), hi = min(a.V, lo + a.per);
@@ -116,7 +120,7 @@ __global__ __launch_bounds__(PART_WAVES * 64) void beam_part_kernel(Beam a) {
   best.clear(a.W);
   auto add = [&](float v, int token) {
     const float y = v < LEAST ? LEAST : v;  // NaN stays
-    sum[token & 1] += exp_of((double)y);
+    sum[token & 1] += exp_of((double)y, table);
   };
   if (wave == 0) {
     const int i = lane < head ? lo + lane : lane >= 32 && tail + lane - 32 < hi ? tail + lane - 32 : -1;
@@ -125,55 +129,48 @@ __global__ __launch_bounds__(PART_WAVES * 64) void beam_part_kernel(Beam a) {
     top = fmaxf(top, v);
     best.add(i >= 0 && v == v ? rank_of(v, i) : 0);
   }
-  // the list's last as a logit: later pieces hold later tokens, so they have to pass it (the odd ones before and
-  // behind do not count: they are of any place)
+  // Each piece's maximum waits in LDS for the bar.
   const Vec* from = reinterpret_cast<const Vec*>(x + lo + head);
-  bool begun = false;
-  for (int b0 = wave * 64; b0 < pieces; b0 += U * PART_WAVES * 64) {
+  float lane_most = -INFINITY;
+  auto place = [&](int n) { return (n * PART_WAVES + wave) * 64 + lane; };  // this lane's n-th piece
+  const int mine = pieces > wave * 64 ? (pieces - wave * 64 + PART_WAVES * 64 - 1) / (PART_WAVES * 64) : 0;
+  for (int n0 = 0; n0 < mine; n0 += U) {
     Vec now[U];
-    bool there[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) now[u] = __builtin_nontemporal_load(from + min(place(n0 + u), pieces - 1));
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = b0 + u * PART_WAVES * 64 + lane;
-      there[u] = i < pieces;
-      now[u] = __builtin_nontemporal_load(from + min(i, pieces - 1));
-    }
-    float most[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      most[u] = -INFINITY;
-      if (there[u]) {
-        const int i = lo + head + (b0 + u * PART_WAVES * 64 + lane) * E;
+      float most = -INFINITY;
+      if (place(n0 + u) < pieces)
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           add((float)now[u][e], e);
-          most[u] = fmaxf(most[u], (float)now[u][e]);
+          most = fmaxf(most, (float)now[u][e]);
         }
-      }
-      top = fmaxf(top, most[u]);
+      if (n0 + u < mine) mosts[n0 + u][threadIdx.x] = most;
+      lane_most = fmaxf(lane_most, most);
     }
-    if (!begun) {
-      begun = true;
-      float lane_most = most[0];
+  }
+  top = fmaxf(top, lane_most);
+  for (int w = 0; w < a.W; ++w) {
+    bar = wave_max(lane_most);
+    const uint64_t who = __ballot(lane_most == bar);
+    if (lane == __builtin_ctzll(who)) lane_most = -INFINITY;
+  }
+  if (lane == 0) bars[wave] = bar;
+  __syncthreads();
 #pragma unroll
-      for (int u = 1; u < U; ++u) lane_most = fmaxf(lane_most, most[u]);
-      for (int w = 0; w < a.W; ++w) {
-        bar = wave_max(lane_most);
-        const uint64_t who = __ballot(lane_most == bar);
-        if (who && lane == __builtin_ctzll(who)) lane_most = -INFINITY;
-      }
-    }
+  for (int w = 0; w < PART_WAVES; ++w) bar = fmaxf(bar, bars[w]);
+  for (int n = 0; n < mine; ++n) {
+    const bool here = mosts[n][threadIdx.x] >= bar && place(n) < pieces;
+    if (!__any(here)) continue;
+    const Vec now = from[min(place(n), pieces - 1)];
+    const int i = lo + head + place(n) * E;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (!__any(there[u] && most[u] >= bar)) continue;
-      const int i = lo + head + (b0 + u * PART_WAVES * 64 + lane) * E;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float v = (float)now[u][e];
-        const bool may = there[u] && v >= bar;
-        if (__any(may)) best.add(may ? rank_of(v, i + e) : 0);
-      }
-      if (best.least) bar = fmaxf(bar, logit_of(best.least));
+    for (int e = 0; e < E; ++e) {
+      const float v = (float)now[e];
+      const bool may = here && v >= bar;
+      if (__any(may)) best.add(may ? rank_of(v, i + e) : 0);
     }
   }
 #pragma unroll
@@ -208,13 +205,13 @@ __global__ __launch_bounds__(PART_WAVES * 64) void beam_part_kernel(Beam a) {
 
 // One request: each beam's parts joined, then the beams. Candidates are in order of (score, beam, place in the
 // beam's order), and a candidate's place among all is the number of those before it, beam by beam.
-__global__ __launch_bounds__(256) void beam_join_kernel(Beam a) {
+__global__ __launch_bounds__(1024) void beam_join_kernel(Beam a) {
   extern __shared__ unsigned char lds[];
   double* keys = reinterpret_cast<double*>(lds);             // [W][W]
   int* toks = reinterpret_cast<int*>(keys + a.W * a.W);      // [W][W]
   int* counts = toks + a.W * a.W;                            // [W]: a beam's candidates
   const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, W = a.W, most = min(W, a.V);
-  for (int w = wave; w < W; w += 4) {
+  for (int w = wave; w < W; w += blockDim.x >> 6) {
     const int row = b * W + w;
     const double score = (double)a.scores[row];
     double key = -INFINITY;
@@ -262,7 +259,7 @@ __global__ __launch_bounds__(256) void beam_join_kernel(Beam a) {
     if (lane == 0) counts[w] = __builtin_popcountll(real);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < W * W; i += 256) {
+  for (int i = threadIdx.x; i < W * W; i += blockDim.x) {
     const int own = i / W, nth = i - own * W;
     if (nth >= counts[own]) continue;
     const double key = keys[i];
@@ -288,20 +285,22 @@ __global__ __launch_bounds__(256) void beam_join_kernel(Beam a) {
   }
 }
 
-// The parts of a beam: enough workgroups for the GPU, of at least 1024 tokens each.
-static int64_t parts_of(int64_t rows, int64_t V) {
-  const int64_t want = (2048 + rows - 1) / rows, most = (V + 1023) / 1024;
-  const int64_t parts = want < most ? want : most;
-  return parts < 1 ? 1 : parts;
+// The parts of a beam: enough workgroups for all CUs at once (8 a CU; twice as many or half measure within 2 %, four
+// times as many 10 % more), of at least 2048 tokens each (1024: 5 beams of 7 requests, 50001 tokens 18.8 us for 16.9),
+// and as few as a part has room for (16 logits less than it has, for a row that starts anywhere).
+static int64_t parts_of(int type, int64_t rows, int64_t V) {
+  const int64_t want = (2048 + rows - 1) / rows, most = (V + 2047) / 2048, room = PART_BYTES / (type == 0 ? 4 : 2) - 16;
+  const int64_t least = (V + room - 1) / room, parts = want < most ? want : most;
+  return parts < least ? least : parts;
 }
 
 }  // namespace bq
 
 using namespace bq;
 
-size_t bq_beam_select_ws_bytes(int64_t B, int64_t W, int64_t V) {
+size_t bq_beam_select_ws_bytes(int type, int64_t B, int64_t W, int64_t V) {
   if (B < 1 || W < 1 || W > MOST_BEAMS || V < 1) return 0;
-  return (size_t)(B * W * parts_of(B * W, V)) * (16 + 8 * W);
+  return (size_t)(B * W * parts_of(type, B * W, V)) * (16 + 8 * W);
 }
 
 int bq_beam_select(const void* logits, int type, int64_t B, int64_t W, int64_t V, int64_t pitch, const float* scores,
@@ -314,8 +313,9 @@ int bq_beam_select(const void* logits, int type, int64_t B, int64_t W, int64_t V
   if (V > 0x7fffffff - 8192 || B > 0x7fffff) return set_error(BQ_ERR_ARG, "%s: size too large", what);
   if (done && (end < 0 || end > 0x7fffffff)) return set_error(BQ_ERR_ARG, "%s: end token %lld", what, (long long)end);
   if (B == 0) return BQ_OK;
+  if (parts_of(type, B * W, V) > 0x7fffffff / (B * W)) return set_error(BQ_ERR_ARG, "%s: size too large", what);
   if (!logits || !scores || !out || !parents || !tokens) return set_error(BQ_ERR_ARG, "%s: null pointer", what);
-  const size_t need = bq_beam_select_ws_bytes(B, W, V);
+  const size_t need = bq_beam_select_ws_bytes(type, B, W, V);
   if (!ws || ws_bytes < need || ((uintptr_t)ws & 15))
     return set_error(BQ_ERR_ARG, "%s: a workspace of %zu bytes, given %zu", what, need, ws ? ws_bytes : 0);
   Beam a;
@@ -327,7 +327,7 @@ int bq_beam_select(const void* logits, int type, int64_t B, int64_t W, int64_t V
   a.W = (int)W;
   a.V = (int)V;
   a.end = end < 0 || end > 0x7fffffff ? -1 : (int)end;
-  a.parts = (int)parts_of(B * W, V);
+  a.parts = (int)parts_of(type, B * W, V);
   a.per = (int)((V + a.parts - 1) / a.parts);
   a.sums = (double2*)ws;
   a.best = (uint64_t*)(a.sums + B * W * a.parts);
@@ -340,6 +340,6 @@ int bq_beam_select(const void* logits, int type, int64_t B, int64_t W, int64_t V
   if (type == 0) beam_part_kernel<float><<<grid, PART_WAVES * 64, 0, st>>>(a);
   else if (type == 1) beam_part_kernel<__bf16><<<grid, PART_WAVES * 64, 0, st>>>(a);
   else beam_part_kernel<_Float16><<<grid, PART_WAVES * 64, 0, st>>>(a);
-  beam_join_kernel<<<(unsigned)B, 256, (size_t)W * W * 12 + W * 4, st>>>(a);
+  beam_join_kernel<<<(unsigned)B, 64 * (W < 16 ? (int)W : 16), (size_t)W * W * 12 + W * 4, st>>>(a);
   return check_launch(what);
 }

@@ -629,9 +629,9 @@ int bq_kv4_copy_pages(const bq_kv4_cache* caches, int64_t count, const int32_t* 
  * the tokens.
  *   out f32 [B, W]: the scores in order; parents i32 [B, W]: their beams, as b W + w; tokens i32 [B, W];
  *   ended u8 [B, W] (nullable): the beam was done or the token is `end`
- * W <= 64. None of the outputs is an input. The logits are read once (twice where they do not fit, from cache);
+ * W <= 64. None of the outputs is an input. The logits are read once (what may hold a candidate twice, from cache);
  * no atomics. ws: bq_beam_select_ws_bytes bytes, 16-byte aligned, need not be cleared. */
-size_t bq_beam_select_ws_bytes(int64_t B, int64_t W, int64_t V);
+size_t bq_beam_select_ws_bytes(int type, int64_t B, int64_t W, int64_t V);
 int bq_beam_select(const void* logits, int type, int64_t B, int64_t W, int64_t V, int64_t pitch, const float* scores,
                    const uint8_t* done, int64_t end, float* out, int32_t* parents, int32_t* tokens, uint8_t* ended,
                    void* ws, size_t ws_bytes, bq_stream_t stream);

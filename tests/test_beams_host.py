@@ -12,7 +12,7 @@ ARG, UNSUPPORTED = _lib.BQ_ERR_ARG, _lib.BQ_ERR_UNSUPPORTED
 
 def test_select_refusals():
     lib = _lib.lib()
-    need = lib.bq_beam_select_ws_bytes(2, 3, 40)
+    need = lib.bq_beam_select_ws_bytes(0, 2, 3, 40)
     assert need > 0
 
     def call(x=16, type=0, B=2, W=3, V=40, scores=16, done=None, end=-1, out=16, parents=16, tokens=16, ws=16, size=need):
@@ -20,13 +20,13 @@ def test_select_refusals():
 
     assert call(type=3) == ARG and call(B=-1) == ARG and call(W=0) == ARG and call(V=0) == ARG
     assert call(W=65) == UNSUPPORTED and "64" in _lib.last_error()
-    assert call(V=2 ** 31) == ARG and call(B=2 ** 24) == ARG
+    assert call(V=2 ** 31) == ARG and call(B=2 ** 24) == ARG and call(B=2 ** 22, W=64, V=10 ** 6) == ARG
     assert call(done=16) == ARG and "end token" in _lib.last_error()
     assert call(B=0, x=None) == 0
     for name in ("x", "scores", "out", "parents", "tokens"):
         assert call(**{name: None}) == ARG and "null" in _lib.last_error()
     assert call(ws=None) == ARG and call(size=need - 1) == ARG and call(ws=24) == ARG
-    assert lib.bq_beam_select_ws_bytes(0, 3, 40) == 0 == lib.bq_beam_select_ws_bytes(1, 65, 40)
+    assert lib.bq_beam_select_ws_bytes(0, 0, 3, 40) == 0 == lib.bq_beam_select_ws_bytes(0, 1, 65, 40)
 
 
 def test_cpu_tensors_are_refused():
