@@ -132,7 +132,7 @@ SIGNATURES = {
     "bq_kv4_attend_ws_bytes": (_c_size, [*[_c_i64] * 5, _c_int]),
     "bq_kv4_attend": (_c_int, [_c_p, _c_p, _c_int, *[_c_i64] * 5, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_f, _c_p,
                                _c_p, _c_i64, _c_i64, _c_p, _c_size, _c_p]),
-    "bq_kv4_attend_chunk_ws_bytes": (_c_size, [_c_int, *[_c_i64] * 6]),
+    "bq_kv4_attend_chunk_ws_bytes": (_c_size, [_c_int, *[_c_i64] * 7]),
     "bq_kv4_attend_chunk": (_c_int, [_c_p, _c_p, _c_int, *[_c_i64] * 4, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_f,
                                      _c_p, _c_p, _c_size, _c_p]),
     "bq_beam_select_ws_bytes": (_c_size, [_c_int, *[_c_i64] * 3]),

@@ -5,25 +5,32 @@
 // tokens: row i is token lens[b] - cu[b + 1] + i and sees the tokens up to itself,
 // out = sum_i p_i v_i with p = softmax(scale q . k_i), zeros where it sees nothing.
 //
-// One pass over the keys with each row's running maximum and sum. The G = q_heads / heads query heads
-// of a key-value head and the chunk's tokens are the rows of one product (row t G + j: token t, head j),
-// so that the codes are expanded once for all that read them. A workgroup of four waves takes a tile of
-// 128 rows, 32 a wave, and 64 keys at a time: the codes, loaded one tile ahead, become bf16 exactly (a
-// code has 2 significant bits, bf16 the exponents of f32) in LDS, two tiles in turn, one barrier a tile.
-// The scores are taken transposed, S^T = k q^T on the 32 x 32 x 16 MFMA, keys in an order (bits 2 and 3 of
-// their number exchanged) that leaves 8 following tokens in 8 following registers of a lane: the
-// exponentials are, register for register, the second operand of O^T = v^T p^T. q enters as the exact sum of
-// bf16 pieces (f32: 3, f16: 2, bf16: 1), p as pieces too (f32: 3, f16: 2, so that p's error is 2^-17 where
-// the output's rounding is 2^-12; bf16: 1, half a step of 2^-8 on each term as the output), with f32
-// accumulation. Tiles of up to 64 rows give two waves the halves of each 64 keys for the same rows; of up
-// to 32, where a product is small beside the reading, each wave takes every fourth 32 keys by itself,
-// without barriers. Such waves are joined in LDS at the end.
+// One pass over the keys with each row's running maximum and sum. The G = q_heads / heads query heads of a key-value
+// head and the chunk's tokens are the rows of one product (row t G + j: token t, head j), so that the codes are
+// expanded once for all that read them. The codes become bf16 exactly (a code has 2 significant bits, bf16 the
+// exponents of f32). q enters as the exact sum of bf16 pieces (f32: 3, f16: 2, bf16: 1), the weights p as pieces too
+// (f32: 3; f16: 2, so that p's error is 2^-17 where the output's rounding is 2^-12; bf16: 1, half a step of 2^-8 on
+// each term as the output), with f32 accumulation; the sum of the weights is of those before they are rounded. The
+// scores are taken transposed, S^T = k q^T on the 32 x 32 x 16 MFMA, keys in an order (bits 2 and 3 of their number
+// exchanged) that leaves 8 following tokens in 8 following registers of a lane: the exponentials are, register for
+// register, the second operand of O^T = v^T p^T.
 //
-// The maximum that is subtracted lags by up to 2^8 (the weights' own size cancels in the quotient) and is
-// a whole number of powers of two, so that a weight is one FMA and one exp2 and all of a row's agree.
+// Wide tiles, of sequences of many rows: a workgroup of four waves takes 128 rows, 32 a wave, and 64 keys at a time,
+// whose codes, loaded one tile ahead, are expanded into LDS, two tiles in turn, one barrier a tile. Bound by the
+// matrix units beside the exponentials and the expansion: 2048 tokens over 16384, 32 heads over 8 of 128, bf16:
+// 560 us, 917 TFLOP/s; 8192 over 8192 567 us, 969 (a plain loop of the MFMA: 2011). f16 473 and f32 372, at 1.5 and 3
+// times the products. Each wave expanding for itself would cost four times the conversions; 64 rows a workgroup twice.
 //
-// A tile's keys are cut into shares of up to `upper` units of 64 where the tiles alone would leave the GPU
-// part empty; a second kernel joins the shares of a row.
+// Narrow tiles, of sequences of few rows, where a product is small beside the reading: 32 rows, of which each wave
+// takes every fourth 32 keys by itself, from memory into operands, joined in LDS at the end. Bound by the reading:
+// 64 sequences of 4000 tokens and one new, bf16: 60 us, 4.6 TB/s (read alone: 7.0); 512 of 1000: 177 us, 3.2 TB/s,
+// where finding the tile, the first loads and the join are a third of a workgroup's time.
+//
+// The maximum that is subtracted lags by up to 2^8 (the weights' own size cancels in the quotient) and is a whole
+// number of powers of two, so that a weight is one FMA and one exp2 and all of a row's agree.
+//
+// A tile's keys are cut into shares of up to `upper` units of 64 where the tiles alone would leave the GPU part empty;
+// a second kernel joins the shares of a row.
 #include "bq_dma.h"
 #include "bq_kv4_pieces.h"
 
@@ -56,25 +63,50 @@ struct Place {
   int base, len;             // the place in the cache of the sequence's first new token, and its tokens
 };
 
-// Tile `place` of what lies before cu[0], of each sequence in turn, or of what lies past the last: of those that
-// tiles of TILE rows take.
+// The tiles of TILE rows of what lies before cu[0] (i = 0), of sequence i - 1, or of what lies past the last: of those
+// that take such tiles.
 template <int TILE>
-__device__ __forceinline__ bool place_of(const Chunk& a, int place, Place* out) {
-  const int lane = threadIdx.x & 63;
-  for (int at = 0; at < a.B + 2; at += 64) {
-    const int i = at + lane;
-    int s = 0, e = 0;
-    if (i <= a.B + 1) {
-      s = i == 0 ? 0 : min(max(a.cu[i - 1], 0), a.n);
-      e = i == a.B + 1 ? a.n : min(max(a.cu[i], 0), a.n);
-    }
-    const int rows = max(0, e - s) * a.group, mine = (rows > a.least) == (TILE == WIDE) ? (rows + TILE - 1) / TILE : 0;
-    int upto = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int y = __shfl_up(upto, d);
-      if (lane >= d) upto += y;
-    }
+__device__ __forceinline__ int tiles_of(const Chunk& a, int i, int* s, int* rows) {
+  if (i > a.B + 1) return 0;
+  *s = i == 0 ? 0 : min(max(a.cu[i - 1], 0), a.n);
+  const int e = i == a.B + 1 ? a.n : min(max(a.cu[i], 0), a.n);
+  *rows = max(0, e - *s) * a.group;
+  return (*rows > a.least) == (TILE == WIDE) ? (*rows + TILE - 1) / TILE : 0;
+}
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ int plus_lanes(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CONTROL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_upto(int v) {  // the lanes' values up to this one's own
+  v = plus_lanes<0x111, 0xF>(v);  // from the lanes 1, 2, 4 and 8 before in a row of 16,
+  v = plus_lanes<0x112, 0xF>(v);
+  v = plus_lanes<0x114, 0xF>(v);
+  v = plus_lanes<0x118, 0xF>(v);
+  v = plus_lanes<0x142, 0xA>(v);  // the last of the row before into the second and fourth,
+  return plus_lanes<0x143, 0xC>(v);  // lane 31's into the upper half
+}
+// Tile `last` from the last one on. A lane sums some sequences first, where there are more than lanes: one after
+// another 64 at a time, each waited for the loads of those before.
+template <int TILE>
+__device__ __forceinline__ bool place_of(const Chunk& a, int last, Place* out) {
+  const int lane = threadIdx.x & 63, each = (a.B + 2 + 63) >> 6;
+  int from = 0, place = 0, s = 0, rows = 0;
+  if (each > 1) {
+    int mine = 0;
+#pragma unroll 4
+    for (int i = 0; i < each; ++i) mine += tiles_of<TILE>(a, lane * each + i, &s, &rows);
+    const int upto = wave_upto(mine);
+    place = __builtin_amdgcn_readlane(upto, 63) - 1 - last;
+    if (place < 0) return false;
+    const int l = __builtin_ctzll(__ballot(upto > place));
+    place -= __builtin_amdgcn_readlane(upto - mine, l);
+    from = l * each;
+  }
+  for (int at = from; at < (each > 1 ? from + each : 64); at += 64) {
+    s = rows = 0;
+    const int mine = tiles_of<TILE>(a, at + lane, &s, &rows), upto = wave_upto(mine);
+    if (each == 1) place = __builtin_amdgcn_readlane(upto, 63) - 1 - last;
+    if (place < 0) return false;
     const uint64_t hit = __ballot(upto > place);
     if (hit) {
       const int l = __builtin_ctzll(hit), seq = at + l;
@@ -85,7 +117,7 @@ __device__ __forceinline__ bool place_of(const Chunk& a, int place, Place* out) 
       out->rows = __builtin_amdgcn_readlane(rows, l);
       out->row0 = place * TILE;
       out->len = real ? max(0, min(a.lens[seq - 1], a.max_len)) : 0;
-      out->base = real ? a.lens[seq - 1] - (__builtin_amdgcn_readlane(e, l) - out->start) : 0;
+      out->base = real ? a.lens[seq - 1] - fdiv(out->rows, a.by_group.mul, a.by_group.shift) : 0;
       return true;
     }
     place -= __builtin_amdgcn_readlane(upto, 63);
@@ -327,17 +359,8 @@ struct Rows {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_exp2f(__fmaf_rn(s[e / 2][8 * (e % 2) + i], a.scale2, -ref));
     const Pieces<PP> f = pieces_of<PP>(x);
-    if constexpr (PP == 1) {  // of the weights as rounded, two at a time
-      const uint4 w = __builtin_bit_cast(uint4, f.p[0]);
-      const v2bf one = {(__bf16)1.f, (__bf16)1.f};
-      float y = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w.x), one, 0.f, false);
-      y = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w.y), one, y, false);
-      y = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w.z), one, y, false);
-      *sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w.w), one, y, false);
-    } else {
-      *sum = __fadd_rn(__fadd_rn(__fadd_rn(x[0], x[1]), __fadd_rn(x[2], x[3])),
-                       __fadd_rn(__fadd_rn(x[4], x[5]), __fadd_rn(x[6], x[7])));
-    }
+    *sum = __fadd_rn(__fadd_rn(__fadd_rn(x[0], x[1]), __fadd_rn(x[2], x[3])),
+                     __fadd_rn(__fadd_rn(x[4], x[5]), __fadd_rn(x[6], x[7])));
     return f;
   }
 
@@ -442,7 +465,7 @@ __device__ __forceinline__ bool job_of(const Chunk& a, int id, Place* at, int* h
   *h = id % a.c.heads;
   const int rest = id / a.c.heads;
   *share = rest % kind.most;
-  if (!place_of<TILE>(a, kind.tiles - 1 - rest / kind.most, at)) return false;
+  if (!place_of<TILE>(a, rest / kind.most, at)) return false;
   const int units = units_of<TILE>(a, *at, at->row0);
   *shares = shares_of(kind.upper, units);
   if (*share >= *shares) return false;
@@ -700,20 +723,15 @@ __device__ __forceinline__ void narrow_tile(const Chunk& a, int id, float* all) 
   r.store(a, at, h, share, shares);
 }
 
-// Both in one launch, the wide tiles first.
-template <typename T, int DIM, bool WIDES, bool FEWS>
+// Both in one launch, the wide tiles first; or narrow ones alone, with less LDS and fewer registers.
+template <typename T, int DIM, bool WIDES>
 __global__ __launch_bounds__(256, 2) void kv4_chunk_kernel(Chunk a) {
   constexpr int BYTES = WIDES ? 4 * KEYS * DIM * 2 : 3 * (DIM / 2 + 2) * 256;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[BYTES];
   const int wides = a.wide.tiles * a.wide.most * a.c.heads;
-  if constexpr (WIDES && FEWS) {
-    if ((int)blockIdx.x < wides) wide_tile<T, DIM>(a, blockIdx.x, lds);
-    else narrow_tile<T, DIM>(a, blockIdx.x - wides, reinterpret_cast<float*>(lds));
-  } else if constexpr (WIDES) {
-    wide_tile<T, DIM>(a, blockIdx.x, lds);
-  } else {
-    narrow_tile<T, DIM>(a, blockIdx.x, reinterpret_cast<float*>(lds));
-  }
+  if constexpr (WIDES)
+    if ((int)blockIdx.x < wides) return wide_tile<T, DIM>(a, blockIdx.x, lds);
+  narrow_tile<T, DIM>(a, blockIdx.x - wides, reinterpret_cast<float*>(lds));
 }
 
 // The shares of each row joined: a wave a row and head.
@@ -782,26 +800,35 @@ __global__ __launch_bounds__(256) void kv4_chunk_join_kernel(Chunk a) {
 
 // How the work is cut, whatever the lengths are.
 //
-// A sequence takes wide tiles from more than FEW_ROWS rows on, of which there are then few that are mostly empty; a
-// call of up to FEW_ALL rows takes narrow tiles alone, and one launch.
+// A sequence takes wide tiles from more than FEW_ROWS rows on (32 sequences of 48 rows beside it, of 3000 tokens: 65 us
+// so, 93 in wide tiles; of 128 rows: 98 in wide tiles, 120 in narrow ones); a call of up to FEW_ALL rows takes narrow
+// tiles alone, for more workgroups (those 48 rows, 1536 in all: 42 us; but 4096 rows so 132 us for 96).
 //
-// Of the shares that a tile may be cut in that number is taken for which the workgroups that run at once, all as
-// long as the longest sequence makes them, and what the join writes and reads cost least. (Taking sequences to
-// be half as long on average cut 64 equal ones of 4000 tokens too often: 62 -> 188 us.)
-constexpr int64_t FEW_ROWS = 64, FEW_ALL = 512;
+// Of the shares that a tile may be cut in that number is taken for which the estimated time is least: of the longest
+// workgroup, of all the work over the workgroups that run at once and the longest begun last, or of whole rounds of
+// equal ones; the workgroups that find no tile; and what the join writes and reads. Narrow tiles' usual length is what
+// the cache's pages hold for each sequence: with the longest sequence's for all, one chunk of 1024 tokens beside 511
+// sequences of one over 1000 took 866 us, so 248.
+constexpr int64_t FEW_ROWS = 64, FEW_ALL = 2048;
+constexpr double FEW_UNIT_US = 1.2, NONE_US = 1.5;  // a unit of a narrow tile's; a workgroup that finds no tile
 struct Cut {
   Chunk::Kind wide, few;
   int64_t least;
 };
-static Chunk::Kind kind_of(int64_t most_tiles, int64_t tiles, int64_t heads, int64_t units, int64_t at_once, double unit_us,
-                           double share_us) {
+static Chunk::Kind kind_of(int64_t most_tiles, int64_t tiles, int64_t heads, int64_t units, double usual, int64_t at_once,
+                           double unit_us, double share_us) {
   Chunk::Kind k = {(int)most_tiles, (int)units, 1};
   double least = 0.0;
   if (tiles < 1) tiles = 1;
   for (int64_t m = 1; m <= 128 && m <= units; ++m) {
-    const int64_t all = tiles * heads * m, each = (units + m - 1) / m;
-    const double rounds = all <= at_once ? 1.0 : (double)all / at_once + 1.0;
-    const double us = rounds * each * unit_us + (m > 1 ? 4.0 + m * share_us : 0.0);
+    const int64_t all = tiles * heads * m, each = (units + m - 1) / m, none = most_tiles * heads * m - all;
+    double length = (double)each;
+    if (all > at_once) {
+      const double work = tiles * heads * usual / at_once + each * (1.0 - (double)at_once / all);
+      const double rounds = (all + at_once - 1) / at_once * usual / m;
+      length = fmax(length, fmax(work, rounds));
+    }
+    const double us = length * unit_us + (none > 0 ? NONE_US * none / at_once : 0.0) + (m > 1 ? 4.0 + m * share_us : 0.0);
     if (m == 1 || us < least) {
       least = us;
       k.upper = (int)each;
@@ -810,23 +837,24 @@ static Chunk::Kind kind_of(int64_t most_tiles, int64_t tiles, int64_t heads, int
   }
   return k;
 }
-static Cut cut_of(int type, int64_t n, int64_t B, int64_t heads, int64_t group, int64_t dim, int64_t max_len) {
+static Cut cut_of(int type, int64_t n, int64_t B, int64_t heads, int64_t group, int64_t dim, int64_t max_len, int64_t tokens) {
   const int64_t units = max_len > 0 ? (max_len + KEYS - 1) / KEYS : 1, begun = B + 2 < n ? B + 2 : n, rows = n * group;
   const double share_us = (double)rows * heads * (2 * 4 * (dim + 2)) / 4e6;  // of all rows, written and read at 4 TB/s
   // workgroups that run at once (two a CU, three where the registers allow), and a unit's time in one of them then
   const int64_t at_once = dim == 64 && type ? 768 : 512;
   const double unit_us = dim == 64 ? (type == 0 ? 3.3 : type == 1 ? 2.0 : 2.4) : type == 0 ? 5.5 : type == 1 ? 2.3 : 3.7;
-  constexpr double FEW_UNIT_US = 2.0;
+  const double mean = B < 1 ? 1.0 : (double)tokens / KEYS / B, usual = mean < units ? mean : (double)units;
   Cut c;
   c.least = rows <= FEW_ALL ? 0x7fffffff : FEW_ROWS;
   if (rows <= FEW_ALL) {
     const int64_t tiles = (rows + FEW - 1) / FEW, some = B < n ? B : n;
     c.wide = {0, 1, 1};
-    c.few = kind_of(rows / FEW + begun, tiles > some ? tiles : some, heads, units, at_once, FEW_UNIT_US, share_us);
+    c.few = kind_of(rows / FEW + begun, tiles > some ? tiles : some, heads, units, usual, at_once, FEW_UNIT_US, share_us);
   } else {
     const int64_t many = rows / (FEW_ROWS + 1);  // sequences of more rows at most
-    c.wide = kind_of(rows / WIDE + (begun < many ? begun : many), rows / WIDE, heads, units, at_once, unit_us, share_us);
-    c.few = kind_of(begun * (FEW_ROWS / FEW), B < 1 ? 1 : B, heads, units, at_once, FEW_UNIT_US, share_us);
+    c.wide = kind_of(rows / WIDE + (begun < many ? begun : many), rows / WIDE, heads, units, (double)units, at_once, unit_us, share_us);
+    const int64_t full = rows / FEW + begun, two = begun * (FEW_ROWS / FEW);
+    c.few = kind_of(full < two ? full : two, B < 1 ? 1 : B, heads, units, usual, at_once, FEW_UNIT_US, share_us);
   }
   return c;
 }
@@ -834,8 +862,8 @@ static Cut cut_of(int type, int64_t n, int64_t B, int64_t heads, int64_t group, 
 template <typename T, int DIM>
 static int launch(const char* what, const Chunk& a, hipStream_t st) {
   auto grid = [&](const Chunk::Kind& k) { return (unsigned)((int64_t)k.tiles * k.most * a.c.heads); };
-  if (a.wide.tiles) kv4_chunk_kernel<T, DIM, true, true><<<grid(a.wide) + grid(a.few), 256, 0, st>>>(a);
-  else kv4_chunk_kernel<T, DIM, false, true><<<grid(a.few), 256, 0, st>>>(a);
+  if (a.wide.tiles) kv4_chunk_kernel<T, DIM, true><<<grid(a.wide) + grid(a.few), 256, 0, st>>>(a);
+  else kv4_chunk_kernel<T, DIM, false><<<grid(a.few), 256, 0, st>>>(a);
   if (a.wide.most > 1 || a.few.most > 1) {
     const int64_t rows = (int64_t)a.n * a.c.heads * a.group;
     kv4_chunk_join_kernel<T, DIM><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(a);
@@ -848,9 +876,9 @@ static int launch(const char* what, const Chunk& a, hipStream_t st) {
 using namespace bq;
 
 size_t bq_kv4_attend_chunk_ws_bytes(int type, int64_t n, int64_t B, int64_t q_heads, int64_t heads, int64_t dim,
-                                    int64_t max_len) {
-  if (n < 1 || B < 0 || heads < 1 || q_heads < heads || dim < 1 || max_len < 0) return 0;
-  const Cut c = cut_of(type, n, B, heads, q_heads / heads, dim, max_len);
+                                    int64_t max_len, int64_t tokens) {
+  if (n < 1 || B < 0 || heads < 1 || q_heads < heads || dim < 1 || max_len < 0 || tokens < 0) return 0;
+  const Cut c = cut_of(type, n, B, heads, q_heads / heads, dim, max_len, tokens);
   const int most = c.wide.most > c.few.most ? c.wide.most : c.few.most;
   return most > 1 ? (size_t)n * q_heads * most * (dim + 2) * 4 : 0;
 }
@@ -872,7 +900,7 @@ int bq_kv4_attend_chunk(const bq_kv4_cache* cache, const void* q, int type, int6
   if (n == 0) return BQ_OK;
   const int64_t group = q_heads / cache->heads;
   if (n * group > 0x7fffffff - 8192) return set_error(BQ_ERR_ARG, "%s: size too large", what);
-  const Cut cut = cut_of(type, n, B, cache->heads, group, cache->dim, max_len);
+  const Cut cut = cut_of(type, n, B, cache->heads, group, cache->dim, max_len, cache->pages * cache->page);
   auto grid = [&](const Chunk::Kind& k) { return (int64_t)k.tiles * k.most * cache->heads; };
   if (grid(cut.wide) + grid(cut.few) > 0x7fffffff || n * q_heads > 0x7fffffffll * 4)
     return set_error(BQ_ERR_ARG, "%s: size too large", what);
@@ -880,7 +908,8 @@ int bq_kv4_attend_chunk(const bq_kv4_cache* cache, const void* q, int type, int6
   const int64_t size = type == KV4_F32 ? 4 : 2;
   if ((((uintptr_t)q | (uintptr_t)out) & 15) || (q_token | q_head) * size % 16)
     return set_error(BQ_ERR_ARG, "%s: rows that are not 16-byte aligned", what);
-  const size_t need = bq_kv4_attend_chunk_ws_bytes(type, n, B, q_heads, cache->heads, cache->dim, max_len);
+  const size_t need = bq_kv4_attend_chunk_ws_bytes(type, n, B, q_heads, cache->heads, cache->dim, max_len,
+                                                   cache->pages * cache->page);
   if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
     return set_error(BQ_ERR_ARG, "%s: a workspace of %zu bytes, given %zu", what, need, ws ? ws_bytes : 0);
   const int64_t held = cache->pages ? width * cache->page : 0;  // tokens that a sequence's pages have room for

@@ -214,7 +214,7 @@ class Cache4:
         if n == 0:
             return out
         q, qs = rows(q, code)
-        need = _chunk_ws_bytes(code, n, B, hq, self.heads, dim, max_len)
+        need = _chunk_ws_bytes(code, n, B, hq, self.heads, dim, max_len, self.pages * self.page)
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         with on(self._index):
             check(lib().bq_kv4_attend_chunk(self._ref, q.data_ptr(), code, n, hq, *qs, table.data_ptr(), B, width,

@@ -550,9 +550,9 @@ int bq_kv4_attend(const bq_kv4_cache* cache, const void* q, int type, int64_t to
                   int64_t max_len, float scale, void* out, float* weights, int64_t w_seq, int64_t w_head, void* ws,
                   size_t ws_bytes, bq_stream_t stream);
 
-/* Workspace bytes of bq_kv4_attend_chunk (0 where the work is not cut). */
+/* Workspace bytes of bq_kv4_attend_chunk (0 where the work is not cut). tokens: of the whole cache, pages * page. */
 size_t bq_kv4_attend_chunk_ws_bytes(int type, int64_t n, int64_t B, int64_t q_heads, int64_t heads, int64_t dim,
-                                    int64_t max_len);
+                                    int64_t max_len, int64_t tokens);
 
 /* Attention of chunks of new tokens over the cache: q [n, q_heads, dim], sequence b's the rows cu[b] ..
  * cu[b + 1] - 1 (cu i32 [B + 1], ascending), the last ones of its lens[b] cached tokens (lens counts them):

@@ -37,12 +37,13 @@ def test_chunk_refusals():
     assert call(q=24) == ARG and call(out=8) == ARG and "aligned" in _lib.last_error()
     assert call(strides=(255, 64)) == ARG and call(type=1, strides=(256, 68)) == ARG
     assert call(n=2 ** 30, hq=64) == ARG and "large" in _lib.last_error()
-    need = lib.bq_kv4_attend_chunk_ws_bytes(0, 3, 1, 4, 2, 64, 100000)
+    tokens = full.pages * full.page
+    need = lib.bq_kv4_attend_chunk_ws_bytes(0, 3, 1, 4, 2, 64, 100000, tokens)
     assert need > 0 and call(max_len=100000, width=4000) == ARG and "workspace" in _lib.last_error()
     assert call(max_len=100000, width=4000, ws=16, ws_bytes=need - 1) == ARG
     assert call(max_len=100000, width=4000, ws=24, ws_bytes=need) == ARG
-    assert lib.bq_kv4_attend_chunk_ws_bytes(0, 3, 1, 4, 2, 64, 100) == 0 == lib.bq_kv4_attend_chunk_ws_bytes(0, 0, 1, 4, 2, 64, 10 ** 6)
-    assert lib.bq_kv4_attend_chunk_ws_bytes(0, 3, 1, 1, 2, 64, 10 ** 6) == 0
+    assert lib.bq_kv4_attend_chunk_ws_bytes(0, 3, 1, 4, 2, 64, 100, tokens) == 0 == lib.bq_kv4_attend_chunk_ws_bytes(0, 0, 1, 4, 2, 64, 10 ** 6, tokens)
+    assert lib.bq_kv4_attend_chunk_ws_bytes(0, 3, 1, 1, 2, 64, 10 ** 6, tokens) == 0
 
 
 def test_chunk_on_the_cpu():

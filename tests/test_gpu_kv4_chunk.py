@@ -96,6 +96,23 @@ def test_chunk_in_shares(dev, kind, dim, group):
     check(got, q, k[:, :, :2048], v[:, :, :2048], there[:, :2048], ln, cu, 2048, kind, scale=0.3)
 
 
+@pytest.mark.parametrize("count,kind,dim", [(62, "f32", 64), (63, "bf16", 128), (200, "f16", 64), (700, "bf16", 64)])
+def test_chunk_many_sequences(dev, count, kind, dim):
+    """More sequences than lanes, most of them of a token or none, one of many rows and some in between."""
+    print(f"kv4 chunk {count} sequences {kind} dim={dim}", flush=True)
+    lens = [(i * 37) % 71 for i in range(count)]
+    new = [min(n, (i * 5) % 3) for i, n in enumerate(lens)]
+    lens[count // 2], new[count // 2] = 300, 200
+    lens[count - 7], new[count - 7] = 90, 30
+    c, table, ln, _ = filled(dev, lens, 1, dim, 32, 21)
+    cu = starts(new) + 3  # rows of no sequence before the first, and past the last
+    q = queries(sum(new) + 7, 4, dim, kind, 6)
+    k, v, there = held(c, table, ln, 300, dev)
+    got = c.attend_chunk(q.to(dev), table.to(dev), ln.to(dev), cu.to(dev), max_len=300)
+    check(got, q, k, v, there, ln, cu, 300, kind)
+    assert not bool(got[:3].any()) and not bool(got[-4:].any())
+
+
 def test_chunk_rows_of_no_sequence(dev):
     """Rows before the first sequence and past the last one, and rows whose token lies before the cache's
     first: zeros."""
