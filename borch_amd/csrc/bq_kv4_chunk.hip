@@ -18,7 +18,7 @@
 // Wide tiles, of sequences of many rows: a workgroup of four waves takes 128 rows, 32 a wave, and 64 keys at a time,
 // whose codes, loaded one tile ahead, are expanded into LDS, two tiles in turn, one barrier a tile. Bound by the
 // matrix units beside the exponentials and the expansion: 2048 tokens over 16384, 32 heads over 8 of 128, bf16:
-// 560 us, 917 TFLOP/s; 8192 over 8192 567 us, 969 (a plain loop of the MFMA: 2011). f16 473 and f32 372, at 1.5 and 3
+// 531 us, 971 TFLOP/s; 8192 over 8192 553 us, 994 (the library's 8192^3 product: 1426). f16 560 and f32 380, at 2 and 3
 // times the products. Each wave expanding for itself would cost four times the conversions; 64 rows a workgroup twice.
 //
 // Narrow tiles, of sequences of few rows, where a product is small beside the reading: 32 rows, of which each wave
@@ -458,14 +458,15 @@ struct Rows {
 };
 
 // Which tile and share a workgroup has; false: none. Tiles from the last down (those with most keys first), the
-// key-value heads side by side.
+// key-value heads side by side, the shares one after another: side by side, four heads' four shares of which some are
+// none left half of the XCDs idle (f32, 512 rows beside 333 and 500: 146 -> 107 us).
 template <int TILE>
 __device__ __forceinline__ bool job_of(const Chunk& a, int id, Place* at, int* h, int* share, int* shares, int* u0, int* u1) {
   const Chunk::Kind& kind = TILE == WIDE ? a.wide : a.few;
   *h = id % a.c.heads;
   const int rest = id / a.c.heads;
-  *share = rest % kind.most;
-  if (!place_of<TILE>(a, rest / kind.most, at)) return false;
+  *share = rest / kind.tiles;
+  if (!place_of<TILE>(a, rest - *share * kind.tiles, at)) return false;
   const int units = units_of<TILE>(a, *at, at->row0);
   *shares = shares_of(kind.upper, units);
   if (*share >= *shares) return false;
@@ -808,15 +809,18 @@ __global__ __launch_bounds__(256) void kv4_chunk_join_kernel(Chunk a) {
 // workgroup, of all the work over the workgroups that run at once and the longest begun last, or of whole rounds of
 // equal ones; the workgroups that find no tile; and what the join writes and reads. Narrow tiles' usual length is what
 // the cache's pages hold for each sequence: with the longest sequence's for all, one chunk of 1024 tokens beside 511
-// sequences of one over 1000 took 866 us, so 248.
+// sequences of one over 1000 took 866 us, so 240. So are wide tiles' where every sequence may have some (three chunks
+// of 512, 500 and 333 tokens over 4096, 1500 and 777, f32: 130 -> 107 us). Narrow tiles beside wide ones are cut only
+// where they would last longer: the join alone, over all rows, is 15 us of 2048 tokens of 32 heads.
 constexpr int64_t FEW_ROWS = 64, FEW_ALL = 2048;
-constexpr double FEW_UNIT_US = 1.2, NONE_US = 1.5;  // a unit of a narrow tile's; a workgroup that finds no tile
+static_assert(2 * (FEW_ROWS + 1) > WIDE);
+constexpr double FEW_UNIT_US = 1.2, NONE_US = 4.0;  // a unit of a narrow tile's; a workgroup that finds no tile
 struct Cut {
   Chunk::Kind wide, few;
   int64_t least;
 };
 static Chunk::Kind kind_of(int64_t most_tiles, int64_t tiles, int64_t heads, int64_t units, double usual, int64_t at_once,
-                           double unit_us, double share_us) {
+                           double unit_us, double share_us, double* took) {
   Chunk::Kind k = {(int)most_tiles, (int)units, 1};
   double least = 0.0;
   if (tiles < 1) tiles = 1;
@@ -828,13 +832,15 @@ static Chunk::Kind kind_of(int64_t most_tiles, int64_t tiles, int64_t heads, int
       const double rounds = (all + at_once - 1) / at_once * usual / m;
       length = fmax(length, fmax(work, rounds));
     }
-    const double us = length * unit_us + (none > 0 ? NONE_US * none / at_once : 0.0) + (m > 1 ? 4.0 + m * share_us : 0.0);
+    const double us = fmax(length * unit_us + (none > 0 ? NONE_US * none / at_once : 0.0), *took) +
+                      (m > 1 ? 4.0 + m * share_us : 0.0);
     if (m == 1 || us < least) {
       least = us;
       k.upper = (int)each;
       k.most = (int)((units + each - 1) / each);
     }
   }
+  *took = least;
   return k;
 }
 static Cut cut_of(int type, int64_t n, int64_t B, int64_t heads, int64_t group, int64_t dim, int64_t max_len, int64_t tokens) {
@@ -844,17 +850,21 @@ static Cut cut_of(int type, int64_t n, int64_t B, int64_t heads, int64_t group, 
   const int64_t at_once = dim == 64 && type ? 768 : 512;
   const double unit_us = dim == 64 ? (type == 0 ? 3.3 : type == 1 ? 2.0 : 2.4) : type == 0 ? 5.5 : type == 1 ? 2.3 : 3.7;
   const double mean = B < 1 ? 1.0 : (double)tokens / KEYS / B, usual = mean < units ? mean : (double)units;
+  double took = 0.0;  // of the wide tiles, beside which the narrow ones run
   Cut c;
   c.least = rows <= FEW_ALL ? 0x7fffffff : FEW_ROWS;
   if (rows <= FEW_ALL) {
     const int64_t tiles = (rows + FEW - 1) / FEW, some = B < n ? B : n;
     c.wide = {0, 1, 1};
-    c.few = kind_of(rows / FEW + begun, tiles > some ? tiles : some, heads, units, usual, at_once, FEW_UNIT_US, share_us);
+    c.few = kind_of(rows / FEW + begun, tiles > some ? tiles : some, heads, units, usual, at_once, FEW_UNIT_US, share_us, &took);
   } else {
     const int64_t many = rows / (FEW_ROWS + 1);  // sequences of more rows at most
-    c.wide = kind_of(rows / WIDE + (begun < many ? begun : many), rows / WIDE, heads, units, (double)units, at_once, unit_us, share_us);
+    // more than FEW_ROWS rows are at most 2 tiles for every WIDE + 1
+    const int64_t tiles = rows / WIDE + (begun < many ? begun : many), most = 2 * rows / (WIDE + 1);
+    c.wide = kind_of(tiles < most ? tiles : most, rows / WIDE, heads, units, B <= rows / WIDE ? usual : (double)units,
+                     at_once, unit_us, share_us, &took);
     const int64_t full = rows / FEW + begun, two = begun * (FEW_ROWS / FEW);
-    c.few = kind_of(full < two ? full : two, B < 1 ? 1 : B, heads, units, usual, at_once, FEW_UNIT_US, share_us);
+    c.few = kind_of(full < two ? full : two, B < 1 ? 1 : B, heads, units, usual, at_once, FEW_UNIT_US, share_us, &took);
   }
   return c;
 }
