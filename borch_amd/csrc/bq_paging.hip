@@ -7,7 +7,9 @@
 // several times is not written to: a sequence whose last page is partly filled and shared takes one of its own
 // when it grows, and the caller moves the tokens there (bq_kv4_copy_pages).
 //
-// All of this is latency: the tables of a few hundred sequences are some 100 KB.
+// All of this is latency: the tables of a few hundred sequences are some 100 KB, and a launch of one workgroup is
+// some eight look-ups one after another. 256 sequences of up to 128 pages: 3 us to cut, 8.6 to grow by a token each;
+// 128 of 512 sequences ended and replaced by prompts of 4000 tokens, 200000 pages: 25 us in five launches.
 #include "bq_kv4.h"
 
 namespace bq {
@@ -41,7 +43,8 @@ __global__ __launch_bounds__(256) void pages_cut_kernel(Tables a, const int* __r
 }
 
 // Every row of the table becomes its parent's: a workgroup takes 2^`shift` columns of all rows through LDS,
-// the last one the lengths. Few columns where there are few rows, for more workgroups.
+// the last one the lengths. 8 columns above 128 rows, for more workgroups (192 rows of 24 pages: 13 us in 16 columns
+// with divisions, so 5), fewer where LDS ends.
 constexpr int FORK_ENTRIES = 16384, FORK_THREADS = 512, FORK_EACH = 4 * FORK_THREADS;
 __global__ __launch_bounds__(FORK_THREADS) void pages_fork_kernel(Tables a, const int* __restrict__ parents, int shift) {
   extern __shared__ int old[];
@@ -72,7 +75,7 @@ __global__ __launch_bounds__(FORK_THREADS) void pages_fork_kernel(Tables a, cons
 // Growing. BLOCK pages' free ones are found as 64 words of 64 bits, a lane's word each. Up to SOLO_PAGES pages the
 // plan's waves read refs themselves, beyond it a launch before it writes the words down. One workgroup plans, since
 // the tables change only where all find room; it also hands out the pages and writes the places, but those of many
-// tokens (SOLO_ROWS) are launches of their own.
+// tokens (SOLO_ROWS) are launches of their own (16000 pages for 512000 tokens: 45 us by the plan, 7 so).
 constexpr int BLOCK = 4096, PLAN_THREADS = 1024, PLAN_WAVES = PLAN_THREADS / 64;
 constexpr int MOST_SEQUENCES = 8192, MOST_BLOCKS = 4096;
 constexpr int64_t SOLO_PAGES = (int64_t)BLOCK * PLAN_WAVES;

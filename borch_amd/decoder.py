@@ -109,6 +109,8 @@ class Decoder(tnn.Module):
         more rows, past the last): a prompt's next piece, one token, or none. The logits of each one's last token
         ``[sequences, vocab]``; those of a sequence without new tokens say nothing, and where not all tokens find
         room (``state.ok`` 0) nothing changes and none do."""
+        if ids.dim() != 1 or not len(ids) or ids.device != state.pages.device:
+            raise RuntimeError(f"read: ids {tuple(ids.shape)} on {ids.device} are the tokens, one at least, on {state.pages.device}")
         got = state.pages.grow(counts, ids.shape[0])
         copy_pages(state.caches, got.moves)
         state.ok = got.ok
@@ -131,6 +133,8 @@ class Decoder(tnn.Module):
                                f"{state.pages.sequences} sequences")
         if ids.shape != (sum(lens),):
             raise RuntimeError(f"ids {tuple(ids.shape)} for prompts of {sum(lens)} tokens")
+        if beams > 64 or not 0 <= end < self.embed.num_embeddings:
+            raise RuntimeError(f"search: {beams} beams (64 at most), end token {end} of {self.embed.num_embeddings}")
         if max(lens) + steps - 1 > state.pages.width * state.pages.page:
             raise RuntimeError(f"search: {max(lens)} tokens and {steps - 1} more in a state of "
                                f"{state.pages.width * state.pages.page} a sequence")

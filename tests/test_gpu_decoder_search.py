@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import borch_amd as bt
+from borch_amd.beams import beam_select
 from borch_amd.decoder import PagedState
 from oracle import beams as O
 from test_gpu_decoder import model_of
@@ -103,6 +104,15 @@ def test_search_refusals(dev):
         PagedState(m, 2, pages=30, width=17, page=32)
     state = PagedState(m, 4, pages=3, width=2, page=32)
     ids = torch.zeros(60, dtype=torch.long, device=dev)
+    counts = torch.tensor([3, 0, 0, 0], dtype=torch.int32, device=dev)
+    for bad in (ids[:0], ids.cpu(), ids.view(2, 30)):
+        with pytest.raises(RuntimeError, match="read: ids"):
+            m.read(state, bad, counts)
+    with pytest.raises(RuntimeError, match="end token 97"):
+        m.search(state, ids, [60], 4, 2, end=97)
+    with pytest.raises(RuntimeError, match="65 beams"):
+        m.search(PagedState(m, 65, pages=3, width=2, page=32), ids, [60], 65, 2)
+    assert not bool(state.pages.lens.any())
     with pytest.raises(RuntimeError, match="4 sequences"):
         m.search(state, ids, [60], 3, 2)
     with pytest.raises(RuntimeError, match="prompts of 50"):
@@ -111,3 +121,37 @@ def test_search_refusals(dev):
         m.search(state, ids, [60], 4, 6)
     with pytest.raises(RuntimeError, match="3 pages"):
         m.search(state, ids, [60], 4, 4)
+
+
+@torch.no_grad()
+def test_search_captured(dev):
+    """A step of the search captured: fork, growth, copies, the model over the caches and the selection, replayed with
+    the host's own work between, against the same search call by call."""
+    print("decoder search captured", flush=True)
+    m = model_of(dev, 3)
+    lens, W, steps, end = [37, 63], 3, 6, 11
+    S = len(lens) * W
+    ids = torch.randint(0, 97, (sum(lens),), generator=torch.Generator().manual_seed(8)).to(dev)
+    want, scores = m.search(PagedState(m, S, pages=40, width=4, page=32), ids, lens, W, steps, end)
+    state = PagedState(m, S, pages=40, width=4, page=32)
+    counts = torch.tensor([37, 0, 0, 63, 0, 0], dtype=torch.int32, device=dev)
+    logits = m.read(state, ids, counts)
+    have = torch.tensor([[0.0, -torch.inf, -torch.inf]] * 2, device=dev)
+    done, one = torch.zeros(2, W, dtype=torch.bool, device=dev), torch.ones(S, dtype=torch.int32, device=dev)
+    tokens = torch.zeros(S, steps + 1, dtype=torch.int32, device=dev)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = beam_select(logits, have, done, end)
+        parents, new = got.parents.view(-1), got.tokens.view(-1)
+        tokens.copy_(torch.cat([tokens[parents][:, 1:], new[:, None]], 1))
+        state.pages.fork(parents)
+        next_logits = m.read(state, new, one)
+        for to, x in ((logits, next_logits), (have, got.scores), (done, got.done)):
+            to.copy_(x)
+    for step in range(steps):
+        graph.replay()
+        assert state.ok.item() == 1
+        assert state.pages.lens.tolist() == [38 + step] * W + [64 + step] * W
+    assert torch.equal(tokens[:, 1:].view(2, W, steps), want)
+    assert float((have - scores).abs().max()) < 2e-3
