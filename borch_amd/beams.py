@@ -37,33 +37,33 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, done: torch.Tensor |
     no_graph("beam_select", logits, scores)
     require_device(logits.device)
     code = type_of(logits, "beam_select")
-    if scores.dim() != 2 or logits.dim() != 2 or logits.shape[0] != scores.numel() or not logits.shape[1] or not scores.shape[1]:
+    index, shape, size = logits.get_device(), scores.shape, logits.shape
+    if len(shape) != 2 or len(size) != 2 or size[0] != shape[0] * shape[1] or not size[1] or not shape[1]:
         raise RuntimeError(f"beam_select: logits {tuple(logits.shape)} are [requests * beams, vocab], scores "
                            f"{tuple(scores.shape)} [requests, beams]")
-    index, shape = logits.get_device(), scores.shape
+    B, W = shape
+    V = size[1]
     if scores.dtype is not torch.float32 or scores.get_device() != index:
         raise TypeError(f"beam_select: scores are float32 on {logits.device}, got {scores.dtype} on {scores.device}")
     if done is not None:
         if done.dtype is not torch.bool or done.get_device() != index or done.shape != shape:
             raise TypeError(f"beam_select: done is bool {tuple(shape)} on {logits.device}, got {done.dtype} "
                             f"{tuple(done.shape)} on {done.device}")
-        if not 0 <= end < logits.shape[1]:
-            raise ValueError(f"beam_select: end token {end} of {logits.shape[1]}, with beams that may be done")
+        if not 0 <= end < V:
+            raise ValueError(f"beam_select: end token {end} of {V}, with beams that may be done")
         done = done.contiguous()
-    if logits.stride(1) != 1 and logits.shape[1] > 1:
-        logits = logits.contiguous()
+    pitch, step = logits.stride()
+    if step != 1 and V > 1:
+        logits, pitch = logits.contiguous(), V
     scores = scores.contiguous()
-    out = Selected(torch.empty_like(scores), torch.empty(shape, dtype=torch.int32, device=logits.device),
-                   torch.empty(shape, dtype=torch.int32, device=logits.device),
-                   torch.empty(shape, dtype=torch.bool, device=logits.device))
-    B, W = shape
+    parents = torch.empty_like(scores, dtype=torch.int32)
+    out = Selected(torch.empty_like(scores), parents, torch.empty_like(parents), torch.empty_like(scores, dtype=torch.bool))
     if B == 0:
         return out
-    V = logits.shape[1]
     need = lib().bq_beam_select_ws_bytes(code, B, W, V)
-    ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    ws = torch.empty(need, dtype=torch.uint8, device=scores.device)
     with on(index):
-        check(lib().bq_beam_select(logits.data_ptr(), code, B, W, V, logits.stride(0), scores.data_ptr(),
+        check(lib().bq_beam_select(logits.data_ptr(), code, B, W, V, pitch, scores.data_ptr(),
                                    None if done is None else done.data_ptr(), end, out.scores.data_ptr(),
                                    out.parents.data_ptr(), out.tokens.data_ptr(), out.done.data_ptr(), ws.data_ptr(), need,
                                    _stream(logits)))
