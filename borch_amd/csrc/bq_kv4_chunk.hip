@@ -19,7 +19,9 @@
 // whose codes, loaded one tile ahead, are expanded into LDS, two tiles in turn, one barrier a tile. Bound by the
 // matrix units beside the exponentials and the expansion: 2048 tokens over 16384, 32 heads over 8 of 128, bf16:
 // 531 us, 971 TFLOP/s; 8192 over 8192 553 us, 994 (the library's 8192^3 product: 1426). f16 560 and f32 380, at 2 and 3
-// times the products. Each wave expanding for itself would cost four times the conversions; 64 rows a workgroup twice.
+// times the products. Reading LDS takes as long as the products of bf16, but with 64 rows a wave, which halves it, one
+// wave a SIMD does not hide the exponentials (804 us where these are 555), and eight waves that share the codes take as
+// long (567; in two halves that take turns between products and exponentials 630).
 //
 // Narrow tiles, of sequences of few rows, where a product is small beside the reading: 32 rows, of which each wave
 // takes every fourth 32 keys by itself, from memory into operands, joined in LDS at the end. Bound by the reading:
