@@ -65,16 +65,6 @@ struct Place {
   int base, len;             // the place in the cache of the sequence's first new token, and its tokens
 };
 
-// The tiles of TILE rows of what lies before cu[0] (i = 0), of sequence i - 1, or of what lies past the last: of those
-// that take such tiles.
-template <int TILE>
-__device__ __forceinline__ int tiles_of(const Chunk& a, int i, int* s, int* rows) {
-  if (i > a.B + 1) return 0;
-  *s = i == 0 ? 0 : min(max(a.cu[i - 1], 0), a.n);
-  const int e = i == a.B + 1 ? a.n : min(max(a.cu[i], 0), a.n);
-  *rows = max(0, e - *s) * a.group;
-  return (*rows > a.least) == (TILE == WIDE) ? (*rows + TILE - 1) / TILE : 0;
-}
 template <int CONTROL, int ROWS>
 __device__ __forceinline__ int plus_lanes(int v) {
   return v + __builtin_amdgcn_update_dpp(0, v, CONTROL, ROWS, 0xF, false);
@@ -87,27 +77,44 @@ __device__ __forceinline__ int wave_upto(int v) {  // the lanes' values up to th
   v = plus_lanes<0x142, 0xA>(v);  // the last of the row before into the second and fourth,
   return plus_lanes<0x143, 0xC>(v);  // lane 31's into the upper half
 }
-// Tile `last` from the last one on. A lane sums some sequences first, where there are more than lanes: one after
-// another 64 at a time, each waited for the loads of those before.
+// Where the i-th of what lies before cu[0], each sequence and what lies past the last ends.
+__device__ __forceinline__ int end_at(const Chunk& a, int i) { return i > a.B ? a.n : min(max(a.cu[i], 0), a.n); }
+// From 64 of those ends, a lane each, and the one before: the rows of each, and its tiles if it takes such.
+template <int TILE>
+__device__ __forceinline__ int tiles_of(const Chunk& a, int end, int before, int* start, int* rows) {
+  *start = __builtin_amdgcn_update_dpp(before, end, 0x138, 0xF, 0xF, false);  // the lane before's
+  *rows = max(0, end - *start) * a.group;
+  return (*rows > a.least) == (TILE == WIDE) ? (*rows + TILE - 1) / TILE : 0;
+}
+// Tile `last` from the last one on. Where there are more sequences than lanes their tiles are summed first, 64 at a
+// time, the loads of eight such on their way (512 sequences: 177 -> 140 us of which this was a third).
 template <int TILE>
 __device__ __forceinline__ bool place_of(const Chunk& a, int last, Place* out) {
-  const int lane = threadIdx.x & 63, each = (a.B + 2 + 63) >> 6;
-  int from = 0, place = 0, s = 0, rows = 0;
-  if (each > 1) {
-    int mine = 0;
-#pragma unroll 4
-    for (int i = 0; i < each; ++i) mine += tiles_of<TILE>(a, lane * each + i, &s, &rows);
-    const int upto = wave_upto(mine);
+  const int lane = threadIdx.x & 63, rounds = (a.B + 2 + 63) >> 6, each = (rounds + 63) >> 6;  // rounds a lane's sum
+  int from = 0, place = 0, s, rows;
+  if (rounds > 1) {
+    int sums = 0, before = 0;
+    for (int r0 = 0; r0 < rounds; r0 += 8) {
+      int ends[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) ends[k] = end_at(a, (r0 + k) * 64 + lane);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int sum = __builtin_amdgcn_readlane(wave_upto(tiles_of<TILE>(a, ends[k], before, &s, &rows)), 63);
+        before = __builtin_amdgcn_readlane(ends[k], 63);
+        sums += lane == (each == 1 ? r0 + k : (r0 + k) / each) ? sum : 0;
+      }
+    }
+    const int upto = wave_upto(sums);
     place = __builtin_amdgcn_readlane(upto, 63) - 1 - last;
     if (place < 0) return false;
     const int l = __builtin_ctzll(__ballot(upto > place));
-    place -= __builtin_amdgcn_readlane(upto - mine, l);
-    from = l * each;
+    place -= __builtin_amdgcn_readlane(upto - sums, l);
+    from = l * each * 64;
   }
-  for (int at = from; at < (each > 1 ? from + each : 64); at += 64) {
-    s = rows = 0;
-    const int mine = tiles_of<TILE>(a, at + lane, &s, &rows), upto = wave_upto(mine);
-    if (each == 1) place = __builtin_amdgcn_readlane(upto, 63) - 1 - last;
+  for (int at = from; at < from + each * 64; at += 64) {
+    const int mine = tiles_of<TILE>(a, end_at(a, at + lane), at ? end_at(a, at - 1) : 0, &s, &rows), upto = wave_upto(mine);
+    if (rounds == 1) place = __builtin_amdgcn_readlane(upto, 63) - 1 - last;
     if (place < 0) return false;
     const uint64_t hit = __ballot(upto > place);
     if (hit) {
@@ -399,8 +406,9 @@ struct Rows {
   }
 
   // What was left out of the products is added to the outputs of the rows that see it, whatever its weight,
-  // and to no other's.
-  __device__ __forceinline__ void add_huge(const Chunk& a, const Place& at, int h, int blk0, int blk1) {
+  // and to no other's: to the N of them from `first` on in out()'s order, y(0) ...
+  template <int N, typename Y>
+  __device__ __forceinline__ void add_huge(const Chunk& a, const Place& at, int h, int blk0, int blk1, int first, Y&& y) {
     const int hh = (threadIdx.x >> 5) & 1;
     for (int blk = blk0; blk < blk1; ++blk) {
       const int64_t r0 = row_of(a, at, h, blk);
@@ -409,16 +417,16 @@ struct Rows {
       for (int t = 0; t < 32; ++t) {
         if (32 * blk + t >= most) break;
 #pragma unroll
-        for (int i = 0; i < DIM / 8; ++i) {  // four channels at a time
-          const int ch = channel(4 * i, hh);
+        for (int i = 0; i < N / 4; ++i) {  // four channels at a time
+          const int ch = channel(first + 4 * i, hh);
           const uint32_t byte = a.c.vs[Kv4At<DIM>::vs(r0 + t, t, ch / 32)];
           if (byte < HUGE) continue;
           const uint32_t w = *reinterpret_cast<const uint16_t*>(a.c.v + Kv4At<DIM>::v(r0 + t, t, ch / (DIM / 16)) +
                                                                 ch % (DIM / 16) / 2);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float y = (float)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w >> (8 * (e / 2)), scale_bits(byte), 0)[e & 1];
-            if (!(fabsf(y) < INFINITY) && 32 * blk + t < end) out(4 * i + e) = __fadd_rn(out(4 * i + e), y);
+            const float v = (float)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w >> (8 * (e / 2)), scale_bits(byte), 0)[e & 1];
+            if (!(fabsf(v) < INFINITY) && 32 * blk + t < end) y(4 * i + e) = __fadd_rn(y(4 * i + e), v);
           }
         }
       }
@@ -436,8 +444,9 @@ struct Rows {
     }
   }
 
-  // Into the output, or as one of the shares of a row.
-  __device__ __forceinline__ void store(const Chunk& a, const Place& at, int h, int share, int shares) {
+  // N outputs from `first` on into the output, or as one of the shares of a row.
+  template <int N, typename Y>
+  __device__ __forceinline__ void store(const Chunk& a, const Place& at, int h, int share, int shares, int first, Y&& y) {
     const int hh = (threadIdx.x >> 5) & 1;
     if (row >= at.rows) return;
     if (shares == 1) {
@@ -445,16 +454,16 @@ struct Rows {
       const float r = __fdiv_rn(1.f, l == 0.f ? 1.f : l);
       T* to = (T*)a.out + ((int64_t)(at.start + t) * a.c.heads * a.group + h * a.group + j) * DIM;
 #pragma unroll
-      for (int x = 0; x < DIM / 2; x += 4)
-        store4(to + channel(x, hh), __fmul_rn(out(x), r), __fmul_rn(out(x + 1), r), __fmul_rn(out(x + 2), r),
-               __fmul_rn(out(x + 3), r));
+      for (int x = 0; x < N; x += 4)
+        store4(to + channel(first + x, hh), __fmul_rn(y(x), r), __fmul_rn(y(x + 1), r), __fmul_rn(y(x + 2), r),
+               __fmul_rn(y(x + 3), r));
     } else {
       const int64_t slot = slot_of(a, at, row, h) + share;
       float* to = a.part + slot * DIM;
 #pragma unroll
-      for (int x = 0; x < DIM / 2; x += 4)
-        *reinterpret_cast<float4*>(to + channel(x, hh)) = make_float4(out(x), out(x + 1), out(x + 2), out(x + 3));
-      if (hh == 0) *reinterpret_cast<float2*>(a.stats + slot * 2) = make_float2(m, l);
+      for (int x = 0; x < N; x += 4)
+        *reinterpret_cast<float4*>(to + channel(first + x, hh)) = make_float4(y(x), y(x + 1), y(x + 2), y(x + 3));
+      if (hh == 0 && first == 0) *reinterpret_cast<float2*>(a.stats + slot * 2) = make_float2(m, l);
     }
   }
 };
@@ -544,9 +553,10 @@ __device__ __forceinline__ void wide_tile(const Chunk& a, int id, unsigned char*
       if (KEYS * u < r.most) r.template keys<2>(a, tk, tv, 0, KEYS * u, now);
     }
   }
-  if (__syncthreads_or(huge)) r.add_huge(a, at, h, 2 * u0, min(2 * u1, (at.len + 31) >> 5));
+  auto y = [&](int x) -> float& { return r.out(x); };
+  if (__syncthreads_or(huge)) r.template add_huge<DIM / 2>(a, at, h, 2 * u0, min(2 * u1, (at.len + 31) >> 5), 0, y);
   r.l = __fadd_rn(r.l, __shfl_xor(r.l, 32));
-  r.store(a, at, h, share, shares);
+  r.template store<DIM / 2>(a, at, h, share, shares, 0, y);
 }
 
 // Sequences of few rows, where the products are small beside the reading: each wave takes every fourth 32 keys for
@@ -701,35 +711,38 @@ __device__ __forceinline__ void narrow_tile(const Chunk& a, int id, float* all) 
     body(blk, blocks[0]);
     if (DEPTH == 2 && blk + 4 < b1) body(blk + 4, blocks[DEPTH - 1]);
   }
-  r.l = __fadd_rn(r.l, __shfl_xor(r.l, 32));
+  // a quarter of the outputs by each wave, from all four
+  constexpr int N = DIM / 8;
+  float* to = all + wave * (WORDS * 64) + lane;
+  to[0] = r.m;
+  to[64] = __fadd_rn(r.l, __shfl_xor(r.l, 32));
+#pragma unroll
+  for (int x = 0; x < DIM / 2; ++x) to[(2 + x) * 64] = r.out(x);
   huge = __syncthreads_or(huge);
-  if (wave) {
-    float* to = all + (wave - 1) * (WORDS * 64) + lane;
-    to[0] = r.m;
-    to[64] = r.l;
+  const float* from = all + lane;
+  float ms[4], f[4], y[N];
 #pragma unroll
-    for (int i = 0; i < 16 * VT; ++i) to[(2 + i) * 64] = r.o[i / 16][i % 16];
-  }
-  __syncthreads();
-  if (wave) return;
-  for (int w = 0; w < 3; ++w) {
-    const float* from = all + w * (WORDS * 64) + lane;
-    const float m1 = from[0], now_m = fmaxf(r.m, m1);
-    const float f0 = r.m == now_m ? 1.f : factor(r.m, now_m, a.scale2), f1 = m1 == now_m ? 1.f : factor(m1, now_m, a.scale2);
-    r.m = now_m;
-    r.l = __fmaf_rn(r.l, f0, __fmul_rn(from[64], f1));
+  for (int w = 0; w < 4; ++w) ms[w] = from[w * (WORDS * 64)];
+  r.m = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
+  r.l = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16 * VT; ++i)
-      r.o[i / 16][i % 16] = __fmaf_rn(r.o[i / 16][i % 16], f0, __fmul_rn(from[(2 + i) * 64], f1));
+  for (int x = 0; x < N; ++x) y[x] = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    f[w] = ms[w] == r.m ? 1.f : factor(ms[w], r.m, a.scale2);
+    r.l = __fmaf_rn(from[w * (WORDS * 64) + 64], f[w], r.l);
+#pragma unroll
+    for (int x = 0; x < N; ++x) y[x] = __fmaf_rn(from[(w * WORDS + 2 + wave * N + x) * 64], f[w], y[x]);
   }
-  if (huge) r.add_huge(a, at, h, 2 * u0, b1);
-  r.store(a, at, h, share, shares);
+  auto part = [&](int x) -> float& { return y[x]; };
+  if (huge) r.template add_huge<N>(a, at, h, 2 * u0, b1, wave * N, part);
+  r.template store<N>(a, at, h, share, shares, wave * N, part);
 }
 
 // Both in one launch, the wide tiles first; or narrow ones alone, with less LDS and fewer registers.
 template <typename T, int DIM, bool WIDES>
 __global__ __launch_bounds__(256, 2) void kv4_chunk_kernel(Chunk a) {
-  constexpr int BYTES = WIDES ? 4 * KEYS * DIM * 2 : 3 * (DIM / 2 + 2) * 256;
+  constexpr int TILES = WIDES ? 4 * KEYS * DIM * 2 : 0, JOIN = 4 * (DIM / 2 + 2) * 256, BYTES = TILES > JOIN ? TILES : JOIN;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[BYTES];
   const int wides = a.wide.tiles * a.wide.most * a.c.heads;
   if constexpr (WIDES)
