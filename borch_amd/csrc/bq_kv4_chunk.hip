@@ -78,7 +78,10 @@ __device__ __forceinline__ int wave_upto(int v) {  // the lanes' values up to th
   return plus_lanes<0x143, 0xC>(v);  // lane 31's into the upper half
 }
 // Where the i-th of what lies before cu[0], each sequence and what lies past the last ends.
-__device__ __forceinline__ int end_at(const Chunk& a, int i) { return i > a.B ? a.n : min(max(a.cu[i], 0), a.n); }
+__device__ __forceinline__ int end_at(const Chunk& a, int i) {
+  const int x = min(max(a.cu[min(i, a.B)], 0), a.n);  // whatever i: loads under a condition would wait for one another
+  return i > a.B ? a.n : x;
+}
 // From 64 of those ends, a lane each, and the one before: the rows of each, and its tiles if it takes such.
 template <int TILE>
 __device__ __forceinline__ int tiles_of(const Chunk& a, int end, int before, int* start, int* rows) {
@@ -87,7 +90,8 @@ __device__ __forceinline__ int tiles_of(const Chunk& a, int end, int before, int
   return (*rows > a.least) == (TILE == WIDE) ? (*rows + TILE - 1) / TILE : 0;
 }
 // Tile `last` from the last one on. Where there are more sequences than lanes their tiles are summed first, 64 at a
-// time, the loads of eight such on their way (512 sequences: 177 -> 140 us of which this was a third).
+// time, the loads of eight such on their way: beside workgroups that stream, each wait is 1 to 2 us (512 sequences of
+// one token: 178 us with one after another, 166 so).
 template <int TILE>
 __device__ __forceinline__ bool place_of(const Chunk& a, int last, Place* out) {
   const int lane = threadIdx.x & 63, rounds = (a.B + 2 + 63) >> 6, each = (rounds + 63) >> 6;  // rounds a lane's sum
@@ -481,8 +485,8 @@ __device__ __forceinline__ bool job_of(const Chunk& a, int id, Place* at, int* h
   const int units = units_of<TILE>(a, *at, at->row0);
   *shares = shares_of(kind.upper, units);
   if (*share >= *shares) return false;
-  *u0 = (int)((int64_t)units * *share / *shares);
-  *u1 = (int)((int64_t)units * (*share + 1) / *shares);
+  *u0 = (uint32_t)units * *share / *shares;  // 2^25 units and 128 shares at most
+  *u1 = (uint32_t)units * (*share + 1) / *shares;
   return true;
 }
 
