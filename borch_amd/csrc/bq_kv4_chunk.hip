@@ -85,7 +85,9 @@ __device__ __forceinline__ int end_at(const Chunk& a, int i) {
 // From 64 of those ends, a lane each, and the one before: the rows of each, and its tiles if it takes such.
 template <int TILE>
 __device__ __forceinline__ int tiles_of(const Chunk& a, int end, int before, int* start, int* rows) {
-  *start = __builtin_amdgcn_update_dpp(before, end, 0x138, 0xF, 0xF, false);  // the lane before's
+  int x = __builtin_amdgcn_update_dpp(before, end, 0x138, 0xF, 0xF, false);  // the lane before's
+  asm("" : "+v"(x));  // no operand of the difference: where `before` is 0 it became a v_subrev_u32_dpp, of the wrong sign
+  *start = x;
   *rows = max(0, end - *start) * a.group;
   return (*rows > a.least) == (TILE == WIDE) ? (*rows + TILE - 1) / TILE : 0;
 }
