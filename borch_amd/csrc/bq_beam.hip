@@ -15,7 +15,7 @@
 // against their maximum. The second launch joins a request's parts and beams.
 //
 // Bound by the exponentials, 10 operations in f64 and as many in 32 bits a logit, beside the reading: 64 requests of
-// 8 beams and 128000 tokens in bf16 (131 MB) take 50 us for the first launch (the vector units busy for two thirds of
+// 8 beams and 128000 tokens in bf16 (131 MB) take 55 us for the first launch (the vector units busy for two thirds of
 // it) and 9 for the second. 4 beams of 32000 in f32: 6 us each, latency.
 #include <math.h>
 

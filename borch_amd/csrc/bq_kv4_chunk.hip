@@ -25,8 +25,8 @@
 //
 // Narrow tiles, of sequences of few rows, where a product is small beside the reading: 32 rows, of which each wave
 // takes every fourth 32 keys by itself, from memory into operands, joined in LDS at the end. Bound by the reading:
-// 64 sequences of 4000 tokens and one new, bf16: 60 us, 4.6 TB/s (read alone: 7.0); 512 of 1000: 177 us, 3.2 TB/s,
-// where finding the tile, the first loads and the join are a third of a workgroup's time.
+// 64 sequences of 4000 tokens and one new, bf16: 60 us, 4.6 TB/s (read alone: 7.0); 512 of 1000: 164 us, 3.4 TB/s,
+// where finding the tile and the first loads are a third of a workgroup's time.
 //
 // The maximum that is subtracted lags by up to 2^8 (the weights' own size cancels in the quotient) and is a whole
 // number of powers of two, so that a weight is one FMA and one exp2 and all of a row's agree.
@@ -830,7 +830,7 @@ __global__ __launch_bounds__(256) void kv4_chunk_join_kernel(Chunk a) {
 // workgroup, of all the work over the workgroups that run at once and the longest begun last, or of whole rounds of
 // equal ones; the workgroups that find no tile; and what the join writes and reads. Narrow tiles' usual length is what
 // the cache's pages hold for each sequence: with the longest sequence's for all, one chunk of 1024 tokens beside 511
-// sequences of one over 1000 took 866 us, so 240. So are wide tiles' where every sequence may have some (three chunks
+// sequences of one over 1000 took 866 us, so 230. So are wide tiles' where every sequence may have some (three chunks
 // of 512, 500 and 333 tokens over 4096, 1500 and 777, f32: 130 -> 107 us). Narrow tiles beside wide ones are cut only
 // where they would last longer: the join alone, over all rows, is 15 us of 2048 tokens of 32 heads.
 constexpr int64_t FEW_ROWS = 64, FEW_ALL = 2048;

@@ -286,6 +286,36 @@ def test_captured(dev):
             (cu, slots, at, moves, [ok])
 
 
+def test_captured_many(dev):
+    """Many pages and many tokens, whose launches share a workspace: captured, replayed with eager calls between."""
+    print("pages captured, many", flush=True)
+    b = Both(dev, 9, 2000, 70000, 8)
+    b.grow([9000, 10, 0, 777, 0, 0, 64, 1, 3], 10000)
+    parents, more, to = (i32(x, dev) for x in ([0] * 9, [1] * 9, [200] * 9))
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        b.gpu.cut(to)
+        b.gpu.fork(parents)
+        got = b.gpu.grow(more, 9001)
+    r = random.Random(7)
+    for step in range(4):
+        p = [r.randrange(9) for _ in range(9)]
+        t = [n - r.randint(0, 5000) for n in b.ref.lens]
+        m = [r.choice([0, 1, 300, 4000]) if sum(t) else 1 for _ in range(9)]
+        m = [0 if sum(m[:i + 1]) > 9001 else n for i, n in enumerate(m)]
+        for x, y in ((parents, p), (more, m), (to, t)):
+            x.copy_(i32(y, dev))
+        graph.replay()
+        b.ref.cut(t)
+        b.ref.fork(p)
+        cu, slots, at, moves, ok = b.ref.grow(m, 9001)
+        b.same()
+        assert (got.cu.tolist(), got.slots.tolist(), got.at.tolist(), got.moves.tolist(), got.ok.tolist()) == \
+            (cu, slots, at, moves, [ok])
+        b.grow([5] * 9, 9000)  # eager, into what is free by now
+
+
 def test_refusals(dev):
     p = paging.Pages.zeros(3, 4, 8, 32, dev)
     x = torch.zeros(3, dtype=torch.int32, device=dev)
