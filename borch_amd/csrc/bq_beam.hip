@@ -57,6 +57,39 @@ __device__ __forceinline__ int token_of(uint64_t r) { return (int)~(uint32_t)r; 
 // The value of the lane before (wave_shr:1); the first lane's is not looked at.
 __device__ __forceinline__ int lane_below(int v) { return __builtin_amdgcn_mov_dpp(v, 0x138, 0xF, 0xF, false); }
 
+// Over the wave's lanes, in a fixed order: from the lanes 1, 2, 4 and 8 before in a row of 16, the row before's last,
+// lane 31's. Lanes that have none before take `none`, or for the maximum their own.
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ double from_lanes(double v, double none) {
+  const uint64_t x = __builtin_bit_cast(uint64_t, v), o = __builtin_bit_cast(uint64_t, none);
+  const uint32_t lo = __builtin_amdgcn_update_dpp((int)o, (int)x, CONTROL, ROWS, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp((int)(o >> 32), (int)(x >> 32), CONTROL, ROWS, 0xF, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double last_lane(double v) {
+  const uint64_t x = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), 63) << 32 |
+                                        (uint32_t)__builtin_amdgcn_readlane((int)x, 63));
+}
+__device__ __forceinline__ double wave_sum(double v) {
+  v += from_lanes<0x111, 0xF>(v, 0.0);
+  v += from_lanes<0x112, 0xF>(v, 0.0);
+  v += from_lanes<0x114, 0xF>(v, 0.0);
+  v += from_lanes<0x118, 0xF>(v, 0.0);
+  v += from_lanes<0x142, 0xA>(v, 0.0);
+  v += from_lanes<0x143, 0xC>(v, 0.0);
+  return last_lane(v);
+}
+__device__ __forceinline__ double wave_top(double v) {
+  v = fmax(v, from_lanes<0x111, 0xF>(v, v));
+  v = fmax(v, from_lanes<0x112, 0xF>(v, v));
+  v = fmax(v, from_lanes<0x114, 0xF>(v, v));
+  v = fmax(v, from_lanes<0x118, 0xF>(v, v));
+  v = fmax(v, from_lanes<0x142, 0xA>(v, v));
+  v = fmax(v, from_lanes<0x143, 0xC>(v, v));
+  return last_lane(v);
+}
+
 // The best `W` so far, in order, lane i the i-th (0: none); `least` the W-th.
 struct List {
   uint64_t mine, least;
@@ -173,8 +206,7 @@ __global__ __launch_bounds__(PART_WAVES * 64) void beam_part_kernel(Beam a) {
       if (__any(may)) best.add(may ? rank_of(v, i + e) : 0);
     }
   }
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  top = wave_max(top);
   if (lane == 0) tops[wave] = top;
   lists[wave][lane] = best.mine;
   __syncthreads();
@@ -188,8 +220,7 @@ __global__ __launch_bounds__(PART_WAVES * 64) void beam_part_kernel(Beam a) {
       for (int i = lo + (int)threadIdx.x; i < hi; i += PART_WAVES * 64) all += exp((double)(float)x[i] - base);
     }
   }
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
+  all = wave_sum(all);
   if (lane == 0) sums[wave] = all;
   __syncthreads();
   if (wave) return;
@@ -229,13 +260,8 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(Beam a) {
         double2 s = make_double2(-INFINITY, 0.0);
         if (p < a.parts) s = a.sums[(size_t)row * a.parts + p];
         nan |= s.y != s.y;
-        double now = s.x;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) now = fmax(now, __shfl_xor(now, d));
-        now = fmax(now, top);
-        double add = s.x > -INFINITY ? s.y * exp(s.x - now) : 0.0;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) add += __shfl_xor(add, d);
+        const double now = fmax(wave_top(s.x), top);
+        const double add = wave_sum(s.x > -INFINITY ? s.y * exp(s.x - now) : 0.0);
         sum = (top > -INFINITY ? sum * exp(top - now) : 0.0) + add;
         top = now;
       }
