@@ -23,9 +23,6 @@
 
 namespace bq {
 
-typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-
 constexpr int MOST_BEAMS = 64, PART_WAVES = 4;
 constexpr int PIECES = 16, PART_BYTES = PIECES * PART_WAVES * 64 * 16;  // 16 bytes each of a lane; of a part
 
@@ -253,6 +250,9 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(Beam a) {
     } else {
       List best;
       best.clear(W);
+      const uint64_t* from = a.best + (size_t)row * a.parts * W;
+      const int all = a.parts * W;
+      uint64_t next = from[min(lane, all - 1)];  // on its way beside the sums
       double top = -INFINITY, sum = 0.0;
       bool nan = false;
       for (int p0 = 0; p0 < a.parts; p0 += 64) {
@@ -265,8 +265,11 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(Beam a) {
         sum = (top > -INFINITY ? sum * exp(top - now) : 0.0) + add;
         top = now;
       }
-      for (int i0 = 0; i0 < a.parts * W; i0 += 64)
-        best.add(i0 + lane < a.parts * W ? a.best[(size_t)row * a.parts * W + i0 + lane] : 0);
+      for (int i = lane; i - lane < all; i += 64) {
+        const uint64_t now = next;
+        next = from[min(i + 64, all - 1)];
+        best.add(i < all ? now : 0);
+      }
       const bool dead = __any(nan) || !(top > -INFINITY && top < INFINITY) || !(fabs(score) < INFINITY);
       if (dead) {
         token = lane;  // nothing tells its tokens apart
