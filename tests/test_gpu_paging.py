@@ -286,6 +286,31 @@ def test_captured(dev):
             (cu, slots, at, moves, [ok])
 
 
+def test_streams(dev):
+    """A step on another stream than the current one's; two states on two streams at once."""
+    print("pages streams", flush=True)
+    both = [Both(dev, 40, 9, 70000, 32) for _ in range(2)]
+    sides = [torch.cuda.Stream(dev) for _ in range(2)]
+    r = random.Random(3)
+    steps = [([r.randint(0, 90) for _ in range(40)], [r.randrange(40) for _ in range(40)]) for _ in range(6)]
+    given = [(i32(m, dev), i32(p, dev)) for m, p in steps]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for m, p in given:
+        for b, side, g in zip(both, sides, got):
+            with torch.cuda.stream(side):
+                g.append(b.gpu.grow(m, 4000))
+                b.gpu.fork(p)
+    torch.cuda.synchronize()
+    for b, g in zip(both, got):
+        for (m, p), x in zip(steps, g):
+            cu, slots, at, moves, ok = b.ref.grow(m, 4000)
+            assert (x.cu.tolist(), x.slots.tolist(), x.at.tolist(), x.moves.tolist(), x.ok.tolist()) == \
+                (cu, slots, at, moves, [ok])
+            b.ref.fork(p)
+        b.same()
+
+
 def test_captured_many(dev):
     """Many pages and many tokens, whose launches share a workspace: captured, replayed with eager calls between."""
     print("pages captured, many", flush=True)
