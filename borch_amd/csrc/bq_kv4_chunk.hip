@@ -824,7 +824,9 @@ __global__ __launch_bounds__(256) void kv4_chunk_join_kernel(Chunk a) {
 //
 // A sequence takes wide tiles from more than FEW_ROWS rows on (32 sequences of 48 rows beside it, of 3000 tokens: 65 us
 // so, 93 in wide tiles; of 128 rows: 98 in wide tiles, 120 in narrow ones); a call of up to FEW_ALL rows takes narrow
-// tiles alone, for more workgroups (those 48 rows, 1536 in all: 42 us; but 4096 rows so 132 us for 96).
+// tiles alone, for more workgroups (those 48 rows, 1536 in all: 42 us; but 4096 rows so 132 us for 96). Above FEW_MOST
+// rows, where every sequence may fill a wide tile, it takes them if the estimates below say so: 512 tokens of 32 heads
+// over 8, bf16, over 4096: 48 us in narrow tiles, 59 in wide ones; over 16384 174 and 165, over 65536 677 and 596.
 //
 // Of the shares that a tile may be cut in that number is taken for which the estimated time is least: of the longest
 // workgroup, of all the work over the workgroups that run at once and the longest begun last, or of whole rounds of
@@ -833,7 +835,7 @@ __global__ __launch_bounds__(256) void kv4_chunk_join_kernel(Chunk a) {
 // sequences of one over 1000 took 866 us, so 230. So are wide tiles' where every sequence may have some (three chunks
 // of 512, 500 and 333 tokens over 4096, 1500 and 777, f32: 130 -> 107 us). Narrow tiles beside wide ones are cut only
 // where they would last longer: the join alone, over all rows, is 15 us of 2048 tokens of 32 heads.
-constexpr int64_t FEW_ROWS = 64, FEW_ALL = 2048;
+constexpr int64_t FEW_ROWS = 64, FEW_ALL = 2048, FEW_MOST = 512;
 static_assert(2 * (FEW_ROWS + 1) > WIDE);
 constexpr double FEW_UNIT_US = 1.2, NONE_US = 4.0;  // a unit of a narrow tile's; a workgroup that finds no tile
 struct Cut {
@@ -871,21 +873,34 @@ static Cut cut_of(int type, int64_t n, int64_t B, int64_t heads, int64_t group, 
   const int64_t at_once = dim == 64 && type ? 768 : 512;
   const double unit_us = dim == 64 ? (type == 0 ? 3.3 : type == 1 ? 2.0 : 2.4) : type == 0 ? 5.5 : type == 1 ? 2.3 : 3.7;
   const double mean = B < 1 ? 1.0 : (double)tokens / KEYS / B, usual = mean < units ? mean : (double)units;
-  double took = 0.0;  // of the wide tiles, beside which the narrow ones run
-  Cut c;
-  c.least = rows <= FEW_ALL ? 0x7fffffff : FEW_ROWS;
-  if (rows <= FEW_ALL) {
+  auto narrow_kind = [&](double each_us, double* took) {
     const int64_t tiles = (rows + FEW - 1) / FEW, some = B < n ? B : n;
-    c.wide = {0, 1, 1};
-    c.few = kind_of(rows / FEW + begun, tiles > some ? tiles : some, heads, units, usual, at_once, FEW_UNIT_US, share_us, &took);
-  } else {
-    const int64_t many = rows / (FEW_ROWS + 1);  // sequences of more rows at most
+    return kind_of(rows / FEW + begun, tiles > some ? tiles : some, heads, units, usual, at_once, each_us, share_us, took);
+  };
+  auto wide_kind = [&](double* took) {
     // more than FEW_ROWS rows are at most 2 tiles for every WIDE + 1
-    const int64_t tiles = rows / WIDE + (begun < many ? begun : many), most = 2 * rows / (WIDE + 1);
-    c.wide = kind_of(tiles < most ? tiles : most, rows / WIDE, heads, units, B <= rows / WIDE ? usual : (double)units,
-                     at_once, unit_us, share_us, &took);
+    const int64_t many = rows / (FEW_ROWS + 1), tiles = rows / WIDE + (begun < many ? begun : many);
+    const int64_t most = 2 * rows / (WIDE + 1);
+    return kind_of(tiles < most ? tiles : most, rows / WIDE, heads, units, B <= rows / WIDE ? usual : (double)units,
+                   at_once, unit_us, share_us, took);
+  };
+  bool wide = rows > FEW_ALL;
+  if (!wide && rows > FEW_MOST && B <= rows / WIDE) {  // a unit of a narrow tile's beside others of the same sequence
+    const double each_us = dim == 64 ? (type == 0 ? 0.8 : type == 1 ? 0.5 : 0.66) : type == 0 ? 1.33 : type == 1 ? 0.66 : 0.97;
+    double narrow_us = 0.0, wide_us = 0.0;
+    narrow_kind(each_us, &narrow_us);
+    wide_kind(&wide_us);
+    wide = wide_us < narrow_us;
+  }
+  double took = 0.0;  // of the wide tiles, beside which the narrow ones run
+  Cut c = {{0, 1, 1}, {}, 0x7fffffff};
+  if (wide) {
+    c.least = FEW_ROWS;
+    c.wide = wide_kind(&took);
     const int64_t full = rows / FEW + begun, two = begun * (FEW_ROWS / FEW);
     c.few = kind_of(full < two ? full : two, B < 1 ? 1 : B, heads, units, usual, at_once, FEW_UNIT_US, share_us, &took);
+  } else {
+    c.few = narrow_kind(FEW_UNIT_US, &took);
   }
   return c;
 }

@@ -64,7 +64,10 @@ def held(c, table, lens, most, dev):
 @pytest.mark.parametrize("lens,new,h,group,page", [
     ([1], [1], 1, 1, 32), ([0, 31, 64, 33], [0, 31, 1, 2], 2, 3, 32), ([300, 5], [40, 5], 3, 1, 64),
     ([129, 0, 700], [129, 0, 33], 2, 4, 128), ([40, 3, 65], [11, 3, 65], 1, 6, 32), ([1000], [7], 1, 16, 256),
-    ([200, 97], [64, 1], 2, 8, 96), ([260, 259, 1], [130, 257, 1], 1, 5, 64), ([513], [512], 1, 1, 64)])
+    ([200, 97], [64, 1], 2, 8, 96), ([260, 259, 1], [130, 257, 1], 1, 5, 64), ([513], [512], 1, 1, 64),
+    # from here on wide tiles, beside narrow ones: more than 2048 rows in all, sequences of more than 64
+    ([400, 33, 700], [140, 1, 3], 1, 16, 32), ([300, 90, 0], [129, 12, 0], 2, 18, 96), ([2100, 64], [2050, 3], 1, 1, 64),
+    ([180] * 17 + [77, 300], [5] * 17 + [4, 127], 1, 16, 64), ([140, 129], [140, 129], 1, 8, 128)])
 def test_chunk_against_float64(dev, kind, dim, lens, new, h, group, page):
     print(f"kv4 chunk {kind} dim={dim} lens={lens} new={new} heads={h}x{group} page={page}", flush=True)
     c, table, ln, _ = filled(dev, lens, h, dim, page, 31)
@@ -79,7 +82,8 @@ def test_chunk_against_float64(dev, kind, dim, lens, new, h, group, page):
     check(c.attend_chunk(qd, td, ld, cd), q[:, :h * group], k, v, there, ln, cu, most, kind)
 
 
-@pytest.mark.parametrize("kind,dim,group", [("f32", 128, 1), ("bf16", 64, 2), ("f16", 128, 4), ("bf16", 128, 7)])
+@pytest.mark.parametrize("kind,dim,group", [("f32", 128, 1), ("bf16", 64, 2), ("f16", 128, 4), ("bf16", 128, 7),
+                                            ("bf16", 64, 20), ("f32", 128, 20), ("f16", 64, 32)])
 def test_chunk_in_shares(dev, kind, dim, group):
     """Few rows over a long axis: a row's keys in many shares, joined; beside them short sequences; a caller's
     max_len beyond every length; lengths cut by it."""
@@ -129,8 +133,9 @@ def test_chunk_rows_of_no_sequence(dev):
     assert not bool(c.attend_chunk(q.to(dev), table.to(dev), ln.to(dev), none.to(dev)).any())
 
 
-def test_chunk_entries_that_are_no_page(dev):
-    print("kv4 chunk bad pages", flush=True)
+@pytest.mark.parametrize("group", [3, 32])
+def test_chunk_entries_that_are_no_page(dev, group):
+    print(f"kv4 chunk bad pages group={group}", flush=True)
     lens, new = [200, 140], [70, 9]
     c, table, ln, _ = filled(dev, lens, 2, 64, 32, 6)
     table = table.clone()
@@ -139,67 +144,68 @@ def test_chunk_entries_that_are_no_page(dev):
     ref = D.Pages(c.k, c.k_scales, c.v, c.v_scales)
     k, v, there = ref.read(table, ln, 224)
     for kind in ("f32", "bf16"):
-        q = queries(sum(new), 6, 64, kind, 1)
+        q = queries(sum(new), 2 * group, 64, kind, 1)
         got = c.attend_chunk(q.to(dev), table.to(dev), ln.to(dev), cu.to(dev))
         check(got, q, k, v, there, ln, cu, 224, kind)
 
 
-@pytest.mark.parametrize("dim,rows", [(64, 8), (128, 8), (128, 40), (64, 100)])
+@pytest.mark.parametrize("dim,rows,group", [(64, 8, 1), (128, 8, 1), (128, 40, 1), (64, 100, 1), (64, 70, 32), (128, 100, 21)])
 @pytest.mark.parametrize("which", ["k", "v"])
 @pytest.mark.parametrize("bad", [0, 40, 97, 99, 101])
-def test_chunk_what_is_not_seen_does_not_count(dev, dim, rows, which, bad):
+def test_chunk_what_is_not_seen_does_not_count(dev, dim, rows, group, which, bad):
     """A NaN among the tokens reaches the rows that see it, a value's in its 32 channels; NaN past the length,
-    in the same page, reaches none. In each form of a tile: a wave by itself, two waves a row, one."""
-    print(f"kv4 chunk NaN dim={dim} rows={rows} {which}[{bad}]", flush=True)
+    in the same page, reaches none. In narrow tiles and (more than 2048 rows) in wide ones."""
+    print(f"kv4 chunk NaN dim={dim} rows={rows} group={group} {which}[{bad}]", flush=True)
     c, table, _, x = filled(dev, [160], 1, dim, 64, 23)
     ln, cu = torch.tensor([100], dtype=torch.int32), starts([rows])
     x = x.clone()
     x[bad, 0 if which == "k" else 1, 33] = math.nan
     c.append(x[:, :1].to(dev), x[:, 1:].to(dev), table.to(dev), torch.tensor([160], dtype=torch.int32, device=dev),
              starts([160]).to(dev))
-    q = queries(rows, 1, dim, "bf16", 2)
+    q = queries(rows, group, dim, "bf16", 2)
     ref = D.Pages(c.k, c.k_scales, c.v, c.v_scales)
     k, v, there = ref.read(table, ln, 100)
     got = c.attend_chunk(q.to(dev), table.to(dev), ln.to(dev), cu.to(dev)).cpu()
     check(got, q, k, v, there, ln, cu, 100, "bf16")
     sees = torch.arange(100 - rows, 100) >= bad
+    sees = sees[:, None].expand(rows, group)
     if which == "v":
-        assert torch.equal(got.isnan().any(-1)[:, 0], sees) and not got[:, :, :32].isnan().any()
+        assert torch.equal(got.isnan().any(-1), sees) and not got[:, :, :32].isnan().any()
     else:
-        assert torch.equal(got.isnan().all(-1)[:, 0], sees) and torch.equal(got.isnan().any(-1)[:, 0], sees)
+        assert torch.equal(got.isnan().all(-1), sees) and torch.equal(got.isnan().any(-1), sees)
 
 
 def test_chunk_infinite_values(dev):
     """A value that the cache holds as infinite, among the newest tokens: infinite where it is seen, not NaN
     where it is not."""
     print("kv4 chunk infinite values", flush=True)
-    for dim, rows in ((64, 8), (128, 50), (128, 90)):
+    for dim, rows, group in ((64, 8, 1), (128, 50, 1), (128, 90, 1), (64, 90, 32), (128, 90, 24)):
         c, table, ln, x = filled(dev, [100], 1, dim, 64, 23)
         x = x.clone()
         x[95, 1, 5], x[97, 1, 40] = 3.3e38, -3.3e38
         c.append(x[:, :1].to(dev), x[:, 1:].to(dev), table.to(dev), ln.to(dev), starts([100]).to(dev))
-        q = queries(rows, 1, dim, "f32", 2)
+        q = queries(rows, group, dim, "f32", 2)
         k, v, there = held(c, table, ln, 100, dev)
         assert bool(v.isinf().any())
-        got = c.attend_chunk(q.to(dev), table.to(dev), ln.to(dev), starts([rows]).to(dev)).cpu()[:, 0]
+        got = c.attend_chunk(q.to(dev), table.to(dev), ln.to(dev), starts([rows]).to(dev)).cpu()
         fine = got[:rows - 5]
         assert bool(torch.isfinite(fine).all())
-        want = torch.zeros(5, dim)
-        want[:, 5] = math.inf
-        want[2:, 40] = -math.inf
+        want = torch.zeros(5, group, dim)
+        want[:, :, 5] = math.inf
+        want[2:, :, 40] = -math.inf
         assert torch.equal(torch.where(got[rows - 5:].isinf(), got[rows - 5:], torch.zeros(())), want)
         assert not bool(got.isnan().any())
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("rows", [3, 40, 130])
-def test_chunk_queries_at_the_ends(dev, kind, rows):
+@pytest.mark.parametrize("rows,heads", [(3, 2), (40, 2), (130, 2), (130, 17)])
+def test_chunk_queries_at_the_ends(dev, kind, rows, heads):
     """Infinite and NaN queries make their own rows NaN and no other; the largest finite ones and scores far
     beyond 2^20 decide by the largest score; zeros weigh all alike."""
-    print(f"kv4 chunk extreme queries {kind} rows={rows}", flush=True)
+    print(f"kv4 chunk extreme queries {kind} rows={rows} heads={heads}", flush=True)
     dim, n = 64, 200
     c, table, ln, _ = filled(dev, [n], 1, dim, 64, 29, "f32")
-    q = queries(rows, 2, dim, kind, 4).float()
+    q = queries(rows, heads, dim, kind, 4).float()
     q[0, 0, 3], q[1, 1, 7] = math.inf, math.nan
     q[2, 0] = 0.0
     q[1, 0] *= 1.0e4 if kind == "f16" else 1e9
@@ -208,7 +214,7 @@ def test_chunk_queries_at_the_ends(dev, kind, rows):
     k, v, there = held(c, table, ln, n, dev)
     got = c.attend_chunk(q.to(dev), table.to(dev), ln.to(dev), cu.to(dev)).cpu()
     assert bool(got[0, 0].isnan().all()) and bool(got[1, 1].isnan().all())
-    others = torch.ones(rows, 2, dtype=torch.bool)
+    others = torch.ones(rows, heads, dtype=torch.bool)
     others[0, 0] = others[1, 1] = False
     assert bool(torch.isfinite(got[others]).all())
     # a row whose scores are far apart takes the value of the largest
@@ -241,6 +247,9 @@ def test_chunk_strides_and_streams(dev):
     lens, new = [150, 90], [40, 33]
     c, table, ln, _ = filled(dev, lens, 2, 64, 32, 3)
     td, ld, cd = table.to(dev), ln.to(dev), starts(new).to(dev)
+    long = queries(73, 128, 64, "f16", 7).to(dev)  # wide tiles
+    assert torch.equal(c.attend_chunk(long.transpose(0, 1).contiguous().transpose(0, 1), td, ld, cd),
+                       c.attend_chunk(long, td, ld, cd))
     q = queries(73, 4, 64, "f16", 6).to(dev)
     want = c.attend_chunk(q, td, ld, cd)
     odd = torch.empty(73 * 4 * 64 + 1, dtype=torch.float16, device=dev)[1:].view(73, 4, 64)
