@@ -9,24 +9,26 @@
 // head and the chunk's tokens are the rows of one product (row t G + j: token t, head j), so that the codes are
 // expanded once for all that read them. The codes become bf16 exactly (a code has 2 significant bits, bf16 the
 // exponents of f32). q enters as the exact sum of bf16 pieces (f32: 3, f16: 2, bf16: 1), the weights p as pieces too
-// (f32: 3; f16: 2, so that p's error is 2^-17 where the output's rounding is 2^-12; bf16: 1, half a step of 2^-8 on
-// each term as the output), with f32 accumulation; the sum of the weights is of those before they are rounded. The
-// scores are taken transposed, S^T = k q^T on the 32 x 32 x 16 MFMA, keys in an order (bits 2 and 3 of their number
+// (f32: 3; the 16-bit types: 2, so that p's error is 2^-16 beside the output's rounding of 2^-11 or 2^-8; with one,
+// bf16's outputs were 2.36e-3 of their size from float64 where rounding them alone is 1.67e-3, in 553 us for 702 of the
+// case below), with f32 accumulation; the sum of the weights is of those before they are rounded. The scores are
+// taken transposed, S^T = k q^T on the 32 x 32 x 16 MFMA, keys in an order (bits 2 and 3 of their number
 // exchanged) that leaves 8 following tokens in 8 following registers of a lane: the exponentials are, register for
 // register, the second operand of O^T = v^T p^T.
 //
 // Wide tiles, of sequences of many rows: a workgroup of four waves takes 128 rows, 32 a wave, and 64 keys at a time,
 // whose codes, loaded one tile ahead, are expanded into LDS, two tiles in turn, one barrier a tile. Bound by the
 // matrix units beside the exponentials and the expansion: 2048 tokens over 16384, 32 heads over 8 of 128, bf16:
-// 531 us, 971 TFLOP/s; 8192 over 8192 553 us, 994 (the library's 8192^3 product: 1426). f16 560 and f32 380, at 2 and 3
-// times the products. Reading LDS takes as long as the products of bf16, but with 64 rows a wave, which halves it, one
-// wave a SIMD does not hide the exponentials (804 us where these are 555), and eight waves that share the codes take as
-// long (567; in two halves that take turns between products and exponentials 630).
+// 702 us, 734 TFLOP/s, at 1.5 times the products (1.10 PFLOP/s of pieces); 8192 over 8192 735 us, 748 (the library's
+// 8192^3 product: 1426). f16 550 and f32 380, at 2 and 3 times the products. With p of bf16 in one piece reading LDS
+// took as long as the products, but with 64 rows a wave, which halves it, one wave a SIMD did not hide the exponentials
+// (804 us where these were 555), and eight waves that share the codes took as long (567; in two halves that take turns
+// between products and exponentials 630).
 //
-// Narrow tiles, of sequences of few rows, where a product is small beside the reading: 32 rows, of which each wave
-// takes every fourth 32 keys by itself, from memory into operands, joined in LDS at the end. Bound by the reading:
-// 64 sequences of 4000 tokens and one new, bf16: 60 us, 4.6 TB/s (read alone: 7.0); 512 of 1000: 164 us, 3.4 TB/s,
-// where finding the tile and the first loads are a third of a workgroup's time.
+// Narrow tiles, of sequences of few rows: 32 rows, of which each wave takes every fourth 32 keys by itself, from
+// memory into operands, joined in LDS at the end. Bound by the reading and the products beside it: 64 sequences of
+// 4000 tokens and one new, bf16: 74 us, 3.7 TB/s (read alone: 7.0; with p in one piece 60 us); 512 of 1000: 180 us,
+// 3.1 TB/s (167), where finding the tile and the first loads are a third of a workgroup's time.
 //
 // The maximum that is subtracted lags by up to 2^8 (the weights' own size cancels in the quotient) and is a whole
 // number of powers of two, so that a weight is one FMA and one exp2 and all of a row's agree.
@@ -279,15 +281,12 @@ __device__ __forceinline__ v16f zeros16() {
   return z;
 }
 
-template <typename T>
-constexpr int W_PIECES = __is_same(T, float) ? 3 : __is_same(T, _Float16) ? 2 : 1;
-
 // What a wave keeps of 32 rows of one key-value head: the queries' pieces, the running maxima and sums, the outputs.
 // Lane (n, hh) has row n; of the queries channels 16 s + 8 hh .. of step s, of the outputs 32 d + 8 i + 4 hh ...
 // With DIRECT the contracted channels of step s are DIM / 2 hh + 8 s .., the outputs VT (8 (i / 4) + 4 hh + i % 4) + d.
 template <typename T, int DIM, bool DIRECT>
 struct Rows {
-  static constexpr int QP = Q_PIECES<T>, PP = W_PIECES<T>, STEPS = DIM / 16, VT = DIM / 32;
+  static constexpr int QP = Q_PIECES<T>, PP = P_PIECES<T>, STEPS = DIM / 16, VT = DIM / 32;
   Pieces<QP> q[STEPS];
   float m, l;
   v16f o[VT];
@@ -397,7 +396,7 @@ struct Rows {
     scores<SUB>(tk, sub, s);
     const float ref = raise<SUB>(a, tok, there, s);
     float sums[2 * SUB];
-    if constexpr (PP == 1) {
+    if constexpr (QP == 1) {  // all weights first, as the registers allow (2048 tokens over 16384: 711 us in turn, 702 so)
       Pieces<PP> f[2 * SUB];
 #pragma unroll
       for (int e = 0; e < 2 * SUB; ++e) f[e] = weights<SUB>(a, s, ref, e, sums + e);
@@ -572,7 +571,7 @@ __device__ __forceinline__ void wide_tile(const Chunk& a, int id, unsigned char*
 // values under the next scores. The four waves are joined at the end.
 template <typename T, int DIM>
 __device__ __forceinline__ void narrow_tile(const Chunk& a, int id, float* all) {
-  constexpr int VT = DIM / 32, CB = DIM / 32, PP = W_PIECES<T>;
+  constexpr int VT = DIM / 32, CB = DIM / 32, PP = P_PIECES<T>;
   constexpr int WORDS = 16 * VT + 2;
   constexpr int DEPTH = sizeof(T) == 4 && DIM == 128 ? 1 : 2;  // blocks on their way, as the registers allow
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hh = lane >> 5;
@@ -869,7 +868,9 @@ static Chunk::Kind kind_of(int64_t most_tiles, int64_t tiles, int64_t heads, int
 static Cut cut_of(int type, int64_t n, int64_t B, int64_t heads, int64_t group, int64_t dim, int64_t max_len, int64_t tokens) {
   const int64_t units = max_len > 0 ? (max_len + KEYS - 1) / KEYS : 1, begun = B + 2 < n ? B + 2 : n, rows = n * group;
   const double share_us = (double)rows * heads * (2 * 4 * (dim + 2)) / 4e6;  // of all rows, written and read at 4 TB/s
-  // workgroups that run at once (two a CU, three where the registers allow), and a unit's time in one of them then
+  // workgroups that run at once (two a CU, three where the registers allow), and a unit's time in one of them then;
+  // bf16's is that of weights in one piece: 2.6 for 64 channels, as measured with two, cuts 8192 tokens over 8192 in
+  // two (562 us for 445), 2.9 for 128 changes nothing
   const int64_t at_once = dim == 64 && type ? 768 : 512;
   const double unit_us = dim == 64 ? (type == 0 ? 3.3 : type == 1 ? 2.0 : 2.4) : type == 0 ? 5.5 : type == 1 ? 2.3 : 3.7;
   const double mean = B < 1 ? 1.0 : (double)tokens / KEYS / B, usual = mean < units ? mean : (double)units;
