@@ -171,11 +171,13 @@ __device__ __forceinline__ int64_t of_lane(int64_t x, int lane) {
 // passes 2^20, to the maximum itself.
 constexpr float FAR = 0x1p20f;
 __device__ __forceinline__ float ref_of(float m, float c) { return m == -INFINITY ? 0.f : rintf(__fmul_rn(m, c)); }
-// From weights of one maximum to those of another.
+// From weights of one maximum to those of another, each by what its side's are relative to.
 __device__ __forceinline__ float factor(float from, float to, float c) {
   if (from == -INFINITY) return 0.f;
   const float a = ref_of(from, c), b = ref_of(to, c);
-  return __builtin_amdgcn_exp2f(fmaxf(fabsf(a), fabsf(b)) > FAR ? __fmul_rn(__fsub_rn(from, to), c) : __fsub_rn(a, b));
+  const bool far_a = fabsf(a) > FAR, far_b = fabsf(b) > FAR;
+  const float far = __fsub_rn(far_a ? from : 0.f, far_b ? to : 0.f), near = __fsub_rn(far_a ? 0.f : a, far_b ? 0.f : b);
+  return __builtin_amdgcn_exp2f(__fmaf_rn(far, c, near));
 }
 
 // Where a 16-byte piece lies in LDS: row `row` of the keys, channels 8 piece ..; channel `ch` of the
