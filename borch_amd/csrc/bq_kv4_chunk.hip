@@ -31,7 +31,8 @@
 // 3.1 TB/s (167), where finding the tile and the first loads are a third of a workgroup's time.
 //
 // The maximum that is subtracted lags by up to 2^8 (the weights' own size cancels in the quotient) and is a whole
-// number of powers of two, so that a weight is one FMA and one exp2 and all of a row's agree.
+// number of powers of two, so that a weight is one FMA and one exp2 and all of a row's agree. In keys whose values are
+// large it does not lag, so that no weight passes 1 there: f32 holds the sums as far as those of such weights.
 //
 // A tile's keys are cut into shares of up to `upper` units of 64 where the tiles alone would leave the GPU part empty;
 // a second kernel joins the shares of a row.
@@ -61,6 +62,7 @@ struct Chunk {
 };
 
 constexpr int WIDE = 128, FEW = 32, KEYS = 64;  // rows a tile, of sequences of many and of few; keys a unit
+constexpr float LAG = 8.f;  // by how many powers of two the maximum that is subtracted may lag
 // A tile's sequence and rows.
 struct Place {
   int b, start, rows, row0;  // b: -1 for rows of no sequence; the first row of q, the sequence's rows, the tile's first
@@ -167,10 +169,10 @@ __device__ __forceinline__ int64_t of_lane(int64_t x, int lane) {
          (int64_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32;
 }
 
-// A row's weights are relative to 2^ref, ref a whole number near its lagging maximum; or, where that
+// A row's weights are relative to 2^ref, ref the next whole number above its lagging maximum; or, where that
 // passes 2^20, to the maximum itself.
 constexpr float FAR = 0x1p20f;
-__device__ __forceinline__ float ref_of(float m, float c) { return m == -INFINITY ? 0.f : rintf(__fmul_rn(m, c)); }
+__device__ __forceinline__ float ref_of(float m, float c) { return m == -INFINITY ? 0.f : ceilf(__fmul_rn(m, c)); }
 // From weights of one maximum to those of another, each by what its side's are relative to.
 __device__ __forceinline__ float factor(float from, float to, float c) {
   if (from == -INFINITY) return 0.f;
@@ -189,8 +191,10 @@ __device__ __forceinline__ int k_at(int row, int piece) {
 __device__ __forceinline__ int v_at(int ch, int piece) { return ch * 128 + ((piece ^ (((ch >> 1) ^ ((ch >> 4) & 3)) & 7)) << 4); }
 
 constexpr uint32_t HUGE = 253;  // scale bytes from here on may make codes infinite or NaN
-// Which of four bytes are: bits 7, 15, ... of the result.
+// Which of four bytes are: bits 7, 15, ... of the result. And those from 191 on, of values of up to 2^66 and more: of
+// smaller ones 2^31 terms with weights of 2^8 stay far below f32's end.
 __device__ __forceinline__ uint32_t huge_of(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x03030303u) & w & 0x80808080u; }
+__device__ __forceinline__ uint32_t large_of(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x41414141u) & w & 0x80808080u; }
 // Byte I of four as a scale of the expanding conversion, which takes a float's exponent and nothing else of it.
 template <int I>
 __device__ __forceinline__ float scale_byte(uint32_t w) {
@@ -240,6 +244,7 @@ struct Codes {
       }
   }
   __device__ __forceinline__ bool huge() const { return huge_of(vs) != 0; }
+  __device__ __forceinline__ bool large() const { return large_of(vs) != 0; }
   // Into a tile in LDS, as bf16. CLEAR: what is not finite among the values becomes 0 (it is added at the end).
   __device__ __forceinline__ void expand_k(unsigned char* tk, int p) const {
     const int t = p >> 2, row = (t & ~12) | ((t & 4) << 1) | ((t & 8) >> 1);
@@ -331,10 +336,10 @@ struct Rows {
     }
   }
 
-  // What is not seen leaves them (keys from `tok`; there: a bit for each 32 that has a page), and the maximum
-  // follows. Returns what is subtracted.
+  // What is not seen leaves them (keys from `tok`; there: a bit for each 32 that has a page). Returns the maximum,
+  // which the one that is subtracted follows where it is `lag` powers of two above.
   template <int SUB>
-  __device__ __forceinline__ float raise(const Chunk& a, int tok, int there, v16f (&s)[SUB]) {
+  __device__ __forceinline__ float raise(const Chunk& a, int tok, int there, v16f (&s)[SUB], float lag) {
     const int hh = (threadIdx.x >> 5) & 1;
     if (tok + 32 * SUB > sure || there != (1 << SUB) - 1)
 #pragma unroll
@@ -349,7 +354,11 @@ struct Rows {
       for (int i = c + 4; i < 16 * SUB; i += 4) tops[c] = fmaxf(tops[c], s[i / 16][i % 16]);
     }
     const float top = max_xor32(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
-    const bool grew = __fmul_rn(__fsub_rn(top, m), a.scale2) > 8.f;
+    follow(a, top, lag);
+    return top;
+  }
+  __device__ __forceinline__ void follow(const Chunk& a, float top, float lag) {
+    const bool grew = __fmul_rn(__fsub_rn(top, m), a.scale2) > lag;
     if (__any(grew)) {
       const float f = grew ? factor(m, top, a.scale2) : 1.f;
       m = grew ? top : m;
@@ -357,6 +366,10 @@ struct Rows {
 #pragma unroll
       for (int d = 0; d < VT; ++d) o[d] *= f;
     }
+  }
+  // What is subtracted from the scores, times the scale.
+  template <int SUB>
+  __device__ __forceinline__ float base(const Chunk& a, v16f (&s)[SUB]) const {
     float ref = ref_of(m, a.scale2);
     const bool far = fabsf(ref) > FAR;
     if (__any(far)) {  // such rows' differences are taken here, exactly as far as f32 goes
@@ -393,10 +406,11 @@ struct Rows {
   // SUB times 32 keys from `tok`, in a tile's places from 32 sub on.
   template <int SUB>
   __device__ __forceinline__ void keys(const Chunk& a, const unsigned char* tk, const unsigned char* tv, int sub, int tok,
-                                       int there) {
+                                       int there, float lag) {
     v16f s[SUB];
     scores<SUB>(tk, sub, s);
-    const float ref = raise<SUB>(a, tok, there, s);
+    raise<SUB>(a, tok, there, s, lag);
+    const float ref = base<SUB>(a, s);
     float sums[2 * SUB];
     if constexpr (QP == 1) {  // all weights first, as the registers allow (2048 tokens over 16384: 711 us in turn, 702 so)
       Pieces<PP> f[2 * SUB];
@@ -516,6 +530,8 @@ __device__ __forceinline__ void wide_tile(const Chunk& a, int id, unsigned char*
   look(u0);
   int there = 0, loaded = 0;  // a bit for each block that has a page: of the unit expanded last, of the codes in `next`
   bool huge = false;          // whether there were values that may not be finite
+  int* large = reinterpret_cast<int*>(lds + 2 * BUF);  // of each buffer: the last unit of large values
+  if (threadIdx.x < 2) large[threadIdx.x] = -1;
   auto load = [&](int u) {
     if (u - first == 64) look(u);
     const int64_t r0 = of_lane(rows[0], u - first), r1 = of_lane(rows[1], u - first);
@@ -531,8 +547,10 @@ __device__ __forceinline__ void wide_tile(const Chunk& a, int id, unsigned char*
     if (gone || KEYS * u + KEYS > at.len) next.cut(gone ? 0 : at.len - KEYS * u - 4 * (p >> 4));
     unsigned char *tk = lds + buf * BUF, *tv = tk + KB;
     next.expand_k(tk, p);
-    if (__any(next.huge())) {
-      huge = true;
+    const bool far_up = __any(next.large());
+    if (far_up) {
+      large[buf] = u;  // by whichever waves
+      huge |= __any(next.huge());
       next.template expand_v<true>(tv, p);
     } else {
       next.template expand_v<false>(tv, p);
@@ -540,6 +558,8 @@ __device__ __forceinline__ void wide_tile(const Chunk& a, int id, unsigned char*
   };
   if (u0 < u1) {
     load(u0);
+    wait_lds();
+    barrier();
     expand(u0, 0);
     if (u0 + 1 < u1) load(u0 + 1);
   }
@@ -552,12 +572,13 @@ __device__ __forceinline__ void wide_tile(const Chunk& a, int id, unsigned char*
       expand(u + 1, buf ^ 1);
       if (u + 2 < u1) load(u + 2);
     }
+    const float lag = __builtin_amdgcn_readfirstlane(large[buf]) == u ? 0.f : LAG;
     if constexpr (Q_PIECES<T> == 3 && DIM == 128) {  // as the registers allow
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        if (KEYS * u + 32 * e < r.most) r.template keys<1>(a, tk, tv, e, KEYS * u + 32 * e, (now >> e) & 1);
+        if (KEYS * u + 32 * e < r.most) r.template keys<1>(a, tk, tv, e, KEYS * u + 32 * e, (now >> e) & 1, lag);
     } else {
-      if (KEYS * u < r.most) r.template keys<2>(a, tk, tv, 0, KEYS * u, now);
+      if (KEYS * u < r.most) r.template keys<2>(a, tk, tv, 0, KEYS * u, now, lag);
     }
   }
   auto y = [&](int x) -> float& { return r.out(x); };
@@ -649,7 +670,7 @@ __device__ __forceinline__ void narrow_tile(const Chunk& a, int id, float* all) 
       for (int p = Q_PIECES<T> - 1; p >= 0; --p) s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, r.q[e].p[p], s[0], 0, 0, 0);
     }
     load_k(c);
-    const float ref = r.template raise<1>(a, 32 * blk, there, s);
+    const float top = r.template raise<1>(a, 32 * blk, there, s, LAG);
     // values past the length, or of no page, read as zeros
     if (!there || 32 * blk + 32 > at.len) {
 #pragma unroll
@@ -662,8 +683,12 @@ __device__ __forceinline__ void narrow_tile(const Chunk& a, int id, float* all) 
             c.vs[e][i / 4] = (c.vs[e][i / 4] & ~(255u << (8 * (i & 3)))) | (127u << (8 * (i & 3)));
           }
     }
-    const bool odd = __any((huge_of(c.vs[0][0]) | huge_of(c.vs[0][1]) | huge_of(c.vs[1][0]) | huge_of(c.vs[1][1])) != 0);
-    huge |= odd;
+    const bool large = __any((large_of(c.vs[0][0]) | large_of(c.vs[0][1]) | large_of(c.vs[1][0]) | large_of(c.vs[1][1])) != 0);
+    if (large) {
+      huge |= __any((huge_of(c.vs[0][0]) | huge_of(c.vs[0][1]) | huge_of(c.vs[1][0]) | huge_of(c.vs[1][1])) != 0);
+      r.follow(a, top, 0.f);
+    }
+    const float ref = r.template base<1>(a, s);
     float sums[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -693,7 +718,7 @@ __device__ __forceinline__ void narrow_tile(const Chunk& a, int id, float* all) 
       };
       four.template operator()<0>();
       four.template operator()<1>();
-      if (odd)  // what is not finite is added at the end
+      if (large)  // what is not finite is added at the end
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -746,10 +771,12 @@ __device__ __forceinline__ void narrow_tile(const Chunk& a, int id, float* all) 
   r.template store<N>(a, at, h, share, shares, wave * N, part);
 }
 
-// Both in one launch, the wide tiles first; or narrow ones alone, with less LDS and fewer registers.
+// Both in one launch, the wide tiles first; or narrow ones alone, with less LDS and fewer registers. Three workgroups a
+// CU where 64 channels of 16-bit types allow it (f16's wide tiles took 176 registers of the 168 by themselves).
 template <typename T, int DIM, bool WIDES>
-__global__ __launch_bounds__(256, 2) void kv4_chunk_kernel(Chunk a) {
+__global__ __launch_bounds__(256, DIM == 64 && sizeof(T) == 2 ? 3 : 2) void kv4_chunk_kernel(Chunk a) {
   constexpr int TILES = WIDES ? 4 * KEYS * DIM * 2 : 0, JOIN = 4 * (DIM / 2 + 2) * 256, BYTES = TILES > JOIN ? TILES : JOIN;
+  static_assert(!WIDES || BYTES >= TILES + 8);  // the tiles, and which of them hold large values
   __shared__ __attribute__((aligned(1024))) unsigned char lds[BYTES];
   const int wides = a.wide.tiles * a.wide.most * a.c.heads;
   if constexpr (WIDES)

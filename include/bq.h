@@ -560,7 +560,8 @@ size_t bq_kv4_attend_chunk_ws_bytes(int type, int64_t n, int64_t B, int64_t q_he
  *   out [n, q_heads, dim] (contiguous, of q's type) = softmax(scale q k^T) v
  * over the values that the cache stands for, zeros where nothing is seen and in rows of no sequence; what a
  * row does not see never reaches its output. f32 accumulation; products to f32's accuracy, but the weights of the
- * 16-bit types to 2^-16. No atomics: the same bits in every run. ws: bq_kv4_attend_chunk_ws_bytes bytes, 16-byte aligned, need not be
+ * 16-bit types to 2^-16; finite where the values are, as long as f32 holds the sum of the |v| that a row sees. No
+ * atomics: the same bits in every run. ws: bq_kv4_attend_chunk_ws_bytes bytes, 16-byte aligned, need not be
  * cleared. */
 int bq_kv4_attend_chunk(const bq_kv4_cache* cache, const void* q, int type, int64_t n, int64_t q_heads, int64_t q_token,
                         int64_t q_head, const int32_t* table, int64_t B, int64_t width, const int32_t* lens,
