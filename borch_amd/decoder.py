@@ -124,8 +124,8 @@ class Decoder(tnn.Module):
 
     @torch.no_grad()
     def search(self, state: "PagedState", ids: torch.Tensor, lens, beams: int, steps: int, end: int = 0):
-        """Beam search of ``steps`` tokens after each of the prompts ``ids [sum(lens)]``, packed, into an empty
-        ``state`` of ``len(lens) * beams`` sequences. ``tokens`` int32 ``[prompts, beams, steps]`` and ``scores``
+        """Beam search of ``steps`` tokens after each of the prompts ``ids [sum(lens)]``, packed, in a ``state`` of
+        ``len(lens) * beams`` sequences; what they hold ends first. ``tokens`` int32 ``[prompts, beams, steps]`` and ``scores``
         f32 ``[prompts, beams]``, the best first; a beam that has ended goes on with ``end``."""
         B, S, dev = len(lens), len(lens) * beams, ids.device
         if state.pages.sequences != S or beams < 1 or steps < 1 or B < 1 or min(lens) < 1:
@@ -144,6 +144,7 @@ class Decoder(tnn.Module):
         scores[:, 0] = 0.0
         done = torch.zeros(B, beams, dtype=torch.bool, device=dev)
         tokens = torch.zeros(S, steps, dtype=torch.int32, device=dev)
+        state.pages.cut(torch.zeros(S, dtype=torch.int32, device=dev))
         logits = self.read(state, ids, counts.view(-1))
         room, one = state.ok, torch.ones(S, dtype=torch.int32, device=dev)
         for t in range(steps):
