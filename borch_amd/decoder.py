@@ -126,7 +126,8 @@ class Decoder(tnn.Module):
     def search(self, state: "PagedState", ids: torch.Tensor, lens, beams: int, steps: int, end: int = 0):
         """Beam search of ``steps`` tokens after each of the prompts ``ids [sum(lens)]``, packed, in a ``state`` of
         ``len(lens) * beams`` sequences; what they hold ends first. ``tokens`` int32 ``[prompts, beams, steps]`` and ``scores``
-        f32 ``[prompts, beams]``, the best first; a beam that has ended goes on with ``end``."""
+        f32 ``[prompts, beams]``, the best first; a beam that has ended goes on with ``end`` and gives its pages
+        back."""
         B, S, dev = len(lens), len(lens) * beams, ids.device
         if state.pages.sequences != S or beams < 1 or steps < 1 or B < 1 or min(lens) < 1:
             raise RuntimeError(f"search: {B} prompts of at least one token, {beams} beams and {steps} steps, in a state of "
@@ -146,14 +147,18 @@ class Decoder(tnn.Module):
         tokens = torch.zeros(S, steps, dtype=torch.int32, device=dev)
         state.pages.cut(torch.zeros(S, dtype=torch.int32, device=dev))
         logits = self.read(state, ids, counts.view(-1))
-        room, one = state.ok, torch.ones(S, dtype=torch.int32, device=dev)
+        room, blank = state.ok, torch.zeros(S + 1, dtype=torch.int32, device=dev)
+        one, none = torch.ones_like(blank[1:]), torch.full_like(blank[1:], -1)
         for t in range(steps):
             scores, parents, new, done = beam_select(logits, scores, done, end)
             tokens = tokens[parents.view(-1)]
             tokens[:, t] = new.view(-1)
             if t + 1 < steps:
-                state.pages.fork(parents.view(-1))
-                logits = self.read(state, new.view(-1), one)
+                over = done.view(-1)
+                state.pages.fork(torch.where(over, none, parents.view(-1)))
+                live = over ^ one
+                packed = blank.scatter(0, live.cumsum(0) * live, new.view(-1))  # those of ended beams at 0, left out
+                logits = self.read(state, packed[1:], live)
                 room = room * state.ok
         if not room.item():
             raise RuntimeError(f"search: the state's {state.pages.pages} pages are too few")
