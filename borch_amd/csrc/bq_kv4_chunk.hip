@@ -850,19 +850,25 @@ __global__ __launch_bounds__(256) void kv4_chunk_join_kernel(Chunk a) {
 
 // How the work is cut, whatever the lengths are.
 //
-// A sequence takes wide tiles from more than FEW_ROWS rows on (32 sequences of 48 rows beside it, of 3000 tokens: 65 us
-// so, 93 in wide tiles; of 128 rows: 98 in wide tiles, 120 in narrow ones); a call of up to FEW_ALL rows takes narrow
-// tiles alone, for more workgroups (those 48 rows, 1536 in all: 42 us; but 4096 rows so 132 us for 96). Above FEW_MOST
-// rows, where every sequence may fill a wide tile, it takes them if the estimates below say so: 512 tokens of 32 heads
-// over 8, bf16, over 4096: 48 us in narrow tiles, 59 in wide ones; over 16384 174 and 165, over 65536 677 and 596.
+// A sequence takes wide tiles from more than FEW_ROWS rows on; a call of up to FEW_ALL rows takes narrow tiles alone,
+// for more workgroups. Above FEW_MOST rows, where every sequence may fill a wide tile, it takes them if the estimates
+// below say so. In narrow and in wide tiles on one card, 32 heads over 8 of 128, bf16 unless said:
+//   24 new tokens in each of 32 sequences of 3000 (3072 rows) 78 and 100 us, 32 of them 103 and 116, 1024 over 8192 in
+//   f16 (4096 rows) 308 and 270: wide ones are taken; 12 in each of the 32 sequences (1536 rows, narrow either way) 55,
+//   and 71 in the launch that has both
+//   512 tokens (2048 rows) over 4096 62 and 72, over 16384 232 and 217, over 65536 925 and 810
+//   128 tokens (512 rows) over 4096 28 and 36, over 16384 72 and 70, over 65536 252 and 218 (f16 288 and 263, f32 376
+//   and 390; narrow ones are taken); 64 tokens over 65536 137 and 163
+//   32 and 17 tokens over 65536 and 50001, 24 heads over 4, f16: 100 and 140
 //
 // Of the shares that a tile may be cut in that number is taken for which the estimated time is least: of the longest
 // workgroup, of all the work over the workgroups that run at once and the longest begun last, or of whole rounds of
 // equal ones; the workgroups that find no tile; and what the join writes and reads. Narrow tiles' usual length is what
 // the cache's pages hold for each sequence: with the longest sequence's for all, one chunk of 1024 tokens beside 511
-// sequences of one over 1000 took 866 us, so 230. So are wide tiles' where every sequence may have some (three chunks
-// of 512, 500 and 333 tokens over 4096, 1500 and 777, f32: 130 -> 107 us). Narrow tiles beside wide ones are cut only
-// where they would last longer: the join alone, over all rows, is 15 us of 2048 tokens of 32 heads.
+// sequences of one over 1000 took 866 us, so 230 (268 with weights in two pieces). So are wide tiles' where every
+// sequence may have some (three chunks of 512, 500 and 333 tokens over 4096, 1500 and 777, f32: 130 -> 107 us). Narrow
+// tiles beside wide ones are cut only where they would last longer: the join alone, over all rows, is 15 us of 2048
+// tokens of 32 heads.
 constexpr int64_t FEW_ROWS = 64, FEW_ALL = 2048, FEW_MOST = 512;
 static_assert(2 * (FEW_ROWS + 1) > WIDE);
 constexpr double FEW_UNIT_US = 1.2, NONE_US = 4.0;  // a unit of a narrow tile's; a workgroup that finds no tile
