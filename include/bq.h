@@ -540,11 +540,12 @@ size_t bq_kv4_attend_ws_bytes(int64_t B, int64_t heads, int64_t rows, int64_t di
  * token t sees the first min(lens[b], max_len) - tokens + 1 + t cached tokens:
  *   out [B, tokens, q_heads, dim] (contiguous, of q's type) = softmax(scale q k^T) v
  * over the values that the cache stands for, zeros where nothing is seen; what a token does not see
- * never reaches its output. f32 accumulation, f32 products to f32's accuracy. weights (nullable) f32,
- * at w_seq and w_head elements from sequence to sequence and head to head, has each cached token's
- * softmax weights added, summed over the queries of its key-value head (no atomics: the same bits in
- * every run; rows of different sequences and heads share no place). ws: bq_kv4_attend_ws_bytes bytes,
- * 16-byte aligned, need not be cleared. */
+ * never reaches its output. f32 accumulation, f32 products to f32's accuracy; finite where the values
+ * are, as long as f32 holds 256 times the sum of the |v| that a token sees. weights (nullable) f32, at
+ * w_seq and w_head elements from sequence to sequence and head to head, has each cached token's softmax
+ * weights added, summed over the queries of its key-value head (no atomics: the same bits in every run;
+ * rows of different sequences and heads share no place). ws: bq_kv4_attend_ws_bytes bytes, 16-byte
+ * aligned, need not be cleared. */
 int bq_kv4_attend(const bq_kv4_cache* cache, const void* q, int type, int64_t tokens, int64_t q_heads, int64_t q_seq,
                   int64_t q_token, int64_t q_head, const int32_t* table, int64_t B, int64_t width, const int32_t* lens,
                   int64_t max_len, float scale, void* out, float* weights, int64_t w_seq, int64_t w_head, void* ws,
