@@ -40,4 +40,6 @@ def test_chunk_large_values(dev, monkeypatch, kind, dim, n, rows, group, where):
     assert bool(torch.isfinite(hv).all()) and float(hv.max()) == 6 * 2.0 ** 125
     got = c.attend_chunk(q.to(dev), table.to(dev), ln.to(dev), cu.to(dev))
     assert bool(torch.isfinite(got).all())
+    for _ in range(3):
+        assert torch.equal(got, c.attend_chunk(q.to(dev), table.to(dev), ln.to(dev), cu.to(dev)))
     C.check(got, q, hk, hv, there, ln, cu, n, kind)
