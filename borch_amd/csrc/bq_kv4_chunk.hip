@@ -853,7 +853,7 @@ __global__ __launch_bounds__(256) void kv4_chunk_join_kernel(Chunk a) {
 // A sequence takes wide tiles from more than FEW_ROWS rows on; a call of up to FEW_ALL rows takes narrow tiles alone,
 // for more workgroups. Above FEW_MOST rows, where every sequence may fill a wide tile, it takes them if the estimates
 // below say so. In narrow and in wide tiles on one card, 32 heads over 8 of 128, bf16 unless said:
-//   24 new tokens in each of 32 sequences of 3000 (3072 rows) 78 and 100 us, 32 of them 103 and 116, 1024 over 8192 in
+//   24 new tokens in each of 32 sequences of 3000 78 and 100 us, 32 of them 103 and 116, 1024 over 8192 in
 //   f16 (4096 rows) 308 and 270: wide ones are taken; 12 in each of the 32 sequences (1536 rows, narrow either way) 55,
 //   and 71 in the launch that has both
 //   512 tokens (2048 rows) over 4096 62 and 72, over 16384 232 and 217, over 65536 925 and 810
