@@ -559,7 +559,7 @@ __device__ __forceinline__ void wide_tile(const Chunk& a, int id, unsigned char*
   if (u0 < u1) {
     load(u0);
     wait_lds();
-    barrier();
+    barrier();  // `large` is set
     expand(u0, 0);
     if (u0 + 1 < u1) load(u0 + 1);
   }

@@ -125,9 +125,9 @@ class Decoder(tnn.Module):
     @torch.no_grad()
     def search(self, state: "PagedState", ids: torch.Tensor, lens, beams: int, steps: int, end: int = 0):
         """Beam search of ``steps`` tokens after each of the prompts ``ids [sum(lens)]``, packed, in a ``state`` of
-        ``len(lens) * beams`` sequences; what they hold ends first. ``tokens`` int32 ``[prompts, beams, steps]`` and ``scores``
-        f32 ``[prompts, beams]``, the best first; a beam that has ended goes on with ``end`` and gives its pages
-        back."""
+        ``len(lens) * beams`` sequences; what they hold ends first. ``tokens`` int32 ``[prompts, beams, steps]``
+        and ``scores`` f32 ``[prompts, beams]``, the best first; a beam that has ended goes on with ``end`` and
+        gives its pages back."""
         B, S, dev = len(lens), len(lens) * beams, ids.device
         if state.pages.sequences != S or beams < 1 or steps < 1 or B < 1 or min(lens) < 1:
             raise RuntimeError(f"search: {B} prompts of at least one token, {beams} beams and {steps} steps, in a state of "
